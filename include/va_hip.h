@@ -464,6 +464,94 @@ typedef struct {
 va_status va_probe_mfma(va_context* ctx, va_probe_kind kind, int random_operands, uint32_t iterations,
                         va_probe_result* out);
 
+/* ---- training and serving of the embeddings a collection holds ----------------------------------
+ * What a program needs around the search: the loss that trains queries against all items of a
+ * collection, the norm and 8-bit coding of an encoder's output, and the clipping of its gradients.
+ * Device pointers and the context's stream as everywhere; nothing here waits on the host except to
+ * grow the scratch arena.  Rows are row-major with a stride in elements; sums, softmax statistics
+ * and norms are fp32 or wider whatever the type. */
+typedef enum { VA_DTYPE_F32 = 0, VA_DTYPE_F16 = 1, VA_DTYPE_BF16 = 2 } va_dtype;
+typedef enum { VA_REDUCE_MEAN = 0, VA_REDUCE_SUM = 1, VA_REDUCE_NONE = 2 } va_reduction;
+
+#define VA_XENT_MAX_DIM 65536u
+
+/* Softmax cross entropy of `rows` hidden rows over `num_items` items (a vocabulary, or the rows of
+ * a collection):  l_tj = scale h_t . w_j + o_j,  lse_t = log sum_j exp l_tj,  loss_t = lse_t - l_{t,y_t}.
+ * The rows x items matrix is never stored.
+ *  - offsets (may be NULL): o_j, constants (no gradient): sampling corrections, and -inf for items
+ *    that are deleted, which have probability and gradient 0 whatever their vector holds.  With
+ *    every item masked, lse is -inf and losses and gradients are 0.  A masked target's loss is +inf.
+ *  - a row whose target is ignore_index has loss 0 and gradient 0; a target outside
+ *    [0, num_items) gives that row a NaN loss and gradient 0. */
+typedef struct {
+    const void* hidden;      /* [rows x dim] */
+    const void* items;       /* [num_items x dim] */
+    const int64_t* targets;  /* [rows] */
+    const float* offsets;    /* [num_items] or NULL */
+    uint64_t hidden_stride;  /* elements between rows */
+    uint64_t items_stride;
+    int64_t ignore_index;
+    uint32_t rows, num_items, dim;
+    va_dtype dtype;          /* of hidden, items and their gradients */
+    float scale;
+} va_xent_desc;
+/* out_loss, out_lse: [rows]; out_reduced: the sum of the losses, or their mean over the rows whose
+ * target is not ignore_index (0 when there is none); NULL exactly when reduction is VA_REDUCE_NONE. */
+va_status va_xent_forward(va_context* ctx, const va_xent_desc* desc, float* out_loss, float* out_lse,
+                          va_reduction reduction, float* out_reduced);
+/* Gradients of the reduced loss (times *grad, 1 when grad is NULL) or, without a reduction, of
+ * sum_t grad[t] loss_t.  lse: va_xent_forward's.  Either output may be NULL. */
+va_status va_xent_backward(va_context* ctx, const va_xent_desc* desc, const float* lse, va_reduction reduction,
+                           const float* grad, void* out_grad_hidden, uint64_t grad_hidden_stride,
+                           void* out_grad_items, uint64_t grad_items_stride);
+
+/* Root-mean-square norm of rows, after the addition of a residual:
+ *   r = x + residual,  i = 1 / sqrt(mean_d r_d^2 + epsilon),  y_d = r_d i w_d.
+ * residual, out_residual (r in the rows' type) and out_inverse_rms (i, [rows] fp32) may be NULL;
+ * outputs may be the inputs they replace.  8-bit outputs: code = round(y / s) (ties to even,
+ * saturating) with s = max |y| / 127 (int8) or / 448 (fp8, e4m3 without infinities) over each group
+ * of `group` dimensions (0: the row; else a power of two from 8 to 512, the last one may be
+ * shorter), written to out_scales [rows x groups]; or with one given scale > 0 and no out_scales
+ * (codes on one grid, as va_i8_scan_topk compares them).  A group of zeros has scale 0; one that
+ * holds NaN or inf has a scale that is not finite. */
+typedef enum { VA_CODE_INT8 = 0, VA_CODE_FP8_E4M3 = 1 } va_code;
+typedef struct {
+    const void* x;           /* [rows x dim] */
+    const void* residual;    /* [rows x dim] or NULL */
+    const void* weight;      /* [dim] */
+    void* out_residual;      /* [rows x dim] or NULL */
+    float* out_inverse_rms;  /* [rows] or NULL */
+    uint64_t x_stride, residual_stride, out_residual_stride; /* elements between rows */
+    uint32_t rows, dim;
+    va_dtype dtype;          /* of x, residual, weight, out_residual and the output rows */
+    float epsilon;
+} va_rms_desc;
+va_status va_rms_norm(va_context* ctx, const va_rms_desc* desc, void* out, uint64_t out_stride);
+va_status va_rms_norm_quantized(va_context* ctx, const va_rms_desc* desc, va_code code, uint32_t group,
+                                float given_scale, void* out_codes, uint64_t codes_stride, float* out_scales);
+/* out = code * scale in `dtype` */
+va_status va_rms_dequantize(va_context* ctx, const void* codes, uint64_t codes_stride, va_code code,
+                            const float* scales, float given_scale, uint32_t rows, uint32_t dim, uint32_t group,
+                            va_dtype dtype, void* out, uint64_t out_stride);
+/* desc: x is r (va_rms_norm's out_residual, or x where there was no residual), no residual and no
+ * outputs.  grad: of y; grad_residual (may be NULL): what reaches r past the norm.  out_grad_x is the
+ * gradient of x and of the residual alike; either output may be NULL. */
+va_status va_rms_norm_backward(va_context* ctx, const va_rms_desc* desc, const void* grad, uint64_t grad_stride,
+                               const void* grad_residual, uint64_t grad_residual_stride, const float* inverse_rms,
+                               void* out_grad_x, uint64_t grad_x_stride, void* out_grad_weight);
+
+/* The 2-norm n of all values of a list of tensors (out_norm, one float; may be NULL), and every
+ * tensor times min(1, max_norm / (n + epsilon)), into `outputs` or in place (outputs NULL).  The
+ * arrays are host memory, read before the call returns; tensors may be empty. */
+typedef struct {
+    void* const* tensors;    /* device, contiguous */
+    void* const* outputs;    /* device, or NULL: in place */
+    const uint64_t* sizes;   /* values of each */
+    const int32_t* dtypes;   /* va_dtype of each */
+    uint32_t count;
+} va_tensor_list;
+va_status va_grad_clip(va_context* ctx, const va_tensor_list* list, float max_norm, float epsilon, float* out_norm);
+
 #ifdef __cplusplus
 }
 #endif

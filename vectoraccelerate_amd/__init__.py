@@ -48,8 +48,20 @@ from .quantization import (
     ScalarQuantizationKernel,
     ScalarQuantKernel,
 )
+from .training import (
+    GradientClipKernel,
+    RMSNormKernel,
+    SoftmaxCrossEntropyKernel,
+    SoftmaxCrossEntropyResult,
+    TensorList,
+)
 
 __all__ = [
+    "GradientClipKernel",
+    "RMSNormKernel",
+    "SoftmaxCrossEntropyKernel",
+    "SoftmaxCrossEntropyResult",
+    "TensorList",
     "MetalComputeProvider",
     "SupportedDistanceMetric",
     "EuclideanDistance",

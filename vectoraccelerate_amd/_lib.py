@@ -35,6 +35,16 @@ VA_MAX_K = 1024
 VA_I8_MAX_DIM = 131071  # va_i8_scan_topk: the int32 dot of two code vectors stays exact
 VA_NOALLOC_SCRATCH_BYTES = 64 << 20
 
+VA_DTYPE_F32 = 0
+VA_DTYPE_F16 = 1
+VA_DTYPE_BF16 = 2
+VA_REDUCE_MEAN = 0
+VA_REDUCE_SUM = 1
+VA_REDUCE_NONE = 2
+VA_CODE_INT8 = 0
+VA_CODE_FP8_E4M3 = 1
+VA_XENT_MAX_DIM = 65536
+
 VA_PROBE_FP32 = 0
 VA_PROBE_FP16 = 1
 VA_PROBE_INT8 = 2
@@ -111,6 +121,13 @@ SIGNATURES: dict[str, tuple] = {
     "va_pq_distance_tables": (_st, [_p, _p, _u32, _u32, _u32, _u32, _p, _p]),
     "va_pq_adc_distances": (_st, [_p, _p, _u32, _p, _u32, _u32, _u32, _p]),
     "va_pq_search": (_st, [_p, _p, _u32, _u32, _u32, _u32, _p, _p, _u32, _u32, _p, _p]),
+    "va_xent_forward": (_st, [_p, _p, _p, _p, _i32, _p]),
+    "va_xent_backward": (_st, [_p, _p, _p, _i32, _p, _p, _u64, _p, _u64]),
+    "va_rms_norm": (_st, [_p, _p, _p, _u64]),
+    "va_rms_norm_quantized": (_st, [_p, _p, _i32, _u32, C.c_float, _p, _u64, _p]),
+    "va_rms_dequantize": (_st, [_p, _p, _u64, _i32, _p, C.c_float, _u32, _u32, _u32, _i32, _p, _u64]),
+    "va_rms_norm_backward": (_st, [_p, _p, _p, _u64, _p, _u64, _p, _p, _u64, _p]),
+    "va_grad_clip": (_st, [_p, _p, C.c_float, C.c_float, _p]),
     "va_probe_mfma": (_st, [_p, _i32, _i32, _u32, _p]),
 }
 
@@ -166,6 +183,56 @@ class ProbeResult(C.Structure):
         ("engine_mhz", C.c_double),
         ("ms", C.c_double),
         ("ops", C.c_double),
+    ]
+
+
+class XentDesc(C.Structure):
+    """va_xent_desc (include/va_hip.h)."""
+
+    _fields_ = [
+        ("hidden", C.c_void_p),
+        ("items", C.c_void_p),
+        ("targets", C.c_void_p),
+        ("offsets", C.c_void_p),
+        ("hidden_stride", C.c_uint64),
+        ("items_stride", C.c_uint64),
+        ("ignore_index", C.c_int64),
+        ("rows", C.c_uint32),
+        ("num_items", C.c_uint32),
+        ("dim", C.c_uint32),
+        ("dtype", C.c_int),
+        ("scale", C.c_float),
+    ]
+
+
+class RmsDesc(C.Structure):
+    """va_rms_desc (include/va_hip.h)."""
+
+    _fields_ = [
+        ("x", C.c_void_p),
+        ("residual", C.c_void_p),
+        ("weight", C.c_void_p),
+        ("out_residual", C.c_void_p),
+        ("out_inverse_rms", C.c_void_p),
+        ("x_stride", C.c_uint64),
+        ("residual_stride", C.c_uint64),
+        ("out_residual_stride", C.c_uint64),
+        ("rows", C.c_uint32),
+        ("dim", C.c_uint32),
+        ("dtype", C.c_int),
+        ("epsilon", C.c_float),
+    ]
+
+
+class TensorListDesc(C.Structure):
+    """va_tensor_list (include/va_hip.h)."""
+
+    _fields_ = [
+        ("tensors", C.c_void_p),
+        ("outputs", C.c_void_p),
+        ("sizes", C.c_void_p),
+        ("dtypes", C.c_void_p),
+        ("count", C.c_uint32),
     ]
 
 

@@ -1,0 +1,192 @@
+// va_clip.hip — the global 2-norm of a list of gradients, and the gradients clipped by it.
+//
+//   n = sqrt(sum over all values g^2)        out = g min(1, max_norm / (n + eps))
+//
+// Bound by memory: the gradients are read twice (the factor is known after the last of them) and
+// written once.  The list travels in the kernels' arguments, kListMax tensors a launch, so a
+// call leaves nothing behind that it would have to wait for.  A tensor is cut into chunks of
+// kChunk values; a workgroup takes chunks in turn and leaves one sum.  Sums are fp64 from the first
+// product on (gradients of any magnitude, no overflow) and joined in a fixed order by every workgroup
+// of the second pass, so results do not depend on the order in which workgroups run.  The second pass
+// starts where the first one ended: what is left of it in the caches is read from there.
+#include <algorithm>
+#include <cmath>
+
+#include "va_internal.hpp"
+
+namespace va {
+namespace {
+
+constexpr uint32_t kChunk = 16384;
+constexpr uint32_t kListMax = 96;     // 3 KiB of arguments
+constexpr uint32_t kMaxSums = 1024;   // workgroups of the first pass, all launches together
+
+struct Entry {
+    const void* in;
+    void* out;
+    uint64_t count;
+    uint32_t chunk0;  // first chunk of the tensor among the launch's
+    uint32_t dtype;
+};
+struct List {
+    Entry e[kListMax];
+    uint32_t n, chunks;
+};
+
+template <class T>
+using Vec8 = T __attribute__((ext_vector_type(8), aligned(sizeof(T))));
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+
+// the tensor that holds chunk c
+__device__ __forceinline__ const Entry& entry_of(const List& l, uint32_t c) {
+    uint32_t lo = 0, hi = l.n - 1;
+    while (lo < hi) {
+        const uint32_t mid = (lo + hi + 1) >> 1;
+        if (l.e[mid].chunk0 <= c) lo = mid;
+        else hi = mid - 1;
+    }
+    return l.e[lo];
+}
+
+__device__ __forceinline__ double block_sum(double v, double* part) {
+    for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d);
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = 0.0;
+    for (uint32_t i = 0; i < blockDim.x / 64; ++i) v += part[i];
+    return v;
+}
+
+template <class T>
+__device__ __forceinline__ double square_sum(const T* p, uint32_t n) {
+    double s[2] = {0.0, 0.0};
+    const uint32_t full = n / 8;
+    for (uint32_t i = threadIdx.x; i < full; i += 256) {
+        const Vec8<T> v = *reinterpret_cast<const Vec8<T>*>(p + 8 * i);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const double x = double(float(v[e]));
+            s[e & 1] = fma(x, x, s[e & 1]);
+        }
+    }
+    const uint32_t i = 8 * full + threadIdx.x;
+    if (i < n) {
+        const double x = double(float(p[i]));
+        s[0] = fma(x, x, s[0]);
+    }
+    return s[0] + s[1];
+}
+
+__global__ __launch_bounds__(256) void clip_norm_kernel(List l, double* sums) {
+    __shared__ double part[4];
+    double s = 0.0;
+    for (uint32_t c = blockIdx.x; c < l.chunks; c += gridDim.x) {
+        const Entry& e = entry_of(l, c);
+        const uint64_t at = uint64_t(c - e.chunk0) * kChunk;
+        const uint32_t n = uint32_t(min(uint64_t(kChunk), e.count - at));
+        if (e.dtype == VA_DTYPE_F32) s += square_sum(static_cast<const float*>(e.in) + at, n);
+        else if (e.dtype == VA_DTYPE_F16) s += square_sum(static_cast<const _Float16*>(e.in) + at, n);
+        else s += square_sum(static_cast<const __bf16*>(e.in) + at, n);
+    }
+    s = block_sum(s, part);
+    if (threadIdx.x == 0) sums[blockIdx.x] = s;
+}
+
+template <class T>
+__device__ __forceinline__ void scale_chunk(const T* in, T* out, uint32_t n, float f) {
+    const uint32_t full = n / 8;
+    for (uint32_t i = threadIdx.x; i < full; i += 256) {
+        const f32x8 v = __builtin_convertvector(*reinterpret_cast<const Vec8<T>*>(in + 8 * i), f32x8) * f;
+        *reinterpret_cast<Vec8<T>*>(out + 8 * i) = __builtin_convertvector(v, Vec8<T>);
+    }
+    const uint32_t i = 8 * full + threadIdx.x;
+    if (i < n) out[i] = T(float(in[i]) * f);
+}
+
+__global__ __launch_bounds__(256) void clip_scale_kernel(List l, const double* __restrict__ sums, uint32_t nsums, float max_norm, float eps,
+                                                         float* out_norm) {
+    __shared__ double part[4];
+    double s = 0.0;
+    for (uint32_t i = threadIdx.x; i < nsums; i += 256) s += sums[i];
+    const double norm = sqrt(block_sum(s, part));
+    // (a comparison that is false for NaN keeps it, as the quotient does)
+    const double q = double(max_norm) / (norm + double(eps));
+    const float f = q > 1.0 ? 1.0f : float(q);
+    if (out_norm && blockIdx.x == 0 && threadIdx.x == 0) *out_norm = float(norm);
+    for (uint32_t i = blockIdx.x; i < l.chunks; i += gridDim.x) {
+        const uint32_t c = l.chunks - 1 - i;
+        const Entry& e = entry_of(l, c);
+        if (f == 1.0f && e.in == e.out) continue;  // in place, and nothing changes
+        const uint64_t at = uint64_t(c - e.chunk0) * kChunk;
+        const uint32_t n = uint32_t(min(uint64_t(kChunk), e.count - at));
+        if (e.dtype == VA_DTYPE_F32) scale_chunk(static_cast<const float*>(e.in) + at, static_cast<float*>(e.out) + at, n, f);
+        else if (e.dtype == VA_DTYPE_F16) scale_chunk(static_cast<const _Float16*>(e.in) + at, static_cast<_Float16*>(e.out) + at, n, f);
+        else scale_chunk(static_cast<const __bf16*>(e.in) + at, static_cast<__bf16*>(e.out) + at, n, f);
+    }
+}
+
+// tensors [i, ...) of the list into one launch's arguments; the first tensor not taken
+va_status take(va_context* ctx, const va_tensor_list* t, uint32_t i, List& l, uint32_t& next) {
+    l.n = 0;
+    uint64_t chunks = 0;
+    for (; i < t->count && l.n < kListMax; ++i) {
+        if (!t->sizes[i]) continue;
+        const uint64_t c = (t->sizes[i] + kChunk - 1) / kChunk;
+        VA_REQUIRE(ctx, chunks + c < 0xFFFFFFFFull, "va_grad_clip: too many values");
+        l.e[l.n++] = Entry{t->tensors[i], t->outputs ? t->outputs[i] : t->tensors[i], t->sizes[i], uint32_t(chunks), uint32_t(t->dtypes[i])};
+        chunks += c;
+    }
+    l.chunks = uint32_t(chunks);
+    next = i;
+    return VA_OK;
+}
+
+}  // namespace
+}  // namespace va
+
+using namespace va;
+
+extern "C" {
+
+va_status va_grad_clip(va_context* ctx, const va_tensor_list* t, float max_norm, float epsilon, float* out_norm) {
+    if (!ctx) return VA_ERR_INVALID_ARG;
+    VA_REQUIRE(ctx, t && (t->count == 0 || (t->tensors && t->sizes && t->dtypes)), "va_grad_clip: NULL list");
+    VA_REQUIRE(ctx, max_norm >= 0.0f, "va_grad_clip: max_norm must not be negative or NaN");
+    VA_REQUIRE(ctx, std::isfinite(epsilon) && epsilon >= 0.0f, "va_grad_clip: epsilon must be finite and not negative");
+    uint64_t total = 0;
+    for (uint32_t i = 0; i < t->count; ++i) {
+        VA_REQUIRE(ctx, t->dtypes[i] == VA_DTYPE_F32 || t->dtypes[i] == VA_DTYPE_F16 || t->dtypes[i] == VA_DTYPE_BF16, "va_grad_clip: tensor %u: unknown type %d", i, int(t->dtypes[i]));
+        const uintptr_t es = t->dtypes[i] == VA_DTYPE_F32 ? 4 : 2;
+        const void* o = t->outputs ? t->outputs[i] : t->tensors[i];
+        VA_REQUIRE(ctx, !t->sizes[i] || (t->tensors[i] && o), "va_grad_clip: tensor %u is NULL", i);
+        VA_REQUIRE(ctx, reinterpret_cast<uintptr_t>(t->tensors[i]) % es == 0 && reinterpret_cast<uintptr_t>(o) % es == 0, "va_grad_clip: tensor %u is not aligned to its type", i);
+        total += (t->sizes[i] + kChunk - 1) / kChunk;
+    }
+    DeviceGuard guard(ctx->device);
+    Scratch sc(ctx);
+    const uint32_t launches = ceil_div(t->count, kListMax);
+    VA_CHECK_STATUS(sc.reserve(Scratch::round((kMaxSums + launches) * sizeof(double))));
+    double* sums = sc.carve<double>(kMaxSums + launches);
+    uint32_t n = 0;
+    List l;
+    for (uint32_t i = 0; i < t->count;) {
+        VA_CHECK_STATUS(take(ctx, t, i, l, i));
+        if (!l.n) break;
+        // the launch's share of the sums, by its share of the chunks
+        const uint32_t grid = uint32_t(std::max<uint64_t>(std::min<uint64_t>(l.chunks, uint64_t(kMaxSums) * l.chunks / std::max<uint64_t>(total, kMaxSums)), 1));
+        clip_norm_kernel<<<dim3(grid), dim3(256), 0, ctx->stream>>>(l, sums + n);
+        VA_CHECK_LAUNCH(ctx);
+        n += grid;
+    }
+    bool told = false;
+    for (uint32_t i = 0; i < t->count || !told;) {
+        VA_CHECK_STATUS(take(ctx, t, i, l, i));
+        if (!l.n && told) break;
+        clip_scale_kernel<<<dim3(std::min(std::max(l.chunks, 1u), 2048u)), dim3(256), 0, ctx->stream>>>(l, sums, n, max_norm, epsilon, told ? nullptr : out_norm);
+        VA_CHECK_LAUNCH(ctx);
+        told = true;
+    }
+    return VA_OK;
+}
+
+}  // extern "C"

@@ -1,0 +1,571 @@
+// va_rmsnorm.hip — root-mean-square norm of rows with the residual's addition, its backward pass,
+// and the output in 8 bits with scales.
+//
+//   r = x + residual     i = 1 / sqrt(mean_d r_d^2 + eps)     y_d = r_d i w_d
+//   codes: s = max |y| over a group / M (M = 127 for int8, 448 for fp8 e4m3), code = round(y / s)
+//   dx = i (w dy - n mean_d(w dy n)) + dresidual,  dw = sum_t dy n,  n = r i
+//
+// Bound by memory: every operand is read once and every result written once.  A row is held in
+// registers by one wave (D <= 2048) or one workgroup (D <= 8192): 8 consecutive values a lane and
+// chunk, so a group's largest value is a few lane exchanges away.  Longer rows are read twice, the
+// second time from cache.  Values are loaded 16 bytes at a time whatever their alignment (global
+// loads on gfx950 need none beyond the element's); a row's last, partial 8 values element by element.
+// Sums are fp32 (a lane's chain of at most 32 values, then a tree).
+#include <algorithm>
+#include <cmath>
+
+#include "va_internal.hpp"
+
+namespace va {
+namespace {
+
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+
+enum Out : int { OUT_SAME = 0, OUT_INT8 = 1, OUT_FP8 = 2 };
+
+template <int DT>
+struct Elem;
+template <>
+struct Elem<VA_DTYPE_F32> {
+    using T = float;
+};
+template <>
+struct Elem<VA_DTYPE_F16> {
+    using T = _Float16;
+};
+template <>
+struct Elem<VA_DTYPE_BF16> {
+    using T = __bf16;
+};
+template <int DT>
+using ElemT = typename Elem<DT>::T;
+
+// 8 consecutive values with no alignment beyond the element's
+template <class T>
+using Vec8 = T __attribute__((ext_vector_type(8), aligned(sizeof(T))));
+
+// values [d, d + 8) of a row as fp32, zeros from D on
+template <class T>
+__device__ __forceinline__ f32x8 load8(const T* row, uint32_t d, uint32_t D) {
+    f32x8 o;
+    if (d + 8 <= D) {
+        const Vec8<T> v = *reinterpret_cast<const Vec8<T>*>(row + d);
+        o = __builtin_convertvector(v, f32x8);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e] = d + e < D ? float(row[d + e]) : 0.0f;
+    }
+    return o;
+}
+template <class T>
+__device__ __forceinline__ void store8(T* row, uint32_t d, uint32_t D, f32x8 v) {
+    const auto o = __builtin_convertvector(v, Vec8<T>);
+    if (d + 8 <= D) {
+        *reinterpret_cast<Vec8<T>*>(row + d) = o;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (d + e < D) row[d + e] = o[e];
+    }
+}
+
+template <int N>
+__device__ __forceinline__ float lanes_sum(float v) {
+#pragma unroll
+    for (int d = 1; d < N; d <<= 1) v += __shfl_xor(v, d);
+    return v;
+}
+// the larger of two magnitudes; NaN stays
+__device__ __forceinline__ float top(float a, float b) { return b > a || b != b ? b : a; }
+
+// a sum over the row's threads (one wave, or the workgroup's four)
+template <int WPR>
+__device__ __forceinline__ float row_sum(float v, float* part) {
+    v = lanes_sum<64>(v);
+    if constexpr (WPR > 1) {
+        __syncthreads();  // the previous row's sums are read
+        if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = (part[0] + part[1]) + (part[2] + part[3]);
+    }
+    return v;
+}
+template <int WPR>
+__device__ __forceinline__ float row_top(float v, float* part) {
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) v = top(v, __shfl_xor(v, d));
+    if constexpr (WPR > 1) {
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = top(top(part[0], part[1]), top(part[2], part[3]));
+    }
+    return v;
+}
+
+struct RmsArgs {
+    const void* x;
+    const void* residual;  // or nullptr
+    const void* weight;
+    void* out_residual;  // or nullptr
+    float* inverse;      // or nullptr
+    void* out;
+    float* scales;  // 8-bit outputs without a given scale
+    uint64_t ldx, ldr, ldro, ldo;
+    uint32_t T, D, group, groups;  // group 0: the row
+    float eps, given;              // given > 0: the scale
+};
+
+__device__ __forceinline__ uint2 codes8(f32x8 y, float inv, bool fp8) {
+    uint32_t w[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        float z[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            z[e] = y[4 * h + e] * inv;
+            const float most = fp8 ? 448.0f : 127.0f;
+            z[e] = z[e] != z[e] ? z[e] : fminf(fmaxf(z[e], -most), most);
+        }
+        if (fp8) {
+            int p = __builtin_amdgcn_cvt_pk_fp8_f32(z[0], z[1], 0, false);
+            w[h] = uint32_t(__builtin_amdgcn_cvt_pk_fp8_f32(z[2], z[3], p, true));
+        } else {
+            w[h] = 0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[h] |= (uint32_t(z[e] == z[e] ? int(rintf(z[e])) : 0) & 0xFFu) << (8 * e);
+        }
+    }
+    return make_uint2(w[0], w[1]);
+}
+__device__ __forceinline__ void store_codes(uint8_t* row, uint32_t d, uint32_t D, uint2 c) {
+    if (d + 8 <= D) {
+        typedef uint32_t u32x2 __attribute__((ext_vector_type(2), aligned(1)));
+        *reinterpret_cast<u32x2*>(row + d) = u32x2{c.x, c.y};
+    } else {
+        for (int e = 0; e < 8; ++e)
+            if (d + e < D) row[d + e] = uint8_t((e < 4 ? c.x >> (8 * e) : c.y >> (8 * (e - 4))) & 0xFFu);
+    }
+}
+
+// WPR waves a row; C chunks of 8 values a lane in registers, or (C == 0) any number, read again
+template <int DT, int OUT, int WPR, int C>
+__global__ __launch_bounds__(256) void rms_norm_kernel(RmsArgs a) {
+    using T = ElemT<DT>;
+    constexpr int NT = 64 * WPR;
+    __shared__ float part[4];
+    const uint32_t t = WPR == 1 ? blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
+    if (t >= a.T) return;  // (a whole wave, or the workgroup)
+    const uint32_t tid = WPR == 1 ? threadIdx.x & 63 : threadIdx.x;
+    const T* x = static_cast<const T*>(a.x) + t * a.ldx;
+    const T* res = a.residual ? static_cast<const T*>(a.residual) + t * a.ldr : nullptr;
+    const T* w = static_cast<const T*>(a.weight);
+    T* ro = a.out_residual ? static_cast<T*>(a.out_residual) + t * a.ldro : nullptr;
+    const uint32_t D = a.D, chunks = C ? C : (D + 8 * NT - 1) / (8 * NT);
+    auto sum8 = [&](uint32_t d) {
+        f32x8 v = load8(x, d, D);
+        if (res) v += load8(res, d, D);
+        return v;
+    };
+    f32x8 r[C ? C : 1];
+    float ss = 0.0f;
+    if constexpr (C > 0) {
+#pragma unroll
+        for (int c = 0; c < C; ++c) r[c] = sum8((c * NT + tid) * 8);
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) ss = fmaf(r[c][e], r[c][e], ss);
+    } else {
+        for (uint32_t c = 0; c < chunks; ++c) {
+            const f32x8 v = sum8((c * NT + tid) * 8);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) ss = fmaf(v[e], v[e], ss);
+        }
+    }
+    ss = row_sum<WPR>(ss, part);
+    const float inv = 1.0f / sqrtf(ss / float(D) + a.eps);
+    if (a.inverse && tid == 0) a.inverse[t] = inv;
+
+    // y of a chunk, the new residual stored on the way (once)
+    auto y_of = [&](uint32_t d, f32x8 v, bool keep) {
+        if (ro && keep) store8(ro, d, D, v);
+        return v * inv * load8(w, d, D);
+    };
+    if constexpr (OUT == OUT_SAME) {
+        T* o = static_cast<T*>(a.out) + t * a.ldo;
+        if constexpr (C > 0) {
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                const uint32_t d = (c * NT + tid) * 8;
+                store8(o, d, D, y_of(d, r[c], true));
+            }
+        } else {
+            for (uint32_t c = 0; c < chunks; ++c) {
+                const uint32_t d = (c * NT + tid) * 8;
+                store8(o, d, D, y_of(d, sum8(d), true));
+            }
+        }
+    } else {
+        constexpr bool fp8 = OUT == OUT_FP8;
+        constexpr float most = fp8 ? 448.0f : 127.0f;
+        uint8_t* o = static_cast<uint8_t*>(a.out) + t * a.ldo;
+        auto biggest = [&](f32x8 y) {
+            float m = fabsf(y[0]);
+#pragma unroll
+            for (int e = 1; e < 8; ++e) m = top(m, fabsf(y[e]));
+            return m;
+        };
+        // the scale of a whole row: one pass over y first
+        float s = a.given;
+        if (a.group == 0 && !(a.given > 0.0f)) {
+            float m = 0.0f;
+            if constexpr (C > 0) {
+#pragma unroll
+                for (int c = 0; c < C; ++c) {
+                    const uint32_t d = (c * NT + tid) * 8;
+                    r[c] = y_of(d, r[c], true);
+                    m = top(m, biggest(r[c]));
+                }
+            } else {
+                for (uint32_t c = 0; c < chunks; ++c) {
+                    const uint32_t d = (c * NT + tid) * 8;
+                    m = top(m, biggest(y_of(d, sum8(d), false)));
+                }
+            }
+            s = row_top<WPR>(m, part) / most;
+            if (tid == 0) a.scales[t] = s;
+        }
+        auto emit = [&](uint32_t d, f32x8 y) {
+            float sc = s;
+            if (a.group) {
+                float m = biggest(y);
+                for (uint32_t k = 1; k < a.group / 8; k <<= 1) m = top(m, __shfl_xor(m, int(k)));
+                sc = m / most;
+                if (d < D && d % a.group == 0) a.scales[uint64_t(t) * a.groups + d / a.group] = sc;
+            }
+            store_codes(o, d, D, codes8(y, sc == 0.0f ? 0.0f : 1.0f / sc, fp8));
+        };
+        if constexpr (C > 0) {
+            const bool have = a.group == 0 && !(a.given > 0.0f);  // r holds y
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                const uint32_t d = (c * NT + tid) * 8;
+                emit(d, have ? r[c] : y_of(d, r[c], true));
+            }
+        } else {
+            for (uint32_t c = 0; c < chunks; ++c) {
+                const uint32_t d = (c * NT + tid) * 8;
+                emit(d, y_of(d, sum8(d), true));
+            }
+        }
+    }
+}
+
+// out = code scale, 8 values a thread
+template <int DT>
+__global__ __launch_bounds__(256) void rms_dequantize_kernel(const uint8_t* __restrict__ codes, const float* __restrict__ scales, uint64_t ldc,
+                                                             uint32_t T, uint32_t D, uint32_t group, uint32_t groups, float given, bool fp8,
+                                                             ElemT<DT>* __restrict__ out, uint64_t ldo) {
+    const uint32_t per = (D + 7) / 8;
+    const uint64_t i = uint64_t(blockIdx.x) * 256 + threadIdx.x;
+    if (i >= uint64_t(T) * per) return;
+    const uint32_t t = uint32_t(i / per), d = uint32_t(i % per) * 8;
+    const float s = given > 0.0f ? given : scales[uint64_t(t) * groups + (group ? d / group : 0)];
+    const uint8_t* c = codes + t * ldc + d;
+    uint32_t w[2] = {0, 0};
+    if (d + 8 <= D) {
+        __builtin_memcpy(w, c, 8);
+    } else {
+        for (int e = 0; e < 8; ++e)
+            if (d + e < D) w[e >> 2] |= uint32_t(c[e]) << (8 * (e & 3));
+    }
+    f32x8 v;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        if (fp8) {
+            v[4 * h] = __builtin_amdgcn_cvt_f32_fp8(int(w[h]), 0);
+            v[4 * h + 1] = __builtin_amdgcn_cvt_f32_fp8(int(w[h]), 1);
+            v[4 * h + 2] = __builtin_amdgcn_cvt_f32_fp8(int(w[h]), 2);
+            v[4 * h + 3] = __builtin_amdgcn_cvt_f32_fp8(int(w[h]), 3);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[4 * h + e] = float(int8_t(w[h] >> (8 * e)));
+        }
+    }
+    store8(out + t * ldo, d, D, v * s);
+}
+
+// ---- backward ------------------------------------------------------------------------------------
+struct RmsGradArgs {
+    const void* grad;
+    const void* r;  // the summed rows of the forward pass
+    const void* weight;
+    const void* grad_residual;  // or nullptr
+    const float* inverse;
+    void* out;    // dx, or nullptr
+    float* part;  // [workgroups][D] shares of dw, or nullptr
+    uint64_t ldg, ldr, ldgr, ldo;
+    uint32_t T, D;
+};
+
+// A wave (or workgroup) takes rows in turn; dw's shares stay in registers (C > 0).
+template <int DT, int WPR, int C>
+__global__ __launch_bounds__(256) void rms_grad_kernel(RmsGradArgs a) {
+    using T = ElemT<DT>;
+    constexpr int NT = 64 * WPR, CC = C ? C : 1;
+    constexpr int ROWS = 4 / WPR;
+    __shared__ float part[4];
+    __shared__ f32x8 join[WPR == 1 && C > 0 ? 256 : 1];
+    const uint32_t tid = WPR == 1 ? threadIdx.x & 63 : threadIdx.x;
+    const uint32_t D = a.D, chunks = C ? C : (D + 8 * NT - 1) / (8 * NT);
+    const T* w = static_cast<const T*>(a.weight);
+    f32x8 dw[CC], wv[CC];
+#pragma unroll
+    for (int c = 0; c < CC; ++c) {
+        dw[c] = f32x8(0.0f);
+        if constexpr (C > 0) wv[c] = load8(w, (c * NT + tid) * 8, D);
+    }
+    for (uint32_t t = blockIdx.x * ROWS + (WPR == 1 ? threadIdx.x >> 6 : 0); t < a.T; t += gridDim.x * ROWS) {
+        const T* g = static_cast<const T*>(a.grad) + t * a.ldg;
+        const T* r = static_cast<const T*>(a.r) + t * a.ldr;
+        const T* gr = a.grad_residual ? static_cast<const T*>(a.grad_residual) + t * a.ldgr : nullptr;
+        const float inv = a.inverse[t];
+        float along = 0.0f;
+        f32x8 gv[CC], nv[CC];
+        auto chunk = [&](uint32_t d, f32x8 wc, f32x8& gg, f32x8& nn) {
+            gg = load8(g, d, D);
+            nn = load8(r, d, D) * inv;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) along = fmaf(gg[e] * wc[e], nn[e], along);
+        };
+        if constexpr (C > 0) {
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                chunk((c * NT + tid) * 8, wv[c], gv[c], nv[c]);
+                dw[c] += gv[c] * nv[c];
+            }
+        } else {
+            for (uint32_t c = 0; c < chunks; ++c) {
+                const uint32_t d = (c * NT + tid) * 8;
+                f32x8 gg, nn;
+                chunk(d, load8(w, d, D), gg, nn);
+            }
+        }
+        along = row_sum<WPR>(along, part) / float(D);
+        if (!a.out) continue;
+        T* o = static_cast<T*>(a.out) + t * a.ldo;
+        auto finish = [&](uint32_t d, f32x8 wc, f32x8 gg, f32x8 nn) {
+            f32x8 v = (gg * wc - nn * along) * inv;
+            if (gr) v += load8(gr, d, D);
+            store8(o, d, D, v);
+        };
+        if constexpr (C > 0) {
+#pragma unroll
+            for (int c = 0; c < C; ++c) finish((c * NT + tid) * 8, wv[c], gv[c], nv[c]);
+        } else {
+            for (uint32_t c = 0; c < chunks; ++c) {
+                const uint32_t d = (c * NT + tid) * 8;
+                f32x8 gg = load8(g, d, D), nn = load8(r, d, D) * inv;
+                finish(d, load8(w, d, D), gg, nn);
+            }
+        }
+    }
+    if constexpr (C > 0) {
+        if (!a.part) return;
+        float* o = a.part + uint64_t(blockIdx.x) * D;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const uint32_t d = (c * NT + tid) * 8;
+            f32x8 v = dw[c];
+            if constexpr (WPR == 1) {
+                __syncthreads();
+                join[threadIdx.x] = v;
+                __syncthreads();
+                if (threadIdx.x >= 64) continue;
+                v = (join[tid] + join[tid + 64]) + (join[tid + 128] + join[tid + 192]);
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (d + e < D) o[d + e] = v[e];
+        }
+    }
+}
+
+// dw's shares of long rows: a workgroup takes 2048 columns of every gridDim.y-th row
+template <int DT>
+__global__ __launch_bounds__(256) void rms_weight_grad_kernel(RmsGradArgs a) {
+    using T = ElemT<DT>;
+    const uint32_t d = (blockIdx.x * 256 + threadIdx.x) * 8;
+    f32x8 dw(0.0f);
+    for (uint32_t t = blockIdx.y; t < a.T; t += gridDim.y)
+        dw += load8(static_cast<const T*>(a.grad) + t * a.ldg, d, a.D) * (load8(static_cast<const T*>(a.r) + t * a.ldr, d, a.D) * a.inverse[t]);
+    for (int e = 0; e < 8; ++e)
+        if (d + e < a.D) a.part[uint64_t(blockIdx.y) * a.D + d + e] = dw[e];
+}
+
+// out[d] = sum of the shares, in a fixed order: 64 columns a workgroup, 16 groups of shares
+template <int DT>
+__global__ __launch_bounds__(1024) void rms_weight_sum_kernel(const float* __restrict__ part, uint32_t shares, uint32_t D, ElemT<DT>* __restrict__ out) {
+    __shared__ float s[16][64];
+    const uint32_t c = threadIdx.x & 63, g = threadIdx.x >> 6, d = blockIdx.x * 64 + c;
+    float v = 0.0f;
+    if (d < D)
+#pragma unroll 8
+        for (uint32_t i = g; i < shares; i += 16) v += part[uint64_t(i) * D + d];
+    s[g][c] = v;
+    __syncthreads();
+    if (g || d >= D) return;
+    for (int i = 1; i < 16; ++i) v += s[i][c];
+    out[d] = ElemT<DT>(v);
+}
+
+// ---- host ------------------------------------------------------------------------------------------
+template <class F>
+va_status by_shape(uint32_t D, F&& f) {
+    using std::integral_constant;
+    const uint32_t c1 = ceil_div(D, 512), c4 = ceil_div(D, 2048);
+    if (c1 <= 1) return f(integral_constant<int, 1>(), integral_constant<int, 1>());
+    if (c1 == 2) return f(integral_constant<int, 1>(), integral_constant<int, 2>());
+    if (c1 == 3) return f(integral_constant<int, 1>(), integral_constant<int, 3>());
+    if (c1 == 4) return f(integral_constant<int, 1>(), integral_constant<int, 4>());
+    if (c4 == 2) return f(integral_constant<int, 4>(), integral_constant<int, 2>());
+    if (c4 <= 4) return f(integral_constant<int, 4>(), integral_constant<int, 4>());
+    return f(integral_constant<int, 4>(), integral_constant<int, 0>());
+}
+template <class F>
+va_status by_dtype(va_dtype t, F&& f) {
+    if (t == VA_DTYPE_F32) return f(std::integral_constant<int, VA_DTYPE_F32>());
+    if (t == VA_DTYPE_F16) return f(std::integral_constant<int, VA_DTYPE_F16>());
+    return f(std::integral_constant<int, VA_DTYPE_BF16>());
+}
+bool known(va_dtype t) { return t == VA_DTYPE_F32 || t == VA_DTYPE_F16 || t == VA_DTYPE_BF16; }
+bool aligned(const void* p, va_dtype t) { return reinterpret_cast<uintptr_t>(p) % (t == VA_DTYPE_F32 ? 4 : 2) == 0; }
+
+va_status check(va_context* ctx, const va_rms_desc* d, const char* who) {
+    VA_REQUIRE(ctx, d, "%s: NULL description", who);
+    VA_REQUIRE(ctx, d->x && d->weight, "%s: NULL pointer", who);
+    VA_REQUIRE(ctx, d->rows > 0 && d->dim > 0, "%s: empty input (%u rows, %u dimensions)", who, d->rows, d->dim);
+    VA_REQUIRE(ctx, known(d->dtype), "%s: unknown type %d", who, int(d->dtype));
+    VA_REQUIRE(ctx, d->x_stride >= d->dim && (!d->residual || d->residual_stride >= d->dim) && (!d->out_residual || d->out_residual_stride >= d->dim),
+               "%s: a row stride is below the dimension", who);
+    VA_REQUIRE(ctx, aligned(d->x, d->dtype) && aligned(d->residual, d->dtype) && aligned(d->weight, d->dtype) && aligned(d->out_residual, d->dtype),
+               "%s: an operand is not aligned to its type", who);
+    VA_REQUIRE(ctx, std::isfinite(d->epsilon) && d->epsilon >= 0.0f, "%s: epsilon must be finite and not negative", who);
+    VA_REQUIRE(ctx, d->dim <= 0x7FFFFFFFu - 16384u, "%s: %u dimensions", who, d->dim);
+    return VA_OK;
+}
+
+template <int OUT>
+va_status forward(va_context* ctx, const va_rms_desc* d, void* out, uint64_t ldo, uint32_t group, float given, float* scales) {
+    RmsArgs a{d->x, d->residual, d->weight, d->out_residual, d->out_inverse_rms, out, scales, d->x_stride, d->residual_stride,
+              d->out_residual_stride, ldo, d->rows, d->dim, group, group ? ceil_div(d->dim, group) : 1u, d->epsilon, given};
+    return by_dtype(d->dtype, [&](auto dt) {
+        return by_shape(d->dim, [&](auto wpr, auto c) {
+            const uint32_t grid = decltype(wpr)::value == 1 ? ceil_div(a.T, 4) : a.T;
+            rms_norm_kernel<decltype(dt)::value, OUT, decltype(wpr)::value, decltype(c)::value><<<dim3(grid), dim3(256), 0, ctx->stream>>>(a);
+            VA_CHECK_LAUNCH(ctx);
+            return VA_OK;
+        });
+    });
+}
+
+va_status check_codes(va_context* ctx, va_code code, uint32_t group, float given, const char* who) {
+    VA_REQUIRE(ctx, code == VA_CODE_INT8 || code == VA_CODE_FP8_E4M3, "%s: unknown code type %d", who, int(code));
+    VA_REQUIRE(ctx, group == 0 || (group >= 8 && group <= 512 && (group & (group - 1)) == 0),
+               "%s: groups of %u (0, or a power of two from 8 to 512)", who, group);
+    VA_REQUIRE(ctx, std::isfinite(given) && given >= 0.0f && (given == 0.0f || group == 0), "%s: a given scale is positive and for the whole tensor", who);
+    return VA_OK;
+}
+
+}  // namespace
+}  // namespace va
+
+using namespace va;
+
+extern "C" {
+
+va_status va_rms_norm(va_context* ctx, const va_rms_desc* d, void* out, uint64_t out_stride) {
+    if (!ctx) return VA_ERR_INVALID_ARG;
+    VA_CHECK_STATUS(check(ctx, d, "va_rms_norm"));
+    VA_REQUIRE(ctx, out && out_stride >= d->dim && aligned(out, d->dtype), "va_rms_norm: the output is NULL, misaligned or its stride below the dimension");
+    DeviceGuard guard(ctx->device);
+    return forward<OUT_SAME>(ctx, d, out, out_stride, 0, 0.0f, nullptr);
+}
+
+va_status va_rms_norm_quantized(va_context* ctx, const va_rms_desc* d, va_code code, uint32_t group, float given_scale, void* out_codes,
+                                uint64_t codes_stride, float* out_scales) {
+    if (!ctx) return VA_ERR_INVALID_ARG;
+    VA_CHECK_STATUS(check(ctx, d, "va_rms_norm_quantized"));
+    VA_CHECK_STATUS(check_codes(ctx, code, group, given_scale, "va_rms_norm_quantized"));
+    VA_REQUIRE(ctx, out_codes && codes_stride >= d->dim, "va_rms_norm_quantized: the codes are NULL or their stride below the dimension");
+    VA_REQUIRE(ctx, (given_scale > 0.0f) == (out_scales == nullptr), "va_rms_norm_quantized: scales are written unless one is given");
+    DeviceGuard guard(ctx->device);
+    return code == VA_CODE_INT8 ? forward<OUT_INT8>(ctx, d, out_codes, codes_stride, group, given_scale, out_scales)
+                                : forward<OUT_FP8>(ctx, d, out_codes, codes_stride, group, given_scale, out_scales);
+}
+
+va_status va_rms_dequantize(va_context* ctx, const void* codes, uint64_t codes_stride, va_code code, const float* scales, float given_scale,
+                            uint32_t rows, uint32_t dim, uint32_t group, va_dtype dtype, void* out, uint64_t out_stride) {
+    if (!ctx) return VA_ERR_INVALID_ARG;
+    VA_CHECK_STATUS(check_codes(ctx, code, group, given_scale, "va_rms_dequantize"));
+    VA_REQUIRE(ctx, codes && out && (given_scale > 0.0f) == (scales == nullptr), "va_rms_dequantize: NULL pointer, or scales beside a given scale");
+    VA_REQUIRE(ctx, rows > 0 && dim > 0, "va_rms_dequantize: empty input (%u rows, %u dimensions)", rows, dim);
+    VA_REQUIRE(ctx, known(dtype) && aligned(out, dtype), "va_rms_dequantize: unknown type or misaligned output");
+    VA_REQUIRE(ctx, codes_stride >= dim && out_stride >= dim, "va_rms_dequantize: a row stride is below the dimension");
+    const uint64_t blocks = (uint64_t(rows) * ((uint64_t(dim) + 7) / 8) + 255) / 256;
+    VA_REQUIRE(ctx, blocks <= 0x7FFFFFFFull, "va_rms_dequantize: too many values");
+    DeviceGuard guard(ctx->device);
+    return by_dtype(dtype, [&](auto dt) {
+        rms_dequantize_kernel<decltype(dt)::value><<<dim3(uint32_t(blocks)), dim3(256), 0, ctx->stream>>>(
+            static_cast<const uint8_t*>(codes), scales, codes_stride, rows, dim, group, group ? ceil_div(dim, group) : 1u, given_scale,
+            code == VA_CODE_FP8_E4M3, static_cast<ElemT<decltype(dt)::value>*>(out), out_stride);
+        VA_CHECK_LAUNCH(ctx);
+        return VA_OK;
+    });
+}
+
+va_status va_rms_norm_backward(va_context* ctx, const va_rms_desc* d, const void* grad, uint64_t grad_stride, const void* grad_residual,
+                               uint64_t grad_residual_stride, const float* inverse_rms, void* out_grad_x, uint64_t grad_x_stride,
+                               void* out_grad_weight) {
+    if (!ctx) return VA_ERR_INVALID_ARG;
+    VA_CHECK_STATUS(check(ctx, d, "va_rms_norm_backward"));
+    VA_REQUIRE(ctx, grad && inverse_rms && (out_grad_x || out_grad_weight), "va_rms_norm_backward: NULL pointer");
+    VA_REQUIRE(ctx, !d->residual && !d->out_residual && !d->out_inverse_rms, "va_rms_norm_backward: x is the summed row; the description has no residual and no output");
+    VA_REQUIRE(ctx, grad_stride >= d->dim && (!grad_residual || grad_residual_stride >= d->dim) && (!out_grad_x || grad_x_stride >= d->dim),
+               "va_rms_norm_backward: a row stride is below the dimension");
+    VA_REQUIRE(ctx, aligned(grad, d->dtype) && aligned(grad_residual, d->dtype) && aligned(out_grad_x, d->dtype) && aligned(out_grad_weight, d->dtype),
+               "va_rms_norm_backward: an operand is not aligned to its type");
+    DeviceGuard guard(ctx->device);
+    RmsGradArgs a{grad, d->x, d->weight, grad_residual, inverse_rms, out_grad_x, nullptr, grad_stride, d->x_stride, grad_residual_stride,
+                  grad_x_stride, d->rows, d->dim};
+    return by_dtype(d->dtype, [&](auto dt) {
+        constexpr int DT = decltype(dt)::value;
+        return by_shape(d->dim, [&](auto wpr, auto c) {
+            constexpr int WPR = decltype(wpr)::value, C = decltype(c)::value;
+            // two workgroups a CU; fewer where their shares of dw would be more than the rows
+            const uint32_t grid = std::min(ceil_div(a.T, 4 / WPR), 2u * uint32_t(ctx->num_cus));
+            const uint32_t shares = C ? grid : std::min(a.T, 256u);
+            Scratch sc(ctx);
+            if (out_grad_weight) {
+                VA_CHECK_STATUS(sc.reserve(Scratch::round(uint64_t(shares) * a.D * 4)));
+                a.part = sc.carve<float>(uint64_t(shares) * a.D);
+            }
+            if (C || a.out) {
+                rms_grad_kernel<DT, WPR, C><<<dim3(grid), dim3(256), 0, ctx->stream>>>(a);
+                VA_CHECK_LAUNCH(ctx);
+            }
+            if (out_grad_weight) {
+                if (!C) {
+                    rms_weight_grad_kernel<DT><<<dim3(ceil_div(a.D, 2048), shares), dim3(256), 0, ctx->stream>>>(a);
+                    VA_CHECK_LAUNCH(ctx);
+                }
+                rms_weight_sum_kernel<DT><<<dim3(ceil_div(a.D, 64)), dim3(1024), 0, ctx->stream>>>(a.part, shares, a.D, static_cast<ElemT<DT>*>(out_grad_weight));
+                VA_CHECK_LAUNCH(ctx);
+            }
+            return VA_OK;
+        });
+    });
+}
+
+}  // extern "C"

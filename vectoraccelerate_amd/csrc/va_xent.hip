@@ -1,0 +1,941 @@
+// va_xent.hip — softmax cross entropy of hidden rows over all items of a collection, and its
+// gradient, without the rows x items matrix.
+//
+//   l_tj = scale h_t . w_j + o_j          lse_t = log sum_j exp l_tj       loss_t = lse_t - l_{t, y_t}
+//   dl_tj = g_t (exp(l_tj - lse_t) - [j = y_t])     dh = scale dl w        dw = scale dl^T h
+//
+// Forward: one product (va_gemm16.hpp) whose epilogue keeps, per row, the running maximum m and
+// z = sum exp(l - m) of the items seen; the workgroups' (m, z) are joined by the finishing kernel.  Backward: the items are taken in
+// pieces; for each piece the logits are computed again, dl leaves the product's epilogue as 16-bit
+// values in a bounded workspace, in both orders, and two more products read it: dh accumulates over
+// the pieces in fp32, dw's rows of the piece are final.  So a training step is four products (one
+// of them the recomputation), and the memory is that of one piece.
+//
+// Precision: fp16 / bf16 operands enter the matrix cores as they are, sums are fp32.  dl is rounded
+// once to the operands' type for the second products (relative 2^-12 / 2^-9 a value, like the
+// rounding of the result), after a scale that takes the largest |g| to 2^14: fp16's range then holds
+// probabilities down to 2^-38 of it, and with one g for all rows the target's -g is exact.  fp32 operands, and dl with them, are two
+// fp16 planes (va_gemm16.hpp).
+//
+// Masks: an item whose offset is -inf has no probability whatever its vector holds (NaN and inf
+// included) and gets a zero gradient; a row without a target has loss 0 and a zero gradient whatever
+// it holds.  When every item is masked, lse = -inf, the losses are 0 and so are the gradients.
+#include <algorithm>
+#include <cfloat>
+#include <cmath>
+
+#include "va_gemm16.hpp"
+
+namespace va {
+namespace {
+
+using g16::f32x16;
+using g16::f32x4;
+using g16::u32x4;
+
+constexpr float kLog2e = 1.44269504088896340736f;
+
+// ---- element types -----------------------------------------------------------------------------
+template <int DT>
+struct Elem;
+template <>
+struct Elem<VA_DTYPE_F32> {
+    using T = float;
+    static __device__ float to_f(T v) { return v; }
+    static __device__ T from_f(float v) { return v; }
+};
+template <>
+struct Elem<VA_DTYPE_F16> {
+    using T = _Float16;
+    static __device__ float to_f(T v) { return float(v); }
+    static __device__ T from_f(float v) { return T(v); }
+};
+template <>
+struct Elem<VA_DTYPE_BF16> {
+    using T = __bf16;
+    static __device__ float to_f(T v) { return float(v); }
+    static __device__ T from_f(float v) { return T(v); }
+};
+template <int DT>
+using ElemT = typename Elem<DT>::T;
+template <bool BF16>
+__device__ __forceinline__ uint16_t bits16(float v) {
+    if constexpr (BF16) return __builtin_bit_cast(uint16_t, __bf16(v));
+    else return __builtin_bit_cast(uint16_t, _Float16(v));
+}
+// v = hi + lo in fp16
+__device__ __forceinline__ void split16(float v, uint16_t& hi, uint16_t& lo) {
+    const _Float16 h = _Float16(v);
+    hi = __builtin_bit_cast(uint16_t, h);
+    lo = __builtin_bit_cast(uint16_t, _Float16(v - float(h)));
+}
+// the power of two that puts |v| in [2^13, 2^14) (1 for 0, inf and NaN)
+__device__ __forceinline__ float scale_to_2p14(float v) {
+    v = fabsf(v);
+    if (!(v > 0.0f) || !(v < INFINITY)) return 1.0f;
+    int e;
+    (void)frexpf(v, &e);  // v = f 2^e, f in [0.5, 1)
+    return ldexpf(1.0f, min(14 - e, 126));
+}
+
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+    for (int d = 32; d; d >>= 1) v = fmaxf(v, __shfl_xor(v, d));
+    return v;
+}
+
+// (m, z) of two disjoint sets of items, joined
+__device__ __forceinline__ void join(float& m, float& z, float m2, float z2) {
+    const float mm = fmaxf(m, m2);
+    const float ref = mm == -INFINITY ? 0.0f : mm;
+    z = z * exp2f((m - ref) * kLog2e) + z2 * exp2f((m2 - ref) * kLog2e);
+    m = mm;
+}
+
+// ---- packing: operands whose rows are not whole 64-value stages, or not 16-bit ---------------------
+// dst[r][k] = src[r][k], zeros for k in [D, Kp)
+__global__ __launch_bounds__(256) void pack16_kernel(const uint16_t* __restrict__ src, uint64_t ld, uint32_t D, uint32_t Kp,
+                                                     uint16_t* __restrict__ dst, uint64_t n8) {
+    for (uint64_t i = uint64_t(blockIdx.x) * 256 + threadIdx.x; i < n8; i += uint64_t(gridDim.x) * 256) {
+        const uint32_t per = Kp / 8;
+        const uint64_t r = i / per;
+        const uint32_t k = uint32_t(i - r * per) * 8;
+        uint16_t v[8];
+        const uint16_t* s = src + r * ld + k;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = k + e < D ? s[e] : uint16_t(0);
+        u32x4 o;
+        __builtin_memcpy(&o, v, 16);
+        *reinterpret_cast<u32x4*>(dst + r * Kp + k) = o;
+    }
+}
+
+// One wave per fp32 row: its planes dst[r] = {hi, lo} (Kp values each, zeros past D), scaled by the
+// power of two that puts its largest entry near 2^14; inv[r] = the inverse.
+__global__ __launch_bounds__(256) void pack32_kernel(const float* __restrict__ src, uint64_t ld, uint32_t R, uint32_t D,
+                                                     uint32_t Kp, uint16_t* __restrict__ dst, float* __restrict__ inv) {
+    const int lane = threadIdx.x & 63;
+    const uint32_t r = blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (r >= R) return;
+    const float* s = src + r * ld;
+    float m = 0.0f;
+    for (uint32_t k = lane; k < D; k += 64) m = fmaxf(m, fabsf(s[k]));
+    const float sc = scale_to_2p14(wave_max(m));
+    if (lane == 0) inv[r] = 1.0f / sc;
+    uint16_t* o = dst + uint64_t(r) * 2 * Kp;
+    for (uint32_t k = 2 * lane; k < Kp; k += 128) {
+        uint16_t h0, l0, h1, l1;
+        split16(k < D ? s[k] * sc : 0.0f, h0, l0);
+        split16(k + 1 < D ? s[k + 1] * sc : 0.0f, h1, l1);
+        *reinterpret_cast<uint32_t*>(o + k) = h0 | uint32_t(h1) << 16;
+        *reinterpret_cast<uint32_t*>(o + Kp + k) = l0 | uint32_t(l1) << 16;
+    }
+}
+
+// out = the bits of the largest |src| (0 before the launch); rows whose drop value says so are left out
+__global__ __launch_bounds__(256) void absmax_kernel(const float* __restrict__ src, uint64_t ld, uint32_t R, uint32_t D,
+                                                     const float* __restrict__ drop, float drop_if, uint32_t* out) {
+    __shared__ float part[4];
+    float m = 0.0f;
+    const int lane = threadIdx.x & 63;
+    for (uint32_t r = blockIdx.x * 4 + (threadIdx.x >> 6); r < R; r += gridDim.x * 4) {
+        if (drop && drop[r] == drop_if) continue;
+        const float* s = src + r * ld;
+        for (uint32_t k = lane; k < D; k += 64) m = fmaxf(m, fabsf(s[k]));
+    }
+    m = wave_max(m);
+    if (lane == 0) part[threadIdx.x >> 6] = m;
+    __syncthreads();
+    if (threadIdx.x == 0)
+        atomicMax(out, __builtin_bit_cast(uint32_t, fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]))));
+}
+
+// dst[d][r] = src[r][d] for r < R, zeros for r in [R, Rp); rows whose drop value says so are zeros.
+// fp32: two planes (lo behind hi's Rp values), scaled by the tensor's power of two (absmax).
+// 64 x 64 tiles through LDS.
+template <int DT>
+__global__ __launch_bounds__(256) void transpose_kernel(const ElemT<DT>* __restrict__ src, uint64_t ld, uint32_t R, uint32_t D,
+                                                        uint32_t Rp, const float* __restrict__ drop, float drop_if,
+                                                        const uint32_t* __restrict__ absmax, uint16_t* __restrict__ dst) {
+    constexpr bool kF32 = DT == VA_DTYPE_F32;
+    __shared__ ElemT<DT> tile[64][64 + (kF32 ? 1 : 2)];
+    const uint32_t r0 = blockIdx.x * 64, d0 = blockIdx.y * 64;
+    const uint32_t c = threadIdx.x & 63, w = threadIdx.x >> 6;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const uint32_t r = r0 + w + 4 * i, d = d0 + c;
+        const bool in = r < R && d < D && !(drop && drop[r] == drop_if);
+        tile[w + 4 * i][c] = in ? src[uint64_t(r) * ld + d] : ElemT<DT>(0.0f);
+    }
+    __syncthreads();
+    const float sc = kF32 ? scale_to_2p14(__builtin_bit_cast(float, *absmax)) : 1.0f;
+    const uint64_t pitch = uint64_t(Rp) * (kF32 ? 2 : 1);
+    const uint32_t rr = (threadIdx.x & 31) * 2;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const uint32_t dl = (threadIdx.x >> 5) + 8 * i, d = d0 + dl;
+        if (d >= D || r0 + rr >= Rp) continue;
+        uint16_t* o = dst + d * pitch + r0 + rr;
+        if constexpr (kF32) {
+            uint16_t h0, l0, h1, l1;
+            split16(tile[rr][dl] * sc, h0, l0);
+            split16(tile[rr + 1][dl] * sc, h1, l1);
+            *reinterpret_cast<uint32_t*>(o) = h0 | uint32_t(h1) << 16;
+            *reinterpret_cast<uint32_t*>(o + Rp) = l0 | uint32_t(l1) << 16;
+        } else {
+            const uint16_t a = __builtin_bit_cast(uint16_t, tile[rr][dl]), b = __builtin_bit_cast(uint16_t, tile[rr + 1][dl]);
+            *reinterpret_cast<uint32_t*>(o) = a | uint32_t(b) << 16;
+        }
+    }
+}
+
+// ---- the logits' epilogues -------------------------------------------------------------------------
+struct LogitArgs {
+    const float* offsets;  // of the launch's first item (nullptr: zeros)
+    const float* qinv;     // fp32 operands: the rows' and the items' inverse scales
+    const float* xinv;
+    float scale;
+    uint32_t rows, items;  // hidden rows; items of this launch
+};
+
+// What the epilogue needs of a tile's items, and the logit of one accumulator.  OFF: there are
+// offsets, or the last tile is not whole (its missing items get offset -inf).
+template <bool OFF, bool PLANES>
+struct LogitShared {
+    float off[OFF ? g16::TR : 1];
+    float inv[PLANES ? g16::TR : 1];
+};
+template <bool OFF, bool PLANES>
+__device__ __forceinline__ f32x4 logits4(const LogitShared<OFF, PLANES>& sm, const f32x16& acc, int j, int r, float c) {
+    f32x4 v;
+    f32x4 o{}, x{};
+    asm volatile("" ::: "memory");  // these reads stay here: hoisted, a tile's would fill the registers
+    if constexpr (OFF) o = *reinterpret_cast<const f32x4*>(sm.off + r);
+    if constexpr (PLANES) x = *reinterpret_cast<const f32x4*>(sm.inv + r);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        float a = acc[4 * j + e];
+        if constexpr (PLANES) a *= x[e];
+        if constexpr (OFF) v[e] = o[e] == -INFINITY ? -INFINITY : fmaf(a, c, o[e]);
+        else v[e] = a * c;
+    }
+    return v;
+}
+
+// exp(v - ref).  The difference is taken first: where v is near ref (the items that matter) it is exact,
+// and it stays in range for offsets as low as the type's lowest value.
+__device__ __forceinline__ float exp_diff(float v, float ref) { return __builtin_amdgcn_exp2f((v - ref) * kLog2e); }
+
+// Forward: the running (m, z) of a lane's items per query; joined over the workgroup at the end of
+// the item and written to part[row * slots + slot].  The target's logit is picked out on the way: with
+// the loss a difference of two logits, both from the same sums, their errors cancel for a row whose
+// target is far ahead of the other items.
+template <bool OFF, bool PLANES>
+struct LseEpi {
+    static constexpr bool kWalk = true;
+    LogitArgs a;
+    const int64_t* targets;
+    uint32_t item0;  // of the launch
+    float* picked;   // [rows] the target's logit
+    float2* part;
+    uint32_t slots, slot0;
+    struct Shared : LogitShared<OFF, PLANES> {
+        float2 red[4][g16::TQ];
+        uint32_t target[g16::TQ];  // within the launch's items (any larger value: elsewhere)
+        float qinv[PLANES ? g16::TQ : 1];
+    };
+    struct State {
+        float m[2], z[2];
+        float off, inv;
+    };
+    template <class Tile>
+    __device__ void begin(State& s, Shared& sm, const Tile& t) {
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            s.m[n] = -INFINITY;
+            s.z[n] = 0.0f;
+        }
+        const uint32_t i = threadIdx.x, q = t.qb * g16::TQ + i;
+        if (i >= uint32_t(g16::TQ)) return;
+        const int64_t y = q < a.rows ? targets[q] - int64_t(item0) : -1;
+        sm.target[i] = y >= 0 && y < int64_t(a.items) ? uint32_t(y) : 0xFFFFFFFFu;
+        if constexpr (PLANES) sm.qinv[i] = q < a.rows ? a.qinv[q] : 0.0f;
+    }
+    template <class Tile>
+    __device__ void load(State& s, const Tile& t, int tid) {
+        const uint32_t r = t.rb * g16::TR + uint32_t(tid);
+        const bool in = tid < g16::TR && r < a.items;
+        if constexpr (OFF) s.off = !in ? -INFINITY : a.offsets ? a.offsets[r] : 0.0f;
+        if constexpr (PLANES) s.inv = in ? a.xinv[r] : 0.0f;
+    }
+    __device__ void publish(State& s, Shared& sm, int tid) {
+        if constexpr (OFF)
+            if (tid < g16::TR) sm.off[tid] = s.off;
+        if constexpr (PLANES)
+            if (tid < g16::TR) sm.inv[tid] = s.inv;
+    }
+    template <class Tile>
+    __device__ void tile(State& s, Shared& sm, const g16::Lane& ln, f32x16 (&acc)[2][2], const Tile& t) {
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            const float c = PLANES ? a.scale * sm.qinv[ln.q(n)] : a.scale;
+            float top = -INFINITY;
+#pragma unroll
+            for (int m = 0; m < 2; ++m)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    f32x4 v = logits4<OFF, PLANES>(sm, acc[m][n], j, ln.r(m, j), c);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        top = fmaxf(top, v[e]);
+                        acc[m][n][4 * j + e] = v[e];
+                    }
+                }
+            const float mm = fmaxf(s.m[n], top);
+            const float ref = mm == -INFINITY ? 0.0f : mm;
+            const float z = s.z[n] * exp_diff(s.m[n], ref);
+            // (a tile holds the target of few rows, most tiles of none of a wave's)
+            const uint32_t y = sm.target[ln.q(n)] - t.rb * g16::TR - uint32_t(ln.wr * 64);
+            if (__any(y < 64u)) {
+                const uint32_t i = y - 4u * uint32_t(ln.hh);  // 32 m + 8 j + e of the lane's values
+                float v = 0.0f;
+#pragma unroll
+                for (int m = 0; m < 2; ++m)
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) v = i == uint32_t(32 * m + 8 * (k >> 2) + (k & 3)) ? acc[m][n][k] : v;
+                if (y < 64u && (i & 4u) == 0u) picked[t.qb * g16::TQ + ln.q(n)] = v;
+            }
+            float zz[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int m = 0; m < 2; ++m)
+#pragma unroll
+                for (int v = 0; v < 16; ++v) zz[v & 3] += exp_diff(acc[m][n][v], ref);
+            s.m[n] = mm;
+            s.z[n] = z + ((zz[0] + zz[1]) + (zz[2] + zz[3]));
+        }
+    }
+    template <class Tile>
+    __device__ void end(State& s, Shared& sm, const g16::Lane& ln, const Tile& t) {
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            join(s.m[n], s.z[n], __shfl_xor(s.m[n], 32), __shfl_xor(s.z[n], 32));
+            if (ln.hh == 0) sm.red[ln.wr][ln.q(n)] = make_float2(s.m[n], s.z[n]);
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        const uint32_t q = threadIdx.x;
+        if (q < uint32_t(g16::TQ) && t.qb * g16::TQ + q < a.rows) {
+            float2 v = sm.red[0][q];
+#pragma unroll
+            for (int w = 1; w < 4; ++w) join(v.x, v.y, sm.red[w][q].x, sm.red[w][q].y);
+            part[uint64_t(t.qb * g16::TQ + q) * slots + slot0 + t.part] = v;
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    }
+};
+
+// Backward: dl of the piece's items, in both orders (either may be absent):
+//   p[t][j]  rows of Vp values a plane (zeros past the last item), the query operand of dh
+//   pt[j][t] rows of Tp values a plane (zeros past the last row), the query operand of dw; whole
+//            tiles of 256 items
+template <bool BF16, bool OFF, bool PLANES>
+struct GradEpi {
+    static constexpr bool kWalk = false;
+    LogitArgs a;
+    const float* gk;   // g_t times dl's factor (0: the row has no gradient)
+    const float* lse;
+    const int64_t* targets;
+    uint32_t item0;    // the piece's first item
+    uint16_t* p;
+    uint16_t* pt;
+    uint32_t Vp, Tp;
+    struct Shared : LogitShared<OFF, PLANES> {
+        float gk[g16::TQ], lse[g16::TQ];
+        uint32_t target[g16::TQ];  // within the piece (any larger value: elsewhere)
+        float inv_q[PLANES ? g16::TQ : 1];
+    };
+    struct State {
+        float off, inv, gk, lse, qinv;
+        uint32_t target;
+    };
+    template <class Tile>
+    __device__ void begin(State&, Shared&, const Tile&) {}
+    template <class Tile>
+    __device__ void load(State& s, const Tile& t, int tid) {
+        const uint32_t r = t.rb * g16::TR + uint32_t(tid), q = t.qb * g16::TQ + uint32_t(tid);
+        const bool in = tid < g16::TR && r < a.items, qin = tid < g16::TQ && q < a.rows;
+        if constexpr (OFF) s.off = !in ? -INFINITY : a.offsets ? a.offsets[r] : 0.0f;
+        if constexpr (PLANES) {
+            s.inv = in ? a.xinv[r] : 0.0f;
+            s.qinv = qin ? a.qinv[q] : 0.0f;
+        }
+        s.gk = qin ? gk[q] : 0.0f;
+        s.lse = qin ? lse[q] : 0.0f;
+        const int64_t y = qin ? targets[q] - int64_t(item0) : -1;
+        s.target = y >= 0 && y < int64_t(a.items) ? uint32_t(y) : 0xFFFFFFFFu;
+    }
+    __device__ void publish(State& s, Shared& sm, int tid) {
+        if (tid >= g16::TQ) return;
+        if constexpr (OFF) sm.off[tid] = s.off;
+        if constexpr (PLANES) {
+            sm.inv[tid] = s.inv;
+            sm.inv_q[tid] = s.qinv;
+        }
+        sm.gk[tid] = s.gk;
+        sm.lse[tid] = s.lse;
+        sm.target[tid] = s.target;
+    }
+    template <class Tile>
+    __device__ void tile(State&, Shared& sm, const g16::Lane& ln, f32x16 (&acc)[2][2], const Tile& t) {
+        const uint32_t r0 = t.rb * g16::TR;
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            const uint32_t q = t.qb * g16::TQ + uint32_t(ln.q(n));
+            const float g = sm.gk[ln.q(n)], ref = sm.lse[ln.q(n)];
+            const float c = PLANES ? a.scale * sm.inv_q[ln.q(n)] : a.scale;
+            const uint32_t y = sm.target[ln.q(n)] - r0;
+            const bool none = g == 0.0f || ref == -INFINITY;
+#pragma unroll
+            for (int m = 0; m < 2; ++m)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t r = uint32_t(ln.r(m, j));
+                    const f32x4 v = logits4<OFF, PLANES>(sm, acc[m][n], j, int(r), c);
+                    uint16_t hi[4], lo[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        float d = exp_diff(v[e], ref);
+                        if (y == r + e && v[e] != -INFINITY) d -= 1.0f;
+                        d = none ? 0.0f : d * g;
+                        if constexpr (PLANES) split16(d, hi[e], lo[e]);
+                        else hi[e] = bits16<BF16>(d);
+                    }
+                    // (a piece's rows are padded to whole 64-item stages: a group of 4 is inside or outside)
+                    if (p && q < a.rows && r0 + r < Vp) {
+                        uint16_t* o = p + uint64_t(q) * Vp * (PLANES ? 2 : 1) + r0 + r;
+                        *reinterpret_cast<uint2*>(o) = make_uint2(hi[0] | uint32_t(hi[1]) << 16, hi[2] | uint32_t(hi[3]) << 16);
+                        if constexpr (PLANES)
+                            *reinterpret_cast<uint2*>(o + Vp) =
+                                make_uint2(lo[0] | uint32_t(lo[1]) << 16, lo[2] | uint32_t(lo[3]) << 16);
+                    }
+                    if (pt && q < Tp) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            uint16_t* o = pt + uint64_t(r0 + r + e) * Tp * (PLANES ? 2 : 1) + q;
+                            o[0] = hi[e];
+                            if constexpr (PLANES) o[Tp] = lo[e];
+                        }
+                    }
+                }
+        }
+    }
+    template <class Tile>
+    __device__ void end(State&, Shared&, const g16::Lane&, const Tile&) {}
+};
+
+// dh: fp32 shares [part][t][Dp], added to over the pieces (first: written)
+struct ShareEpi {
+    static constexpr bool kWalk = false;
+    float* out;
+    uint32_t rows, D, Dp;
+    bool first;
+    struct Shared {};
+    struct State {};
+    template <class Tile>
+    __device__ void begin(State&, Shared&, const Tile&) {}
+    template <class Tile>
+    __device__ void load(State&, const Tile&, int) {}
+    __device__ void publish(State&, Shared&, int) {}
+    template <class Tile>
+    __device__ void tile(State&, Shared&, const g16::Lane& ln, f32x16 (&acc)[2][2], const Tile& t) {
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            const uint32_t q = t.qb * g16::TQ + uint32_t(ln.q(n));
+            if (q >= rows) continue;
+            float* o = out + (uint64_t(t.part) * rows + q) * Dp;
+#pragma unroll
+            for (int m = 0; m < 2; ++m)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t d = t.rb * g16::TR + uint32_t(ln.r(m, j));
+                    if (d >= D) continue;  // (rows hold Dp = whole groups of 4)
+                    f32x4 v;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[e] = acc[m][n][4 * j + e];
+                    if (!first) v += *reinterpret_cast<const f32x4*>(o + d);
+                    *reinterpret_cast<f32x4*>(o + d) = v;
+                }
+        }
+    }
+    template <class Tile>
+    __device__ void end(State&, Shared&, const g16::Lane&, const Tile&) {}
+};
+
+// dw: the piece's rows, final
+template <int DT>
+struct ItemGradEpi {
+    static constexpr bool kWalk = false;
+    ElemT<DT>* out;
+    uint64_t ld;
+    uint32_t rows, D;
+    const float* mul;        // scale over dl's factor
+    const uint32_t* absmax;  // fp32: of the hidden rows (their planes' scale)
+    bool vec;                // rows of four values are aligned
+    struct Shared {
+        float mul;
+    };
+    struct State {};
+    template <class Tile>
+    __device__ void begin(State&, Shared&, const Tile&) {}
+    template <class Tile>
+    __device__ void load(State&, const Tile&, int) {}
+    __device__ void publish(State&, Shared& sm, int tid) {
+        if (tid == 0) sm.mul = *mul / (DT == VA_DTYPE_F32 ? scale_to_2p14(__builtin_bit_cast(float, *absmax)) : 1.0f);
+    }
+    template <class Tile>
+    __device__ void tile(State&, Shared& sm, const g16::Lane& ln, f32x16 (&acc)[2][2], const Tile& t) {
+        const float s = sm.mul;
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            const uint32_t q = t.qb * g16::TQ + uint32_t(ln.q(n));
+            if (q >= rows) continue;
+            ElemT<DT>* o = out + q * ld;
+#pragma unroll
+            for (int m = 0; m < 2; ++m)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t d = t.rb * g16::TR + uint32_t(ln.r(m, j));
+                    if (d >= D) continue;
+                    struct alignas(4 * sizeof(ElemT<DT>)) V4 {
+                        ElemT<DT> v[4];
+                    } v;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v.v[e] = Elem<DT>::from_f(acc[m][n][4 * j + e] * s);
+                    if (vec && d + 4 <= D) *reinterpret_cast<V4*>(o + d) = v;
+                    else
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (d + e < D) o[d + e] = v.v[e];
+                }
+        }
+    }
+    template <class Tile>
+    __device__ void end(State&, Shared&, const g16::Lane&, const Tile&) {}
+};
+
+// ---- finishing kernels ---------------------------------------------------------------------------
+// One wave per row: the shares joined into lse, and the loss.
+__global__ __launch_bounds__(256) void xent_finish_kernel(const int64_t* __restrict__ targets, uint32_t T, uint32_t V, int64_t ignore,
+                                                          const float2* __restrict__ part, const float* __restrict__ picked,
+                                                          uint32_t slots, float* __restrict__ loss, float* __restrict__ lse) {
+    const int lane = threadIdx.x & 63;
+    const uint32_t t = blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (t >= T) return;
+    float m = -INFINITY, z = 0.0f;
+    for (uint32_t i = lane; i < slots; i += 64) {
+        const float2 p = part[uint64_t(t) * slots + i];
+        join(m, z, p.x, p.y);
+    }
+#pragma unroll
+    for (int d = 32; d; d >>= 1) join(m, z, __shfl_xor(m, d), __shfl_xor(z, d));
+    if (lane) return;
+    const float l = m == -INFINITY && z == 0.0f ? -INFINITY : m + logf(z);
+    const int64_t y = targets[t];
+    float out = 0.0f;
+    if (y != ignore) {
+        out = NAN;  // a target outside the collection
+        if (y >= 0 && y < int64_t(V)) {
+            const float v = picked[t];
+            // log z + (m - v): the two large terms cancel before the small one is added
+            out = l == -INFINITY ? 0.0f : v == -INFINITY ? INFINITY : logf(z) + (m - v);
+        }
+    }
+    lse[t] = l;
+    loss[t] = out;
+}
+
+// The sum or mean of the losses over the rows with a target.  One workgroup.
+__global__ __launch_bounds__(1024) void xent_reduce_kernel(const float* __restrict__ loss, const int64_t* __restrict__ targets,
+                                                           uint32_t T, int64_t ignore, bool mean, float* out) {
+    __shared__ double sum[16];
+    __shared__ uint32_t cnt[16];
+    double s = 0.0;
+    uint32_t c = 0;
+    for (uint32_t t = threadIdx.x; t < T; t += 1024)
+        if (targets[t] != ignore) {
+            s += double(loss[t]);
+            ++c;
+        }
+    for (int d = 32; d; d >>= 1) {
+        s += __shfl_xor(s, d);
+        c += __shfl_xor(c, d);
+    }
+    if ((threadIdx.x & 63) == 0) {
+        sum[threadIdx.x >> 6] = s;
+        cnt[threadIdx.x >> 6] = c;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int i = 1; i < 16; ++i) {
+            s += sum[i];
+            c += cnt[i];
+        }
+        *out = float(mean ? (c ? s / double(c) : 0.0) : s);
+    }
+}
+
+// gk[t] = g_t c, *mul = scale / c: g_t is the gradient that reaches the row's loss, 0 for a row
+// without a target, c takes the largest |g_t| to 2^14.  Clears absmax[0..2).  One workgroup.
+__global__ __launch_bounds__(1024) void xent_gradient_kernel(const float* __restrict__ grad, const int64_t* __restrict__ targets,
+                                                             uint32_t T, uint32_t V, int64_t ignore, int reduction, float scale,
+                                                             float* __restrict__ gk, float* __restrict__ mul, uint32_t* absmax) {
+    __shared__ float top[16];
+    __shared__ uint32_t cnt[16];
+    if (threadIdx.x < 2) absmax[threadIdx.x] = 0;
+    float m = 0.0f;
+    uint32_t c = 0;
+    for (uint32_t t = threadIdx.x; t < T; t += 1024) {
+        const int64_t y = targets[t];
+        if (y == ignore) continue;
+        ++c;
+        if (reduction == VA_REDUCE_NONE && y >= 0 && y < int64_t(V)) m = fmaxf(m, fabsf(grad[t]));
+    }
+    for (int d = 32; d; d >>= 1) {
+        m = fmaxf(m, __shfl_xor(m, d));
+        c += __shfl_xor(c, d);
+    }
+    if ((threadIdx.x & 63) == 0) {
+        top[threadIdx.x >> 6] = m;
+        cnt[threadIdx.x >> 6] = c;
+    }
+    __syncthreads();
+    m = top[0];
+    c = cnt[0];
+    for (int i = 1; i < 16; ++i) {
+        m = fmaxf(m, top[i]);
+        c += cnt[i];
+    }
+    float g = 1.0f;
+    if (reduction != VA_REDUCE_NONE) {
+        if (grad) g = *grad;
+        if (reduction == VA_REDUCE_MEAN) g /= float(max(c, 1u));
+        m = fabsf(g);
+    }
+    const bool plain = !(m > 0.0f) || !(m < INFINITY);
+    if (plain) m = 16384.0f;
+    for (uint32_t t = threadIdx.x; t < T; t += 1024) {
+        const int64_t y = targets[t];
+        const bool in = y != ignore && y >= 0 && y < int64_t(V);
+        gk[t] = in ? (reduction == VA_REDUCE_NONE ? grad[t] : g) / m * 16384.0f : 0.0f;
+    }
+    if (threadIdx.x == 0) *mul = scale * (m / 16384.0f);
+}
+
+// dh[t][d] = mul sum over the shares (zero for a row without a gradient)
+template <int DT>
+__global__ __launch_bounds__(256) void share_sum_kernel(const float* __restrict__ share, uint32_t parts, uint32_t T, uint32_t D,
+                                                        uint32_t Dp, const float* __restrict__ gk, const float* __restrict__ mul,
+                                                        const uint32_t* __restrict__ absmax, ElemT<DT>* __restrict__ out, uint64_t ld) {
+    const uint32_t per = Dp / 4;
+    const uint64_t i = uint64_t(blockIdx.x) * 256 + threadIdx.x;
+    if (i >= uint64_t(T) * per) return;
+    const uint32_t t = uint32_t(i / per), d = uint32_t(i % per) * 4;
+    f32x4 v{0.0f, 0.0f, 0.0f, 0.0f};
+    for (uint32_t s = 0; s < parts; ++s) v += *reinterpret_cast<const f32x4*>(share + (uint64_t(s) * T + t) * Dp + d);
+    const float m = *mul / (DT == VA_DTYPE_F32 ? scale_to_2p14(__builtin_bit_cast(float, *absmax)) : 1.0f);
+    const bool none = gk[t] == 0.0f;
+    for (int e = 0; e < 4 && d + e < D; ++e) out[t * ld + d + e] = Elem<DT>::from_f(none ? 0.0f : v[e] * m);
+}
+
+// ---- host ------------------------------------------------------------------------------------------
+size_t elem_size(va_dtype t) { return t == VA_DTYPE_F32 ? 4 : 2; }
+
+// Rows that the product can read where they are: 16-bit, whole stages, aligned.
+bool direct(va_dtype dt, const void* p, uint64_t ld, uint32_t D) {
+    return dt != VA_DTYPE_F32 && D % g16::KC == 0 && ld % 8 == 0 && reinterpret_cast<uintptr_t>(p) % 16 == 0;
+}
+size_t packed_bytes(va_dtype dt, uint64_t rows, uint32_t Kp) { return rows * Kp * (dt == VA_DTYPE_F32 ? 4 : 2); }
+
+va_status pack(va_context* ctx, va_dtype dt, const void* src, uint64_t ld, uint32_t R, uint32_t D, uint32_t Kp, void* dst, float* inv) {
+    if (dt == VA_DTYPE_F32) {
+        pack32_kernel<<<dim3(ceil_div(R, 4)), dim3(256), 0, ctx->stream>>>(static_cast<const float*>(src), ld, R, D, Kp,
+                                                                           static_cast<uint16_t*>(dst), inv);
+    } else {
+        const uint64_t n8 = uint64_t(R) * (Kp / 8);
+        pack16_kernel<<<dim3(uint32_t(std::min<uint64_t>((n8 + 255) / 256, 16384))), dim3(256), 0, ctx->stream>>>(
+            static_cast<const uint16_t*>(src), ld, D, Kp, static_cast<uint16_t*>(dst), n8);
+    }
+    VA_CHECK_LAUNCH(ctx);
+    return VA_OK;
+}
+
+va_status transpose(va_context* ctx, va_dtype dt, const void* src, uint64_t ld, uint32_t R, uint32_t D, uint32_t Rp, const float* drop,
+                    float drop_if, const uint32_t* absmax, uint16_t* dst) {
+    const dim3 grid(Rp / 64, ceil_div(D, 64));
+    if (dt == VA_DTYPE_F32)
+        transpose_kernel<VA_DTYPE_F32><<<grid, dim3(256), 0, ctx->stream>>>(static_cast<const float*>(src), ld, R, D, Rp, drop, drop_if, absmax, dst);
+    else if (dt == VA_DTYPE_F16)
+        transpose_kernel<VA_DTYPE_F16><<<grid, dim3(256), 0, ctx->stream>>>(static_cast<const _Float16*>(src), ld, R, D, Rp, drop, drop_if, absmax, dst);
+    else
+        transpose_kernel<VA_DTYPE_BF16><<<grid, dim3(256), 0, ctx->stream>>>(static_cast<const __bf16*>(src), ld, R, D, Rp, drop, drop_if, absmax, dst);
+    VA_CHECK_LAUNCH(ctx);
+    return VA_OK;
+}
+
+const char* at(const void* p, uint64_t ld, uint64_t row, va_dtype dt) { return static_cast<const char*>(p) + row * ld * elem_size(dt); }
+
+template <class F>
+va_status by_type(va_dtype dt, bool off, F&& f) {
+    if (dt == VA_DTYPE_F32) return off ? f(std::false_type(), std::true_type(), std::true_type()) : f(std::false_type(), std::false_type(), std::true_type());
+    if (dt == VA_DTYPE_F16) return off ? f(std::false_type(), std::true_type(), std::false_type()) : f(std::false_type(), std::false_type(), std::false_type());
+    return off ? f(std::true_type(), std::true_type(), std::false_type()) : f(std::true_type(), std::false_type(), std::false_type());
+}
+
+va_status check_desc(va_context* ctx, const va_xent_desc* d, const char* who) {
+    VA_REQUIRE(ctx, d != nullptr, "%s: NULL description", who);
+    VA_REQUIRE(ctx, d->hidden && d->items && d->targets, "%s: NULL pointer", who);
+    VA_REQUIRE(ctx, d->rows > 0 && d->num_items > 0 && d->dim > 0, "%s: empty input (%u rows, %u items, %u dimensions)", who, d->rows,
+               d->num_items, d->dim);
+    VA_REQUIRE(ctx, d->dtype == VA_DTYPE_F32 || d->dtype == VA_DTYPE_F16 || d->dtype == VA_DTYPE_BF16, "%s: unknown type %d", who, int(d->dtype));
+    VA_REQUIRE(ctx, d->dim <= VA_XENT_MAX_DIM, "%s: %u dimensions (at most %u)", who, d->dim, VA_XENT_MAX_DIM);
+    VA_REQUIRE(ctx, d->num_items < 0xFFFFFF00u && d->rows < 0xFFFFFF00u, "%s: too many rows or items", who);
+    VA_REQUIRE(ctx, d->hidden_stride >= d->dim && d->items_stride >= d->dim, "%s: a row stride is below the dimension", who);
+    VA_REQUIRE(ctx, std::isfinite(d->scale), "%s: the scale is not finite", who);
+    const size_t es = elem_size(d->dtype);
+    VA_REQUIRE(ctx, reinterpret_cast<uintptr_t>(d->hidden) % es == 0 && reinterpret_cast<uintptr_t>(d->items) % es == 0,
+               "%s: rows or items are not aligned to their type", who);
+    return VA_OK;
+}
+
+uint32_t round_up(uint32_t v, uint32_t m) { return (v + m - 1) / m * m; }
+
+// The largest piece of items (a multiple of 256) whose per-item workspace stays within `budget`.
+uint32_t piece_items(uint32_t V, size_t per_item, size_t budget) {
+    const uint64_t n = std::max<uint64_t>(budget / std::max<size_t>(per_item, 1) / 256, 1) * 256;
+    return uint32_t(std::min<uint64_t>(n, round_up(V, 256)));
+}
+
+constexpr size_t kPackBudget = size_t(256) << 20;  // packed items of one piece
+constexpr size_t kGradBudget = size_t(512) << 20;  // one order of dl of one piece
+
+}  // namespace
+}  // namespace va
+
+using namespace va;
+
+extern "C" {
+
+va_status va_xent_forward(va_context* ctx, const va_xent_desc* d, float* out_loss, float* out_lse, va_reduction reduction, float* out_reduced) {
+    if (!ctx) return VA_ERR_INVALID_ARG;
+    VA_CHECK_STATUS(check_desc(ctx, d, "va_xent_forward"));
+    VA_REQUIRE(ctx, out_loss && out_lse, "va_xent_forward: NULL output");
+    VA_REQUIRE(ctx, reduction == VA_REDUCE_MEAN || reduction == VA_REDUCE_SUM || reduction == VA_REDUCE_NONE, "va_xent_forward: unknown reduction %d", int(reduction));
+    VA_REQUIRE(ctx, (reduction == VA_REDUCE_NONE) == (out_reduced == nullptr), "va_xent_forward: a reduced loss goes with a reduction");
+    DeviceGuard guard(ctx->device);
+    const uint32_t T = d->rows, V = d->num_items, D = d->dim, Kp = round_up(D, g16::KC);
+    const va_dtype dt = d->dtype;
+    const size_t es = elem_size(dt), planes = dt == VA_DTYPE_F32 ? 2 : 1;
+    const bool qd = direct(dt, d->hidden, d->hidden_stride, D), xd = direct(dt, d->items, d->items_stride, D);
+    const uint32_t piece = xd ? round_up(V, 256) : piece_items(V, packed_bytes(dt, 1, Kp), kPackBudget);
+    const uint32_t pieces = ceil_div(V, piece), nq = ceil_div(T, 256);
+    const uint32_t cus = std::max(uint32_t(ctx->num_cus), kXcds) / kXcds * kXcds;
+    // parts per query block: whole multiples of the XCDs when there are that many
+    uint32_t parts = std::max(cus / nq, 1u);
+    if (parts > kXcds) parts = parts / kXcds * kXcds;
+    parts = std::min(parts, ceil_div(std::min(piece, V), 256));
+    const uint32_t last_parts = std::min(parts, ceil_div(V - (pieces - 1) * piece, 256));  // (of the last piece)
+    const uint32_t slots = parts * (pieces - 1) + last_parts;
+
+    Scratch sc(ctx);
+    const size_t need = (qd ? 0 : Scratch::round(packed_bytes(dt, T, Kp)) + Scratch::round(T * 4ull)) +
+                        (xd ? 0 : Scratch::round(packed_bytes(dt, piece, Kp)) + Scratch::round(piece * 4ull)) +
+                        Scratch::round(uint64_t(T) * slots * sizeof(float2)) + Scratch::round(T * 4ull);
+    VA_CHECK_STATUS(sc.reserve(need));
+    float2* part = sc.carve<float2>(uint64_t(T) * slots);
+    float* picked = sc.carve<float>(T);
+    char* qp = nullptr;
+    char* xp = nullptr;
+    float* qinv = nullptr;
+    float* xinv = nullptr;
+    if (!qd) {
+        qp = sc.carve<char>(packed_bytes(dt, T, Kp));
+        qinv = sc.carve<float>(T);
+        VA_CHECK_STATUS(pack(ctx, dt, d->hidden, d->hidden_stride, T, D, Kp, qp, qinv));
+    }
+    if (!xd) {
+        xp = sc.carve<char>(packed_bytes(dt, piece, Kp));
+        xinv = sc.carve<float>(piece);
+    }
+    VA_CHECK_STATUS(sc.verify(need));
+    for (uint32_t c = 0; c < pieces; ++c) {
+        const uint32_t v0 = c * piece, n = std::min(piece, V - v0);
+        const char* items = at(d->items, d->items_stride, v0, dt);
+        if (!xd) VA_CHECK_STATUS(pack(ctx, dt, items, d->items_stride, n, D, Kp, xp, xinv));
+        g16::Args a;
+        a.q = g16::Operand{qd ? d->hidden : qp, qd ? d->hidden_stride * es : uint64_t(Kp) * 2 * planes, T, uint32_t(Kp * 2)};
+        a.x = g16::Operand{xd ? items : xp, xd ? d->items_stride * es : uint64_t(Kp) * 2 * planes, n, uint32_t(Kp * 2)};
+        a.kstages = Kp / g16::KC;
+        a.nq = nq;
+        a.nr = ceil_div(n, 256);
+        a.parts = c + 1 < pieces ? parts : last_parts;
+        VA_CHECK_STATUS(by_type(dt, d->offsets || n % g16::TR, [&](auto bf, auto off, auto pl) {
+            LseEpi<decltype(off)::value, decltype(pl)::value> e;
+            e.a = LogitArgs{d->offsets ? d->offsets + v0 : nullptr, qinv, xinv, d->scale, T, n};
+            e.targets = d->targets;
+            e.item0 = v0;
+            e.picked = picked;
+            e.part = part;
+            e.slots = slots;
+            e.slot0 = c * parts;
+            return g16::launch<decltype(bf)::value, decltype(pl)::value>(ctx, a, e);
+        }));
+    }
+    xent_finish_kernel<<<dim3(ceil_div(T, 4)), dim3(256), 0, ctx->stream>>>(d->targets, T, V, d->ignore_index, part, picked, slots, out_loss, out_lse);
+    VA_CHECK_LAUNCH(ctx);
+    if (out_reduced) {
+        xent_reduce_kernel<<<dim3(1), dim3(1024), 0, ctx->stream>>>(out_loss, d->targets, T, d->ignore_index, reduction == VA_REDUCE_MEAN, out_reduced);
+        VA_CHECK_LAUNCH(ctx);
+    }
+    return VA_OK;
+}
+
+va_status va_xent_backward(va_context* ctx, const va_xent_desc* d, const float* lse, va_reduction reduction, const float* grad,
+                           void* out_grad_hidden, uint64_t grad_hidden_stride, void* out_grad_items, uint64_t grad_items_stride) {
+    if (!ctx) return VA_ERR_INVALID_ARG;
+    VA_CHECK_STATUS(check_desc(ctx, d, "va_xent_backward"));
+    VA_REQUIRE(ctx, lse, "va_xent_backward: NULL log-sum-exp");
+    VA_REQUIRE(ctx, reduction == VA_REDUCE_MEAN || reduction == VA_REDUCE_SUM || reduction == VA_REDUCE_NONE, "va_xent_backward: unknown reduction %d", int(reduction));
+    VA_REQUIRE(ctx, reduction != VA_REDUCE_NONE || grad, "va_xent_backward: without a reduction the rows' gradients are needed");
+    VA_REQUIRE(ctx, out_grad_hidden || out_grad_items, "va_xent_backward: no output");
+    VA_REQUIRE(ctx, (!out_grad_hidden || grad_hidden_stride >= d->dim) && (!out_grad_items || grad_items_stride >= d->dim),
+               "va_xent_backward: a gradient's row stride is below the dimension");
+    DeviceGuard guard(ctx->device);
+    const uint32_t T = d->rows, V = d->num_items, D = d->dim, Kp = round_up(D, g16::KC), Tp = round_up(T, g16::KC), Dp = round_up(D, 4);
+    const va_dtype dt = d->dtype;
+    const bool f32 = dt == VA_DTYPE_F32;
+    const size_t es = elem_size(dt), planes = f32 ? 2 : 1;
+    const bool qd = direct(dt, d->hidden, d->hidden_stride, D), xd = direct(dt, d->items, d->items_stride, D);
+    VA_REQUIRE(ctx, (!out_grad_hidden || reinterpret_cast<uintptr_t>(out_grad_hidden) % es == 0) &&
+                        (!out_grad_items || reinterpret_cast<uintptr_t>(out_grad_items) % es == 0),
+               "va_xent_backward: a gradient is not aligned to its type");
+    // the piece: dl within its budget (in either order), the packed and transposed items too
+    uint32_t piece = piece_items(V, uint64_t(Tp) * 2 * planes, kGradBudget);
+    piece = std::min(piece, piece_items(V, packed_bytes(dt, 1, Kp), kPackBudget));
+    // dl's rows of a piece within the products' 32-bit offsets
+    piece = std::min<uint32_t>(piece, uint32_t(kDmaMaxBytes / 256 / (2 * planes)) / 256 * 256);
+    VA_REQUIRE(ctx, uint64_t(Tp) * 2 * planes * 256 <= kDmaMaxBytes, "va_xent_backward: %u rows (at most %u)", T, uint32_t(kDmaMaxBytes / (512 * planes)));
+    const uint32_t pieces = ceil_div(V, piece), nq = ceil_div(T, 256), nd = ceil_div(D, 256);
+    const uint32_t Vpmax = round_up(std::min(piece, V), g16::KC);
+    const uint32_t cus = std::max(uint32_t(ctx->num_cus), kXcds) / kXcds * kXcds;
+    // dh has few tiles and a long sum: shares of it until the chip is filled once
+    const uint32_t kst = Vpmax / g16::KC * (f32 ? 3 : 1);
+    const uint32_t parts = std::min(std::max(cus / (nq * nd), 1u), std::max(kst / 4, 1u));
+
+    const size_t p_bytes = out_grad_hidden ? uint64_t(T) * Vpmax * 2 * planes : 0;
+    const size_t pt_bytes = out_grad_items ? uint64_t(std::min(piece, round_up(V, 256))) * Tp * 2 * planes : 0;
+    const size_t wt_bytes = out_grad_hidden ? uint64_t(D) * Vpmax * 2 * planes : 0;
+    const size_t ht_bytes = out_grad_items ? uint64_t(D) * Tp * 2 * planes : 0;
+    const size_t share_n = out_grad_hidden ? uint64_t(parts) * T * Dp : 0;
+    const size_t qp_bytes = qd ? 0 : packed_bytes(dt, T, Kp), xp_bytes = xd ? 0 : packed_bytes(dt, std::min(piece, V), Kp);
+    Scratch sc(ctx);
+    const size_t need = Scratch::round(p_bytes) + Scratch::round(pt_bytes) + Scratch::round(wt_bytes) + Scratch::round(ht_bytes) +
+                        Scratch::round(share_n * 4) + Scratch::round(qp_bytes) + Scratch::round(xp_bytes) + 2 * Scratch::round(T * 4ull) +
+                        Scratch::round(piece * 4ull) + Scratch::round(16);
+    VA_CHECK_STATUS(sc.reserve(need));
+    uint16_t* p = out_grad_hidden ? sc.carve<uint16_t>(p_bytes / 2) : nullptr;
+    uint16_t* pt = out_grad_items ? sc.carve<uint16_t>(pt_bytes / 2) : nullptr;
+    uint16_t* wt = sc.carve<uint16_t>(wt_bytes / 2);
+    uint16_t* ht = sc.carve<uint16_t>(ht_bytes / 2);
+    float* share = sc.carve<float>(share_n);
+    char* qp = sc.carve<char>(qp_bytes);
+    char* xp = sc.carve<char>(xp_bytes);
+    float* gk = sc.carve<float>(T);
+    float* qinv = sc.carve<float>(T);
+    float* xinv = sc.carve<float>(piece);
+    float* mul = sc.carve<float>(4);
+    uint32_t* absmax = reinterpret_cast<uint32_t*>(mul + 1);  // of the hidden rows, of the items
+    VA_CHECK_STATUS(sc.verify(need));
+
+    xent_gradient_kernel<<<dim3(1), dim3(1024), 0, ctx->stream>>>(grad, d->targets, T, V, d->ignore_index, int(reduction), d->scale, gk, mul, absmax);
+    VA_CHECK_LAUNCH(ctx);
+    if (f32) {
+        auto top = [&](const void* src, uint64_t ld, uint32_t R, const float* drop, float drop_if, uint32_t* out) {
+            absmax_kernel<<<dim3(std::min<uint32_t>(ceil_div(R, 4), 2048)), dim3(256), 0, ctx->stream>>>(static_cast<const float*>(src), ld, R, D, drop, drop_if, out);
+        };
+        if (out_grad_items) top(d->hidden, d->hidden_stride, T, gk, 0.0f, absmax);
+        if (out_grad_hidden) top(d->items, d->items_stride, V, d->offsets, -INFINITY, absmax + 1);
+        VA_CHECK_LAUNCH(ctx);
+    }
+    if (!qd) VA_CHECK_STATUS(pack(ctx, dt, d->hidden, d->hidden_stride, T, D, Kp, qp, qinv));
+    if (out_grad_items) VA_CHECK_STATUS(transpose(ctx, dt, d->hidden, d->hidden_stride, T, D, Tp, gk, 0.0f, absmax, ht));
+    for (uint32_t c = 0; c < pieces; ++c) {
+        const uint32_t v0 = c * piece, n = std::min(piece, V - v0), Vp = round_up(n, g16::KC);
+        const char* items = at(d->items, d->items_stride, v0, dt);
+        const float* offsets = d->offsets ? d->offsets + v0 : nullptr;
+        if (!xd) VA_CHECK_STATUS(pack(ctx, dt, items, d->items_stride, n, D, Kp, xp, xinv));
+        g16::Args a;
+        a.q = g16::Operand{qd ? d->hidden : qp, qd ? d->hidden_stride * es : uint64_t(Kp) * 2 * planes, T, uint32_t(Kp * 2)};
+        a.x = g16::Operand{xd ? items : xp, xd ? d->items_stride * es : uint64_t(Kp) * 2 * planes, n, uint32_t(Kp * 2)};
+        a.kstages = Kp / g16::KC;
+        a.nq = nq;
+        a.nr = ceil_div(n, 256);
+        a.parts = 1;
+        VA_CHECK_STATUS(by_type(dt, offsets || n % g16::TR, [&](auto bf, auto off, auto pl) {
+            GradEpi<decltype(bf)::value, decltype(off)::value, decltype(pl)::value> e;
+            e.a = LogitArgs{offsets, qinv, xinv, d->scale, T, n};
+            e.gk = gk;
+            e.lse = lse;
+            e.targets = d->targets;
+            e.item0 = v0;
+            e.p = p;
+            e.pt = pt;
+            e.Vp = Vp;
+            e.Tp = Tp;
+            return g16::launch<decltype(bf)::value, decltype(pl)::value>(ctx, a, e);
+        }));
+        if (out_grad_hidden) {
+            VA_CHECK_STATUS(transpose(ctx, dt, items, d->items_stride, n, D, Vp, offsets, -INFINITY, absmax + 1, wt));
+            g16::Args b;
+            b.q = g16::Operand{p, uint64_t(Vp) * 2 * planes, T, Vp * 2};
+            b.x = g16::Operand{wt, uint64_t(Vp) * 2 * planes, D, Vp * 2};
+            b.kstages = Vp / g16::KC;
+            b.nq = nq;
+            b.nr = nd;
+            b.parts = parts;
+            const ShareEpi e{share, T, D, Dp, c == 0};
+            VA_CHECK_STATUS(f32 ? (g16::launch<false, true>(ctx, b, e))
+                                : dt == VA_DTYPE_F16 ? (g16::launch<false, false>(ctx, b, e)) : (g16::launch<true, false>(ctx, b, e)));
+        }
+        if (out_grad_items) {
+            g16::Args b;
+            b.q = g16::Operand{pt, uint64_t(Tp) * 2 * planes, n, Tp * 2};
+            b.x = g16::Operand{ht, uint64_t(Tp) * 2 * planes, D, Tp * 2};
+            b.kstages = Tp / g16::KC;
+            b.nq = ceil_div(n, 256);
+            b.nr = nd;
+            b.parts = 1;
+            const uintptr_t o = reinterpret_cast<uintptr_t>(out_grad_items) + uint64_t(v0) * grad_items_stride * es;
+            const bool vec = o % (4 * es) == 0 && grad_items_stride % 4 == 0;
+            auto go = [&](auto DT, auto bf, auto pl) {
+                constexpr int kT = decltype(DT)::value;
+                ItemGradEpi<kT> e{reinterpret_cast<ElemT<kT>*>(o), grad_items_stride, n, D, mul, absmax, vec};
+                return g16::launch<decltype(bf)::value, decltype(pl)::value>(ctx, b, e);
+            };
+            VA_CHECK_STATUS(f32 ? go(std::integral_constant<int, VA_DTYPE_F32>(), std::false_type(), std::true_type())
+                            : dt == VA_DTYPE_F16 ? go(std::integral_constant<int, VA_DTYPE_F16>(), std::false_type(), std::false_type())
+                                                 : go(std::integral_constant<int, VA_DTYPE_BF16>(), std::true_type(), std::false_type()));
+        }
+    }
+    if (out_grad_hidden) {
+        const dim3 grid(ceil_div(uint64_t(T) * (Dp / 4), 256));
+        auto sum = [&](auto k, auto* o) {
+            k<<<grid, dim3(256), 0, ctx->stream>>>(share, parts, T, D, Dp, gk, mul, absmax + 1, o, grad_hidden_stride);
+        };
+        if (f32) sum(&share_sum_kernel<VA_DTYPE_F32>, static_cast<float*>(out_grad_hidden));
+        else if (dt == VA_DTYPE_F16) sum(&share_sum_kernel<VA_DTYPE_F16>, static_cast<_Float16*>(out_grad_hidden));
+        else sum(&share_sum_kernel<VA_DTYPE_BF16>, static_cast<__bf16*>(out_grad_hidden));
+        VA_CHECK_LAUNCH(ctx);
+    }
+    return VA_OK;
+}
+
+}  // extern "C"

@@ -1,0 +1,346 @@
+"""Training and serving of the embeddings that a collection holds.
+
+SoftmaxCrossEntropyKernel  the loss of hidden rows against every item of a collection, and its gradient
+RMSNormKernel              root-mean-square norm with the residual's addition, its backward pass, and
+                           its output in 8 bits with scales (the codes of the int8 scan)
+GradientClipKernel         the global norm of a list of gradients, and the gradients clipped by it
+
+The reference has no counterpart of these.  They follow its kernel classes: ``encode*`` takes device
+tensors, checks them and enqueues on the context's stream (inputs must be ready for that stream, and
+tensors must live until the work is done); the other methods allocate the outputs, order the call after
+torch's current stream and wait.  All arithmetic runs in libva_hip.so.
+"""
+from __future__ import annotations
+
+import ctypes as C
+from dataclasses import dataclass
+
+from . import _lib
+from .context import GPUContext, VectorError, dptr
+
+_REDUCTIONS = {"mean": _lib.VA_REDUCE_MEAN, "sum": _lib.VA_REDUCE_SUM, "none": _lib.VA_REDUCE_NONE}
+_DTYPES: dict = {}
+_CODES: dict = {}
+
+
+def _torch():
+    import torch
+
+    if not _DTYPES:
+        _DTYPES.update({torch.float32: _lib.VA_DTYPE_F32, torch.float16: _lib.VA_DTYPE_F16, torch.bfloat16: _lib.VA_DTYPE_BF16})
+        _CODES.update({torch.int8: _lib.VA_CODE_INT8, torch.float8_e4m3fn: _lib.VA_CODE_FP8_E4M3})
+    return torch
+
+
+def _dtype(t, name: str) -> int:
+    _torch()
+    d = _DTYPES.get(t.dtype)
+    if d is None:
+        raise VectorError.invalidInput(f"{name}: unsupported type {t.dtype} (float32, float16 or bfloat16)")
+    return d
+
+
+def _rows(t, name: str, like=None, shape=None) -> tuple[int, int]:
+    """(device pointer, elements between rows) of a device matrix whose rows are contiguous; checked
+    against `like`'s type and device and against `shape`."""
+    if not t.is_cuda:
+        raise VectorError.invalidInput(f"{name}: expected a device (CUDA) tensor")
+    if t.dim() != 2:
+        raise VectorError.invalidInput(f"{name}: expected a matrix, got {t.dim()} dimensions")
+    if shape is not None and tuple(t.shape) != tuple(shape):
+        if t.shape[1] != shape[1]:
+            raise VectorError.dimensionMismatch(shape[1], t.shape[1])
+        raise VectorError.invalidInput(f"{name}: expected {shape[0]} rows, got {t.shape[0]}")
+    if like is not None:
+        if t.dtype != like.dtype:
+            raise VectorError.invalidInput(f"{name}: expected {like.dtype}, got {t.dtype}")
+        if t.device != like.device:
+            raise VectorError.invalidInput(f"{name}: on {t.device}, expected {like.device}")
+    rows, dim = t.shape
+    sr, sd = t.stride()
+    if dim > 1 and sd != 1:
+        raise VectorError.invalidInput(f"{name}: the values of a row must be contiguous")
+    if rows > 1 and sr < dim:
+        raise VectorError.invalidInput(f"{name}: rows overlap")
+    return t.data_ptr(), sr if rows > 1 else max(sr, dim)
+
+
+def _vector(t, name: str, dtype, count: int, like) -> int:
+    """Device pointer of a contiguous vector of `count` values of `dtype` on `like`'s device."""
+    if t.dtype != dtype or t.numel() != count or t.device != like.device or not t.is_contiguous():
+        raise VectorError.invalidInput(
+            f"{name}: expected {count} contiguous values of {dtype} on {like.device}, got {tuple(t.shape)} of {t.dtype} on {t.device}")
+    return t.data_ptr()
+
+
+@dataclass
+class SoftmaxCrossEntropyResult:
+    """Device tensors: per-row loss and log-sum-exp, and the reduced loss (None without a reduction)."""
+
+    loss: object
+    logSumExp: object
+    reduced: object
+
+
+class SoftmaxCrossEntropyKernel:
+    """Softmax cross entropy of hidden rows [T x D] over all items [V x D] of a collection.
+
+    logits = scale * hidden @ items.T + offsets;  loss_t = logsumexp(logits_t) - logits_t[target_t].
+    The logits are never stored.  offsets (fp32 [V] or None) are constants: corrections of a sampled
+    softmax, and -inf for deleted items, which have no probability and no gradient whatever their
+    vectors hold.  Rows whose target is ``ignoreIndex`` have loss 0 and gradient 0; a target outside
+    the collection gives a NaN loss and gradient 0.  Targets are int64.  hidden and items are float32,
+    float16 or bfloat16 alike, their rows may be strided.
+    """
+
+    name = "SoftmaxCrossEntropyKernel"
+
+    def __init__(self, context: GPUContext):
+        self.context = context
+
+    def _describe(self, hidden, items, targets, scale, offsets, ignoreIndex):
+        torch = _torch()
+        dtype = _dtype(hidden, "hidden")
+        hp, hs = _rows(hidden, "hidden")
+        ip, is_ = _rows(items, "items", hidden, (items.shape[0], hidden.shape[1]))
+        T, D = hidden.shape
+        V = items.shape[0]
+        return _lib.XentDesc(hp, ip, _vector(targets, "targets", torch.int64, T, hidden),
+                             _vector(offsets, "offsets", torch.float32, V, hidden) if offsets is not None else None,
+                             hs, is_, int(ignoreIndex), T, V, D, dtype, float(scale))
+
+    def encodeForward(self, hidden, items, targets, outLoss, outLogSumExp, outReduced=None, reduction: str = "mean",
+                      scale: float = 1.0, offsets=None, ignoreIndex: int = -100) -> None:
+        """outLoss and outLogSumExp: fp32 [T]; outReduced (one fp32 value or None): the reduced loss."""
+        c, f32 = self.context, _torch().float32
+        d = self._describe(hidden, items, targets, scale, offsets, ignoreIndex)
+        mode = _reduction(reduction) if outReduced is not None else _lib.VA_REDUCE_NONE
+        if outReduced is not None and mode == _lib.VA_REDUCE_NONE:
+            raise VectorError.invalidInput("a reduced loss needs a reduction")
+        c.check(c.lib.va_xent_forward(c.handle, C.byref(d), _vector(outLoss, "outLoss", f32, d.rows, hidden),
+                                      _vector(outLogSumExp, "outLogSumExp", f32, d.rows, hidden), mode,
+                                      _vector(outReduced, "outReduced", f32, 1, hidden) if outReduced is not None else None),
+                "va_xent_forward")
+
+    def encodeBackward(self, hidden, items, targets, logSumExp, outGradHidden=None, outGradItems=None, grad=None,
+                       reduction: str = "mean", scale: float = 1.0, offsets=None, ignoreIndex: int = -100) -> None:
+        """Gradients of the reduced loss times ``grad`` (one fp32 value; None: 1), or with reduction "none"
+        of sum(grad * loss) for grad of [T].  logSumExp is encodeForward's; the outputs have the
+        type and shape of what they are the gradient of, and either may be None."""
+        c, f32 = self.context, _torch().float32
+        d = self._describe(hidden, items, targets, scale, offsets, ignoreIndex)
+        mode = _reduction(reduction)
+        if mode == _lib.VA_REDUCE_NONE and grad is None:
+            raise VectorError.invalidInput("without a reduction the rows' gradients are needed")
+        count = d.rows if mode == _lib.VA_REDUCE_NONE else 1
+        hp, hs = _rows(outGradHidden, "outGradHidden", hidden, hidden.shape) if outGradHidden is not None else (None, 0)
+        ip, is_ = _rows(outGradItems, "outGradItems", hidden, items.shape) if outGradItems is not None else (None, 0)
+        c.check(c.lib.va_xent_backward(c.handle, C.byref(d), _vector(logSumExp, "logSumExp", f32, d.rows, hidden), mode,
+                                       _vector(grad, "grad", f32, count, hidden) if grad is not None else None, hp, hs, ip, is_),
+                "va_xent_backward")
+
+    def forward(self, hidden, items, targets, reduction: str = "mean", scale: float = 1.0, offsets=None,
+                ignoreIndex: int = -100) -> SoftmaxCrossEntropyResult:
+        c, torch = self.context, _torch()
+        T = hidden.shape[0]
+        loss, lse = c.empty((T,), torch.float32), c.empty((T,), torch.float32)
+        reduced = c.empty((1,), torch.float32) if _reduction(reduction) != _lib.VA_REDUCE_NONE else None
+        c.order_after_torch()
+        self.encodeForward(hidden, items, targets, loss, lse, reduced, reduction, scale, offsets, ignoreIndex)
+        c.synchronize()
+        return SoftmaxCrossEntropyResult(loss, lse, reduced)
+
+    def backward(self, hidden, items, targets, logSumExp, grad=None, reduction: str = "mean", scale: float = 1.0, offsets=None,
+                 ignoreIndex: int = -100):
+        """(gradient of hidden, gradient of items)."""
+        c = self.context
+        gh, gi = c.empty(hidden.shape, hidden.dtype), c.empty(items.shape, items.dtype)
+        c.order_after_torch()
+        self.encodeBackward(hidden, items, targets, logSumExp, gh, gi, grad, reduction, scale, offsets, ignoreIndex)
+        c.synchronize()
+        return gh, gi
+
+
+def _reduction(name: str) -> int:
+    if name not in _REDUCTIONS:
+        raise VectorError.invalidInput(f"unknown reduction {name!r} (mean, sum or none)")
+    return _REDUCTIONS[name]
+
+
+class RMSNormKernel:
+    """y = r / sqrt(mean(r^2) + epsilon) * weight with r = x + residual, over rows [T x D].
+
+    x, residual, weight and the outputs are float32, float16 or bfloat16 alike; rows may be strided,
+    and an output may be the input that it replaces.  The 8-bit forms write codes (int8, or
+    float8_e4m3fn) with a scale for each row (groupSize 0) or for each group of ``groupSize``
+    dimensions (a power of two from 8 to 512), or on the one grid of ``givenScale``.
+    """
+
+    name = "RMSNormKernel"
+
+    def __init__(self, context: GPUContext):
+        self.context = context
+
+    @staticmethod
+    def _describe(x, weight, residual, outResidual, outInverseRms, epsilon):
+        torch = _torch()
+        dtype = _dtype(x, "x")
+        xp, xs = _rows(x, "x")
+        T, D = x.shape
+        rp, rs = _rows(residual, "residual", x, x.shape) if residual is not None else (None, 0)
+        op, os_ = _rows(outResidual, "outResidual", x, x.shape) if outResidual is not None else (None, 0)
+        ip = _vector(outInverseRms, "outInverseRms", torch.float32, T, x) if outInverseRms is not None else None
+        if weight.numel() != D:
+            raise VectorError.dimensionMismatch(D, weight.numel())
+        return _lib.RmsDesc(xp, rp, _vector(weight, "weight", x.dtype, D, x), op, ip, xs, rs, os_, T, D, dtype, float(epsilon))
+
+    @staticmethod
+    def _codes(codes, x_shape, like):
+        _torch()
+        code = _CODES.get(codes.dtype)
+        if code is None:
+            raise VectorError.invalidInput(f"codes: unsupported type {codes.dtype} (int8 or float8_e4m3fn)")
+        p, s = _rows(codes, "codes", None, x_shape)
+        if codes.device != like.device:
+            raise VectorError.invalidInput(f"codes: on {codes.device}, expected {like.device}")
+        return code, p, s
+
+    @staticmethod
+    def _scales(scales, givenScale, groupSize, T, D, like):
+        if (scales is None) == (givenScale is None):
+            raise VectorError.invalidInput("either scales or a given scale")
+        if givenScale is not None:
+            if not float(givenScale) > 0.0:
+                raise VectorError.invalidInput(f"a given scale must be positive, got {givenScale}")
+            return None
+        groups = -(-D // groupSize) if groupSize else 1
+        return _vector(scales, "scales", _torch().float32, T * groups, like)
+
+    def encode(self, x, weight, out, residual=None, outResidual=None, outInverseRms=None, epsilon: float = 1e-6) -> None:
+        c = self.context
+        d = self._describe(x, weight, residual, outResidual, outInverseRms, epsilon)
+        op, os_ = _rows(out, "out", x, x.shape)
+        c.check(c.lib.va_rms_norm(c.handle, C.byref(d), op, os_), "va_rms_norm")
+
+    def encodeQuantized(self, x, weight, outCodes, outScales=None, residual=None, outResidual=None, outInverseRms=None,
+                        groupSize: int = 0, givenScale: float | None = None, epsilon: float = 1e-6) -> None:
+        c = self.context
+        d = self._describe(x, weight, residual, outResidual, outInverseRms, epsilon)
+        code, cp, cs = self._codes(outCodes, x.shape, x)
+        sp = self._scales(outScales, givenScale, groupSize, d.rows, d.dim, x)
+        c.check(c.lib.va_rms_norm_quantized(c.handle, C.byref(d), code, int(groupSize), float(givenScale or 0.0), cp, cs, sp),
+                "va_rms_norm_quantized")
+
+    def encodeDequantize(self, codes, scales, out, groupSize: int = 0, givenScale: float | None = None) -> None:
+        """out = code * scale in out's type."""
+        c = self.context
+        dtype = _dtype(out, "out")
+        op, os_ = _rows(out, "out")
+        T, D = out.shape
+        code, cp, cs = self._codes(codes, out.shape, out)
+        sp = self._scales(scales, givenScale, groupSize, T, D, out)
+        c.check(c.lib.va_rms_dequantize(c.handle, cp, cs, code, sp, float(givenScale or 0.0), T, D, int(groupSize), dtype, op, os_),
+                "va_rms_dequantize")
+
+    def encodeBackward(self, grad, summed, weight, inverseRms, outGradX=None, outGradWeight=None, gradResidual=None) -> None:
+        """``summed`` is x + residual as the forward pass stored it (x where there was no residual), inverseRms
+        its outInverseRms, gradResidual what reaches the new residual from behind.  outGradX is the
+        gradient of x and of the residual alike."""
+        c = self.context
+        d = self._describe(summed, weight, None, None, None, 0.0)
+        gp, gs = _rows(grad, "grad", summed, summed.shape)
+        rp, rs = _rows(gradResidual, "gradResidual", summed, summed.shape) if gradResidual is not None else (None, 0)
+        xp, xs = _rows(outGradX, "outGradX", summed, summed.shape) if outGradX is not None else (None, 0)
+        wp = _vector(outGradWeight, "outGradWeight", summed.dtype, d.dim, summed) if outGradWeight is not None else None
+        c.check(c.lib.va_rms_norm_backward(c.handle, C.byref(d), gp, gs, rp, rs,
+                                           _vector(inverseRms, "inverseRms", _torch().float32, d.rows, summed), xp, xs, wp),
+                "va_rms_norm_backward")
+
+    def forward(self, x, weight, residual=None, epsilon: float = 1e-6):
+        """(y, x + residual, inverse rms)."""
+        c, torch = self.context, _torch()
+        y, r = c.empty(x.shape, x.dtype), c.empty(x.shape, x.dtype) if residual is not None else x
+        inv = c.empty((x.shape[0],), torch.float32)
+        c.order_after_torch()
+        self.encode(x, weight, y, residual, r if residual is not None else None, inv, epsilon)
+        c.synchronize()
+        return y, r, inv
+
+    def quantize(self, x, weight, residual=None, code=None, groupSize: int = 0, givenScale: float | None = None, epsilon: float = 1e-6):
+        """(codes, scales or None, x + residual); code: torch.int8 (the default) or torch.float8_e4m3fn."""
+        c, torch = self.context, _torch()
+        T, D = x.shape
+        codes = c.empty((T, D), code or torch.int8)
+        scales = c.empty((T, -(-D // groupSize) if groupSize else 1), torch.float32) if givenScale is None else None
+        r = c.empty(x.shape, x.dtype) if residual is not None else x
+        c.order_after_torch()
+        self.encodeQuantized(x, weight, codes, scales, residual, r if residual is not None else None, None, groupSize, givenScale, epsilon)
+        c.synchronize()
+        return codes, scales, r
+
+    def backward(self, grad, summed, weight, inverseRms, gradResidual=None):
+        """(gradient of x and of the residual, gradient of weight)."""
+        c = self.context
+        gx, gw = c.empty(summed.shape, summed.dtype), c.empty(weight.shape, weight.dtype)
+        c.order_after_torch()
+        self.encodeBackward(grad, summed, weight, inverseRms, gx, gw, gradResidual)
+        c.synchronize()
+        return gx, gw
+
+
+class TensorList:
+    """Device tensors of a call, listed once: their addresses, sizes and types.  The tensors are kept
+    alive; a tensor that is replaced (not written in place) needs a new list."""
+
+    def __init__(self, tensors, outputs=None):
+        _torch()
+        self.tensors = list(tensors)
+        self.outputs = list(outputs) if outputs is not None else None
+        if self.outputs is not None and len(self.outputs) != len(self.tensors):
+            raise VectorError.invalidInput(f"{len(self.tensors)} tensors and {len(self.outputs)} outputs")
+        for i, t in enumerate(self.tensors):
+            _dtype(t, f"tensor {i}")
+            dptr(t)
+            if t.device != self.tensors[0].device:
+                raise VectorError.invalidInput(f"tensor {i}: on {t.device}, expected {self.tensors[0].device}")
+            if self.outputs is not None:
+                o = self.outputs[i]
+                dptr(o)
+                if o.dtype != t.dtype or o.numel() != t.numel() or o.device != t.device:
+                    raise VectorError.invalidInput(f"output {i}: expected {t.numel()} values of {t.dtype} on {t.device}")
+        n = len(self.tensors)
+        self._in = (C.c_void_p * n)(*[t.data_ptr() for t in self.tensors])
+        self._out = (C.c_void_p * n)(*[t.data_ptr() for t in self.outputs]) if self.outputs is not None else None
+        self._sizes = (C.c_uint64 * n)(*[t.numel() for t in self.tensors])
+        self._dtypes = (C.c_int32 * n)(*[_DTYPES[t.dtype] for t in self.tensors])
+        cast = lambda a: C.cast(a, C.c_void_p) if a is not None else None  # noqa: E731
+        self.desc = _lib.TensorListDesc(cast(self._in), cast(self._out), cast(self._sizes), cast(self._dtypes), n)
+
+
+class GradientClipKernel:
+    """norm = sqrt(sum of the squares of all values of a list of tensors); every tensor times
+    min(1, maxNorm / (norm + epsilon)), in place or into the list's outputs.  Types may be mixed."""
+
+    name = "GradientClipKernel"
+
+    def __init__(self, context: GPUContext):
+        self.context = context
+
+    def tensorList(self, tensors, outputs=None) -> TensorList:
+        return TensorList(tensors, outputs)
+
+    def encode(self, tensors: TensorList, maxNorm: float, outNorm=None, epsilon: float = 1e-6) -> None:
+        """outNorm: one fp32 value on the device, or None."""
+        c = self.context
+        if outNorm is not None and (outNorm.dtype != _torch().float32 or outNorm.numel() != 1 or not outNorm.is_cuda):
+            raise VectorError.invalidInput("outNorm: expected one float32 value on the device")
+        c.check(c.lib.va_grad_clip(c.handle, C.byref(tensors.desc), float(maxNorm), float(epsilon), dptr(outNorm) or None), "va_grad_clip")
+
+    def clip(self, tensors, maxNorm: float, epsilon: float = 1e-6) -> float:
+        """Clips the tensors in place and returns their norm before."""
+        c = self.context
+        norm = c.empty((1,), _torch().float32)
+        c.order_after_torch()
+        self.encode(TensorList(tensors), maxNorm, norm, epsilon)
+        c.synchronize()
+        return float(norm.item())
