@@ -130,7 +130,7 @@ struct Lane {
 //   begin(State&, smem, tile)   a new item's first tile (barriers follow before the epilogue)
 //   load(State&, tile, tid)     before the main loop: starts what the tile's epilogue reads
 //   publish(State&, smem, tid)  after the main loop, before the barrier
-//   tile(State&, smem, lane, acc, tile)
+//   tile(State&, smem, lane, acc, tile, spare)  spare: 4 KiB of LDS of the wave's own
 //   end(State&, smem, lane, tile)  after an item's last tile
 template <bool BF16, bool PLANES, class Epi>
 __global__ __launch_bounds__(64 * WAVES, 4) void gemm16_kernel(Args a, Epi epi) {
@@ -259,7 +259,11 @@ __global__ __launch_bounds__(64 * WAVES, 4) void gemm16_kernel(Args a, Epi epi) 
             open();
             issue(s0, 0);
         }
-        epi.tile(st, smem, ln, acc, here);
+        // what the epilogue computes from the lane is computed there: kept through the main loop, its
+        // addresses would take the registers that the fragments need
+        Lane le = ln;
+        asm volatile("" : "+v"(le.l32), "+v"(le.hh));
+        epi.tile(st, smem, le, acc, here, lds + STAGE + wave * 4096);
         if (last) {
             epi.end(st, smem, ln, here);
             if (!tile.ok) break;

@@ -152,41 +152,64 @@ __global__ __launch_bounds__(256) void absmax_kernel(const float* __restrict__ s
 
 // dst[d][r] = src[r][d] for r < R, zeros for r in [R, Rp); rows whose drop value says so are zeros.
 // fp32: two planes (lo behind hi's Rp values), scaled by the tensor's power of two (absmax).
-// 64 x 64 tiles through LDS.
+// 64 x 64 tiles through LDS, laid out as GradEpi's: 8 values a thread and load, and 8 a store.
 template <int DT>
 __global__ __launch_bounds__(256) void transpose_kernel(const ElemT<DT>* __restrict__ src, uint64_t ld, uint32_t R, uint32_t D,
                                                         uint32_t Rp, const float* __restrict__ drop, float drop_if,
                                                         const uint32_t* __restrict__ absmax, uint16_t* __restrict__ dst) {
     constexpr bool kF32 = DT == VA_DTYPE_F32;
-    __shared__ ElemT<DT> tile[64][64 + (kF32 ? 1 : 2)];
+    constexpr int PL = kF32 ? 2 : 1;
+    typedef ElemT<DT> in8 __attribute__((ext_vector_type(8), aligned(sizeof(ElemT<DT>))));
+    typedef short s16x4 __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
+    __shared__ __attribute__((aligned(16))) char tile[PL][64 * 128];
     const uint32_t r0 = blockIdx.x * 64, d0 = blockIdx.y * 64;
-    const uint32_t c = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int tid = threadIdx.x;
+    const float sc = kF32 ? scale_to_2p14(__builtin_bit_cast(float, *absmax)) : 1.0f;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        const uint32_t r = r0 + w + 4 * i, d = d0 + c;
-        const bool in = r < R && d < D && !(drop && drop[r] == drop_if);
-        tile[w + 4 * i][c] = in ? src[uint64_t(r) * ld + d] : ElemT<DT>(0.0f);
+    for (int i = 0; i < 2; ++i) {
+        const int rl = (tid >> 3) + 32 * i, c = tid & 7;
+        const uint32_t r = r0 + rl, d = d0 + 8 * c;
+        uint16_t h[8] = {}, l[8] = {};
+        if (r < R && d < D && !(drop && drop[r] == drop_if)) {
+            const ElemT<DT>* s = src + uint64_t(r) * ld + d;
+            ElemT<DT> v[8];
+            if (d + 8 <= D) {
+                const in8 w = *reinterpret_cast<const in8*>(s);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = w[e];
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = d + e < D ? s[e] : ElemT<DT>(0.0f);
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                if constexpr (kF32) split16(v[e] * sc, h[e], l[e]);
+                else h[e] = __builtin_bit_cast(uint16_t, v[e]);
+            }
+        }
+        __builtin_memcpy(tile[0] + rl * 128 + 16 * (c ^ (rl & 7)), h, 16);
+        if constexpr (kF32) __builtin_memcpy(tile[PL - 1] + rl * 128 + 16 * (c ^ (rl & 7)), l, 16);
     }
     __syncthreads();
-    const float sc = kF32 ? scale_to_2p14(__builtin_bit_cast(float, *absmax)) : 1.0f;
-    const uint64_t pitch = uint64_t(Rp) * (kF32 ? 2 : 1);
-    const uint32_t rr = (threadIdx.x & 31) * 2;
+    // wave w takes the d-values 16 w .. 16 w + 15 of the tile: lane (i, g) d 16 w + i, r 8 g .. and 32 + 8 g ..
+    const int lane = tid & 63, w = tid >> 6, g = lane >> 4;
+    const uint32_t d = d0 + uint32_t(16 * w + (lane & 15));
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const uint32_t dl = (threadIdx.x >> 5) + 8 * i, d = d0 + dl;
-        if (d >= D || r0 + rr >= Rp) continue;
-        uint16_t* o = dst + d * pitch + r0 + rr;
-        if constexpr (kF32) {
-            uint16_t h0, l0, h1, l1;
-            split16(tile[rr][dl] * sc, h0, l0);
-            split16(tile[rr + 1][dl] * sc, h1, l1);
-            *reinterpret_cast<uint32_t*>(o) = h0 | uint32_t(h1) << 16;
-            *reinterpret_cast<uint32_t*>(o + Rp) = l0 | uint32_t(l1) << 16;
-        } else {
-            const uint16_t a = __builtin_bit_cast(uint16_t, tile[rr][dl]), b = __builtin_bit_cast(uint16_t, tile[rr + 1][dl]);
-            *reinterpret_cast<uint32_t*>(o) = a | uint32_t(b) << 16;
+    for (int pl = 0; pl < PL; ++pl)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            struct alignas(16) {
+                s16x4 v[2];
+            } o;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int r = 32 * i + 8 * g + 4 * h + ((lane & 15) >> 2), c = 2 * w + ((lane & 3) >> 1);
+                const uint32_t at = lds_addr_of(tile[pl]) + uint32_t(r * 128 + 16 * (c ^ (r & 7)) + 8 * (lane & 1));
+                o.v[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_s16x4>(at));
+            }
+            if (d < D) *reinterpret_cast<u32x4*>(dst + (uint64_t(d) * PL + pl) * Rp + r0 + 32 * i + 8 * g) = __builtin_bit_cast(u32x4, o);
         }
-    }
 }
 
 // ---- the logits' epilogues -------------------------------------------------------------------------
@@ -275,7 +298,7 @@ struct LseEpi {
             if (tid < g16::TR) sm.inv[tid] = s.inv;
     }
     template <class Tile>
-    __device__ void tile(State& s, Shared& sm, const g16::Lane& ln, f32x16 (&acc)[2][2], const Tile& t) {
+    __device__ void tile(State& s, Shared& sm, const g16::Lane& ln, f32x16 (&acc)[2][2], const Tile& t, char*) {
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
             const float c = PLANES ? a.scale * sm.qinv[ln.q(n)] : a.scale;
@@ -384,16 +407,59 @@ struct GradEpi {
         sm.lse[tid] = s.lse;
         sm.target[tid] = s.target;
     }
+    // One plane of the wave's 32 rows x 64 items of query block n, through its 4 KiB of LDS: [t][j] rows of
+    // 128 bytes, 16-byte chunks swizzled by t & 7 (both the 8-byte writes and the reads then touch every
+    // bank equally).  p leaves in whole 128-byte lines; for pt, ds_read_tr16 hands each lane four
+    // consecutive t of one j, so 8 t are one 16-byte store and a row's 32 t are 64 bytes.  (Stored straight
+    // from the accumulators, 8 and 2 bytes a lane, the same tile took three times as long.)
+    __device__ void put(const char* spare, const g16::Lane& ln, int n, const uint32_t q0, const uint32_t r0, uint32_t plane) {
+        typedef short s16x4 __attribute__((ext_vector_type(4)));
+        typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
+        const int lane = ln.hh * 32 + ln.l32;
+        asm volatile("" ::: "memory");  // the writes come first (a wave's LDS accesses execute in order)
+        if (p && r0 < Vp) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int t = 8 * i + (lane >> 3), c = lane & 7;
+                const u32x4 v = *reinterpret_cast<const u32x4*>(spare + t * 128 + 16 * (c ^ (t & 7)));
+                if (q0 + t < a.rows)
+                    *reinterpret_cast<u32x4*>(p + uint64_t(q0 + t) * Vp * (PLANES ? 2 : 1) + plane * Vp + r0 + 8 * c) = v;
+            }
+        }
+        if (pt && q0 < Tp) {
+            const int g = lane >> 4;
+#pragma unroll
+            for (int jb = 0; jb < 4; ++jb) {
+                struct alignas(16) {
+                    s16x4 v[2];
+                } o;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int t = 8 * g + 4 * h + ((lane & 15) >> 2), c = 2 * jb + ((lane & 3) >> 1);
+                    const uint32_t at = lds_addr_of(spare) + uint32_t(t * 128 + 16 * (c ^ (t & 7)) + 8 * (lane & 1));
+                    o.v[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_s16x4>(at));
+                }
+                *reinterpret_cast<u32x4*>(pt + uint64_t(r0 + 16 * jb + (lane & 15)) * Tp * (PLANES ? 2 : 1) + plane * Tp + q0 + 8 * g) =
+                    __builtin_bit_cast(u32x4, o);
+            }
+        }
+        asm volatile("" ::: "memory");  // and the reads before what is written next
+    }
     template <class Tile>
-    __device__ void tile(State&, Shared& sm, const g16::Lane& ln, f32x16 (&acc)[2][2], const Tile& t) {
-        const uint32_t r0 = t.rb * g16::TR;
+    __device__ void tile(State&, Shared& sm, const g16::Lane& ln, f32x16 (&acc)[2][2], const Tile& t, char* spare) {
+        const uint32_t r0 = t.rb * g16::TR, rw = r0 + uint32_t(ln.wr * 64);
+        const int swz = ln.l32 & 7;
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
-            const uint32_t q = t.qb * g16::TQ + uint32_t(ln.q(n));
             const float g = sm.gk[ln.q(n)], ref = sm.lse[ln.q(n)];
             const float c = PLANES ? a.scale * sm.inv_q[ln.q(n)] : a.scale;
             const uint32_t y = sm.target[ln.q(n)] - r0;
             const bool none = g == 0.0f || ref == -INFINITY;
+            const uint32_t q0 = t.qb * g16::TQ + uint32_t(ln.wq * 64 + 32 * n);
+            auto write = [&](int m, int j, const uint16_t (&v)[4]) {
+                *reinterpret_cast<uint2*>(spare + ln.l32 * 128 + 16 * ((4 * m + j) ^ swz) + 8 * ln.hh) =
+                    make_uint2(v[0] | uint32_t(v[1]) << 16, v[2] | uint32_t(v[3]) << 16);
+            };
 #pragma unroll
             for (int m = 0; m < 2; ++m)
 #pragma unroll
@@ -406,26 +472,28 @@ struct GradEpi {
                         float d = exp_diff(v[e], ref);
                         if (y == r + e && v[e] != -INFINITY) d -= 1.0f;
                         d = none ? 0.0f : d * g;
-                        if constexpr (PLANES) split16(d, hi[e], lo[e]);
-                        else hi[e] = bits16<BF16>(d);
-                    }
-                    // (a piece's rows are padded to whole 64-item stages: a group of 4 is inside or outside)
-                    if (p && q < a.rows && r0 + r < Vp) {
-                        uint16_t* o = p + uint64_t(q) * Vp * (PLANES ? 2 : 1) + r0 + r;
-                        *reinterpret_cast<uint2*>(o) = make_uint2(hi[0] | uint32_t(hi[1]) << 16, hi[2] | uint32_t(hi[3]) << 16);
-                        if constexpr (PLANES)
-                            *reinterpret_cast<uint2*>(o + Vp) =
-                                make_uint2(lo[0] | uint32_t(lo[1]) << 16, lo[2] | uint32_t(lo[3]) << 16);
-                    }
-                    if (pt && q < Tp) {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            uint16_t* o = pt + uint64_t(r0 + r + e) * Tp * (PLANES ? 2 : 1) + q;
-                            o[0] = hi[e];
-                            if constexpr (PLANES) o[Tp] = lo[e];
+                        if constexpr (PLANES) {
+                            split16(d, hi[e], lo[e]);
+                            acc[m][n][4 * j + e] = d;
+                        } else {
+                            hi[e] = bits16<BF16>(d);
                         }
                     }
+                    write(m, j, hi);
                 }
+            put(spare, ln, n, q0, rw, 0);
+            if constexpr (PLANES) {
+#pragma unroll
+                for (int m = 0; m < 2; ++m)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        uint16_t hi[4], lo[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) split16(acc[m][n][4 * j + e], hi[e], lo[e]);
+                        write(m, j, lo);
+                    }
+                put(spare, ln, n, q0, rw, 1);
+            }
         }
     }
     template <class Tile>
@@ -446,7 +514,7 @@ struct ShareEpi {
     __device__ void load(State&, const Tile&, int) {}
     __device__ void publish(State&, Shared&, int) {}
     template <class Tile>
-    __device__ void tile(State&, Shared&, const g16::Lane& ln, f32x16 (&acc)[2][2], const Tile& t) {
+    __device__ void tile(State&, Shared&, const g16::Lane& ln, f32x16 (&acc)[2][2], const Tile& t, char*) {
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
             const uint32_t q = t.qb * g16::TQ + uint32_t(ln.q(n));
@@ -492,7 +560,7 @@ struct ItemGradEpi {
         if (tid == 0) sm.mul = *mul / (DT == VA_DTYPE_F32 ? scale_to_2p14(__builtin_bit_cast(float, *absmax)) : 1.0f);
     }
     template <class Tile>
-    __device__ void tile(State&, Shared& sm, const g16::Lane& ln, f32x16 (&acc)[2][2], const Tile& t) {
+    __device__ void tile(State&, Shared& sm, const g16::Lane& ln, f32x16 (&acc)[2][2], const Tile& t, char*) {
         const float s = sm.mul;
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
