@@ -68,6 +68,18 @@ def test_single_rows_to_many_over_a_long_collection(ctx, T, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("T,V,D", [(260, 25_101, 520), (129, 49_200, 64), (513, 16_640, 300)])
+def test_large_tiles(ctx, T, V, D, dtype):
+    """Products of so many tiles that all of them take the largest."""
+    h, w, y, g = _inputs(T, V, D, dtype, V)
+    y[::7] = IGNORE
+    off = torch.randn(V, generator=g)
+    off[torch.rand(V, generator=g) < 0.1] = -torch.inf
+    off[y.cpu().clamp(min=0)] = 0.5
+    _check(ctx, h, w, y, scale=3.0, offsets=off.cuda())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("T", [3, 70])
 def test_offsets_and_masks(ctx, T, dtype):
     """Corrections; masked items that hold NaN and infinities; a masked target; the type's lowest value."""

@@ -1,14 +1,18 @@
-// va_gemm16.hpp — the matrix product of two row-major 16-bit operands over their common (row)
-// dimension, with the epilogue a template argument: every product of the softmax cross entropy
-// (va_xent.hip) is one of these.
+// va_gemm16.hpp — the matrix product of two 16-bit operands, with the epilogue a template argument:
+// every product of the softmax cross entropy (va_xent.hip) is one of these.
 //
-//   acc[q][r] = sum_k Q[q][k] X[r][k]        Q: [queries x pitch], X: [rows x pitch], fp16 or bf16
+//   acc[q][r] = sum_k Q[q][k] X[r][k]        fp16 or bf16
 //
-// One workgroup computes tiles of 256 queries x 256 rows with sixteen waves of 64 x 64 (2 x 2
-// blocks of v_mfma_f32_32x32x16, 64 fp32 accumulators a lane, four waves per SIMD).  64 k-values
-// of both operands move global -> LDS by direct loads into one of two 64 KiB slots while the
+// Either operand is stored with k along its rows (Q[q] is a row) or across them (k is the row: QK, XK).
+//
+// A wave computes 64 queries x 64 rows (2 x 2 blocks of v_mfma_f32_32x32x16, 64 fp32 accumulators a
+// lane), a workgroup WQ x WR such waves: 4 x 4 for large products (256 x 256, four waves per SIMD, one
+// workgroup a CU), fewer where tiles of that size would leave CUs without work.  64 k-values
+// of both operands move global -> LDS by direct loads into one of two slots while the
 // other is computed on; LDS rows are 128 bytes with their 16-byte chunks swizzled by the row, so
-// fragment reads are conflict-free.  The launch is persistent: a workgroup walks its tiles, and the
+// fragment reads are conflict-free.  An operand stored across k is staged as it lies, 64 rows of the
+// tile's width, and ds_read_tr16 turns it on the way into the fragments (a lane receives four k of one
+// column); its 64-byte segments are swizzled by k, so that four k-rows meet in no bank.  The launch is persistent: a workgroup walks its tiles, and the
 // next tile's first stage streams in during the epilogue.
 //
 // Operands of fp32 values come as two fp16 planes (value = (hi + lo) 2^-e with one exponent a row
@@ -16,6 +20,8 @@
 // accumulators.  lo lo is below 2^-22 of the product and is left out; what remains is exact to
 // about 2^-22 a term, the same as an fp32 fma chain of a few terms.
 #pragma once
+
+#include <algorithm>
 
 #include "va_internal.hpp"
 
@@ -28,24 +34,33 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
-constexpr int TQ = 256, TR = 256, KC = 64, WAVES = 16;
-constexpr int ROWB = KC * 2;                 // bytes of an LDS row
-constexpr int OPB = TQ * ROWB;               // bytes of one operand's stage
-constexpr int STAGE = 2 * OPB;
-constexpr int LDS_BYTES = 2 * STAGE;
-constexpr int LPW = OPB / 1024 / WAVES;      // 1 KiB direct loads per wave, operand and stage
+constexpr int KC = 64;
+constexpr int ROWB = KC * 2;  // bytes of an LDS row (k along the rows)
+
+template <int WQ_, int WR_>
+struct Shape {
+    static constexpr int WQ = WQ_, WR = WR_, WAVES = WQ * WR, THREADS = 64 * WAVES;
+    static constexpr int TQ = 64 * WQ, TR = 64 * WR;
+    static constexpr int QB = TQ * ROWB, XB = TR * ROWB, STAGE = QB + XB, LDS = 2 * STAGE;
+    // waves per SIMD that the registers allow for: all of a CU's (16 waves), or two workgroups' and more
+    static constexpr int PER_SIMD = WAVES == 16 ? 4 : 2;
+    static_assert(THREADS >= TQ && THREADS >= TR, "one thread per query and row");
+    static_assert(WAVES * 4096 <= STAGE, "the epilogue's LDS fits in one slot");
+};
+using Large = Shape<4, 4>;
 
 struct Operand {
-    const void* p = nullptr;  // row 0
-    uint64_t pitch = 0;       // bytes between rows (a multiple of 16)
-    uint32_t rows = 0;
-    uint32_t plane = 0;       // bytes from a row's hi plane to its lo plane (PLANES only)
+    const void* p = nullptr;   // row 0
+    uint64_t pitch = 0;        // bytes between rows (a multiple of 16)
+    uint32_t rows = 0;         // k along the rows: queries (rows) of the product; across: values of k
+    uint32_t width = 0;        // bytes of a row (k along the rows: whole stages; else a multiple of 16)
+    uint32_t plane = 0;        // bytes from a row's hi plane to its lo plane (PLANES only)
 };
 
 struct Args {
     Operand q, x;
-    uint32_t kstages = 0;  // stages of 64 k-values of one plane (rows are zero-padded to them)
-    uint32_t nq = 0, nr = 0;  // blocks of 256
+    uint32_t kstages = 0;  // stages of 64 k-values of one plane (operands are zero-padded to them)
+    uint32_t nq = 0, nr = 0;  // blocks of the shape's queries and rows
     uint32_t parts = 1;  // walk: workgroups per query block; tiles: shares of the k-stages
 };
 
@@ -124,43 +139,129 @@ struct Lane {
     __device__ int r(int m, int j) const { return wr * 64 + 32 * m + 8 * j + 4 * hh; }
 };
 
+// One operand's way into LDS and out of it: W waves along it, of WAVES in the workgroup.  KM: stored
+// across k.
+template <bool KM, bool PLANES, int W, int WAVES>
+struct Feed {
+    static constexpr int LPW = 8 * W / WAVES;       // 1 KiB direct loads per wave and stage
+    static constexpr int KROW = 128 * W;            // bytes of a k-row (KM)
+    static constexpr uint32_t SEGX = W == 1 ? 1 : 3;  // the segment is xored by (k >> SEGS) & SEGX
+    static constexpr uint32_t SEGS = W == 1 ? 1 : 0;
+    const char* base;  // of the tile
+    uint32_t records;  // bytes behind it (k along the rows)
+    uint64_t left;     // (KM)
+    uint32_t pitch, plane;
+    uint32_t voff[LPW];
+    uint32_t lds_at;   // of the wave's first load, within a stage
+    uint32_t frag[KM ? 2 : 1];  // fragment addresses within a stage
+    int swz, hh;
+
+    // Direct loads: wave w fills the 1 KiB groups g = w + WAVES i.  k along the rows: rows 8 g .. 8 g + 7, lane
+    // L row 8 g + L / 8, physical chunk L % 8 = logical chunk (L % 8) ^ ((row >> 1) & 7).  Across: whole k-rows,
+    // each lane one 16-byte chunk, the chunk's segment (four chunks) xored.  Rows past the operand's last one
+    // lie past its descriptor and land as zeros.
+    __device__ void init(const Operand& o, int wave, int lane, uint32_t at, int wtile) {
+        pitch = uint32_t(o.pitch);
+        plane = PLANES ? o.plane : 0;
+        lds_at = at + uint32_t(wave) * 1024u;
+        const int l32 = lane & 31;
+        hh = lane >> 5;
+        if constexpr (KM) {
+#pragma unroll
+            for (int i = 0; i < LPW; ++i) {
+                const uint32_t byte = uint32_t(1024 * (wave + WAVES * i) + 16 * lane);
+                const uint32_t k = byte / KROW, c = byte % KROW / 16;
+                voff[i] = k * pitch + 16u * ((((c >> 2) ^ ((k >> SEGS) & SEGX)) << 2) | (c & 3u));
+            }
+            const int e = (lane & 15) >> 2;
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+                frag[n] = at + uint32_t((8 * hh + e) * KROW + (((2 * wtile + n) ^ ((e >> SEGS) & SEGX)) << 6) + 32 * ((lane >> 4) & 1) + 8 * (lane & 3));
+        } else {
+#pragma unroll
+            for (int i = 0; i < LPW; ++i) {
+                const uint32_t row = uint32_t(8 * (wave + WAVES * i) + (lane >> 3));
+                voff[i] = row * pitch + 16u * uint32_t((lane & 7) ^ ((row >> 1) & 7));
+            }
+            frag[0] = at + uint32_t((wtile * 64 + l32) * ROWB);
+            swz = (l32 >> 1) & 7;
+        }
+    }
+    // the operand's block b of 64 W queries (rows)
+    __device__ void open(const Operand& o, uint32_t b) {
+        if constexpr (KM) {
+            base = static_cast<const char*>(o.p) + b * uint32_t(KROW);
+            left = (o.rows - 1) * o.pitch + o.width - b * uint32_t(KROW);
+        } else {
+            base = static_cast<const char*>(o.p) + uint64_t(b) * (64u * W) * o.pitch;
+            records = (min(64u * W, o.rows - b * (64u * W)) - 1u) * pitch + o.width + plane;
+        }
+    }
+    // stage k (of the plane `lo`) into the slot at LDS address `slot`; !ok: zeros
+    __device__ void issue(uint32_t k, bool lo, bool ok, uint32_t slot) const {
+        if constexpr (KM) {
+            const uint64_t skip = uint64_t(k) * KC * pitch;
+            const dma_rsrc r = make_dma_rsrc(base + skip + (lo ? plane : 0u),
+                                             ok && skip < left ? uint32_t(min(left - skip, uint64_t(kDmaMaxBytes))) : 0u);
+#pragma unroll
+            for (int i = 0; i < LPW; ++i) lds_dma16(r, voff[i], slot + lds_at + uint32_t(1024 * WAVES * i));
+        } else {
+            const dma_rsrc r = make_dma_rsrc(base, records);
+            const uint32_t so = ok ? k * uint32_t(ROWB) + (lo ? plane : 0u) : 0u;
+#pragma unroll
+            for (int i = 0; i < LPW; ++i) lds_dma16_so(r, ok ? voff[i] : kDmaSkip, so, slot + lds_at + uint32_t(1024 * WAVES * i));
+        }
+    }
+    // the fragment of the wave's 32-query (row) block n, k-step t of the slot
+    __device__ u32x4 read(const char* slot, int n, int t) const {
+        if constexpr (KM) {
+            typedef short s16x4 __attribute__((ext_vector_type(4)));
+            typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
+            struct alignas(16) {
+                s16x4 v[2];
+            } o;
+            const uint32_t at = lds_addr_of(slot) + frag[n] + uint32_t(t * 16 * KROW);
+            o.v[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_s16x4>(at));
+            o.v[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_s16x4>(at + 4 * KROW));
+            return __builtin_bit_cast(u32x4, o);
+        } else {
+            return *reinterpret_cast<const u32x4*>(slot + frag[0] + n * 32 * ROWB + 16 * ((2 * t + hh) ^ swz));
+        }
+    }
+};
+
 // Epi: struct with
-//   static constexpr bool kWalk
+//   Shape, static constexpr bool kWalk
 //   struct State (per thread, lives through the main loop)
 //   begin(State&, smem, tile)   a new item's first tile (barriers follow before the epilogue)
 //   load(State&, tile, tid)     before the main loop: starts what the tile's epilogue reads
 //   publish(State&, smem, tid)  after the main loop, before the barrier
 //   tile(State&, smem, lane, acc, tile, spare)  spare: 4 KiB of LDS of the wave's own
 //   end(State&, smem, lane, tile)  after an item's last tile
-template <bool BF16, bool PLANES, class Epi>
-__global__ __launch_bounds__(64 * WAVES, 4) void gemm16_kernel(Args a, Epi epi) {
+template <bool BF16, bool PLANES, bool QK, bool XK, class Epi>
+__global__ __launch_bounds__(Epi::Shape::THREADS, Epi::Shape::PER_SIMD) void gemm16_kernel(Args a, Epi epi) {
+    using Sh = typename Epi::Shape;
+    constexpr int STAGE = Sh::STAGE;
     extern __shared__ __attribute__((aligned(1024))) char lds[];
     __shared__ typename Epi::Shared smem;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const Lane ln{wave & 3, wave >> 2, lane & 31, lane >> 5};
+    const Lane ln{wave % Sh::WQ, wave / Sh::WQ, lane & 31, lane >> 5};
 
     Tiles<Epi::kWalk> tile;
     tile.first(a);
     if (!tile.ok) return;
 
-    // Direct loads: wave w fills the 1 KiB groups g = w + 16 i (rows 8 g .. 8 g + 7) of each operand;
-    // lane L loads row 8 g + L / 8, physical chunk L % 8 = logical chunk (L % 8) ^ ((row >> 1) & 7).
-    // Rows past the operand's last one lie past its descriptor and land as zeros.
-    const uint32_t qpitch = uint32_t(a.q.pitch), xpitch = uint32_t(a.x.pitch);
-    const uint32_t row0 = uint32_t(8 * wave + (lane >> 3));
-    const uint32_t ch = 16u * uint32_t((lane & 7) ^ ((row0 >> 1) & 7));  // 8 * 16 rows on: the same swizzle
     const uint32_t total_stages = PLANES ? 3 * a.kstages : a.kstages;
-    const uint32_t kbytes = a.kstages * uint32_t(ROWB);
     const uint32_t lds0 = lds_addr_of(lds);
-    dma_rsrc qres, xres;
+    Feed<QK, PLANES, Sh::WQ, Sh::WAVES> fq_;
+    Feed<XK, PLANES, Sh::WR, Sh::WAVES> fx_;
+    fq_.init(a.q, wave, lane, 0, ln.wq);
+    fx_.init(a.x, wave, lane, Sh::QB, ln.wr);
     uint32_t s0, s1;  // the tile's stages
     auto open = [&]() {
-        const uint32_t q0 = tile.qb * TQ, r0 = tile.rb * TR;
-        qres = make_dma_rsrc(static_cast<const char*>(a.q.p) + q0 * a.q.pitch,
-                             (min(uint32_t(TQ), a.q.rows - q0) - 1u) * qpitch + kbytes + (PLANES ? a.q.plane : 0u));
-        xres = make_dma_rsrc(static_cast<const char*>(a.x.p) + r0 * a.x.pitch,
-                             (min(uint32_t(TR), a.x.rows - r0) - 1u) * xpitch + kbytes + (PLANES ? a.x.plane : 0u));
+        fq_.open(a.q, tile.qb);
+        fx_.open(a.x, tile.rb);
         if constexpr (Epi::kWalk) {
             s0 = 0;
             s1 = total_stages;
@@ -172,45 +273,36 @@ __global__ __launch_bounds__(64 * WAVES, 4) void gemm16_kernel(Args a, Epi epi) 
     // stage s of the tile into slot `slot` (past the last stage: zeros)
     auto issue = [&](uint32_t s, uint32_t slot) {
         const bool ok = s < s1;
-        uint32_t qo, xo;
-        if constexpr (PLANES) {
-            const uint32_t seg = s / a.kstages, k = (s - seg * a.kstages) * uint32_t(ROWB);
-            qo = k + (seg == 2 ? a.q.plane : 0u);
-            xo = k + (seg == 1 ? a.x.plane : 0u);
-        } else {
-            qo = xo = s * uint32_t(ROWB);
-        }
-        const uint32_t sb = lds0 + slot * uint32_t(STAGE) + uint32_t(wave) * 1024u;
-#pragma unroll
-        for (int i = 0; i < LPW; ++i) {
-            const uint32_t row = row0 + uint32_t(8 * WAVES * i), at = sb + uint32_t(1024 * WAVES * i);
-            lds_dma16_so(qres, ok ? row * qpitch + ch : kDmaSkip, ok ? qo : 0u, at);
-            lds_dma16_so(xres, ok ? row * xpitch + ch : kDmaSkip, ok ? xo : 0u, at + uint32_t(OPB));
-        }
+        const uint32_t k = PLANES ? s / 3u : s, seg = PLANES ? s - 3u * k : 0u;  // (a k's planes are read together)
+        const uint32_t sb = lds0 + slot * uint32_t(STAGE);
+        fq_.issue(k, seg == 2, ok, sb);
+        fx_.issue(k, seg == 1, ok, sb);
     };
 
-    const int swz = (ln.l32 >> 1) & 7;
-    const uint32_t q_at = uint32_t((ln.wq * 64 + ln.l32) * ROWB), x_at = uint32_t(OPB + (ln.wr * 64 + ln.l32) * ROWB);
     f32x16 acc[2][2];
     u32x4 fx[2][2], fq[2][2];
     auto read_frags = [&](int buf, uint32_t slot, int t) {
         const char* base = lds + slot * STAGE;
-        const uint32_t ko = 16u * uint32_t((2 * t + ln.hh) ^ swz);
 #pragma unroll
-        for (int m = 0; m < 2; ++m) fx[buf][m] = *reinterpret_cast<const u32x4*>(base + x_at + m * 32 * ROWB + ko);
+        for (int m = 0; m < 2; ++m) fx[buf][m] = fx_.read(base, m, t);
 #pragma unroll
-        for (int n = 0; n < 2; ++n) fq[buf][n] = *reinterpret_cast<const u32x4*>(base + q_at + n * 32 * ROWB + ko);
+        for (int n = 0; n < 2; ++n) fq[buf][n] = fq_.read(base, n, t);
     };
     auto mma = [&](int buf) {
 #pragma unroll
         for (int m = 0; m < 2; ++m)
 #pragma unroll
             for (int n = 0; n < 2; ++n) acc[m][n] = mfma<BF16>(fx[buf][m], fq[buf][n], acc[m][n]);
-        // the next k-step's four fragment reads go between the four MFMAs
+        // the next k-step's fragment reads (two a fragment across k) go between the four MFMAs
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < 2; ++i) {
             __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, XK ? 2 : 1, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, QK ? 2 : 1, 0);
         }
     };
     // a workgroup barrier that leaves the direct loads in flight; this wave's LDS reads are done
@@ -230,7 +322,7 @@ __global__ __launch_bounds__(64 * WAVES, 4) void gemm16_kernel(Args a, Epi epi) 
                 for (int v = 0; v < 16; ++v) acc[m][n][v] = 0.0f;
         barrier();  // every wave is past the previous tile's main loop: slot 1 is free
         issue(s0 + 1, 1);
-        wait_vmcnt<2 * LPW>();  // stage 0 (older than stage 1's loads)
+        wait_vmcnt<8 / Sh::WQ + 8 / Sh::WR>();  // stage 0 (older than stage 1's loads)
         barrier();
         read_frags(0, 0, 0);
         const uint32_t ns = s1 - s0;
@@ -273,19 +365,31 @@ __global__ __launch_bounds__(64 * WAVES, 4) void gemm16_kernel(Args a, Epi epi) 
     wait_vmcnt<0>();
 }
 
-// Persistent launch: one workgroup per CU (the LDS of a tile fills one), a multiple of the XCDs.
-template <bool BF16, bool PLANES, class Epi>
+// Workgroups of a shape that a CU holds: its LDS (with up to 2 KiB of the epilogue's beside two slots; the
+// largest shape is alone anyway), its registers, its 32 waves.
+template <class Sh>
+constexpr uint32_t per_cu() {
+    constexpr uint32_t lds = 163840 / (Sh::LDS + 2048), waves = 4 * Sh::PER_SIMD / Sh::WAVES;
+    return std::max(std::min(lds, waves), 1u);
+}
+// Persistent launch: as many workgroups as the chip holds, a multiple of the XCDs.
+template <class Sh>
+uint32_t grid_max(const va_context* ctx) {
+    return std::max(uint32_t(ctx->num_cus), kXcds) / kXcds * kXcds * per_cu<Sh>();
+}
+template <bool BF16, bool PLANES, bool QK, bool XK, class Epi>
 va_status launch(va_context* ctx, const Args& a, const Epi& epi) {
+    using Sh = typename Epi::Shape;
+    static_assert(sizeof(typename Epi::Shared) + Sh::LDS <= 163840, "a workgroup's LDS");
     const uint64_t tiles = uint64_t(a.nq) * (Epi::kWalk ? a.parts : a.nr * uint64_t(a.parts));
     if (tiles == 0) return VA_OK;
     if (tiles > 0x7FFFFFF0ull || 256 * std::max(a.q.pitch, a.x.pitch) > kDmaMaxBytes)
         return fail(ctx, VA_ERR_INVALID_ARG, "matrix product too large: %llu tiles, rows of %llu and %llu bytes",
                     (unsigned long long)tiles, (unsigned long long)a.q.pitch, (unsigned long long)a.x.pitch);
-    const uint64_t cus = std::max<uint64_t>(uint64_t(ctx->num_cus), kXcds) / kXcds * kXcds;
-    const uint64_t grid = std::min((tiles + kXcds - 1) / kXcds * kXcds, cus);
-    auto kern = &gemm16_kernel<BF16, PLANES, Epi>;
-    VA_CHECK_HIP(ctx, hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, LDS_BYTES));
-    kern<<<dim3(uint32_t(grid)), dim3(64 * WAVES), LDS_BYTES, ctx->stream>>>(a, epi);
+    const uint64_t grid = std::min<uint64_t>((tiles + kXcds - 1) / kXcds * kXcds, grid_max<Sh>(ctx));
+    auto kern = &gemm16_kernel<BF16, PLANES, QK, XK, Epi>;
+    VA_CHECK_HIP(ctx, hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, Sh::LDS));
+    kern<<<dim3(uint32_t(grid)), dim3(Sh::THREADS), Sh::LDS, ctx->stream>>>(a, epi);
     VA_CHECK_LAUNCH(ctx);
     return VA_OK;
 }

@@ -7,7 +7,7 @@
 // Forward: one product (va_gemm16.hpp) whose epilogue keeps, per row, the running maximum m and
 // z = sum exp(l - m) of the items seen; the workgroups' (m, z) are joined by the finishing kernel.  Backward: the items are taken in
 // pieces; for each piece the logits are computed again, dl leaves the product's epilogue as 16-bit
-// values in a bounded workspace, in both orders, and two more products read it: dh accumulates over
+// values in a bounded workspace, and two more products read it, along its rows and across them: dh accumulates over
 // the pieces in fp32, dw's rows of the piece are final.  So a training step is four products (one
 // of them the recomputation), and the memory is that of one piece.
 //
@@ -92,124 +92,109 @@ __device__ __forceinline__ void join(float& m, float& z, float m2, float z2) {
     m = mm;
 }
 
-// ---- packing: operands whose rows are not whole 64-value stages, or not 16-bit ---------------------
-// dst[r][k] = src[r][k], zeros for k in [D, Kp)
+// ---- packing: operands whose rows are not whole 64-value stages, not 16-bit, or must not be read -----
+// dst[r][k] = src[r][k], zeros for k in [D, Kp); rows whose drop value says so are zeros
 __global__ __launch_bounds__(256) void pack16_kernel(const uint16_t* __restrict__ src, uint64_t ld, uint32_t D, uint32_t Kp,
-                                                     uint16_t* __restrict__ dst, uint64_t n8) {
+                                                     const float* __restrict__ drop, float drop_if, uint16_t* __restrict__ dst, uint64_t n8) {
+    typedef uint16_t u16x8 __attribute__((ext_vector_type(8), aligned(2)));
+    const uint32_t per = Kp / 8;
     for (uint64_t i = uint64_t(blockIdx.x) * 256 + threadIdx.x; i < n8; i += uint64_t(gridDim.x) * 256) {
-        const uint32_t per = Kp / 8;
         const uint64_t r = i / per;
         const uint32_t k = uint32_t(i - r * per) * 8;
-        uint16_t v[8];
+        u16x8 v = {};
         const uint16_t* s = src + r * ld + k;
+        if (!(drop && drop[r] == drop_if)) {
+            if (k + 8 <= D) {
+                v = *reinterpret_cast<const u16x8*>(s);
+            } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = k + e < D ? s[e] : uint16_t(0);
-        u32x4 o;
-        __builtin_memcpy(&o, v, 16);
-        *reinterpret_cast<u32x4*>(dst + r * Kp + k) = o;
+                for (int e = 0; e < 8; ++e) v[e] = k + e < D ? s[e] : uint16_t(0);
+            }
+        }
+        *reinterpret_cast<u32x4*>(dst + r * Kp + k) = __builtin_bit_cast(u32x4, v);
     }
 }
 
 // One wave per fp32 row: its planes dst[r] = {hi, lo} (Kp values each, zeros past D), scaled by the
-// power of two that puts its largest entry near 2^14; inv[r] = the inverse.
-__global__ __launch_bounds__(256) void pack32_kernel(const float* __restrict__ src, uint64_t ld, uint32_t R, uint32_t D,
-                                                     uint32_t Kp, uint16_t* __restrict__ dst, float* __restrict__ inv) {
+// power of two that puts the row's largest entry, or the tensor's (absmax), near 2^14; inv[r] = the
+// inverse.  Rows whose drop value says so are zeros.
+__global__ __launch_bounds__(256) void pack32_kernel(const float* __restrict__ src, uint64_t ld, uint32_t R, uint32_t D, uint32_t Kp,
+                                                     const uint32_t* __restrict__ absmax, const float* __restrict__ drop, float drop_if,
+                                                     uint16_t* __restrict__ dst, float* __restrict__ inv) {
+    typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
     const int lane = threadIdx.x & 63;
     const uint32_t r = blockIdx.x * 4 + (threadIdx.x >> 6);
     if (r >= R) return;
     const float* s = src + r * ld;
-    float m = 0.0f;
-    for (uint32_t k = lane; k < D; k += 64) m = fmaxf(m, fabsf(s[k]));
-    const float sc = scale_to_2p14(wave_max(m));
+    const bool none = drop && drop[r] == drop_if;
+    auto load4 = [&](uint32_t k) {
+        f32x4 v{0.0f, 0.0f, 0.0f, 0.0f};
+        if (none) return v;
+        if (k + 4 <= D) return f32x4(*reinterpret_cast<const f32x4u*>(s + k));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = k + e < D ? s[k + e] : 0.0f;
+        return v;
+    };
+    // up to 1024 values of the row stay in registers between the two passes
+    f32x4 held[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) held[i] = load4(256 * i + 4 * lane);
+    float sc;
+    if (absmax) {
+        sc = scale_to_2p14(__builtin_bit_cast(float, *absmax));
+    } else {
+        float m = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) m = fmaxf(m, fabsf(held[i][e]));
+        for (uint32_t k = 1024 + 4 * lane; k < D; k += 256) {
+            const f32x4 v = load4(k);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) m = fmaxf(m, fabsf(v[e]));
+        }
+        sc = scale_to_2p14(wave_max(m));
+    }
     if (lane == 0) inv[r] = 1.0f / sc;
     uint16_t* o = dst + uint64_t(r) * 2 * Kp;
-    for (uint32_t k = 2 * lane; k < Kp; k += 128) {
-        uint16_t h0, l0, h1, l1;
-        split16(k < D ? s[k] * sc : 0.0f, h0, l0);
-        split16(k + 1 < D ? s[k + 1] * sc : 0.0f, h1, l1);
-        *reinterpret_cast<uint32_t*>(o + k) = h0 | uint32_t(h1) << 16;
-        *reinterpret_cast<uint32_t*>(o + Kp + k) = l0 | uint32_t(l1) << 16;
+    auto put = [&](uint32_t k, f32x4 v) {
+        uint16_t h[4], l[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) split16(v[e] * sc, h[e], l[e]);
+        *reinterpret_cast<uint2*>(o + k) = make_uint2(h[0] | uint32_t(h[1]) << 16, h[2] | uint32_t(h[3]) << 16);
+        *reinterpret_cast<uint2*>(o + Kp + k) = make_uint2(l[0] | uint32_t(l[1]) << 16, l[2] | uint32_t(l[3]) << 16);
+    };
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t k = 256 * i + 4 * lane;
+        if (k < Kp) put(k, held[i]);
     }
+    for (uint32_t k = 1024 + 4 * lane; k < Kp; k += 256) put(k, load4(k));
 }
 
 // out = the bits of the largest |src| (0 before the launch); rows whose drop value says so are left out
 __global__ __launch_bounds__(256) void absmax_kernel(const float* __restrict__ src, uint64_t ld, uint32_t R, uint32_t D,
                                                      const float* __restrict__ drop, float drop_if, uint32_t* out) {
+    typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
     __shared__ float part[4];
     float m = 0.0f;
     const int lane = threadIdx.x & 63;
     for (uint32_t r = blockIdx.x * 4 + (threadIdx.x >> 6); r < R; r += gridDim.x * 4) {
         if (drop && drop[r] == drop_if) continue;
         const float* s = src + r * ld;
-        for (uint32_t k = lane; k < D; k += 64) m = fmaxf(m, fabsf(s[k]));
+        const uint32_t full = D / 4 * 4;
+#pragma unroll 4
+        for (uint32_t k = 4 * lane; k < full; k += 256) {
+            const f32x4 v = *reinterpret_cast<const f32x4u*>(s + k);
+            m = fmaxf(fmaxf(m, fmaxf(fabsf(v[0]), fabsf(v[1]))), fmaxf(fabsf(v[2]), fabsf(v[3])));
+        }
+        if (full + lane < D) m = fmaxf(m, fabsf(s[full + lane]));
     }
     m = wave_max(m);
     if (lane == 0) part[threadIdx.x >> 6] = m;
     __syncthreads();
     if (threadIdx.x == 0)
         atomicMax(out, __builtin_bit_cast(uint32_t, fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]))));
-}
-
-// dst[d][r] = src[r][d] for r < R, zeros for r in [R, Rp); rows whose drop value says so are zeros.
-// fp32: two planes (lo behind hi's Rp values), scaled by the tensor's power of two (absmax).
-// 64 x 64 tiles through LDS, laid out as GradEpi's: 8 values a thread and load, and 8 a store.
-template <int DT>
-__global__ __launch_bounds__(256) void transpose_kernel(const ElemT<DT>* __restrict__ src, uint64_t ld, uint32_t R, uint32_t D,
-                                                        uint32_t Rp, const float* __restrict__ drop, float drop_if,
-                                                        const uint32_t* __restrict__ absmax, uint16_t* __restrict__ dst) {
-    constexpr bool kF32 = DT == VA_DTYPE_F32;
-    constexpr int PL = kF32 ? 2 : 1;
-    typedef ElemT<DT> in8 __attribute__((ext_vector_type(8), aligned(sizeof(ElemT<DT>))));
-    typedef short s16x4 __attribute__((ext_vector_type(4)));
-    typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
-    __shared__ __attribute__((aligned(16))) char tile[PL][64 * 128];
-    const uint32_t r0 = blockIdx.x * 64, d0 = blockIdx.y * 64;
-    const int tid = threadIdx.x;
-    const float sc = kF32 ? scale_to_2p14(__builtin_bit_cast(float, *absmax)) : 1.0f;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int rl = (tid >> 3) + 32 * i, c = tid & 7;
-        const uint32_t r = r0 + rl, d = d0 + 8 * c;
-        uint16_t h[8] = {}, l[8] = {};
-        if (r < R && d < D && !(drop && drop[r] == drop_if)) {
-            const ElemT<DT>* s = src + uint64_t(r) * ld + d;
-            ElemT<DT> v[8];
-            if (d + 8 <= D) {
-                const in8 w = *reinterpret_cast<const in8*>(s);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = w[e];
-            } else {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = d + e < D ? s[e] : ElemT<DT>(0.0f);
-            }
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                if constexpr (kF32) split16(v[e] * sc, h[e], l[e]);
-                else h[e] = __builtin_bit_cast(uint16_t, v[e]);
-            }
-        }
-        __builtin_memcpy(tile[0] + rl * 128 + 16 * (c ^ (rl & 7)), h, 16);
-        if constexpr (kF32) __builtin_memcpy(tile[PL - 1] + rl * 128 + 16 * (c ^ (rl & 7)), l, 16);
-    }
-    __syncthreads();
-    // wave w takes the d-values 16 w .. 16 w + 15 of the tile: lane (i, g) d 16 w + i, r 8 g .. and 32 + 8 g ..
-    const int lane = tid & 63, w = tid >> 6, g = lane >> 4;
-    const uint32_t d = d0 + uint32_t(16 * w + (lane & 15));
-#pragma unroll
-    for (int pl = 0; pl < PL; ++pl)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            struct alignas(16) {
-                s16x4 v[2];
-            } o;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int r = 32 * i + 8 * g + 4 * h + ((lane & 15) >> 2), c = 2 * w + ((lane & 3) >> 1);
-                const uint32_t at = lds_addr_of(tile[pl]) + uint32_t(r * 128 + 16 * (c ^ (r & 7)) + 8 * (lane & 1));
-                o.v[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_s16x4>(at));
-            }
-            if (d < D) *reinterpret_cast<u32x4*>(dst + (uint64_t(d) * PL + pl) * Rp + r0 + 32 * i + 8 * g) = __builtin_bit_cast(u32x4, o);
-        }
 }
 
 // ---- the logits' epilogues -------------------------------------------------------------------------
@@ -223,13 +208,13 @@ struct LogitArgs {
 
 // What the epilogue needs of a tile's items, and the logit of one accumulator.  OFF: there are
 // offsets, or the last tile is not whole (its missing items get offset -inf).
-template <bool OFF, bool PLANES>
+template <bool OFF, bool PLANES, int TR>
 struct LogitShared {
-    float off[OFF ? g16::TR : 1];
-    float inv[PLANES ? g16::TR : 1];
+    float off[OFF ? TR : 1];
+    float inv[PLANES ? TR : 1];
 };
-template <bool OFF, bool PLANES>
-__device__ __forceinline__ f32x4 logits4(const LogitShared<OFF, PLANES>& sm, const f32x16& acc, int j, int r, float c) {
+template <bool OFF, bool PLANES, int TR>
+__device__ __forceinline__ f32x4 logits4(const LogitShared<OFF, PLANES, TR>& sm, const f32x16& acc, int j, int r, float c) {
     f32x4 v;
     f32x4 o{}, x{};
     asm volatile("" ::: "memory");  // these reads stay here: hoisted, a tile's would fill the registers
@@ -253,8 +238,10 @@ __device__ __forceinline__ float exp_diff(float v, float ref) { return __builtin
 // the item and written to part[row * slots + slot].  The target's logit is picked out on the way: with
 // the loss a difference of two logits, both from the same sums, their errors cancel for a row whose
 // target is far ahead of the other items.
-template <bool OFF, bool PLANES>
+template <class Sh, bool OFF, bool PLANES>
 struct LseEpi {
+    using Shape = Sh;
+    static constexpr int TQ = Sh::TQ, TR = Sh::TR;
     static constexpr bool kWalk = true;
     LogitArgs a;
     const int64_t* targets;
@@ -262,10 +249,10 @@ struct LseEpi {
     float* picked;   // [rows] the target's logit
     float2* part;
     uint32_t slots, slot0;
-    struct Shared : LogitShared<OFF, PLANES> {
-        float2 red[4][g16::TQ];
-        uint32_t target[g16::TQ];  // within the launch's items (any larger value: elsewhere)
-        float qinv[PLANES ? g16::TQ : 1];
+    struct Shared : LogitShared<OFF, PLANES, TR> {
+        float2 red[Sh::WR][TQ];
+        uint32_t target[TQ];  // within the launch's items (any larger value: elsewhere)
+        float qinv[PLANES ? TQ : 1];
     };
     struct State {
         float m[2], z[2];
@@ -278,24 +265,24 @@ struct LseEpi {
             s.m[n] = -INFINITY;
             s.z[n] = 0.0f;
         }
-        const uint32_t i = threadIdx.x, q = t.qb * g16::TQ + i;
-        if (i >= uint32_t(g16::TQ)) return;
+        const uint32_t i = threadIdx.x, q = t.qb * TQ + i;
+        if (i >= uint32_t(TQ)) return;
         const int64_t y = q < a.rows ? targets[q] - int64_t(item0) : -1;
         sm.target[i] = y >= 0 && y < int64_t(a.items) ? uint32_t(y) : 0xFFFFFFFFu;
         if constexpr (PLANES) sm.qinv[i] = q < a.rows ? a.qinv[q] : 0.0f;
     }
     template <class Tile>
     __device__ void load(State& s, const Tile& t, int tid) {
-        const uint32_t r = t.rb * g16::TR + uint32_t(tid);
-        const bool in = tid < g16::TR && r < a.items;
+        const uint32_t r = t.rb * TR + uint32_t(tid);
+        const bool in = tid < TR && r < a.items;
         if constexpr (OFF) s.off = !in ? -INFINITY : a.offsets ? a.offsets[r] : 0.0f;
         if constexpr (PLANES) s.inv = in ? a.xinv[r] : 0.0f;
     }
     __device__ void publish(State& s, Shared& sm, int tid) {
         if constexpr (OFF)
-            if (tid < g16::TR) sm.off[tid] = s.off;
+            if (tid < TR) sm.off[tid] = s.off;
         if constexpr (PLANES)
-            if (tid < g16::TR) sm.inv[tid] = s.inv;
+            if (tid < TR) sm.inv[tid] = s.inv;
     }
     template <class Tile>
     __device__ void tile(State& s, Shared& sm, const g16::Lane& ln, f32x16 (&acc)[2][2], const Tile& t, char*) {
@@ -307,7 +294,7 @@ struct LseEpi {
             for (int m = 0; m < 2; ++m)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    f32x4 v = logits4<OFF, PLANES>(sm, acc[m][n], j, ln.r(m, j), c);
+                    f32x4 v = logits4<OFF, PLANES, TR>(sm, acc[m][n], j, ln.r(m, j), c);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         top = fmaxf(top, v[e]);
@@ -318,7 +305,7 @@ struct LseEpi {
             const float ref = mm == -INFINITY ? 0.0f : mm;
             const float z = s.z[n] * exp_diff(s.m[n], ref);
             // (a tile holds the target of few rows, most tiles of none of a wave's)
-            const uint32_t y = sm.target[ln.q(n)] - t.rb * g16::TR - uint32_t(ln.wr * 64);
+            const uint32_t y = sm.target[ln.q(n)] - t.rb * TR - uint32_t(ln.wr * 64);
             if (__any(y < 64u)) {
                 const uint32_t i = y - 4u * uint32_t(ln.hh);  // 32 m + 8 j + e of the lane's values
                 float v = 0.0f;
@@ -326,7 +313,7 @@ struct LseEpi {
                 for (int m = 0; m < 2; ++m)
 #pragma unroll
                     for (int k = 0; k < 16; ++k) v = i == uint32_t(32 * m + 8 * (k >> 2) + (k & 3)) ? acc[m][n][k] : v;
-                if (y < 64u && (i & 4u) == 0u) picked[t.qb * g16::TQ + ln.q(n)] = v;
+                if (y < 64u && (i & 4u) == 0u) picked[t.qb * TQ + ln.q(n)] = v;
             }
             float zz[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -346,22 +333,22 @@ struct LseEpi {
         }
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
         const uint32_t q = threadIdx.x;
-        if (q < uint32_t(g16::TQ) && t.qb * g16::TQ + q < a.rows) {
+        if (q < uint32_t(TQ) && t.qb * TQ + q < a.rows) {
             float2 v = sm.red[0][q];
 #pragma unroll
-            for (int w = 1; w < 4; ++w) join(v.x, v.y, sm.red[w][q].x, sm.red[w][q].y);
-            part[uint64_t(t.qb * g16::TQ + q) * slots + slot0 + t.part] = v;
+            for (int w = 1; w < Sh::WR; ++w) join(v.x, v.y, sm.red[w][q].x, sm.red[w][q].y);
+            part[uint64_t(t.qb * TQ + q) * slots + slot0 + t.part] = v;
         }
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
     }
 };
 
-// Backward: dl of the piece's items, in both orders (either may be absent):
-//   p[t][j]  rows of Vp values a plane (zeros past the last item), the query operand of dh
-//   pt[j][t] rows of Tp values a plane (zeros past the last row), the query operand of dw; whole
-//            tiles of 256 items
-template <bool BF16, bool OFF, bool PLANES>
+// Backward: dl of the piece's items, p[t][j]: Vp values a plane and row, zeros past the last item, rows
+// `pitch` values apart.
+template <class Sh, bool BF16, bool OFF, bool PLANES>
 struct GradEpi {
+    using Shape = Sh;
+    static constexpr int TQ = Sh::TQ, TR = Sh::TR;
     static constexpr bool kWalk = false;
     LogitArgs a;
     const float* gk;   // g_t times dl's factor (0: the row has no gradient)
@@ -369,12 +356,11 @@ struct GradEpi {
     const int64_t* targets;
     uint32_t item0;    // the piece's first item
     uint16_t* p;
-    uint16_t* pt;
-    uint32_t Vp, Tp;
-    struct Shared : LogitShared<OFF, PLANES> {
-        float gk[g16::TQ], lse[g16::TQ];
-        uint32_t target[g16::TQ];  // within the piece (any larger value: elsewhere)
-        float inv_q[PLANES ? g16::TQ : 1];
+    uint32_t Vp, pitch;
+    struct Shared : LogitShared<OFF, PLANES, TR> {
+        float gk[TQ], lse[TQ];
+        uint32_t target[TQ];  // within the piece (any larger value: elsewhere)
+        float inv_q[PLANES ? TQ : 1];
     };
     struct State {
         float off, inv, gk, lse, qinv;
@@ -384,8 +370,8 @@ struct GradEpi {
     __device__ void begin(State&, Shared&, const Tile&) {}
     template <class Tile>
     __device__ void load(State& s, const Tile& t, int tid) {
-        const uint32_t r = t.rb * g16::TR + uint32_t(tid), q = t.qb * g16::TQ + uint32_t(tid);
-        const bool in = tid < g16::TR && r < a.items, qin = tid < g16::TQ && q < a.rows;
+        const uint32_t r = t.rb * TR + uint32_t(tid), q = t.qb * TQ + uint32_t(tid);
+        const bool in = tid < TR && r < a.items, qin = tid < TQ && q < a.rows;
         if constexpr (OFF) s.off = !in ? -INFINITY : a.offsets ? a.offsets[r] : 0.0f;
         if constexpr (PLANES) {
             s.inv = in ? a.xinv[r] : 0.0f;
@@ -397,57 +383,36 @@ struct GradEpi {
         s.target = y >= 0 && y < int64_t(a.items) ? uint32_t(y) : 0xFFFFFFFFu;
     }
     __device__ void publish(State& s, Shared& sm, int tid) {
-        if (tid >= g16::TQ) return;
-        if constexpr (OFF) sm.off[tid] = s.off;
-        if constexpr (PLANES) {
-            sm.inv[tid] = s.inv;
-            sm.inv_q[tid] = s.qinv;
-        }
+        if constexpr (OFF)
+            if (tid < TR) sm.off[tid] = s.off;
+        if constexpr (PLANES)
+            if (tid < TR) sm.inv[tid] = s.inv;
+        if (tid >= TQ) return;
+        if constexpr (PLANES) sm.inv_q[tid] = s.qinv;
         sm.gk[tid] = s.gk;
         sm.lse[tid] = s.lse;
         sm.target[tid] = s.target;
     }
-    // One plane of the wave's 32 rows x 64 items of query block n, through its 4 KiB of LDS: [t][j] rows of
-    // 128 bytes, 16-byte chunks swizzled by t & 7 (both the 8-byte writes and the reads then touch every
-    // bank equally).  p leaves in whole 128-byte lines; for pt, ds_read_tr16 hands each lane four
-    // consecutive t of one j, so 8 t are one 16-byte store and a row's 32 t are 64 bytes.  (Stored straight
-    // from the accumulators, 8 and 2 bytes a lane, the same tile took three times as long.)
-    __device__ void put(const char* spare, const g16::Lane& ln, int n, const uint32_t q0, const uint32_t r0, uint32_t plane) {
-        typedef short s16x4 __attribute__((ext_vector_type(4)));
-        typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
+    // One plane of the wave's 32 rows x 64 items from its 4 KiB of LDS: [t][j] rows of 128 bytes, 16-byte chunks
+    // swizzled by t & 7 (the 8-byte writes and the reads then touch every bank equally); whole 128-byte
+    // lines go out.  (Stored straight from the accumulators, 8 bytes a lane, a tile took three times as long.)
+    __device__ void put(const char* spare, const g16::Lane& ln, const uint32_t q0, const uint32_t r0, uint32_t plane) {
         const int lane = ln.hh * 32 + ln.l32;
         asm volatile("" ::: "memory");  // the writes come first (a wave's LDS accesses execute in order)
-        if (p && r0 < Vp) {
+        if (r0 < Vp) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int t = 8 * i + (lane >> 3), c = lane & 7;
                 const u32x4 v = *reinterpret_cast<const u32x4*>(spare + t * 128 + 16 * (c ^ (t & 7)));
                 if (q0 + t < a.rows)
-                    *reinterpret_cast<u32x4*>(p + uint64_t(q0 + t) * Vp * (PLANES ? 2 : 1) + plane * Vp + r0 + 8 * c) = v;
-            }
-        }
-        if (pt && q0 < Tp) {
-            const int g = lane >> 4;
-#pragma unroll
-            for (int jb = 0; jb < 4; ++jb) {
-                struct alignas(16) {
-                    s16x4 v[2];
-                } o;
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int t = 8 * g + 4 * h + ((lane & 15) >> 2), c = 2 * jb + ((lane & 3) >> 1);
-                    const uint32_t at = lds_addr_of(spare) + uint32_t(t * 128 + 16 * (c ^ (t & 7)) + 8 * (lane & 1));
-                    o.v[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_s16x4>(at));
-                }
-                *reinterpret_cast<u32x4*>(pt + uint64_t(r0 + 16 * jb + (lane & 15)) * Tp * (PLANES ? 2 : 1) + plane * Tp + q0 + 8 * g) =
-                    __builtin_bit_cast(u32x4, o);
+                    *reinterpret_cast<u32x4*>(p + uint64_t(q0 + t) * pitch + plane * Vp + r0 + 8 * c) = v;
             }
         }
         asm volatile("" ::: "memory");  // and the reads before what is written next
     }
     template <class Tile>
     __device__ void tile(State&, Shared& sm, const g16::Lane& ln, f32x16 (&acc)[2][2], const Tile& t, char* spare) {
-        const uint32_t r0 = t.rb * g16::TR, rw = r0 + uint32_t(ln.wr * 64);
+        const uint32_t r0 = t.rb * TR, rw = r0 + uint32_t(ln.wr * 64);
         const int swz = ln.l32 & 7;
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
@@ -455,7 +420,7 @@ struct GradEpi {
             const float c = PLANES ? a.scale * sm.inv_q[ln.q(n)] : a.scale;
             const uint32_t y = sm.target[ln.q(n)] - r0;
             const bool none = g == 0.0f || ref == -INFINITY;
-            const uint32_t q0 = t.qb * g16::TQ + uint32_t(ln.wq * 64 + 32 * n);
+            const uint32_t q0 = t.qb * TQ + uint32_t(ln.wq * 64 + 32 * n);
             auto write = [&](int m, int j, const uint16_t (&v)[4]) {
                 *reinterpret_cast<uint2*>(spare + ln.l32 * 128 + 16 * ((4 * m + j) ^ swz) + 8 * ln.hh) =
                     make_uint2(v[0] | uint32_t(v[1]) << 16, v[2] | uint32_t(v[3]) << 16);
@@ -465,7 +430,7 @@ struct GradEpi {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const uint32_t r = uint32_t(ln.r(m, j));
-                    const f32x4 v = logits4<OFF, PLANES>(sm, acc[m][n], j, int(r), c);
+                    const f32x4 v = logits4<OFF, PLANES, TR>(sm, acc[m][n], j, int(r), c);
                     uint16_t hi[4], lo[4];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
@@ -481,7 +446,7 @@ struct GradEpi {
                     }
                     write(m, j, hi);
                 }
-            put(spare, ln, n, q0, rw, 0);
+            put(spare, ln, q0, rw, 0);
             if constexpr (PLANES) {
 #pragma unroll
                 for (int m = 0; m < 2; ++m)
@@ -492,7 +457,7 @@ struct GradEpi {
                         for (int e = 0; e < 4; ++e) split16(acc[m][n][4 * j + e], hi[e], lo[e]);
                         write(m, j, lo);
                     }
-                put(spare, ln, n, q0, rw, 1);
+                put(spare, ln, q0, rw, 1);
             }
         }
     }
@@ -501,7 +466,10 @@ struct GradEpi {
 };
 
 // dh: fp32 shares [part][t][Dp], added to over the pieces (first: written)
+template <class Sh>
 struct ShareEpi {
+    using Shape = Sh;
+    static constexpr int TQ = Sh::TQ, TR = Sh::TR;
     static constexpr bool kWalk = false;
     float* out;
     uint32_t rows, D, Dp;
@@ -517,14 +485,14 @@ struct ShareEpi {
     __device__ void tile(State&, Shared&, const g16::Lane& ln, f32x16 (&acc)[2][2], const Tile& t, char*) {
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
-            const uint32_t q = t.qb * g16::TQ + uint32_t(ln.q(n));
+            const uint32_t q = t.qb * TQ + uint32_t(ln.q(n));
             if (q >= rows) continue;
             float* o = out + (uint64_t(t.part) * rows + q) * Dp;
 #pragma unroll
             for (int m = 0; m < 2; ++m)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const uint32_t d = t.rb * g16::TR + uint32_t(ln.r(m, j));
+                    const uint32_t d = t.rb * TR + uint32_t(ln.r(m, j));
                     if (d >= D) continue;  // (rows hold Dp = whole groups of 4)
                     f32x4 v;
 #pragma unroll
@@ -539,8 +507,10 @@ struct ShareEpi {
 };
 
 // dw: the piece's rows, final
-template <int DT>
+template <class Sh, int DT>
 struct ItemGradEpi {
+    using Shape = Sh;
+    static constexpr int TQ = Sh::TQ, TR = Sh::TR;
     static constexpr bool kWalk = false;
     ElemT<DT>* out;
     uint64_t ld;
@@ -564,14 +534,14 @@ struct ItemGradEpi {
         const float s = sm.mul;
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
-            const uint32_t q = t.qb * g16::TQ + uint32_t(ln.q(n));
+            const uint32_t q = t.qb * TQ + uint32_t(ln.q(n));
             if (q >= rows) continue;
             ElemT<DT>* o = out + q * ld;
 #pragma unroll
             for (int m = 0; m < 2; ++m)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const uint32_t d = t.rb * g16::TR + uint32_t(ln.r(m, j));
+                    const uint32_t d = t.rb * TR + uint32_t(ln.r(m, j));
                     if (d >= D) continue;
                     struct alignas(4 * sizeof(ElemT<DT>)) V4 {
                         ElemT<DT> v[4];
@@ -698,17 +668,24 @@ __global__ __launch_bounds__(1024) void xent_gradient_kernel(const float* __rest
     if (threadIdx.x == 0) *mul = scale * (m / 16384.0f);
 }
 
-// dh[t][d] = mul sum over the shares (zero for a row without a gradient)
+// dh[t][d] = mul sum over the shares (zero for a row without a gradient).  64 groups of four values a
+// workgroup, its four waves a quarter of the shares each.
 template <int DT>
 __global__ __launch_bounds__(256) void share_sum_kernel(const float* __restrict__ share, uint32_t parts, uint32_t T, uint32_t D,
                                                         uint32_t Dp, const float* __restrict__ gk, const float* __restrict__ mul,
                                                         const uint32_t* __restrict__ absmax, ElemT<DT>* __restrict__ out, uint64_t ld) {
-    const uint32_t per = Dp / 4;
-    const uint64_t i = uint64_t(blockIdx.x) * 256 + threadIdx.x;
-    if (i >= uint64_t(T) * per) return;
-    const uint32_t t = uint32_t(i / per), d = uint32_t(i % per) * 4;
+    __shared__ f32x4 part[4][64];
+    const uint32_t per = Dp / 4, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const uint64_t i = uint64_t(blockIdx.x) * 64 + lane, n = uint64_t(T) * per;
     f32x4 v{0.0f, 0.0f, 0.0f, 0.0f};
-    for (uint32_t s = 0; s < parts; ++s) v += *reinterpret_cast<const f32x4*>(share + (uint64_t(s) * T + t) * Dp + d);
+    if (i < n)
+#pragma unroll 8
+        for (uint32_t s = w; s < parts; s += 4) v += *reinterpret_cast<const f32x4*>(share + (uint64_t(s) * n + i) * 4);
+    part[w][lane] = v;
+    __syncthreads();
+    if (w || i >= n) return;
+    v = (v + part[1][lane]) + (part[2][lane] + part[3][lane]);
+    const uint32_t t = uint32_t(i / per), d = uint32_t(i % per) * 4;
     const float m = *mul / (DT == VA_DTYPE_F32 ? scale_to_2p14(__builtin_bit_cast(float, *absmax)) : 1.0f);
     const bool none = gk[t] == 0.0f;
     for (int e = 0; e < 4 && d + e < D; ++e) out[t * ld + d + e] = Elem<DT>::from_f(none ? 0.0f : v[e] * m);
@@ -723,33 +700,46 @@ bool direct(va_dtype dt, const void* p, uint64_t ld, uint32_t D) {
 }
 size_t packed_bytes(va_dtype dt, uint64_t rows, uint32_t Kp) { return rows * Kp * (dt == VA_DTYPE_F32 ? 4 : 2); }
 
-va_status pack(va_context* ctx, va_dtype dt, const void* src, uint64_t ld, uint32_t R, uint32_t D, uint32_t Kp, void* dst, float* inv) {
+va_status pack(va_context* ctx, va_dtype dt, const void* src, uint64_t ld, uint32_t R, uint32_t D, uint32_t Kp, const uint32_t* absmax,
+               const float* drop, float drop_if, void* dst, float* inv) {
     if (dt == VA_DTYPE_F32) {
-        pack32_kernel<<<dim3(ceil_div(R, 4)), dim3(256), 0, ctx->stream>>>(static_cast<const float*>(src), ld, R, D, Kp,
+        pack32_kernel<<<dim3(ceil_div(R, 4)), dim3(256), 0, ctx->stream>>>(static_cast<const float*>(src), ld, R, D, Kp, absmax, drop, drop_if,
                                                                            static_cast<uint16_t*>(dst), inv);
     } else {
         const uint64_t n8 = uint64_t(R) * (Kp / 8);
         pack16_kernel<<<dim3(uint32_t(std::min<uint64_t>((n8 + 255) / 256, 16384))), dim3(256), 0, ctx->stream>>>(
-            static_cast<const uint16_t*>(src), ld, D, Kp, static_cast<uint16_t*>(dst), n8);
+            static_cast<const uint16_t*>(src), ld, D, Kp, drop, drop_if, static_cast<uint16_t*>(dst), n8);
     }
     VA_CHECK_LAUNCH(ctx);
     return VA_OK;
 }
 
-va_status transpose(va_context* ctx, va_dtype dt, const void* src, uint64_t ld, uint32_t R, uint32_t D, uint32_t Rp, const float* drop,
-                    float drop_if, const uint32_t* absmax, uint16_t* dst) {
-    const dim3 grid(Rp / 64, ceil_div(D, 64));
-    if (dt == VA_DTYPE_F32)
-        transpose_kernel<VA_DTYPE_F32><<<grid, dim3(256), 0, ctx->stream>>>(static_cast<const float*>(src), ld, R, D, Rp, drop, drop_if, absmax, dst);
-    else if (dt == VA_DTYPE_F16)
-        transpose_kernel<VA_DTYPE_F16><<<grid, dim3(256), 0, ctx->stream>>>(static_cast<const _Float16*>(src), ld, R, D, Rp, drop, drop_if, absmax, dst);
-    else
-        transpose_kernel<VA_DTYPE_BF16><<<grid, dim3(256), 0, ctx->stream>>>(static_cast<const __bf16*>(src), ld, R, D, Rp, drop, drop_if, absmax, dst);
-    VA_CHECK_LAUNCH(ctx);
-    return VA_OK;
-}
-
 const char* at(const void* p, uint64_t ld, uint64_t row, va_dtype dt) { return static_cast<const char*>(p) + row * ld * elem_size(dt); }
+
+// The shape of a product's workgroups: 256 x 256 tiles (the least operand traffic) where they fill most
+// of the chip or the operands are that large; smaller ones where those would leave CUs without work.
+template <class F>
+va_status by_shape(int shape, F&& f) {
+    if (shape == 0) return f(g16::Large());
+    if (shape == 1) return f(g16::Shape<2, 2>());
+    return f(g16::Shape<1, 2>());
+}
+struct Blocks {
+    int shape;
+    uint32_t tq, tr, grid;  // grid: the most workgroups of a launch
+    uint32_t nq(uint64_t Q) const { return uint32_t((Q + tq - 1) / tq); }
+    uint32_t nr(uint64_t R) const { return uint32_t((R + tr - 1) / tr); }
+};
+// `shares`: how many shares of the sum the caller can make of each tile
+Blocks blocks_for(const va_context* ctx, uint64_t Q, uint64_t R, uint32_t shares = 1) {
+    const Blocks all[3] = {{0, 256, 256, g16::grid_max<g16::Large>(ctx)},
+                           {1, 128, 128, g16::grid_max<g16::Shape<2, 2>>(ctx)},
+                           {2, 64, 128, g16::grid_max<g16::Shape<1, 2>>(ctx)}};
+    const uint64_t enough = all[0].grid * 3 / 4;
+    for (int i = 0; i < 2; ++i)
+        if (Q > all[i].tq / 2 && uint64_t(all[i].nq(Q)) * all[i].nr(R) * shares >= enough) return all[i];
+    return all[2];
+}
 
 template <class F>
 va_status by_type(va_dtype dt, bool off, F&& f) {
@@ -783,7 +773,10 @@ uint32_t piece_items(uint32_t V, size_t per_item, size_t budget) {
 }
 
 constexpr size_t kPackBudget = size_t(256) << 20;  // packed items of one piece
-constexpr size_t kGradBudget = size_t(512) << 20;  // one order of dl of one piece
+constexpr size_t kGradBudget = size_t(512) << 20;  // dl of one piece
+// Values between dl's rows: with the rows a power of two apart, a tile's 256 rows meet in few memory
+// channels.
+constexpr uint32_t kRowPad = 64;
 
 }  // namespace
 }  // namespace va
@@ -804,13 +797,14 @@ va_status va_xent_forward(va_context* ctx, const va_xent_desc* d, float* out_los
     const size_t es = elem_size(dt), planes = dt == VA_DTYPE_F32 ? 2 : 1;
     const bool qd = direct(dt, d->hidden, d->hidden_stride, D), xd = direct(dt, d->items, d->items_stride, D);
     const uint32_t piece = xd ? round_up(V, 256) : piece_items(V, packed_bytes(dt, 1, Kp), kPackBudget);
-    const uint32_t pieces = ceil_div(V, piece), nq = ceil_div(T, 256);
-    const uint32_t cus = std::max(uint32_t(ctx->num_cus), kXcds) / kXcds * kXcds;
+    const uint32_t pieces = ceil_div(V, piece);
+    const Blocks bl = blocks_for(ctx, T, std::min(piece, V));
+    const uint32_t nq = bl.nq(T);
     // parts per query block: whole multiples of the XCDs when there are that many
-    uint32_t parts = std::max(cus / nq, 1u);
+    uint32_t parts = std::max(bl.grid / nq, 1u);
     if (parts > kXcds) parts = parts / kXcds * kXcds;
-    parts = std::min(parts, ceil_div(std::min(piece, V), 256));
-    const uint32_t last_parts = std::min(parts, ceil_div(V - (pieces - 1) * piece, 256));  // (of the last piece)
+    parts = std::min(parts, bl.nr(std::min(piece, V)));
+    const uint32_t last_parts = std::min(parts, bl.nr(V - (pieces - 1) * piece));  // (of the last piece)
     const uint32_t slots = parts * (pieces - 1) + last_parts;
 
     Scratch sc(ctx);
@@ -827,7 +821,7 @@ va_status va_xent_forward(va_context* ctx, const va_xent_desc* d, float* out_los
     if (!qd) {
         qp = sc.carve<char>(packed_bytes(dt, T, Kp));
         qinv = sc.carve<float>(T);
-        VA_CHECK_STATUS(pack(ctx, dt, d->hidden, d->hidden_stride, T, D, Kp, qp, qinv));
+        VA_CHECK_STATUS(pack(ctx, dt, d->hidden, d->hidden_stride, T, D, Kp, nullptr, nullptr, 0.0f, qp, qinv));
     }
     if (!xd) {
         xp = sc.carve<char>(packed_bytes(dt, piece, Kp));
@@ -837,24 +831,27 @@ va_status va_xent_forward(va_context* ctx, const va_xent_desc* d, float* out_los
     for (uint32_t c = 0; c < pieces; ++c) {
         const uint32_t v0 = c * piece, n = std::min(piece, V - v0);
         const char* items = at(d->items, d->items_stride, v0, dt);
-        if (!xd) VA_CHECK_STATUS(pack(ctx, dt, items, d->items_stride, n, D, Kp, xp, xinv));
+        if (!xd) VA_CHECK_STATUS(pack(ctx, dt, items, d->items_stride, n, D, Kp, nullptr, nullptr, 0.0f, xp, xinv));
         g16::Args a;
-        a.q = g16::Operand{qd ? d->hidden : qp, qd ? d->hidden_stride * es : uint64_t(Kp) * 2 * planes, T, uint32_t(Kp * 2)};
-        a.x = g16::Operand{xd ? items : xp, xd ? d->items_stride * es : uint64_t(Kp) * 2 * planes, n, uint32_t(Kp * 2)};
+        a.q = g16::Operand{qd ? d->hidden : qp, qd ? d->hidden_stride * es : uint64_t(Kp) * 2 * planes, T, Kp * 2, Kp * 2};
+        a.x = g16::Operand{xd ? items : xp, xd ? d->items_stride * es : uint64_t(Kp) * 2 * planes, n, Kp * 2, Kp * 2};
         a.kstages = Kp / g16::KC;
         a.nq = nq;
-        a.nr = ceil_div(n, 256);
+        a.nr = bl.nr(n);
         a.parts = c + 1 < pieces ? parts : last_parts;
-        VA_CHECK_STATUS(by_type(dt, d->offsets || n % g16::TR, [&](auto bf, auto off, auto pl) {
-            LseEpi<decltype(off)::value, decltype(pl)::value> e;
-            e.a = LogitArgs{d->offsets ? d->offsets + v0 : nullptr, qinv, xinv, d->scale, T, n};
-            e.targets = d->targets;
-            e.item0 = v0;
-            e.picked = picked;
-            e.part = part;
-            e.slots = slots;
-            e.slot0 = c * parts;
-            return g16::launch<decltype(bf)::value, decltype(pl)::value>(ctx, a, e);
+        VA_CHECK_STATUS(by_shape(bl.shape, [&](auto sh) {
+            using Sh = decltype(sh);
+            return by_type(dt, d->offsets || n % Sh::TR, [&](auto bf, auto off, auto pl) {
+                LseEpi<Sh, decltype(off)::value, decltype(pl)::value> e;
+                e.a = LogitArgs{d->offsets ? d->offsets + v0 : nullptr, qinv, xinv, d->scale, T, n};
+                e.targets = d->targets;
+                e.item0 = v0;
+                e.picked = picked;
+                e.part = part;
+                e.slots = slots;
+                e.slot0 = c * parts;
+                return g16::launch<decltype(bf)::value, decltype(pl)::value, false, false>(ctx, a, e);
+            });
         }));
     }
     xent_finish_kernel<<<dim3(ceil_div(T, 4)), dim3(256), 0, ctx->stream>>>(d->targets, T, V, d->ignore_index, part, picked, slots, out_loss, out_lse);
@@ -877,42 +874,35 @@ va_status va_xent_backward(va_context* ctx, const va_xent_desc* d, const float* 
     VA_REQUIRE(ctx, (!out_grad_hidden || grad_hidden_stride >= d->dim) && (!out_grad_items || grad_items_stride >= d->dim),
                "va_xent_backward: a gradient's row stride is below the dimension");
     DeviceGuard guard(ctx->device);
-    const uint32_t T = d->rows, V = d->num_items, D = d->dim, Kp = round_up(D, g16::KC), Tp = round_up(T, g16::KC), Dp = round_up(D, 4);
+    const uint32_t T = d->rows, V = d->num_items, D = d->dim, Kp = round_up(D, g16::KC), Dp = round_up(D, 4);
     const va_dtype dt = d->dtype;
     const bool f32 = dt == VA_DTYPE_F32;
     const size_t es = elem_size(dt), planes = f32 ? 2 : 1;
-    const bool qd = direct(dt, d->hidden, d->hidden_stride, D), xd = direct(dt, d->items, d->items_stride, D);
+    // masked items may hold anything, and dh sums over them: their rows are read as zeros
+    const bool xd = direct(dt, d->items, d->items_stride, D) && !d->offsets;
     VA_REQUIRE(ctx, (!out_grad_hidden || reinterpret_cast<uintptr_t>(out_grad_hidden) % es == 0) &&
                         (!out_grad_items || reinterpret_cast<uintptr_t>(out_grad_items) % es == 0),
                "va_xent_backward: a gradient is not aligned to its type");
-    // the piece: dl within its budget (in either order), the packed and transposed items too
-    uint32_t piece = piece_items(V, uint64_t(Tp) * 2 * planes, kGradBudget);
-    piece = std::min(piece, piece_items(V, packed_bytes(dt, 1, Kp), kPackBudget));
-    // dl's rows of a piece within the products' 32-bit offsets
-    piece = std::min<uint32_t>(piece, uint32_t(kDmaMaxBytes / 256 / (2 * planes)) / 256 * 256);
-    VA_REQUIRE(ctx, uint64_t(Tp) * 2 * planes * 256 <= kDmaMaxBytes, "va_xent_backward: %u rows (at most %u)", T, uint32_t(kDmaMaxBytes / (512 * planes)));
-    const uint32_t pieces = ceil_div(V, piece), nq = ceil_div(T, 256), nd = ceil_div(D, 256);
+    // the piece: dl and the packed items within their budgets, dl's rows within the products' 32-bit offsets
+    uint32_t piece = piece_items(V, uint64_t(T) * 2 * planes, kGradBudget);
+    if (!xd) piece = std::min(piece, piece_items(V, packed_bytes(dt, 1, Kp), kPackBudget));
+    piece = std::min<uint32_t>(piece, (uint32_t(kDmaMaxBytes / 256 / 2) - kRowPad) / uint32_t(planes) / 256 * 256);
+    const uint32_t pieces = ceil_div(V, piece);
     const uint32_t Vpmax = round_up(std::min(piece, V), g16::KC);
-    const uint32_t cus = std::max(uint32_t(ctx->num_cus), kXcds) / kXcds * kXcds;
-    // dh has few tiles and a long sum: shares of it until the chip is filled once
-    const uint32_t kst = Vpmax / g16::KC * (f32 ? 3 : 1);
-    const uint32_t parts = std::min(std::max(cus / (nq * nd), 1u), std::max(kst / 4, 1u));
+    const uint32_t most = std::min(piece, V);
+    // dh has few tiles and a long sum: shares of it until the chip is filled once, eight stages at least each
+    const uint32_t kst = Vpmax / g16::KC * (f32 ? 3 : 1), shares = std::max(kst / 8, 1u);
+    const Blocks lb = blocks_for(ctx, T, most), hb = blocks_for(ctx, T, D, shares), wb = blocks_for(ctx, most, D);
+    const uint32_t parts = std::min(std::max(hb.grid / (hb.nq(T) * hb.nr(D)), 1u), shares);
 
-    const size_t p_bytes = out_grad_hidden ? uint64_t(T) * Vpmax * 2 * planes : 0;
-    const size_t pt_bytes = out_grad_items ? uint64_t(std::min(piece, round_up(V, 256))) * Tp * 2 * planes : 0;
-    const size_t wt_bytes = out_grad_hidden ? uint64_t(D) * Vpmax * 2 * planes : 0;
-    const size_t ht_bytes = out_grad_items ? uint64_t(D) * Tp * 2 * planes : 0;
+    const size_t p_bytes = uint64_t(T) * (Vpmax * planes + kRowPad) * 2;
     const size_t share_n = out_grad_hidden ? uint64_t(parts) * T * Dp : 0;
-    const size_t qp_bytes = qd ? 0 : packed_bytes(dt, T, Kp), xp_bytes = xd ? 0 : packed_bytes(dt, std::min(piece, V), Kp);
+    const size_t qp_bytes = packed_bytes(dt, T, Kp), xp_bytes = xd ? 0 : packed_bytes(dt, std::min(piece, V), Kp);
     Scratch sc(ctx);
-    const size_t need = Scratch::round(p_bytes) + Scratch::round(pt_bytes) + Scratch::round(wt_bytes) + Scratch::round(ht_bytes) +
-                        Scratch::round(share_n * 4) + Scratch::round(qp_bytes) + Scratch::round(xp_bytes) + 2 * Scratch::round(T * 4ull) +
-                        Scratch::round(piece * 4ull) + Scratch::round(16);
+    const size_t need = Scratch::round(p_bytes) + Scratch::round(share_n * 4) + Scratch::round(qp_bytes) + Scratch::round(xp_bytes) +
+                        2 * Scratch::round(T * 4ull) + Scratch::round(piece * 4ull) + Scratch::round(16);
     VA_CHECK_STATUS(sc.reserve(need));
-    uint16_t* p = out_grad_hidden ? sc.carve<uint16_t>(p_bytes / 2) : nullptr;
-    uint16_t* pt = out_grad_items ? sc.carve<uint16_t>(pt_bytes / 2) : nullptr;
-    uint16_t* wt = sc.carve<uint16_t>(wt_bytes / 2);
-    uint16_t* ht = sc.carve<uint16_t>(ht_bytes / 2);
+    uint16_t* p = sc.carve<uint16_t>(p_bytes / 2);
     float* share = sc.carve<float>(share_n);
     char* qp = sc.carve<char>(qp_bytes);
     char* xp = sc.carve<char>(xp_bytes);
@@ -926,75 +916,86 @@ va_status va_xent_backward(va_context* ctx, const va_xent_desc* d, const float* 
     xent_gradient_kernel<<<dim3(1), dim3(1024), 0, ctx->stream>>>(grad, d->targets, T, V, d->ignore_index, int(reduction), d->scale, gk, mul, absmax);
     VA_CHECK_LAUNCH(ctx);
     if (f32) {
+        // one scale a tensor: both tensors are summed over in the second products
         auto top = [&](const void* src, uint64_t ld, uint32_t R, const float* drop, float drop_if, uint32_t* out) {
-            absmax_kernel<<<dim3(std::min<uint32_t>(ceil_div(R, 4), 2048)), dim3(256), 0, ctx->stream>>>(static_cast<const float*>(src), ld, R, D, drop, drop_if, out);
+            absmax_kernel<<<dim3(std::min<uint32_t>(ceil_div(R, 16), 512)), dim3(256), 0, ctx->stream>>>(static_cast<const float*>(src), ld, R, D, drop, drop_if, out);
         };
-        if (out_grad_items) top(d->hidden, d->hidden_stride, T, gk, 0.0f, absmax);
-        if (out_grad_hidden) top(d->items, d->items_stride, V, d->offsets, -INFINITY, absmax + 1);
+        top(d->hidden, d->hidden_stride, T, gk, 0.0f, absmax);
+        top(d->items, d->items_stride, V, d->offsets, -INFINITY, absmax + 1);
         VA_CHECK_LAUNCH(ctx);
     }
-    if (!qd) VA_CHECK_STATUS(pack(ctx, dt, d->hidden, d->hidden_stride, T, D, Kp, qp, qinv));
-    if (out_grad_items) VA_CHECK_STATUS(transpose(ctx, dt, d->hidden, d->hidden_stride, T, D, Tp, gk, 0.0f, absmax, ht));
+    VA_CHECK_STATUS(pack(ctx, dt, d->hidden, d->hidden_stride, T, D, Kp, f32 ? absmax : nullptr, gk, 0.0f, qp, qinv));
     for (uint32_t c = 0; c < pieces; ++c) {
         const uint32_t v0 = c * piece, n = std::min(piece, V - v0), Vp = round_up(n, g16::KC);
         const char* items = at(d->items, d->items_stride, v0, dt);
         const float* offsets = d->offsets ? d->offsets + v0 : nullptr;
-        if (!xd) VA_CHECK_STATUS(pack(ctx, dt, items, d->items_stride, n, D, Kp, xp, xinv));
+        if (!xd) VA_CHECK_STATUS(pack(ctx, dt, items, d->items_stride, n, D, Kp, f32 ? absmax + 1 : nullptr, offsets, -INFINITY, xp, xinv));
+        const g16::Operand rows{qp, uint64_t(Kp) * 2 * planes, T, Kp * 2, Kp * 2};
+        const g16::Operand cols{xd ? items : xp, xd ? d->items_stride * es : uint64_t(Kp) * 2 * planes, n, Kp * 2, Kp * 2};
+        const uint32_t pitch = Vp * uint32_t(planes) + kRowPad;
+        const g16::Operand dl{p, uint64_t(pitch) * 2, T, Vp * 2, Vp * 2};
         g16::Args a;
-        a.q = g16::Operand{qd ? d->hidden : qp, qd ? d->hidden_stride * es : uint64_t(Kp) * 2 * planes, T, uint32_t(Kp * 2)};
-        a.x = g16::Operand{xd ? items : xp, xd ? d->items_stride * es : uint64_t(Kp) * 2 * planes, n, uint32_t(Kp * 2)};
+        a.q = rows;
+        a.x = cols;
         a.kstages = Kp / g16::KC;
-        a.nq = nq;
-        a.nr = ceil_div(n, 256);
+        a.nq = lb.nq(T);
+        a.nr = lb.nr(n);
         a.parts = 1;
-        VA_CHECK_STATUS(by_type(dt, offsets || n % g16::TR, [&](auto bf, auto off, auto pl) {
-            GradEpi<decltype(bf)::value, decltype(off)::value, decltype(pl)::value> e;
-            e.a = LogitArgs{offsets, qinv, xinv, d->scale, T, n};
-            e.gk = gk;
-            e.lse = lse;
-            e.targets = d->targets;
-            e.item0 = v0;
-            e.p = p;
-            e.pt = pt;
-            e.Vp = Vp;
-            e.Tp = Tp;
-            return g16::launch<decltype(bf)::value, decltype(pl)::value>(ctx, a, e);
+        VA_CHECK_STATUS(by_shape(lb.shape, [&](auto sh) {
+            using Sh = decltype(sh);
+            return by_type(dt, offsets || n % Sh::TR, [&](auto bf, auto off, auto pl) {
+                GradEpi<Sh, decltype(bf)::value, decltype(off)::value, decltype(pl)::value> e;
+                e.a = LogitArgs{offsets, qinv, xinv, d->scale, T, n};
+                e.gk = gk;
+                e.lse = lse;
+                e.targets = d->targets;
+                e.item0 = v0;
+                e.p = p;
+                e.Vp = Vp;
+                e.pitch = pitch;
+                return g16::launch<decltype(bf)::value, decltype(pl)::value, false, false>(ctx, a, e);
+            });
         }));
         if (out_grad_hidden) {
-            VA_CHECK_STATUS(transpose(ctx, dt, items, d->items_stride, n, D, Vp, offsets, -INFINITY, absmax + 1, wt));
+            // dh[t][d] = sum_j dl[t][j] w[j][d]: the items are stored across the sum
             g16::Args b;
-            b.q = g16::Operand{p, uint64_t(Vp) * 2 * planes, T, Vp * 2};
-            b.x = g16::Operand{wt, uint64_t(Vp) * 2 * planes, D, Vp * 2};
+            b.q = dl;
+            b.x = cols;
             b.kstages = Vp / g16::KC;
-            b.nq = nq;
-            b.nr = nd;
+            b.nq = hb.nq(T);
+            b.nr = hb.nr(D);
             b.parts = parts;
-            const ShareEpi e{share, T, D, Dp, c == 0};
-            VA_CHECK_STATUS(f32 ? (g16::launch<false, true>(ctx, b, e))
-                                : dt == VA_DTYPE_F16 ? (g16::launch<false, false>(ctx, b, e)) : (g16::launch<true, false>(ctx, b, e)));
+            VA_CHECK_STATUS(by_shape(hb.shape, [&](auto sh) {
+                const ShareEpi<decltype(sh)> e{share, T, D, Dp, c == 0};
+                return f32 ? g16::launch<false, true, false, true>(ctx, b, e)
+                           : dt == VA_DTYPE_F16 ? g16::launch<false, false, false, true>(ctx, b, e) : g16::launch<true, false, false, true>(ctx, b, e);
+            }));
         }
         if (out_grad_items) {
+            // dw[j][d] = sum_t dl[t][j] h[t][d]: both are
             g16::Args b;
-            b.q = g16::Operand{pt, uint64_t(Tp) * 2 * planes, n, Tp * 2};
-            b.x = g16::Operand{ht, uint64_t(Tp) * 2 * planes, D, Tp * 2};
-            b.kstages = Tp / g16::KC;
-            b.nq = ceil_div(n, 256);
-            b.nr = nd;
+            b.q = dl;
+            b.x = rows;
+            b.kstages = ceil_div(T, g16::KC);
+            b.nq = wb.nq(n);
+            b.nr = wb.nr(D);
             b.parts = 1;
             const uintptr_t o = reinterpret_cast<uintptr_t>(out_grad_items) + uint64_t(v0) * grad_items_stride * es;
             const bool vec = o % (4 * es) == 0 && grad_items_stride % 4 == 0;
-            auto go = [&](auto DT, auto bf, auto pl) {
-                constexpr int kT = decltype(DT)::value;
-                ItemGradEpi<kT> e{reinterpret_cast<ElemT<kT>*>(o), grad_items_stride, n, D, mul, absmax, vec};
-                return g16::launch<decltype(bf)::value, decltype(pl)::value>(ctx, b, e);
-            };
-            VA_CHECK_STATUS(f32 ? go(std::integral_constant<int, VA_DTYPE_F32>(), std::false_type(), std::true_type())
-                            : dt == VA_DTYPE_F16 ? go(std::integral_constant<int, VA_DTYPE_F16>(), std::false_type(), std::false_type())
-                                                 : go(std::integral_constant<int, VA_DTYPE_BF16>(), std::true_type(), std::false_type()));
+            VA_CHECK_STATUS(by_shape(wb.shape, [&](auto sh) {
+                auto go = [&](auto DT, auto bf, auto pl) {
+                    constexpr int kT = decltype(DT)::value;
+                    ItemGradEpi<decltype(sh), kT> e{reinterpret_cast<ElemT<kT>*>(o), grad_items_stride, n, D, mul, absmax, vec};
+                    return g16::launch<decltype(bf)::value, decltype(pl)::value, true, true>(ctx, b, e);
+                };
+                return f32 ? go(std::integral_constant<int, VA_DTYPE_F32>(), std::false_type(), std::true_type())
+                           : dt == VA_DTYPE_F16 ? go(std::integral_constant<int, VA_DTYPE_F16>(), std::false_type(), std::false_type())
+                                                : go(std::integral_constant<int, VA_DTYPE_BF16>(), std::true_type(), std::false_type());
+            }));
         }
     }
     if (out_grad_hidden) {
-        const dim3 grid(ceil_div(uint64_t(T) * (Dp / 4), 256));
+        const dim3 grid(ceil_div(uint64_t(T) * (Dp / 4), 64));
         auto sum = [&](auto k, auto* o) {
             k<<<grid, dim3(256), 0, ctx->stream>>>(share, parts, T, D, Dp, gk, mul, absmax + 1, o, grad_hidden_stride);
         };
