@@ -22,6 +22,7 @@
 #pragma once
 
 #include <algorithm>
+#include <type_traits>
 
 #include "va_internal.hpp"
 
@@ -55,6 +56,8 @@ struct Operand {
     uint32_t rows = 0;         // k along the rows: queries (rows) of the product; across: values of k
     uint32_t width = 0;        // bytes of a row (k along the rows: whole stages; else a multiple of 16)
     uint32_t plane = 0;        // bytes from a row's hi plane to its lo plane (PLANES only)
+    const void* other = nullptr;  // read instead of p (the same layout) when *choose is not zero
+    const uint32_t* choose = nullptr;
 };
 
 struct Args {
@@ -189,27 +192,27 @@ struct Feed {
     }
     // the operand's block b of 64 W queries (rows)
     __device__ void open(const Operand& o, uint32_t b) {
+        const uint32_t* choose = o.choose;
+        const void *one = o.p, *two = o.other;
+        const char* p = static_cast<const char*>(choose && *choose ? two : one);
         if constexpr (KM) {
-            base = static_cast<const char*>(o.p) + b * uint32_t(KROW);
+            base = p + b * uint32_t(KROW);
             left = (o.rows - 1) * o.pitch + o.width - b * uint32_t(KROW);
         } else {
-            base = static_cast<const char*>(o.p) + uint64_t(b) * (64u * W) * o.pitch;
+            base = p + uint64_t(b) * (64u * W) * o.pitch;
             records = (min(64u * W, o.rows - b * (64u * W)) - 1u) * pitch + o.width + plane;
         }
     }
-    // stage k (of the plane `lo`) into the slot at LDS address `slot`; !ok: zeros
-    __device__ void issue(uint32_t k, bool lo, bool ok, uint32_t slot) const {
+    // load i of stage k (of the plane `lo`) into the slot at LDS address `slot`; !ok: zeros
+    __device__ void issue(uint32_t k, bool lo, bool ok, uint32_t slot, int i) const {
         if constexpr (KM) {
             const uint64_t skip = uint64_t(k) * KC * pitch;
             const dma_rsrc r = make_dma_rsrc(base + skip + (lo ? plane : 0u),
                                              ok && skip < left ? uint32_t(min(left - skip, uint64_t(kDmaMaxBytes))) : 0u);
-#pragma unroll
-            for (int i = 0; i < LPW; ++i) lds_dma16(r, voff[i], slot + lds_at + uint32_t(1024 * WAVES * i));
+            lds_dma16(r, voff[i], slot + lds_at + uint32_t(1024 * WAVES * i));
         } else {
             const dma_rsrc r = make_dma_rsrc(base, records);
-            const uint32_t so = ok ? k * uint32_t(ROWB) + (lo ? plane : 0u) : 0u;
-#pragma unroll
-            for (int i = 0; i < LPW; ++i) lds_dma16_so(r, ok ? voff[i] : kDmaSkip, so, slot + lds_at + uint32_t(1024 * WAVES * i));
+            lds_dma16_so(r, ok ? voff[i] : kDmaSkip, ok ? k * uint32_t(ROWB) + (lo ? plane : 0u) : 0u, slot + lds_at + uint32_t(1024 * WAVES * i));
         }
     }
     // the fragment of the wave's 32-query (row) block n, k-step t of the slot
@@ -231,12 +234,13 @@ struct Feed {
 };
 
 // Epi: struct with
-//   Shape, static constexpr bool kWalk
+//   Shape, static constexpr bool kWalk, kStores
 //   struct State (per thread, lives through the main loop)
 //   begin(State&, smem, tile)   a new item's first tile (barriers follow before the epilogue)
 //   load(State&, tile, tid)     before the main loop: starts what the tile's epilogue reads
 //   publish(State&, smem, tid)  after the main loop, before the barrier
-//   tile(State&, smem, lane, acc, tile, spare)  spare: 4 KiB of LDS of the wave's own
+//   tile(State&, smem, lane, acc, tile, spare, settle)  spare: 4 KiB of LDS of the wave's own; with kStores,
+//                               settle() before the first store to memory
 //   end(State&, smem, lane, tile)  after an item's last tile
 template <bool BF16, bool PLANES, bool QK, bool XK, class Epi>
 __global__ __launch_bounds__(Epi::Shape::THREADS, Epi::Shape::PER_SIMD) void gemm16_kernel(Args a, Epi epi) {
@@ -270,48 +274,62 @@ __global__ __launch_bounds__(Epi::Shape::THREADS, Epi::Shape::PER_SIMD) void gem
             s1 = uint32_t(uint64_t(total_stages) * (tile.part + 1) / a.parts);
         }
     };
-    // stage s of the tile into slot `slot` (past the last stage: zeros)
-    auto issue = [&](uint32_t s, uint32_t slot) {
+    // load i of the tile's stage s into slot `slot` (past the last stage: zeros)
+    constexpr int LQ = decltype(fq_)::LPW, LX = decltype(fx_)::LPW;
+    auto issue_one = [&](uint32_t s, uint32_t slot, int i) {
         const bool ok = s < s1;
         const uint32_t k = PLANES ? s / 3u : s, seg = PLANES ? s - 3u * k : 0u;  // (a k's planes are read together)
         const uint32_t sb = lds0 + slot * uint32_t(STAGE);
-        fq_.issue(k, seg == 2, ok, sb);
-        fx_.issue(k, seg == 1, ok, sb);
+        if (i < LQ) fq_.issue(k, seg == 2, ok, sb, i);
+        else fx_.issue(k, seg == 1, ok, sb, i - LQ);
+    };
+    auto issue = [&](uint32_t s, uint32_t slot) {
+#pragma unroll
+        for (int i = 0; i < LQ + LX; ++i) issue_one(s, slot, i);
     };
 
     f32x16 acc[2][2];
     u32x4 fx[2][2], fq[2][2];
-    auto read_frags = [&](int buf, uint32_t slot, int t) {
+    auto read_one = [&](int buf, uint32_t slot, int t, int i) {
         const char* base = lds + slot * STAGE;
-#pragma unroll
-        for (int m = 0; m < 2; ++m) fx[buf][m] = fx_.read(base, m, t);
-#pragma unroll
-        for (int n = 0; n < 2; ++n) fq[buf][n] = fq_.read(base, n, t);
+        if (i < 2) fx[buf][i] = fx_.read(base, i, t);
+        else fq[buf][i - 2] = fq_.read(base, i - 2, t);
     };
-    auto mma = [&](int buf) {
+    // One k-step: four MFMAs, and behind each of them, in this order, the read of one of the next k-step's
+    // fragments and a share of the loads into the slot that this stage leaves.
+    auto step = [&](int cur, uint32_t slot_next, int t_next, auto more, uint32_t s_load, uint32_t slot_load) {
 #pragma unroll
-        for (int m = 0; m < 2; ++m)
+        for (int i = 0; i < 4; ++i) {
+            const int m = i & 1, n = i >> 1;
+            acc[m][n] = mfma<BF16>(fx[cur][m], fq[cur][n], acc[m][n]);
+            __builtin_amdgcn_sched_barrier(0);
+            read_one(cur ^ 1, slot_next, t_next, (i & 1) * 2 + (i >> 1));
+            if constexpr (decltype(more)::value) {
 #pragma unroll
-            for (int n = 0; n < 2; ++n) acc[m][n] = mfma<BF16>(fx[buf][m], fq[buf][n], acc[m][n]);
-        // the next k-step's fragment reads (two a fragment across k) go between the four MFMAs
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(0x100, XK ? 2 : 1, 0);
-        }
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(0x100, QK ? 2 : 1, 0);
+                for (int l = i * (LQ + LX) / 4; l < (i + 1) * (LQ + LX) / 4; ++l) issue_one(s_load, slot_load, l);
+            }
+            __builtin_amdgcn_sched_barrier(0);
         }
     };
     // a workgroup barrier that leaves the direct loads in flight; this wave's LDS reads are done
     auto barrier = [&]() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
+    // stage i of the tile's; more: stage i + 2 follows
+    auto stage = [&](uint32_t i, auto more) {
+        const uint32_t slot = i & 1u;
+#pragma unroll
+        for (int t = 0; t < KC / 16 - 1; ++t) step(t & 1, slot, t + 1, std::false_type(), 0, 0);
+        // the last k-step's fragments are in registers: publish the next stage, free this slot
+        wait_vmcnt<0>();
+        barrier();
+        __builtin_amdgcn_sched_barrier(0);
+        step((KC / 16 - 1) & 1, slot ^ 1u, 0, more, s0 + i + 2, slot);
+    };
 
     typename Epi::State st;
     open();
     epi.begin(st, smem, tile);
     issue(s0, 0);  // later tiles: during the previous epilogue
+    bool settled = false;
     for (;;) {
         epi.load(st, tile, tid);
 #pragma unroll
@@ -322,27 +340,16 @@ __global__ __launch_bounds__(Epi::Shape::THREADS, Epi::Shape::PER_SIMD) void gem
                 for (int v = 0; v < 16; ++v) acc[m][n][v] = 0.0f;
         barrier();  // every wave is past the previous tile's main loop: slot 1 is free
         issue(s0 + 1, 1);
-        wait_vmcnt<8 / Sh::WQ + 8 / Sh::WR>();  // stage 0 (older than stage 1's loads)
-        barrier();
-        read_frags(0, 0, 0);
-        const uint32_t ns = s1 - s0;
-        for (uint32_t s = 0; s < ns; ++s) {
-            const uint32_t slot = s & 1u;
-#pragma unroll
-            for (int t = 0; t < KC / 16; ++t) {
-                const int cur = t & 1;
-                if (t == KC / 16 - 1) {
-                    // this k-step's fragments are in registers: publish the next stage, free this slot
-                    wait_vmcnt<0>();
-                    barrier();
-                    if (s + 2 < ns) issue(s0 + s + 2, slot);
-                    read_frags(cur ^ 1, slot ^ 1u, 0);
-                } else {
-                    read_frags(cur ^ 1, slot, t + 1);
-                }
-                mma(cur);
-            }
+        if (!settled) {
+            wait_vmcnt<LQ + LX>();  // stage 0 (older than stage 1's loads)
+            barrier();
         }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) read_one(0, 0, 0, i);
+        const uint32_t ns = s1 - s0;
+        uint32_t i = 0;
+        for (; i + 2 < ns; ++i) stage(i, std::true_type());
+        for (; i < ns; ++i) stage(i, std::false_type());
         epi.publish(st, smem, tid);
         __syncthreads();  // every wave is past the main loop: slot 0 is free
         const Tiles<Epi::kWalk> here = tile;
@@ -355,7 +362,10 @@ __global__ __launch_bounds__(Epi::Shape::THREADS, Epi::Shape::PER_SIMD) void gem
         // addresses would take the registers that the fragments need
         Lane le = ln;
         asm volatile("" : "+v"(le.l32), "+v"(le.hh));
-        epi.tile(st, smem, le, acc, here, lds + STAGE + wave * 4096);
+        // An epilogue that stores much waits for the next tile's first stage before its first store: behind the
+        // stores, that wait would be for all of them.
+        settled = Epi::kStores;
+        epi.tile(st, smem, le, acc, here, lds + STAGE + wave * 4096, [] { wait_vmcnt<0>(); });
         if (last) {
             epi.end(st, smem, ln, here);
             if (!tile.ok) break;

@@ -34,6 +34,7 @@ using g16::f32x4;
 using g16::u32x4;
 
 constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLn2 = 0.69314718055994530942f;
 
 // ---- element types -----------------------------------------------------------------------------
 template <int DT>
@@ -93,9 +94,10 @@ __device__ __forceinline__ void join(float& m, float& z, float m2, float z2) {
 }
 
 // ---- packing: operands whose rows are not whole 64-value stages, not 16-bit, or must not be read -----
-// dst[r][k] = src[r][k], zeros for k in [D, Kp); rows whose drop value says so are zeros
+// dst[r][k] = src[r][k], zeros for k in [D, Kp); rows whose drop value says so are zeros.  Nothing if *run_if is zero.
 __global__ __launch_bounds__(256) void pack16_kernel(const uint16_t* __restrict__ src, uint64_t ld, uint32_t D, uint32_t Kp,
-                                                     const float* __restrict__ drop, float drop_if, uint16_t* __restrict__ dst, uint64_t n8) {
+                                                     const float* __restrict__ drop, float drop_if, const uint32_t* run_if, uint16_t* __restrict__ dst, uint64_t n8) {
+    if (run_if && *run_if == 0) return;
     typedef uint16_t u16x8 __attribute__((ext_vector_type(8), aligned(2)));
     const uint32_t per = Kp / 8;
     for (uint64_t i = uint64_t(blockIdx.x) * 256 + threadIdx.x; i < n8; i += uint64_t(gridDim.x) * 256) {
@@ -172,6 +174,20 @@ __global__ __launch_bounds__(256) void pack32_kernel(const float* __restrict__ s
     for (uint32_t k = 1024 + 4 * lane; k < Kp; k += 256) put(k, load4(k));
 }
 
+// *odd = 1 (0 before the launch) if a masked item holds NaN or inf, or if an offset is finite and beyond
+// 1e37 (log2 e times it may not be).  One wave per 64 items; masked rows are read.
+__global__ __launch_bounds__(256) void xent_odd_kernel(const uint16_t* __restrict__ items, uint64_t ld, const float* __restrict__ offsets, uint32_t V,
+                                                       uint32_t D, uint32_t exponent, uint32_t* odd) {
+    const uint32_t lane = threadIdx.x & 63, j0 = (blockIdx.x * 4 + (threadIdx.x >> 6)) * 64;
+    const float o = j0 + lane < V ? offsets[j0 + lane] : 0.0f;
+    bool bad = fabsf(o) > 1e37f && fabsf(o) < INFINITY;
+    for (uint64_t masked = __ballot(o == -INFINITY); masked; masked &= masked - 1) {
+        const uint16_t* row = items + (j0 + uint32_t(__builtin_ctzll(masked))) * ld;
+        for (uint32_t d = lane; d < D; d += 64) bad |= (row[d] & exponent) == exponent;
+    }
+    if (__any(bad) && lane == 0) *odd = 1;
+}
+
 // out = the bits of the largest |src| (0 before the launch); rows whose drop value says so are left out
 __global__ __launch_bounds__(256) void absmax_kernel(const float* __restrict__ src, uint64_t ld, uint32_t R, uint32_t D,
                                                      const float* __restrict__ drop, float drop_if, uint32_t* out) {
@@ -198,51 +214,72 @@ __global__ __launch_bounds__(256) void absmax_kernel(const float* __restrict__ s
 }
 
 // ---- the logits' epilogues -------------------------------------------------------------------------
+// The offsets of a launch: none, none but -inf for the items missing from the last tile, or any.
+enum Offsets : int { OFF_NONE = 0, OFF_EDGE = 1, OFF_ANY = 2 };
+
 struct LogitArgs {
     const float* offsets;  // of the launch's first item (nullptr: zeros)
+    const uint32_t* odd;   // OFF_ANY: zero if no masked item holds NaN or inf and no offset is near fp32's
+                           // limits (nullptr: not known)
     const float* qinv;     // fp32 operands: the rows' and the items' inverse scales
     const float* xinv;
     float scale;
     uint32_t rows, items;  // hidden rows; items of this launch
 };
 
-// What the epilogue needs of a tile's items, and the logit of one accumulator.  OFF: there are
-// offsets, or the last tile is not whole (its missing items get offset -inf).
-template <bool OFF, bool PLANES, int TR>
+// The epilogues work on logits in the unit of a binary exponent (log2 e of them: one fma takes an
+// accumulator there, and exp2 of a difference is one instruction more than the subtraction) unless that could
+// go wrong: odd offsets (masked items are then told by their offset whatever their accumulator holds, and
+// differences are taken before they are scaled: an offset of the type's lowest value stays in range) and fp32
+// operands (whose items have scales of their own) keep natural units.
+template <int OFF, bool PLANES, int TR>
 struct LogitShared {
     float off[OFF ? TR : 1];
     float inv[PLANES ? TR : 1];
 };
-template <bool OFF, bool PLANES, int TR>
+template <bool NATURAL, int OFF, bool PLANES, int TR>
 __device__ __forceinline__ f32x4 logits4(const LogitShared<OFF, PLANES, TR>& sm, const f32x16& acc, int j, int r, float c) {
     f32x4 v;
     f32x4 o{}, x{};
-    asm volatile("" ::: "memory");  // these reads stay here: hoisted, a tile's would fill the registers
-    if constexpr (OFF) o = *reinterpret_cast<const f32x4*>(sm.off + r);
+    // these reads stay here, and the groups in order: mixed, a tile's would fill the registers
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (OFF != OFF_NONE) o = *reinterpret_cast<const f32x4*>(sm.off + r);
     if constexpr (PLANES) x = *reinterpret_cast<const f32x4*>(sm.inv + r);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
         float a = acc[4 * j + e];
         if constexpr (PLANES) a *= x[e];
-        if constexpr (OFF) v[e] = o[e] == -INFINITY ? -INFINITY : fmaf(a, c, o[e]);
-        else v[e] = a * c;
+        if constexpr (OFF == OFF_NONE) v[e] = a * c;
+        else v[e] = NATURAL && o[e] == -INFINITY ? -INFINITY : fmaf(a, c, o[e]);
     }
     return v;
 }
-
-// exp(v - ref).  The difference is taken first: where v is near ref (the items that matter) it is exact,
-// and it stays in range for offsets as low as the type's lowest value.
-__device__ __forceinline__ float exp_diff(float v, float ref) { return __builtin_amdgcn_exp2f((v - ref) * kLog2e); }
+template <bool NATURAL>
+__device__ __forceinline__ float exp_diff(float v, float ref) {
+    return __builtin_amdgcn_exp2f(NATURAL ? (v - ref) * kLog2e : v - ref);
+}
+// whether a launch keeps natural units (uniform)
+template <int OFF, bool PLANES>
+__device__ __forceinline__ bool keeps_natural(const LogitArgs& a) {
+    if constexpr (PLANES) return true;
+    if constexpr (OFF != OFF_ANY) return false;
+    return __builtin_amdgcn_readfirstlane(a.odd ? *a.odd : 1u) != 0u;
+}
+__device__ __forceinline__ float offset_of(const LogitArgs& a, bool in, uint32_t r, bool natural) {
+    const float o = !in ? -INFINITY : a.offsets ? a.offsets[r] : 0.0f;
+    return natural ? o : o * kLog2e;
+}
 
 // Forward: the running (m, z) of a lane's items per query; joined over the workgroup at the end of
 // the item and written to part[row * slots + slot].  The target's logit is picked out on the way: with
 // the loss a difference of two logits, both from the same sums, their errors cancel for a row whose
 // target is far ahead of the other items.
-template <class Sh, bool OFF, bool PLANES>
+template <class Sh, int OFF, bool PLANES>
 struct LseEpi {
     using Shape = Sh;
     static constexpr int TQ = Sh::TQ, TR = Sh::TR;
-    static constexpr bool kWalk = true;
+    static constexpr bool kWalk = true, kStores = false;
     LogitArgs a;
     const int64_t* targets;
     uint32_t item0;  // of the launch
@@ -257,9 +294,11 @@ struct LseEpi {
     struct State {
         float m[2], z[2];
         float off, inv;
+        bool natural;
     };
     template <class Tile>
     __device__ void begin(State& s, Shared& sm, const Tile& t) {
+        s.natural = keeps_natural<OFF, PLANES>(a);
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
             s.m[n] = -INFINITY;
@@ -275,61 +314,74 @@ struct LseEpi {
     __device__ void load(State& s, const Tile& t, int tid) {
         const uint32_t r = t.rb * TR + uint32_t(tid);
         const bool in = tid < TR && r < a.items;
-        if constexpr (OFF) s.off = !in ? -INFINITY : a.offsets ? a.offsets[r] : 0.0f;
+        if constexpr (OFF != OFF_NONE) s.off = offset_of(a, in, r, s.natural);
         if constexpr (PLANES) s.inv = in ? a.xinv[r] : 0.0f;
     }
     __device__ void publish(State& s, Shared& sm, int tid) {
-        if constexpr (OFF)
+        if constexpr (OFF != OFF_NONE)
             if (tid < TR) sm.off[tid] = s.off;
         if constexpr (PLANES)
             if (tid < TR) sm.inv[tid] = s.inv;
     }
-    template <class Tile>
-    __device__ void tile(State& s, Shared& sm, const g16::Lane& ln, f32x16 (&acc)[2][2], const Tile& t, char*) {
+    template <bool NATURAL, class Tile>
+    __device__ void block(State& s, Shared& sm, const g16::Lane& ln, f32x16 (&acc)[2][2], const Tile& t, int n) {
+        const float c = (PLANES ? a.scale * sm.qinv[ln.q(n)] : a.scale) * (NATURAL ? 1.0f : kLog2e);
+        float top = -INFINITY;
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                f32x4 v = logits4<NATURAL, OFF, PLANES, TR>(sm, acc[m][n], j, ln.r(m, j), c);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    top = fmaxf(top, v[e]);
+                    acc[m][n][4 * j + e] = v[e];
+                }
+            }
+        const float mm = fmaxf(s.m[n], top);
+        const float ref = mm == -INFINITY ? 0.0f : mm;
+        const float z = s.z[n] * exp_diff<NATURAL>(s.m[n], ref);
+        // (a tile holds the target of few rows, most tiles of none of a wave's)
+        const uint32_t y = sm.target[ln.q(n)] - t.rb * TR - uint32_t(ln.wr * 64);
+        if (__any(y < 64u)) {
+            const uint32_t i = y - 4u * uint32_t(ln.hh);  // 32 m + 8 j + e of the lane's values
+            float v = 0.0f;
+#pragma unroll
+            for (int m = 0; m < 2; ++m)
+#pragma unroll
+                for (int k = 0; k < 16; ++k) v = i == uint32_t(32 * m + 8 * (k >> 2) + (k & 3)) ? acc[m][n][k] : v;
+            if (y < 64u && (i & 4u) == 0u) picked[t.qb * TQ + ln.q(n)] = NATURAL ? v : v * kLn2;
+        }
+        float zz[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) zz[v & 3] += exp_diff<NATURAL>(acc[m][n][v], ref);
+        s.m[n] = mm;
+        s.z[n] = z + ((zz[0] + zz[1]) + (zz[2] + zz[3]));
+    }
+    template <class Tile, class Settle>
+    __device__ void tile(State& s, Shared& sm, const g16::Lane& ln, f32x16 (&acc)[2][2], const Tile& t, char*, Settle) {
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
-            const float c = PLANES ? a.scale * sm.qinv[ln.q(n)] : a.scale;
-            float top = -INFINITY;
-#pragma unroll
-            for (int m = 0; m < 2; ++m)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    f32x4 v = logits4<OFF, PLANES, TR>(sm, acc[m][n], j, ln.r(m, j), c);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        top = fmaxf(top, v[e]);
-                        acc[m][n][4 * j + e] = v[e];
-                    }
-                }
-            const float mm = fmaxf(s.m[n], top);
-            const float ref = mm == -INFINITY ? 0.0f : mm;
-            const float z = s.z[n] * exp_diff(s.m[n], ref);
-            // (a tile holds the target of few rows, most tiles of none of a wave's)
-            const uint32_t y = sm.target[ln.q(n)] - t.rb * TR - uint32_t(ln.wr * 64);
-            if (__any(y < 64u)) {
-                const uint32_t i = y - 4u * uint32_t(ln.hh);  // 32 m + 8 j + e of the lane's values
-                float v = 0.0f;
-#pragma unroll
-                for (int m = 0; m < 2; ++m)
-#pragma unroll
-                    for (int k = 0; k < 16; ++k) v = i == uint32_t(32 * m + 8 * (k >> 2) + (k & 3)) ? acc[m][n][k] : v;
-                if (y < 64u && (i & 4u) == 0u) picked[t.qb * TQ + ln.q(n)] = v;
+            if constexpr (PLANES) {
+                block<true>(s, sm, ln, acc, t, n);
+            } else if constexpr (OFF != OFF_ANY) {
+                block<false>(s, sm, ln, acc, t, n);
+            } else {
+                if (s.natural) block<true>(s, sm, ln, acc, t, n);
+                else block<false>(s, sm, ln, acc, t, n);
             }
-            float zz[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int m = 0; m < 2; ++m)
-#pragma unroll
-                for (int v = 0; v < 16; ++v) zz[v & 3] += exp_diff(acc[m][n][v], ref);
-            s.m[n] = mm;
-            s.z[n] = z + ((zz[0] + zz[1]) + (zz[2] + zz[3]));
         }
     }
     template <class Tile>
     __device__ void end(State& s, Shared& sm, const g16::Lane& ln, const Tile& t) {
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
-            join(s.m[n], s.z[n], __shfl_xor(s.m[n], 32), __shfl_xor(s.z[n], 32));
-            if (ln.hh == 0) sm.red[ln.wr][ln.q(n)] = make_float2(s.m[n], s.z[n]);
+            // (natural units from here; a row's largest logit and its target's are scaled alike)
+            float m = s.natural ? s.m[n] : s.m[n] * kLn2;
+            join(m, s.z[n], __shfl_xor(m, 32), __shfl_xor(s.z[n], 32));
+            if (ln.hh == 0) sm.red[ln.wr][ln.q(n)] = make_float2(m, s.z[n]);
         }
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
         const uint32_t q = threadIdx.x;
@@ -345,11 +397,11 @@ struct LseEpi {
 
 // Backward: dl of the piece's items, p[t][j]: Vp values a plane and row, zeros past the last item, rows
 // `pitch` values apart.
-template <class Sh, bool BF16, bool OFF, bool PLANES>
+template <class Sh, bool BF16, int OFF, bool PLANES>
 struct GradEpi {
     using Shape = Sh;
     static constexpr int TQ = Sh::TQ, TR = Sh::TR;
-    static constexpr bool kWalk = false;
+    static constexpr bool kWalk = false, kStores = true;
     LogitArgs a;
     const float* gk;   // g_t times dl's factor (0: the row has no gradient)
     const float* lse;
@@ -365,25 +417,35 @@ struct GradEpi {
     struct State {
         float off, inv, gk, lse, qinv;
         uint32_t target;
+        bool natural;
     };
     template <class Tile>
-    __device__ void begin(State&, Shared&, const Tile&) {}
+    __device__ void begin(State& s, Shared&, const Tile&) {
+        s.natural = keeps_natural<OFF, PLANES>(a);
+    }
     template <class Tile>
     __device__ void load(State& s, const Tile& t, int tid) {
         const uint32_t r = t.rb * TR + uint32_t(tid), q = t.qb * TQ + uint32_t(tid);
         const bool in = tid < TR && r < a.items, qin = tid < TQ && q < a.rows;
-        if constexpr (OFF) s.off = !in ? -INFINITY : a.offsets ? a.offsets[r] : 0.0f;
+        if constexpr (OFF != OFF_NONE) s.off = offset_of(a, in, r, s.natural);
         if constexpr (PLANES) {
             s.inv = in ? a.xinv[r] : 0.0f;
             s.qinv = qin ? a.qinv[q] : 0.0f;
         }
         s.gk = qin ? gk[q] : 0.0f;
         s.lse = qin ? lse[q] : 0.0f;
+        // a row without a gradient, or without any item: every probability is exp(-huge) = 0
+        if (s.gk == 0.0f || s.lse == -INFINITY) {
+            s.gk = 0.0f;
+            s.lse = FLT_MAX;
+        } else if (!s.natural) {
+            s.lse *= kLog2e;
+        }
         const int64_t y = qin ? targets[q] - int64_t(item0) : -1;
         s.target = y >= 0 && y < int64_t(a.items) ? uint32_t(y) : 0xFFFFFFFFu;
     }
     __device__ void publish(State& s, Shared& sm, int tid) {
-        if constexpr (OFF)
+        if constexpr (OFF != OFF_NONE)
             if (tid < TR) sm.off[tid] = s.off;
         if constexpr (PLANES)
             if (tid < TR) sm.inv[tid] = s.inv;
@@ -410,42 +472,52 @@ struct GradEpi {
         }
         asm volatile("" ::: "memory");  // and the reads before what is written next
     }
-    template <class Tile>
-    __device__ void tile(State&, Shared& sm, const g16::Lane& ln, f32x16 (&acc)[2][2], const Tile& t, char* spare) {
+    static __device__ void write(char* spare, const g16::Lane& ln, int m, int j, const uint16_t (&v)[4]) {
+        *reinterpret_cast<uint2*>(spare + ln.l32 * 128 + 16 * ((4 * m + j) ^ (ln.l32 & 7)) + 8 * ln.hh) =
+            make_uint2(v[0] | uint32_t(v[1]) << 16, v[2] | uint32_t(v[3]) << 16);
+    }
+    // TARGETS: one of the wave's rows has its target among the block's items
+    template <bool NATURAL, bool TARGETS>
+    __device__ void block(Shared& sm, const g16::Lane& ln, f32x16 (&acc)[2][2], uint32_t y, int n, char* spare) {
+        const float g = sm.gk[ln.q(n)], ref = sm.lse[ln.q(n)];
+        const float c = (PLANES ? a.scale * sm.inv_q[ln.q(n)] : a.scale) * (NATURAL ? 1.0f : kLog2e);
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int r = ln.r(m, j);
+                const f32x4 v = logits4<NATURAL, OFF, PLANES, TR>(sm, acc[m][n], j, r, c);
+                uint16_t hi[4], lo[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float d = exp_diff<NATURAL>(v[e], ref);
+                    if (TARGETS && y == uint32_t(r + e) && v[e] != -INFINITY) d -= 1.0f;
+                    d *= g;
+                    if constexpr (PLANES) {
+                        split16(d, hi[e], lo[e]);
+                        acc[m][n][4 * j + e] = d;
+                    } else {
+                        hi[e] = bits16<BF16>(d);
+                    }
+                }
+                write(spare, ln, m, j, hi);
+            }
+    }
+    template <class Tile, class Settle>
+    __device__ void tile(State& s, Shared& sm, const g16::Lane& ln, f32x16 (&acc)[2][2], const Tile& t, char* spare, Settle settle) {
         const uint32_t r0 = t.rb * TR, rw = r0 + uint32_t(ln.wr * 64);
-        const int swz = ln.l32 & 7;
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
-            const float g = sm.gk[ln.q(n)], ref = sm.lse[ln.q(n)];
-            const float c = PLANES ? a.scale * sm.inv_q[ln.q(n)] : a.scale;
-            const uint32_t y = sm.target[ln.q(n)] - r0;
-            const bool none = g == 0.0f || ref == -INFINITY;
-            const uint32_t q0 = t.qb * TQ + uint32_t(ln.wq * 64 + 32 * n);
-            auto write = [&](int m, int j, const uint16_t (&v)[4]) {
-                *reinterpret_cast<uint2*>(spare + ln.l32 * 128 + 16 * ((4 * m + j) ^ swz) + 8 * ln.hh) =
-                    make_uint2(v[0] | uint32_t(v[1]) << 16, v[2] | uint32_t(v[3]) << 16);
-            };
-#pragma unroll
-            for (int m = 0; m < 2; ++m)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const uint32_t r = uint32_t(ln.r(m, j));
-                    const f32x4 v = logits4<OFF, PLANES, TR>(sm, acc[m][n], j, int(r), c);
-                    uint16_t hi[4], lo[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        float d = exp_diff(v[e], ref);
-                        if (y == r + e && v[e] != -INFINITY) d -= 1.0f;
-                        d = none ? 0.0f : d * g;
-                        if constexpr (PLANES) {
-                            split16(d, hi[e], lo[e]);
-                            acc[m][n][4 * j + e] = d;
-                        } else {
-                            hi[e] = bits16<BF16>(d);
-                        }
-                    }
-                    write(m, j, hi);
-                }
+            const uint32_t q0 = t.qb * TQ + uint32_t(ln.wq * 64 + 32 * n), y = sm.target[ln.q(n)] - r0;
+            const bool hit = __any(y - uint32_t(ln.wr * 64) < 64u);
+            if constexpr (PLANES) {
+                block<true, true>(sm, ln, acc, y, n, spare);
+            } else {
+                if (OFF == OFF_ANY && s.natural) block<true, true>(sm, ln, acc, y, n, spare);
+                else if (hit) block<false, true>(sm, ln, acc, y, n, spare);
+                else block<false, false>(sm, ln, acc, y, n, spare);
+            }
+            if (n == 0) settle();
             put(spare, ln, q0, rw, 0);
             if constexpr (PLANES) {
 #pragma unroll
@@ -455,7 +527,7 @@ struct GradEpi {
                         uint16_t hi[4], lo[4];
 #pragma unroll
                         for (int e = 0; e < 4; ++e) split16(acc[m][n][4 * j + e], hi[e], lo[e]);
-                        write(m, j, lo);
+                        write(spare, ln, m, j, lo);
                     }
                 put(spare, ln, q0, rw, 1);
             }
@@ -470,7 +542,7 @@ template <class Sh>
 struct ShareEpi {
     using Shape = Sh;
     static constexpr int TQ = Sh::TQ, TR = Sh::TR;
-    static constexpr bool kWalk = false;
+    static constexpr bool kWalk = false, kStores = true;
     float* out;
     uint32_t rows, D, Dp;
     bool first;
@@ -481,8 +553,9 @@ struct ShareEpi {
     template <class Tile>
     __device__ void load(State&, const Tile&, int) {}
     __device__ void publish(State&, Shared&, int) {}
-    template <class Tile>
-    __device__ void tile(State&, Shared&, const g16::Lane& ln, f32x16 (&acc)[2][2], const Tile& t, char*) {
+    template <class Tile, class Settle>
+    __device__ void tile(State&, Shared&, const g16::Lane& ln, f32x16 (&acc)[2][2], const Tile& t, char*, Settle settle) {
+        settle();
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
             const uint32_t q = t.qb * TQ + uint32_t(ln.q(n));
@@ -511,7 +584,7 @@ template <class Sh, int DT>
 struct ItemGradEpi {
     using Shape = Sh;
     static constexpr int TQ = Sh::TQ, TR = Sh::TR;
-    static constexpr bool kWalk = false;
+    static constexpr bool kWalk = false, kStores = true;
     ElemT<DT>* out;
     uint64_t ld;
     uint32_t rows, D;
@@ -529,8 +602,9 @@ struct ItemGradEpi {
     __device__ void publish(State&, Shared& sm, int tid) {
         if (tid == 0) sm.mul = *mul / (DT == VA_DTYPE_F32 ? scale_to_2p14(__builtin_bit_cast(float, *absmax)) : 1.0f);
     }
-    template <class Tile>
-    __device__ void tile(State&, Shared& sm, const g16::Lane& ln, f32x16 (&acc)[2][2], const Tile& t, char*) {
+    template <class Tile, class Settle>
+    __device__ void tile(State&, Shared& sm, const g16::Lane& ln, f32x16 (&acc)[2][2], const Tile& t, char*, Settle settle) {
+        settle();
         const float s = sm.mul;
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
@@ -622,13 +696,13 @@ __global__ __launch_bounds__(1024) void xent_reduce_kernel(const float* __restri
 }
 
 // gk[t] = g_t c, *mul = scale / c: g_t is the gradient that reaches the row's loss, 0 for a row
-// without a target, c takes the largest |g_t| to 2^14.  Clears absmax[0..2).  One workgroup.
+// without a target, c takes the largest |g_t| to 2^14.  Clears absmax[0..3).  One workgroup.
 __global__ __launch_bounds__(1024) void xent_gradient_kernel(const float* __restrict__ grad, const int64_t* __restrict__ targets,
                                                              uint32_t T, uint32_t V, int64_t ignore, int reduction, float scale,
                                                              float* __restrict__ gk, float* __restrict__ mul, uint32_t* absmax) {
     __shared__ float top[16];
     __shared__ uint32_t cnt[16];
-    if (threadIdx.x < 2) absmax[threadIdx.x] = 0;
+    if (threadIdx.x < 3) absmax[threadIdx.x] = 0;
     float m = 0.0f;
     uint32_t c = 0;
     for (uint32_t t = threadIdx.x; t < T; t += 1024) {
@@ -701,14 +775,14 @@ bool direct(va_dtype dt, const void* p, uint64_t ld, uint32_t D) {
 size_t packed_bytes(va_dtype dt, uint64_t rows, uint32_t Kp) { return rows * Kp * (dt == VA_DTYPE_F32 ? 4 : 2); }
 
 va_status pack(va_context* ctx, va_dtype dt, const void* src, uint64_t ld, uint32_t R, uint32_t D, uint32_t Kp, const uint32_t* absmax,
-               const float* drop, float drop_if, void* dst, float* inv) {
+               const float* drop, float drop_if, void* dst, float* inv, const uint32_t* run_if = nullptr) {
     if (dt == VA_DTYPE_F32) {
         pack32_kernel<<<dim3(ceil_div(R, 4)), dim3(256), 0, ctx->stream>>>(static_cast<const float*>(src), ld, R, D, Kp, absmax, drop, drop_if,
                                                                            static_cast<uint16_t*>(dst), inv);
     } else {
         const uint64_t n8 = uint64_t(R) * (Kp / 8);
         pack16_kernel<<<dim3(uint32_t(std::min<uint64_t>((n8 + 255) / 256, 16384))), dim3(256), 0, ctx->stream>>>(
-            static_cast<const uint16_t*>(src), ld, D, Kp, drop, drop_if, static_cast<uint16_t*>(dst), n8);
+            static_cast<const uint16_t*>(src), ld, D, Kp, drop, drop_if, run_if, static_cast<uint16_t*>(dst), n8);
     }
     VA_CHECK_LAUNCH(ctx);
     return VA_OK;
@@ -741,11 +815,18 @@ Blocks blocks_for(const va_context* ctx, uint64_t Q, uint64_t R, uint32_t shares
     return all[2];
 }
 
+// f(bf16, offsets, planes) of a launch over n items of a tile width
 template <class F>
-va_status by_type(va_dtype dt, bool off, F&& f) {
-    if (dt == VA_DTYPE_F32) return off ? f(std::false_type(), std::true_type(), std::true_type()) : f(std::false_type(), std::false_type(), std::true_type());
-    if (dt == VA_DTYPE_F16) return off ? f(std::false_type(), std::true_type(), std::false_type()) : f(std::false_type(), std::false_type(), std::false_type());
-    return off ? f(std::true_type(), std::true_type(), std::false_type()) : f(std::true_type(), std::false_type(), std::false_type());
+va_status by_type(va_dtype dt, bool offsets, bool edge, F&& f) {
+    using std::integral_constant;
+    const integral_constant<int, OFF_NONE> none{};
+    const integral_constant<int, OFF_EDGE> some{};
+    const integral_constant<int, OFF_ANY> any{};
+    const std::false_type no{};
+    const std::true_type yes{};
+    if (dt == VA_DTYPE_F32) return offsets || edge ? f(no, any, yes) : f(no, none, yes);
+    if (dt == VA_DTYPE_F16) return offsets ? f(no, any, no) : edge ? f(no, some, no) : f(no, none, no);
+    return offsets ? f(yes, any, no) : edge ? f(yes, some, no) : f(yes, none, no);
 }
 
 va_status check_desc(va_context* ctx, const va_xent_desc* d, const char* who) {
@@ -761,6 +842,21 @@ va_status check_desc(va_context* ctx, const va_xent_desc* d, const char* who) {
     const size_t es = elem_size(d->dtype);
     VA_REQUIRE(ctx, reinterpret_cast<uintptr_t>(d->hidden) % es == 0 && reinterpret_cast<uintptr_t>(d->items) % es == 0,
                "%s: rows or items are not aligned to their type", who);
+    return VA_OK;
+}
+
+// A scale at which the logits' other unit might overflow: natural units (as with odd offsets).
+bool wild_scale(const va_xent_desc* d) { return fabsf(d->scale) > 1e18f; }
+// Whether offsets are looked over first, so that usual ones take the shorter epilogue: 16-bit operands, and
+// products that are bound by the matrix cores (4096 rows x 262,144 items of 768: the check takes 10 us and
+// saves 150; a product that streams its items hides the longer epilogue).
+bool worth_checking(const va_xent_desc* d, const Blocks& b) {
+    return d->offsets && d->dtype != VA_DTYPE_F32 && !wild_scale(d) && b.shape == 0;
+}
+va_status find_odd(va_context* ctx, const va_xent_desc* d, uint32_t* odd) {
+    xent_odd_kernel<<<dim3(ceil_div(d->num_items, 256)), dim3(256), 0, ctx->stream>>>(
+        static_cast<const uint16_t*>(d->items), d->items_stride, d->offsets, d->num_items, d->dim, d->dtype == VA_DTYPE_F16 ? 0x7C00u : 0x7F80u, odd);
+    VA_CHECK_LAUNCH(ctx);
     return VA_OK;
 }
 
@@ -799,6 +895,7 @@ va_status va_xent_forward(va_context* ctx, const va_xent_desc* d, float* out_los
     const uint32_t piece = xd ? round_up(V, 256) : piece_items(V, packed_bytes(dt, 1, Kp), kPackBudget);
     const uint32_t pieces = ceil_div(V, piece);
     const Blocks bl = blocks_for(ctx, T, std::min(piece, V));
+    const bool wild = wild_scale(d), checks = worth_checking(d, bl);
     const uint32_t nq = bl.nq(T);
     // parts per query block: whole multiples of the XCDs when there are that many
     uint32_t parts = std::max(bl.grid / nq, 1u);
@@ -810,10 +907,16 @@ va_status va_xent_forward(va_context* ctx, const va_xent_desc* d, float* out_los
     Scratch sc(ctx);
     const size_t need = (qd ? 0 : Scratch::round(packed_bytes(dt, T, Kp)) + Scratch::round(T * 4ull)) +
                         (xd ? 0 : Scratch::round(packed_bytes(dt, piece, Kp)) + Scratch::round(piece * 4ull)) +
-                        Scratch::round(uint64_t(T) * slots * sizeof(float2)) + Scratch::round(T * 4ull);
+                        Scratch::round(uint64_t(T) * slots * sizeof(float2)) + Scratch::round(T * 4ull) + Scratch::round(4);
     VA_CHECK_STATUS(sc.reserve(need));
     float2* part = sc.carve<float2>(uint64_t(T) * slots);
     float* picked = sc.carve<float>(T);
+    uint32_t* odd = nullptr;
+    if (checks) {
+        odd = sc.carve<uint32_t>(1);
+        VA_CHECK_STATUS(fill_u32(ctx, odd, 1, 0));
+        VA_CHECK_STATUS(find_odd(ctx, d, odd));
+    }
     char* qp = nullptr;
     char* xp = nullptr;
     float* qinv = nullptr;
@@ -841,9 +944,9 @@ va_status va_xent_forward(va_context* ctx, const va_xent_desc* d, float* out_los
         a.parts = c + 1 < pieces ? parts : last_parts;
         VA_CHECK_STATUS(by_shape(bl.shape, [&](auto sh) {
             using Sh = decltype(sh);
-            return by_type(dt, d->offsets || n % Sh::TR, [&](auto bf, auto off, auto pl) {
+            return by_type(dt, d->offsets || wild, n % Sh::TR, [&](auto bf, auto off, auto pl) {
                 LseEpi<Sh, decltype(off)::value, decltype(pl)::value> e;
-                e.a = LogitArgs{d->offsets ? d->offsets + v0 : nullptr, qinv, xinv, d->scale, T, n};
+                e.a = LogitArgs{d->offsets ? d->offsets + v0 : nullptr, odd, qinv, xinv, d->scale, T, n};
                 e.targets = d->targets;
                 e.item0 = v0;
                 e.picked = picked;
@@ -878,8 +981,11 @@ va_status va_xent_backward(va_context* ctx, const va_xent_desc* d, const float* 
     const va_dtype dt = d->dtype;
     const bool f32 = dt == VA_DTYPE_F32;
     const size_t es = elem_size(dt), planes = f32 ? 2 : 1;
-    // masked items may hold anything, and dh sums over them: their rows are read as zeros
-    const bool xd = direct(dt, d->items, d->items_stride, D) && !d->offsets;
+    // masked items may hold anything, and dh sums over them: their rows are read as zeros, from a copy, unless
+    // they are known to be finite
+    const bool in_place = direct(dt, d->items, d->items_stride, D);
+    const bool checks = worth_checking(d, blocks_for(ctx, T, V)), wild = wild_scale(d);
+    const bool xd = in_place && !d->offsets;
     VA_REQUIRE(ctx, (!out_grad_hidden || reinterpret_cast<uintptr_t>(out_grad_hidden) % es == 0) &&
                         (!out_grad_items || reinterpret_cast<uintptr_t>(out_grad_items) % es == 0),
                "va_xent_backward: a gradient is not aligned to its type");
@@ -900,7 +1006,7 @@ va_status va_xent_backward(va_context* ctx, const va_xent_desc* d, const float* 
     const size_t qp_bytes = packed_bytes(dt, T, Kp), xp_bytes = xd ? 0 : packed_bytes(dt, std::min(piece, V), Kp);
     Scratch sc(ctx);
     const size_t need = Scratch::round(p_bytes) + Scratch::round(share_n * 4) + Scratch::round(qp_bytes) + Scratch::round(xp_bytes) +
-                        2 * Scratch::round(T * 4ull) + Scratch::round(piece * 4ull) + Scratch::round(16);
+                        2 * Scratch::round(T * 4ull) + Scratch::round(piece * 4ull) + Scratch::round(32);
     VA_CHECK_STATUS(sc.reserve(need));
     uint16_t* p = sc.carve<uint16_t>(p_bytes / 2);
     float* share = sc.carve<float>(share_n);
@@ -909,8 +1015,9 @@ va_status va_xent_backward(va_context* ctx, const va_xent_desc* d, const float* 
     float* gk = sc.carve<float>(T);
     float* qinv = sc.carve<float>(T);
     float* xinv = sc.carve<float>(piece);
-    float* mul = sc.carve<float>(4);
+    float* mul = sc.carve<float>(8);
     uint32_t* absmax = reinterpret_cast<uint32_t*>(mul + 1);  // of the hidden rows, of the items
+    uint32_t* odd = checks ? absmax + 2 : nullptr;
     VA_CHECK_STATUS(sc.verify(need));
 
     xent_gradient_kernel<<<dim3(1), dim3(1024), 0, ctx->stream>>>(grad, d->targets, T, V, d->ignore_index, int(reduction), d->scale, gk, mul, absmax);
@@ -924,14 +1031,21 @@ va_status va_xent_backward(va_context* ctx, const va_xent_desc* d, const float* 
         top(d->items, d->items_stride, V, d->offsets, -INFINITY, absmax + 1);
         VA_CHECK_LAUNCH(ctx);
     }
+    if (checks) VA_CHECK_STATUS(find_odd(ctx, d, odd));
     VA_CHECK_STATUS(pack(ctx, dt, d->hidden, d->hidden_stride, T, D, Kp, f32 ? absmax : nullptr, gk, 0.0f, qp, qinv));
+    // read in place unless a masked item is odd (the copy then has the rows' own pitch)
+    const bool either = in_place && checks && d->items_stride == Kp;
     for (uint32_t c = 0; c < pieces; ++c) {
         const uint32_t v0 = c * piece, n = std::min(piece, V - v0), Vp = round_up(n, g16::KC);
         const char* items = at(d->items, d->items_stride, v0, dt);
         const float* offsets = d->offsets ? d->offsets + v0 : nullptr;
-        if (!xd) VA_CHECK_STATUS(pack(ctx, dt, items, d->items_stride, n, D, Kp, f32 ? absmax + 1 : nullptr, offsets, -INFINITY, xp, xinv));
+        if (!xd) VA_CHECK_STATUS(pack(ctx, dt, items, d->items_stride, n, D, Kp, f32 ? absmax + 1 : nullptr, offsets, -INFINITY, xp, xinv, either ? odd : nullptr));
         const g16::Operand rows{qp, uint64_t(Kp) * 2 * planes, T, Kp * 2, Kp * 2};
-        const g16::Operand cols{xd ? items : xp, xd ? d->items_stride * es : uint64_t(Kp) * 2 * planes, n, Kp * 2, Kp * 2};
+        g16::Operand cols{xd || either ? items : xp, xd ? d->items_stride * es : uint64_t(Kp) * 2 * planes, n, Kp * 2, Kp * 2};
+        if (either) {
+            cols.other = xp;
+            cols.choose = odd;
+        }
         const uint32_t pitch = Vp * uint32_t(planes) + kRowPad;
         const g16::Operand dl{p, uint64_t(pitch) * 2, T, Vp * 2, Vp * 2};
         g16::Args a;
@@ -943,9 +1057,9 @@ va_status va_xent_backward(va_context* ctx, const va_xent_desc* d, const float* 
         a.parts = 1;
         VA_CHECK_STATUS(by_shape(lb.shape, [&](auto sh) {
             using Sh = decltype(sh);
-            return by_type(dt, offsets || n % Sh::TR, [&](auto bf, auto off, auto pl) {
+            return by_type(dt, offsets || wild, n % Sh::TR, [&](auto bf, auto off, auto pl) {
                 GradEpi<Sh, decltype(bf)::value, decltype(off)::value, decltype(pl)::value> e;
-                e.a = LogitArgs{offsets, qinv, xinv, d->scale, T, n};
+                e.a = LogitArgs{offsets, odd, qinv, xinv, d->scale, T, n};
                 e.gk = gk;
                 e.lse = lse;
                 e.targets = d->targets;
