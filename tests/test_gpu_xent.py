@@ -60,7 +60,7 @@ def test_sizes(ctx, T, V, D, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("T", [1, 5, 20, 50, 90, 150])
+@pytest.mark.parametrize("T", [1, 5, 20, 50, 90, 150, 200])
 def test_single_rows_to_many_over_a_long_collection(ctx, T, dtype):
     """More items than one round of every workgroup, a peaked softmax."""
     h, w, y, _ = _inputs(T, 70_001, 48, dtype, T, spread=3.0)
@@ -80,10 +80,10 @@ def test_large_tiles(ctx, T, V, D, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("T", [3, 70])
-def test_offsets_and_masks(ctx, T, dtype):
+@pytest.mark.parametrize("T,D", [(3, 72), (70, 72), (220, 72), (3, 65), (70, 66), (220, 33)])
+def test_offsets_and_masks(ctx, T, D, dtype):
     """Corrections; masked items that hold NaN and infinities; a masked target; the type's lowest value."""
-    h, w, y, g = _inputs(T, 900, 72, dtype, 11 + T)
+    h, w, y, g = _inputs(T, 900, D, dtype, 11 + T)
     off = torch.randn(900, generator=g) * 2.0
     masked = torch.rand(900, generator=g) < 0.3
     masked[y.cpu()] = False
@@ -120,10 +120,10 @@ def test_every_item_masked(ctx, T, value, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("T", [6, 130])
-def test_ignored_and_invalid_targets(ctx, T, dtype):
+@pytest.mark.parametrize("T,D", [(6, 64), (130, 64), (40, 50), (260, 77)])
+def test_ignored_and_invalid_targets(ctx, T, D, dtype):
     """Rows without a target hold NaN and infinities and change nothing; invalid targets give a NaN loss only."""
-    h, w, y, _ = _inputs(T, 400, 64, dtype, 3)
+    h, w, y, _ = _inputs(T, 400, D, dtype, 3)
     y[::3] = IGNORE
     _check(ctx, h, w, y)
     y[1], y[2] = 400, -1
@@ -157,7 +157,7 @@ def test_upstream_gradients(ctx, reduction, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("T,D,pad,shift", [(5, 64, 8, 0), (70, 64, 3, 0), (70, 128, 64, 1), (40, 50, 13, 1)])
+@pytest.mark.parametrize("T,D,pad,shift", [(5, 64, 8, 0), (70, 64, 3, 0), (70, 128, 64, 1), (40, 50, 13, 1), (9, 50, 14, 2), (200, 70, 2, 0), (200, 33, 1, 0)])
 def test_strided_and_misaligned_rows(ctx, T, D, pad, shift, dtype):
     """Rows within wider rows, starting off any alignment but the element's; what lies between is NaN."""
     h, w, y, _ = _inputs(T, 530, D, dtype, 23)

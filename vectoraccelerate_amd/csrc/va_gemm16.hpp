@@ -1,28 +1,35 @@
-// va_gemm16.hpp — the matrix product of two 16-bit operands, with the epilogue a template argument:
-// every product of the softmax cross entropy (va_xent.hip) is one of these.
+// va_gemm16.hpp — the matrix product of two operands, with the epilogue a template argument: every product
+// of the softmax cross entropy (va_xent.hip, va_xent_grad.hip) is one of these.
 //
-//   acc[q][r] = sum_k Q[q][k] X[r][k]        fp16 or bf16
+//   acc[q][r] = sum_k Q[q][k] X[r][k]        fp16, bf16 or fp32
 //
 // Either operand is stored with k along its rows (Q[q] is a row) or across them (k is the row: QK, XK).
 //
 // A wave computes 64 queries x 64 rows (2 x 2 blocks of v_mfma_f32_32x32x16, 64 fp32 accumulators a
-// lane), a workgroup WQ x WR such waves: 4 x 4 for large products (256 x 256, four waves per SIMD, one
-// workgroup a CU), fewer where tiles of that size would leave CUs without work.  64 k-values
+// lane; NB = 1: 32 queries), a workgroup WQ x WR such waves: 4 x 4 for large products (256 x 256, four waves per
+// SIMD, one workgroup a CU), fewer where tiles of that size would leave CUs without work.  128 bytes of k (a stage)
 // of both operands move global -> LDS by direct loads into one of two slots while the
 // other is computed on; LDS rows are 128 bytes with their 16-byte chunks swizzled by the row, so
-// fragment reads are conflict-free.  An operand stored across k is staged as it lies, 64 rows of the
+// fragment reads are conflict-free.  An operand stored across k is staged as it lies, the stage's k-rows of the
 // tile's width, and ds_read_tr16 turns it on the way into the fragments (a lane receives four k of one
-// column); its 64-byte segments are swizzled by k, so that four k-rows meet in no bank.  The launch is persistent: a workgroup walks its tiles, and the
+// column); its 64-byte segments are swizzled by k, so that four k-rows meet in no bank.  Rows need no
+// alignment but a dword's, and k may end anywhere: behind the end the row operand's values are cleared in its
+// fragments, and the query operand's are zeros in memory.  The launch is persistent: a workgroup walks its tiles, and the
 // next tile's first stage streams in during the epilogue.
 //
-// Operands of fp32 values come as two fp16 planes (value = (hi + lo) 2^-e with one exponent a row
-// or tensor): a product is then hi hi + hi lo + lo hi, three passes over k with the same
-// accumulators.  lo lo is below 2^-22 of the product and is left out; what remains is exact to
-// about 2^-22 a term, the same as an fp32 fma chain of a few terms.
+// fp32 operands come in two ways.  As they are, on v_mfma_f32_32x32x2: a fragment's 16 bytes are four k-values
+// instead of eight, everything else is alike; a sixteenth of the 16-bit rate, which is enough while the
+// operands' bytes are what takes the time.  Or as two fp16 planes (value = (hi + lo) 2^-e with one
+// exponent a row or tensor): a product is then hi hi + hi lo + lo hi, three passes over k with the same
+// accumulators.  lo lo is below 2^-22 of the product and is left out; what remains is exact to about 2^-22 a
+// term, the same as an fp32 fma chain of a few terms.
 #pragma once
 
 #include <algorithm>
+#include <mutex>
+#include <set>
 #include <type_traits>
+#include <utility>
 
 #include "va_internal.hpp"
 
@@ -35,13 +42,17 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
-constexpr int KC = 64;
-constexpr int ROWB = KC * 2;  // bytes of an LDS row (k along the rows)
+constexpr int ROWB = 128;  // bytes of an LDS row (k along the rows)
 
-template <int WQ_, int WR_>
+// What the operands are made of.
+enum Kind : int { F16 = 0, BF16 = 1, PLANES = 2, F32 = 3 };
+constexpr int size_of(int kind) { return kind == F32 ? 4 : 2; }
+constexpr int stage_of(int kind) { return ROWB / size_of(kind); }  // k-values of a stage (of one plane)
+
+template <int WQ_, int WR_, int NB_ = 2>
 struct Shape {
-    static constexpr int WQ = WQ_, WR = WR_, WAVES = WQ * WR, THREADS = 64 * WAVES;
-    static constexpr int TQ = 64 * WQ, TR = 64 * WR;
+    static constexpr int WQ = WQ_, WR = WR_, NB = NB_, WAVES = WQ * WR, THREADS = 64 * WAVES;
+    static constexpr int TQ = 32 * NB * WQ, TR = 64 * WR;
     static constexpr int QB = TQ * ROWB, XB = TR * ROWB, STAGE = QB + XB, LDS = 2 * STAGE;
     // waves per SIMD that the registers allow for: all of a CU's (16 waves), or two workgroups' and more
     static constexpr int PER_SIMD = WAVES == 16 ? 4 : 2;
@@ -54,15 +65,18 @@ struct Operand {
     const void* p = nullptr;   // row 0
     uint64_t pitch = 0;        // bytes between rows (a multiple of 16)
     uint32_t rows = 0;         // k along the rows: queries (rows) of the product; across: values of k
-    uint32_t width = 0;        // bytes of a row (k along the rows: whole stages; else a multiple of 16)
-    uint32_t plane = 0;        // bytes from a row's hi plane to its lo plane (PLANES only)
-    const void* other = nullptr;  // read instead of p (the same layout) when *choose is not zero
+    uint32_t width = 0;        // bytes of a row that may be read (of one plane; whole dwords)
+    uint32_t plane = 0;        // bytes from a row's hi plane to its lo plane (PLANES)
+    // read instead when *choose is not zero: a copy with rows of other_pitch bytes
+    const void* other = nullptr;
+    uint64_t other_pitch = 0;
     const uint32_t* choose = nullptr;
 };
 
 struct Args {
     Operand q, x;
-    uint32_t kstages = 0;  // stages of 64 k-values of one plane (operands are zero-padded to them)
+    uint32_t kstages = 0;  // stages of k of one plane
+    uint32_t tail = 0;     // bytes of k in the last stage (0: all of it); x along the rows only
     uint32_t nq = 0, nr = 0;  // blocks of the shape's queries and rows
     uint32_t parts = 1;  // walk: workgroups per query block; tiles: shares of the k-stages
 };
@@ -127,29 +141,43 @@ struct Tiles {
     }
 };
 
-template <bool BF16>
+template <int KIND>
 __device__ __forceinline__ f32x16 mfma(u32x4 x, u32x4 q, f32x16 c) {
-    if constexpr (BF16)
+    if constexpr (KIND == F32) {
+        // (both operands' fragments hold the same four k of each half)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(__builtin_bit_cast(f32x4, x)[e], __builtin_bit_cast(f32x4, q)[e], c, 0, 0, 0);
+        return c;
+    } else if constexpr (KIND == BF16) {
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, q), c, 0, 0, 0);
-    else
+    } else {
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, x), __builtin_bit_cast(f16x8, q), c, 0, 0, 0);
+    }
 }
 
 // The lane's place in a tile: acc[m][n][4 j + e] is query q(n) against row r(m, j) + e.
+template <int NB>
 struct Lane {
     int wq, wr, l32, hh;
-    __device__ int q(int n) const { return wq * 64 + 32 * n + l32; }
+    __device__ int q(int n) const { return wq * 32 * NB + 32 * n + l32; }
     __device__ int r(int m, int j) const { return wr * 64 + 32 * m + 8 * j + 4 * hh; }
 };
 
-// One operand's way into LDS and out of it: W waves along it, of WAVES in the workgroup.  KM: stored
-// across k.
-template <bool KM, bool PLANES, int W, int WAVES>
+// One operand's way into LDS and out of it: W waves of 32 N queries (rows) along it, of WAVES in the workgroup.
+// KM: stored across k (N = 2).
+template <bool KM, int KIND, int W, int WAVES, int N = 2>
 struct Feed {
-    static constexpr int LPW = 8 * W / WAVES;       // 1 KiB direct loads per wave and stage
-    static constexpr int KROW = 128 * W;            // bytes of a k-row (KM)
-    static constexpr uint32_t SEGX = W == 1 ? 1 : 3;  // the segment is xored by (k >> SEGS) & SEGX
-    static constexpr uint32_t SEGS = W == 1 ? 1 : 0;
+    static_assert(N == 2 || !KM, "narrow waves only along k");
+    static constexpr int ES = size_of(KIND), KV = stage_of(KIND);
+    static constexpr int LPW = 4 * N * W / WAVES;   // 1 KiB direct loads per wave and stage
+    static constexpr int KROW = 64 * ES * W;        // bytes of a k-row (KM)
+    // the place of a k-row's 16-byte chunk c: 16-bit values, its segment (four chunks) xored by k; fp32, its half
+    // of 256 bytes by bit 2 of k (the two k-rows that a fragment reads at once are four apart)
+    static __device__ uint32_t placed(uint32_t k, uint32_t c) {
+        if constexpr (ES == 4) return c ^ ((k & 4u) << 1);
+        else return W == 1 ? c ^ ((k << 1) & 4u) : c ^ ((k & 3u) << 2);
+    }
+    const char* p;
     const char* base;  // of the tile
     uint32_t records;  // bytes behind it (k along the rows)
     uint64_t left;     // (KM)
@@ -164,8 +192,13 @@ struct Feed {
     // each lane one 16-byte chunk, the chunk's segment (four chunks) xored.  Rows past the operand's last one
     // lie past its descriptor and land as zeros.
     __device__ void init(const Operand& o, int wave, int lane, uint32_t at, int wtile) {
-        pitch = uint32_t(o.pitch);
-        plane = PLANES ? o.plane : 0;
+        const uint32_t* choose = o.choose;
+        const void *one = o.p, *two = o.other;
+        const uint64_t pitch1 = o.pitch, pitch2 = o.other_pitch;
+        const bool copy = choose && *choose;
+        p = static_cast<const char*>(copy ? two : one);
+        pitch = uint32_t(copy ? pitch2 : pitch1);
+        plane = KIND == PLANES ? o.plane : 0;
         lds_at = at + uint32_t(wave) * 1024u;
         const int l32 = lane & 31;
         hh = lane >> 5;
@@ -174,39 +207,41 @@ struct Feed {
             for (int i = 0; i < LPW; ++i) {
                 const uint32_t byte = uint32_t(1024 * (wave + WAVES * i) + 16 * lane);
                 const uint32_t k = byte / KROW, c = byte % KROW / 16;
-                voff[i] = k * pitch + 16u * ((((c >> 2) ^ ((k >> SEGS) & SEGX)) << 2) | (c & 3u));
+                voff[i] = k * pitch + 16u * placed(k, c);
             }
             const int e = (lane & 15) >> 2;
 #pragma unroll
-            for (int n = 0; n < 2; ++n)
-                frag[n] = at + uint32_t((8 * hh + e) * KROW + (((2 * wtile + n) ^ ((e >> SEGS) & SEGX)) << 6) + 32 * ((lane >> 4) & 1) + 8 * (lane & 3));
+            for (int n = 0; n < 2; ++n) {
+                if constexpr (ES == 4)  // column l32 of block n, k-row 4 hh (+ 8 t + e)
+                    frag[n] = at + uint32_t(4 * hh * KROW) + 16u * placed(4u * uint32_t(hh), uint32_t(8 * (2 * wtile + n) + (l32 >> 2))) + 4u * uint32_t(l32 & 3);
+                else  // k-row 8 hh + e, 4 columns of the half block (lane >> 4) & 1
+                    frag[n] = at + uint32_t((8 * hh + e) * KROW) +
+                              16u * placed(uint32_t(e), uint32_t(4 * (2 * wtile + n) + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1))) + 8u * uint32_t(lane & 1);
+            }
         } else {
 #pragma unroll
             for (int i = 0; i < LPW; ++i) {
                 const uint32_t row = uint32_t(8 * (wave + WAVES * i) + (lane >> 3));
                 voff[i] = row * pitch + 16u * uint32_t((lane & 7) ^ ((row >> 1) & 7));
             }
-            frag[0] = at + uint32_t((wtile * 64 + l32) * ROWB);
+            frag[0] = at + uint32_t((wtile * 32 * N + l32) * ROWB);
             swz = (l32 >> 1) & 7;
         }
     }
-    // the operand's block b of 64 W queries (rows)
+    // the operand's block b of 32 N W queries (rows)
     __device__ void open(const Operand& o, uint32_t b) {
-        const uint32_t* choose = o.choose;
-        const void *one = o.p, *two = o.other;
-        const char* p = static_cast<const char*>(choose && *choose ? two : one);
         if constexpr (KM) {
             base = p + b * uint32_t(KROW);
-            left = (o.rows - 1) * o.pitch + o.width - b * uint32_t(KROW);
+            left = uint64_t(o.rows - 1) * pitch + o.width - b * uint32_t(KROW);
         } else {
-            base = p + uint64_t(b) * (64u * W) * o.pitch;
-            records = (min(64u * W, o.rows - b * (64u * W)) - 1u) * pitch + o.width + plane;
+            base = p + uint64_t(b) * (32u * N * W) * pitch;
+            records = (min(32u * N * W, o.rows - b * (32u * N * W)) - 1u) * pitch + o.width + plane;
         }
     }
     // load i of stage k (of the plane `lo`) into the slot at LDS address `slot`; !ok: zeros
     __device__ void issue(uint32_t k, bool lo, bool ok, uint32_t slot, int i) const {
         if constexpr (KM) {
-            const uint64_t skip = uint64_t(k) * KC * pitch;
+            const uint64_t skip = uint64_t(k) * KV * pitch;
             const dma_rsrc r = make_dma_rsrc(base + skip + (lo ? plane : 0u),
                                              ok && skip < left ? uint32_t(min(left - skip, uint64_t(kDmaMaxBytes))) : 0u);
             lds_dma16(r, voff[i], slot + lds_at + uint32_t(1024 * WAVES * i));
@@ -215,9 +250,15 @@ struct Feed {
             lds_dma16_so(r, ok ? voff[i] : kDmaSkip, ok ? k * uint32_t(ROWB) + (lo ? plane : 0u) : 0u, slot + lds_at + uint32_t(1024 * WAVES * i));
         }
     }
-    // the fragment of the wave's 32-query (row) block n, k-step t of the slot
+    // the fragment of the wave's 32-query (row) block n, k-step t of the slot (32 bytes of k: this lane's half)
     __device__ u32x4 read(const char* slot, int n, int t) const {
-        if constexpr (KM) {
+        if constexpr (KM && ES == 4) {
+            const char* at = slot + frag[n] + t * 8 * KROW;
+            u32x4 o;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = *reinterpret_cast<const uint32_t*>(at + e * KROW);
+            return o;
+        } else if constexpr (KM) {
             typedef short s16x4 __attribute__((ext_vector_type(4)));
             typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
             struct alignas(16) {
@@ -231,6 +272,17 @@ struct Feed {
             return *reinterpret_cast<const u32x4*>(slot + frag[0] + n * 32 * ROWB + 16 * ((2 * t + hh) ^ swz));
         }
     }
+    // clears what a fragment of k-step t holds from byte `tail` of the stage on
+    __device__ u32x4 cut(u32x4 v, int t, uint32_t tail) const {
+        int have = int(tail) - 16 * (2 * t + hh);
+        asm volatile("" : "+v"(have));  // computed here: kept through the main loop, the masks would spill its registers
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int b = have - 4 * e;
+            v[e] &= b >= 4 ? ~0u : b == 2 ? 0xFFFFu : 0u;
+        }
+        return v;
+    }
 };
 
 // Epi: struct with
@@ -242,7 +294,7 @@ struct Feed {
 //   tile(State&, smem, lane, acc, tile, spare, settle)  spare: 4 KiB of LDS of the wave's own; with kStores,
 //                               settle() before the first store to memory
 //   end(State&, smem, lane, tile)  after an item's last tile
-template <bool BF16, bool PLANES, bool QK, bool XK, class Epi>
+template <int KIND, bool QK, bool XK, class Epi>
 __global__ __launch_bounds__(Epi::Shape::THREADS, Epi::Shape::PER_SIMD) void gemm16_kernel(Args a, Epi epi) {
     using Sh = typename Epi::Shape;
     constexpr int STAGE = Sh::STAGE;
@@ -250,16 +302,17 @@ __global__ __launch_bounds__(Epi::Shape::THREADS, Epi::Shape::PER_SIMD) void gem
     __shared__ typename Epi::Shared smem;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const Lane ln{wave % Sh::WQ, wave / Sh::WQ, lane & 31, lane >> 5};
+    const Lane<Sh::NB> ln{wave % Sh::WQ, wave / Sh::WQ, lane & 31, lane >> 5};
+    constexpr int NB = Sh::NB;
 
     Tiles<Epi::kWalk> tile;
     tile.first(a);
     if (!tile.ok) return;
 
-    const uint32_t total_stages = PLANES ? 3 * a.kstages : a.kstages;
+    const uint32_t total_stages = KIND == PLANES ? 3 * a.kstages : a.kstages;
     const uint32_t lds0 = lds_addr_of(lds);
-    Feed<QK, PLANES, Sh::WQ, Sh::WAVES> fq_;
-    Feed<XK, PLANES, Sh::WR, Sh::WAVES> fx_;
+    Feed<QK, KIND, Sh::WQ, Sh::WAVES, Sh::NB> fq_;
+    Feed<XK, KIND, Sh::WR, Sh::WAVES> fx_;
     fq_.init(a.q, wave, lane, 0, ln.wq);
     fx_.init(a.x, wave, lane, Sh::QB, ln.wr);
     uint32_t s0, s1;  // the tile's stages
@@ -278,7 +331,7 @@ __global__ __launch_bounds__(Epi::Shape::THREADS, Epi::Shape::PER_SIMD) void gem
     constexpr int LQ = decltype(fq_)::LPW, LX = decltype(fx_)::LPW;
     auto issue_one = [&](uint32_t s, uint32_t slot, int i) {
         const bool ok = s < s1;
-        const uint32_t k = PLANES ? s / 3u : s, seg = PLANES ? s - 3u * k : 0u;  // (a k's planes are read together)
+        const uint32_t k = KIND == PLANES ? s / 3u : s, seg = KIND == PLANES ? s - 3u * k : 0u;  // (a k's planes are read together)
         const uint32_t sb = lds0 + slot * uint32_t(STAGE);
         if (i < LQ) fq_.issue(k, seg == 2, ok, sb, i);
         else fx_.issue(k, seg == 1, ok, sb, i - LQ);
@@ -288,41 +341,53 @@ __global__ __launch_bounds__(Epi::Shape::THREADS, Epi::Shape::PER_SIMD) void gem
         for (int i = 0; i < LQ + LX; ++i) issue_one(s, slot, i);
     };
 
-    f32x16 acc[2][2];
-    u32x4 fx[2][2], fq[2][2];
+    f32x16 acc[2][NB];
+    u32x4 fx[2][2], fq[2][NB];
     auto read_one = [&](int buf, uint32_t slot, int t, int i) {
         const char* base = lds + slot * STAGE;
         if (i < 2) fx[buf][i] = fx_.read(base, i, t);
         else fq[buf][i - 2] = fq_.read(base, i - 2, t);
     };
-    // One k-step: four MFMAs, and behind each of them, in this order, the read of one of the next k-step's
+    // One k-step: four MFMAs (NB = 1: two), and behind each of them, in this order, the read of one of the next k-step's
     // fragments and a share of the loads into the slot that this stage leaves.
-    auto step = [&](int cur, uint32_t slot_next, int t_next, auto more, uint32_t s_load, uint32_t slot_load) {
+    auto step = [&](int cur, uint32_t slot_next, int t_next, auto more, uint32_t s_load, uint32_t slot_load, bool ends) {
+        if constexpr (!XK && !decltype(more)::value) {
+            if (ends) {
+                const int t = (t_next + 3) & 3;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+                for (int m = 0; m < 2; ++m) fx[cur][m] = fx_.cut(fx[cur][m], t, a.tail);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 2 * NB; ++i) {
             const int m = i & 1, n = i >> 1;
-            acc[m][n] = mfma<BF16>(fx[cur][m], fq[cur][n], acc[m][n]);
+            acc[m][n] = mfma<KIND>(fx[cur][m], fq[cur][n], acc[m][n]);
             __builtin_amdgcn_sched_barrier(0);
-            read_one(cur ^ 1, slot_next, t_next, (i & 1) * 2 + (i >> 1));
+            if (NB == 2) {
+                read_one(cur ^ 1, slot_next, t_next, (i & 1) * 2 + (i >> 1));
+            } else {
+                read_one(cur ^ 1, slot_next, t_next, i);
+                if (i) read_one(cur ^ 1, slot_next, t_next, 2);
+            }
             if constexpr (decltype(more)::value) {
 #pragma unroll
-                for (int l = i * (LQ + LX) / 4; l < (i + 1) * (LQ + LX) / 4; ++l) issue_one(s_load, slot_load, l);
+                for (int l = i * (LQ + LX) / (2 * NB); l < (i + 1) * (LQ + LX) / (2 * NB); ++l) issue_one(s_load, slot_load, l);
             }
             __builtin_amdgcn_sched_barrier(0);
         }
     };
     // a workgroup barrier that leaves the direct loads in flight; this wave's LDS reads are done
     auto barrier = [&]() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
-    // stage i of the tile's; more: stage i + 2 follows
-    auto stage = [&](uint32_t i, auto more) {
+    // stage i of the tile's; more: stage i + 2 follows; ends: k ends within it
+    auto stage = [&](uint32_t i, auto more, bool ends) {
         const uint32_t slot = i & 1u;
 #pragma unroll
-        for (int t = 0; t < KC / 16 - 1; ++t) step(t & 1, slot, t + 1, std::false_type(), 0, 0);
+        for (int t = 0; t < 3; ++t) step(t & 1, slot, t + 1, std::integral_constant<bool, false>(), 0, 0, ends && !decltype(more)::value);
         // the last k-step's fragments are in registers: publish the next stage, free this slot
         wait_vmcnt<0>();
         barrier();
         __builtin_amdgcn_sched_barrier(0);
-        step((KC / 16 - 1) & 1, slot ^ 1u, 0, more, s0 + i + 2, slot);
+        step(1, slot ^ 1u, 0, more, s0 + i + 2, slot, ends);
     };
 
     typename Epi::State st;
@@ -335,7 +400,7 @@ __global__ __launch_bounds__(Epi::Shape::THREADS, Epi::Shape::PER_SIMD) void gem
 #pragma unroll
         for (int m = 0; m < 2; ++m)
 #pragma unroll
-            for (int n = 0; n < 2; ++n)
+            for (int n = 0; n < NB; ++n)
 #pragma unroll
                 for (int v = 0; v < 16; ++v) acc[m][n][v] = 0.0f;
         barrier();  // every wave is past the previous tile's main loop: slot 1 is free
@@ -345,11 +410,11 @@ __global__ __launch_bounds__(Epi::Shape::THREADS, Epi::Shape::PER_SIMD) void gem
             barrier();
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) read_one(0, 0, 0, i);
+        for (int i = 0; i < 2 + NB; ++i) read_one(0, 0, 0, i);
         const uint32_t ns = s1 - s0;
         uint32_t i = 0;
-        for (; i + 2 < ns; ++i) stage(i, std::true_type());
-        for (; i < ns; ++i) stage(i, std::false_type());
+        for (; i + 2 < ns; ++i) stage(i, std::true_type(), false);
+        for (; i < ns; ++i) stage(i, std::false_type(), !XK && a.tail && s0 + i + 1 == total_stages);
         epi.publish(st, smem, tid);
         __syncthreads();  // every wave is past the main loop: slot 0 is free
         const Tiles<Epi::kWalk> here = tile;
@@ -360,7 +425,7 @@ __global__ __launch_bounds__(Epi::Shape::THREADS, Epi::Shape::PER_SIMD) void gem
         }
         // what the epilogue computes from the lane is computed there: kept through the main loop, its
         // addresses would take the registers that the fragments need
-        Lane le = ln;
+        Lane<Sh::NB> le = ln;
         asm volatile("" : "+v"(le.l32), "+v"(le.hh));
         // An epilogue that stores much waits for the next tile's first stage before its first store: behind the
         // stores, that wait would be for all of them.
@@ -387,18 +452,29 @@ template <class Sh>
 uint32_t grid_max(const va_context* ctx) {
     return std::max(uint32_t(ctx->num_cus), kXcds) / kXcds * kXcds * per_cu<Sh>();
 }
-template <bool BF16, bool PLANES, bool QK, bool XK, class Epi>
+// Lets a kernel take `bytes` of dynamic LDS on the device; the runtime is asked once per kernel and device.
+inline hipError_t allow_lds(const void* kern, int bytes, int device) {
+    static std::mutex lock;
+    static std::set<std::pair<const void*, int>> done;
+    std::lock_guard<std::mutex> hold(lock);
+    if (done.count({kern, device})) return hipSuccess;
+    const hipError_t e = hipFuncSetAttribute(kern, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == hipSuccess) done.insert({kern, device});
+    return e;
+}
+template <int KIND, bool QK, bool XK, class Epi>
 va_status launch(va_context* ctx, const Args& a, const Epi& epi) {
     using Sh = typename Epi::Shape;
     static_assert(sizeof(typename Epi::Shared) + Sh::LDS <= 163840, "a workgroup's LDS");
     const uint64_t tiles = uint64_t(a.nq) * (Epi::kWalk ? a.parts : a.nr * uint64_t(a.parts));
     if (tiles == 0) return VA_OK;
-    if (tiles > 0x7FFFFFF0ull || 256 * std::max(a.q.pitch, a.x.pitch) > kDmaMaxBytes)
-        return fail(ctx, VA_ERR_INVALID_ARG, "matrix product too large: %llu tiles, rows of %llu and %llu bytes",
-                    (unsigned long long)tiles, (unsigned long long)a.q.pitch, (unsigned long long)a.x.pitch);
+    const uint64_t pitch = std::max(std::max(a.q.pitch, a.x.pitch), std::max(a.q.other_pitch, a.x.other_pitch));
+    if (tiles > 0x7FFFFFF0ull || 256 * pitch > kDmaMaxBytes)
+        return fail(ctx, VA_ERR_INVALID_ARG, "matrix product too large: %llu tiles, rows of %llu bytes", (unsigned long long)tiles,
+                    (unsigned long long)pitch);
     const uint64_t grid = std::min<uint64_t>((tiles + kXcds - 1) / kXcds * kXcds, grid_max<Sh>(ctx));
-    auto kern = &gemm16_kernel<BF16, PLANES, QK, XK, Epi>;
-    VA_CHECK_HIP(ctx, hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, Sh::LDS));
+    auto kern = &gemm16_kernel<KIND, QK, XK, Epi>;
+    VA_CHECK_HIP(ctx, allow_lds(reinterpret_cast<const void*>(kern), Sh::LDS, ctx->device));
     kern<<<dim3(uint32_t(grid)), dim3(Sh::THREADS), Sh::LDS, ctx->stream>>>(a, epi);
     VA_CHECK_LAUNCH(ctx);
     return VA_OK;
