@@ -9,7 +9,7 @@
 // lane; NB = 1: 32 queries), a workgroup WQ x WR such waves: 4 x 4 for large products (256 x 256, four waves per
 // SIMD, one workgroup a CU), fewer where tiles of that size would leave CUs without work.  128 bytes of k (a stage)
 // of both operands move global -> LDS by direct loads into one of two slots while the
-// other is computed on; LDS rows are 128 bytes with their 16-byte chunks swizzled by the row, so
+// other is computed on (four slots where a launch does not fill the chip and waits for each stage); LDS rows are 128 bytes with their 16-byte chunks swizzled by the row, so
 // fragment reads are conflict-free.  An operand stored across k is staged as it lies, the stage's k-rows of the
 // tile's width, and ds_read_tr16 turns it on the way into the fragments (a lane receives four k of one
 // column); its 64-byte segments are swizzled by k, so that four k-rows meet in no bank.  Rows need no
@@ -49,13 +49,14 @@ enum Kind : int { F16 = 0, BF16 = 1, PLANES = 2, F32 = 3 };
 constexpr int size_of(int kind) { return kind == F32 ? 4 : 2; }
 constexpr int stage_of(int kind) { return ROWB / size_of(kind); }  // k-values of a stage (of one plane)
 
-template <int WQ_, int WR_, int NB_ = 2>
+template <int WQ_, int WR_, int NB_ = 2, int SLOTS_ = 2>
 struct Shape {
+    static constexpr int SLOTS = SLOTS_;  // a power of two
     static constexpr int WQ = WQ_, WR = WR_, NB = NB_, WAVES = WQ * WR, THREADS = 64 * WAVES;
     static constexpr int TQ = 32 * NB * WQ, TR = 64 * WR;
-    static constexpr int QB = TQ * ROWB, XB = TR * ROWB, STAGE = QB + XB, LDS = 2 * STAGE;
+    static constexpr int QB = TQ * ROWB, XB = TR * ROWB, STAGE = QB + XB, LDS = SLOTS * STAGE;
     // waves per SIMD that the registers allow for: all of a CU's (16 waves), or two workgroups' and more
-    static constexpr int PER_SIMD = WAVES == 16 ? 4 : 2;
+    static constexpr int PER_SIMD = WAVES == 16 ? 4 : SLOTS == 2 ? 2 : 1;
     static_assert(THREADS >= TQ && THREADS >= TR, "one thread per query and row");
     static_assert(WAVES * 4096 <= STAGE, "the epilogue's LDS fits in one slot");
 };
@@ -378,23 +379,36 @@ __global__ __launch_bounds__(Epi::Shape::THREADS, Epi::Shape::PER_SIMD) void gem
     };
     // a workgroup barrier that leaves the direct loads in flight; this wave's LDS reads are done
     auto barrier = [&]() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
-    // stage i of the tile's; more: stage i + 2 follows; ends: k ends within it
-    auto stage = [&](uint32_t i, auto more, bool ends) {
-        const uint32_t slot = i & 1u;
+    // waits for all but the youngest `stages` stages of direct loads
+    constexpr int SLOTS = Sh::SLOTS, L = LQ + LX;
+    static_assert((SLOTS & (SLOTS - 1)) == 0 && L * (SLOTS - 1) < 64 && SLOTS <= 4, "slots");
+    auto wait_but = [&](int stages) {
+        if (SLOTS > 3 && stages >= 3) wait_vmcnt<(SLOTS > 3 ? 3 : 0) * L>();
+        else if (SLOTS > 2 && stages == 2) wait_vmcnt<(SLOTS > 2 ? 2 : 0) * L>();
+        else if (stages == 1) wait_vmcnt<L>();
+        else wait_vmcnt<0>();
+    };
+    // stage i of the tile's ns; more: stage i + SLOTS follows; ends: k ends within it
+    auto stage = [&](uint32_t i, uint32_t ns, auto more, bool ends) {
+        const uint32_t slot = i & (SLOTS - 1);
 #pragma unroll
         for (int t = 0; t < 3; ++t) step(t & 1, slot, t + 1, std::integral_constant<bool, false>(), 0, 0, ends && !decltype(more)::value);
         // the last k-step's fragments are in registers: publish the next stage, free this slot
-        wait_vmcnt<0>();
+        if (decltype(more)::value) wait_but(SLOTS - 2);
+        else wait_but(min(SLOTS - 2, int(ns) - 2 - int(i)));
         barrier();
         __builtin_amdgcn_sched_barrier(0);
-        step(1, slot ^ 1u, 0, more, s0 + i + 2, slot, ends);
+        step(1, (slot + 1) & (SLOTS - 1), 0, more, s0 + i + SLOTS, slot, ends);
     };
 
     typename Epi::State st;
     open();
+    // the first tile's stages before anything that waits for memory; later tiles' first ones during the epilogues
+#pragma unroll
+    for (int k = 0; k < SLOTS; ++k)
+        if (k == 0 || uint32_t(k) < s1 - s0) issue(s0 + k, k);
     epi.begin(st, smem, tile);
-    issue(s0, 0);  // later tiles: during the previous epilogue
-    bool settled = false;
+    bool settled = false, first = true;
     for (;;) {
         epi.load(st, tile, tid);
 #pragma unroll
@@ -403,18 +417,23 @@ __global__ __launch_bounds__(Epi::Shape::THREADS, Epi::Shape::PER_SIMD) void gem
             for (int n = 0; n < NB; ++n)
 #pragma unroll
                 for (int v = 0; v < 16; ++v) acc[m][n][v] = 0.0f;
-        barrier();  // every wave is past the previous tile's main loop: slot 1 is free
-        issue(s0 + 1, 1);
+        const uint32_t ns = s1 - s0;
+        if (!first) {
+            barrier();  // every wave is past the previous tile's epilogue: the other slots are free
+#pragma unroll
+            for (int k = 1; k < SLOTS; ++k)
+                if (uint32_t(k) < ns) issue(s0 + k, k);
+        }
+        first = false;
         if (!settled) {
-            wait_vmcnt<LQ + LX>();  // stage 0 (older than stage 1's loads)
+            wait_but(min(SLOTS, int(ns)) - 1);  // stage 0 (older than the others' loads)
             barrier();
         }
 #pragma unroll
         for (int i = 0; i < 2 + NB; ++i) read_one(0, 0, 0, i);
-        const uint32_t ns = s1 - s0;
         uint32_t i = 0;
-        for (; i + 2 < ns; ++i) stage(i, std::true_type(), false);
-        for (; i < ns; ++i) stage(i, std::false_type(), !XK && a.tail && s0 + i + 1 == total_stages);
+        for (; i + SLOTS < ns; ++i) stage(i, ns, std::true_type(), false);
+        for (; i < ns; ++i) stage(i, ns, std::false_type(), !XK && a.tail && s0 + i + 1 == total_stages);
         epi.publish(st, smem, tid);
         __syncthreads();  // every wave is past the main loop: slot 0 is free
         const Tiles<Epi::kWalk> here = tile;
@@ -444,8 +463,8 @@ __global__ __launch_bounds__(Epi::Shape::THREADS, Epi::Shape::PER_SIMD) void gem
 // largest shape is alone anyway), its registers, its 32 waves.
 template <class Sh>
 constexpr uint32_t per_cu() {
-    constexpr uint32_t lds = 163840 / (Sh::LDS + 2048), waves = 4 * Sh::PER_SIMD / Sh::WAVES;
-    return std::max(std::min(lds, waves), 1u);
+    constexpr uint32_t lds = 163840 / (Sh::LDS + 2048), waves = std::max(4 * Sh::PER_SIMD / Sh::WAVES, 1);
+    return Sh::SLOTS > 2 ? 1u : std::max(std::min(lds, waves), 1u);
 }
 // Persistent launch: as many workgroups as the chip holds, a multiple of the XCDs.
 template <class Sh>

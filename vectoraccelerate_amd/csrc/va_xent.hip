@@ -400,7 +400,7 @@ va_status va_xent_forward(va_context* ctx, const va_xent_desc* d, float* out_los
     // Offsets are looked over first where the shorter epilogue counts: 16-bit products on the matrix cores'
     // time (4096 rows x 262,144 items of 768: the check takes 15 us and saves 100; a product that streams its
     // items hides the longer epilogue).
-    const bool wild = wild_scale(d), checks = d->offsets && kind < g16::PLANES && !wild && bl.shape == 0;
+    const bool wild = wild_scale(d), checks = d->offsets && kind < g16::PLANES && !wild && bl.shape == LARGE;
     const uint32_t nq = bl.nq(T);
     // parts per query block: whole multiples of the XCDs when there are that many
     uint32_t parts = std::max(bl.grid / nq, 1u);

@@ -191,25 +191,35 @@ va_status check_desc(va_context* ctx, const va_xent_desc* d, const char* who);
 // A scale at which the logits' other unit might overflow: natural units (as with odd offsets).
 inline bool wild_scale(const va_xent_desc* d) { return fabsf(d->scale) > 1e18f; }
 
-// The shapes of a product's workgroups.
+// The shapes of a product's workgroups.  Deep ones have four slots: alone on their CU, three stages in flight.
+using Medium = g16::Shape<2, 2>;
+using Small = g16::Shape<1, 2>;
+using DeepMedium = g16::Shape<2, 2, 2, 4>;
+using DeepSmall = g16::Shape<1, 2, 2, 4>;
+// 32 queries, along k: fp32 products as they are, which 64 padded ones would bind to the matrix cores.
+using Narrow = g16::Shape<1, 2, 1>;
+using DeepNarrow = g16::Shape<1, 2, 1, 4>;
+enum ShapeId : int { LARGE = 0, MEDIUM = 1, SMALL = 2, NARROW = 3, DEEP_MEDIUM = 4, DEEP_SMALL = 5, DEEP_NARROW = 6 };
 template <class F>
 va_status by_shape(int shape, F&& f) {
-    if (shape == 0) return f(g16::Large());
-    if (shape == 1) return f(g16::Shape<2, 2>());
-    return f(g16::Shape<1, 2>());
+    switch (shape) {
+        case LARGE: return f(g16::Large());
+        case MEDIUM: return f(Medium());
+        case SMALL: return f(Small());
+        case DEEP_MEDIUM: return f(DeepMedium());
+        default: return f(DeepSmall());
+    }
 }
-// (32 queries: fp32 products as they are, which 64 padded ones would bind to the matrix cores; their query
-// operand along k)
-using Narrow = g16::Shape<1, 2, 1>;
 template <int KIND, class F>
 va_status by_shape_of(int shape, F&& f) {
     if constexpr (KIND == g16::F32) {
-        if (shape == 3) return f(Narrow());
+        if (shape == NARROW) return f(Narrow());
+        if (shape == DEEP_NARROW) return f(DeepNarrow());
     }
     return by_shape(shape, f);
 }
 struct Blocks {
-    int shape;              // of by_shape; 3: Narrow
+    int shape;              // ShapeId
     uint32_t tq, tr, grid;  // grid: the most workgroups of a launch
     uint32_t parts;         // shares of the sum of each tile
     uint32_t nq(uint64_t Q) const { return uint32_t((Q + tq - 1) / tq); }
@@ -221,28 +231,31 @@ struct Blocks {
 // of whole rounds, which the rule gives to the large tiles), one of 64 x 128 (three a CU) 0.48 to 0.59; measured on
 // 1023 x 49,999 x 300 and 4096 x 262,144 x 768.  `shares`: how many shares of the sum the caller can make.
 inline Blocks blocks_for(const va_context* ctx, uint64_t Q, uint64_t R, uint32_t shares = 1, bool narrow = false) {
-    if (narrow) {
-        Blocks b{3, 32, 128, g16::grid_max<Narrow>(ctx), 1};
-        b.parts = uint32_t(std::min<uint64_t>(std::max<uint64_t>(b.grid / (uint64_t(b.nq(Q)) * b.nr(R)), 1), shares));
-        return b;
-    }
-    Blocks all[3] = {{0, 256, 256, g16::grid_max<g16::Large>(ctx), 1},
-                     {1, 128, 128, g16::grid_max<g16::Shape<2, 2>>(ctx), 1},
-                     {2, 64, 128, g16::grid_max<g16::Shape<1, 2>>(ctx), 1}};
-    const double round[3] = {1.0, 0.56, 0.5};
-    int best = 0;
+    Blocks all[4] = {{LARGE, 256, 256, g16::grid_max<g16::Large>(ctx), 1},
+                     {MEDIUM, 128, 128, g16::grid_max<Medium>(ctx), 1},
+                     {SMALL, 64, 128, g16::grid_max<Small>(ctx), 1},
+                     {NARROW, 32, 128, g16::grid_max<Narrow>(ctx), 1}};
+    const double round[4] = {1.0, 0.56, 0.5, 0.5};
+    int best = -1;
     double least = 0.0;
-    for (int i = 0; i < 3; ++i) {
+    for (int i = narrow ? 3 : 0; i < (narrow ? 4 : 3); ++i) {
         const uint64_t tiles = uint64_t(all[i].nq(Q)) * all[i].nr(R);
         all[i].parts = uint32_t(std::min<uint64_t>(std::max<uint64_t>(all[i].grid / tiles, 1), shares));
         const double t = double((tiles * all[i].parts + all[i].grid - 1) / all[i].grid) / all[i].parts * round[i];
-        if (i == 0 || t < least) {
+        if (best < 0 || t < least) {
             best = i;
             least = t;
         }
     }
-    return all[best];
+    Blocks b = all[best];
+    // one workgroup a CU, or fewer: the time is that of a tile's loads
+    if (b.shape != LARGE && uint64_t(b.nq(Q)) * b.nr(R) * b.parts <= uint64_t(ctx->num_cus)) {
+        b.shape += DEEP_MEDIUM - MEDIUM;
+        b.grid = g16::grid_max<DeepSmall>(ctx);
+    }
+    return b;
 }
+static_assert(DEEP_SMALL - SMALL == DEEP_MEDIUM - MEDIUM && DEEP_NARROW - NARROW == DEEP_MEDIUM - MEDIUM, "deep shapes follow the others");
 
 // f(kind, offsets) of a launch; edge: the last tile is not whole
 template <class F>
