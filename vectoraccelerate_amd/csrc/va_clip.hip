@@ -5,9 +5,9 @@
 // Bound by memory: the gradients are read twice (the factor is known after the last of them) and
 // written once.  The list travels in the kernels' arguments, kListMax tensors a launch, so a
 // call leaves nothing behind that it would have to wait for.  A tensor is cut into chunks of
-// kChunk values; a workgroup takes chunks in turn and leaves one sum.  Sums are fp64 from the first
-// product on (gradients of any magnitude, no overflow) and joined in a fixed order by every workgroup
-// of the second pass, so results do not depend on the order in which workgroups run.  The second pass
+// kChunk values, whose loads are issued together; a workgroup takes a run of chunks and leaves one sum.  Sums are
+// fp64 from the first product on (gradients of any magnitude, no overflow) and joined in a fixed order by every
+// workgroup of the second pass, so results do not depend on the order in which workgroups run.  The second pass
 // starts where the first one ended: what is left of it in the caches is read from there.
 #include <algorithm>
 #include <cmath>
@@ -18,8 +18,8 @@ namespace va {
 namespace {
 
 constexpr uint32_t kChunk = 16384;
-constexpr uint32_t kListMax = 96;     // 3 KiB of arguments
-constexpr uint32_t kMaxSums = 1024;   // workgroups of the first pass, all launches together
+constexpr uint32_t kListMax = 124;    // just under 4 KiB of arguments
+constexpr uint32_t kMaxSums = 2048;   // workgroups of the first pass, all launches together: eight a CU
 
 struct Entry {
     const void* in;
@@ -32,20 +32,17 @@ struct List {
     Entry e[kListMax];
     uint32_t n, chunks;
 };
+static_assert(sizeof(List) + 64 <= 4096, "kernel arguments");
 
 template <class T>
 using Vec8 = T __attribute__((ext_vector_type(8), aligned(sizeof(T))));
 typedef float f32x8 __attribute__((ext_vector_type(8)));
 
-// the tensor that holds chunk c
-__device__ __forceinline__ const Entry& entry_of(const List& l, uint32_t c) {
-    uint32_t lo = 0, hi = l.n - 1;
-    while (lo < hi) {
-        const uint32_t mid = (lo + hi + 1) >> 1;
-        if (l.e[mid].chunk0 <= c) lo = mid;
-        else hi = mid - 1;
-    }
-    return l.e[lo];
+// the tensor that holds chunk c, found by the whole wave: lane i looks at tensors i, 64 + i
+__device__ __forceinline__ uint32_t tensor_of(const List& l, uint32_t c) {
+    uint32_t n = 0;
+    for (uint32_t i = threadIdx.x & 63; i < (l.n + 63) / 64 * 64; i += 64) n += uint32_t(__popcll(__ballot(i < l.n && l.e[min(i, l.n - 1)].chunk0 <= c)));
+    return __builtin_amdgcn_readfirstlane(n) - 1;
 }
 
 __device__ __forceinline__ double block_sum(double v, double* part) {
@@ -58,17 +55,31 @@ __device__ __forceinline__ double block_sum(double v, double* part) {
 }
 
 template <class T>
+__device__ __forceinline__ void add_squares(double (&s)[2], Vec8<T> v) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const double x = double(float(v[e]));
+        s[e & 1] = fma(x, x, s[e & 1]);
+    }
+}
+template <class T>
 __device__ __forceinline__ double square_sum(const T* p, uint32_t n) {
     double s[2] = {0.0, 0.0};
-    const uint32_t full = n / 8;
-    for (uint32_t i = threadIdx.x; i < full; i += 256) {
-        const Vec8<T> v = *reinterpret_cast<const Vec8<T>*>(p + 8 * i);
+    if (n == kChunk) {
+        constexpr int R = sizeof(T) == 4 ? 4 : 8;  // 128 bytes a thread in flight
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const double x = double(float(v[e]));
-            s[e & 1] = fma(x, x, s[e & 1]);
+        for (uint32_t b = 0; b < kChunk / 2048; b += R) {
+            Vec8<T> v[R];
+#pragma unroll
+            for (int r = 0; r < R; ++r) v[r] = *reinterpret_cast<const Vec8<T>*>(p + 2048 * (b + r) + 8 * threadIdx.x);
+#pragma unroll
+            for (int r = 0; r < R; ++r) add_squares<T>(s, v[r]);
         }
+        return s[0] + s[1];
     }
+    const uint32_t full = n / 8;
+#pragma unroll 4
+    for (uint32_t i = threadIdx.x; i < full; i += 256) add_squares<T>(s, *reinterpret_cast<const Vec8<T>*>(p + 8 * i));
     const uint32_t i = 8 * full + threadIdx.x;
     if (i < n) {
         const double x = double(float(p[i]));
@@ -80,8 +91,11 @@ __device__ __forceinline__ double square_sum(const T* p, uint32_t n) {
 __global__ __launch_bounds__(256) void clip_norm_kernel(List l, double* sums) {
     __shared__ double part[4];
     double s = 0.0;
-    for (uint32_t c = blockIdx.x; c < l.chunks; c += gridDim.x) {
-        const Entry& e = entry_of(l, c);
+    const uint32_t c0 = uint32_t(uint64_t(l.chunks) * blockIdx.x / gridDim.x), c1 = uint32_t(uint64_t(l.chunks) * (blockIdx.x + 1) / gridDim.x);
+    uint32_t i = tensor_of(l, c0);
+    for (uint32_t c = c0; c < c1; ++c) {
+        if (i + 1 < l.n && l.e[i + 1].chunk0 <= c) ++i;  // (no tensor of a list is empty)
+        const Entry& e = l.e[i];
         const uint64_t at = uint64_t(c - e.chunk0) * kChunk;
         const uint32_t n = uint32_t(min(uint64_t(kChunk), e.count - at));
         if (e.dtype == VA_DTYPE_F32) s += square_sum(static_cast<const float*>(e.in) + at, n);
@@ -94,11 +108,25 @@ __global__ __launch_bounds__(256) void clip_norm_kernel(List l, double* sums) {
 
 template <class T>
 __device__ __forceinline__ void scale_chunk(const T* in, T* out, uint32_t n, float f) {
-    const uint32_t full = n / 8;
-    for (uint32_t i = threadIdx.x; i < full; i += 256) {
-        const f32x8 v = __builtin_convertvector(*reinterpret_cast<const Vec8<T>*>(in + 8 * i), f32x8) * f;
-        *reinterpret_cast<Vec8<T>*>(out + 8 * i) = __builtin_convertvector(v, Vec8<T>);
+    auto put = [&](uint32_t at, Vec8<T> v) {
+        const f32x8 x = __builtin_convertvector(v, f32x8) * f;
+        *reinterpret_cast<Vec8<T>*>(out + at) = __builtin_convertvector(x, Vec8<T>);
+    };
+    if (n == kChunk) {
+        constexpr int R = sizeof(T) == 4 ? 4 : 8;
+#pragma unroll
+        for (uint32_t b = 0; b < kChunk / 2048; b += R) {
+            Vec8<T> v[R];
+#pragma unroll
+            for (int r = 0; r < R; ++r) v[r] = *reinterpret_cast<const Vec8<T>*>(in + 2048 * (b + r) + 8 * threadIdx.x);
+#pragma unroll
+            for (int r = 0; r < R; ++r) put(2048 * (b + r) + 8 * threadIdx.x, v[r]);
+        }
+        return;
     }
+    const uint32_t full = n / 8;
+#pragma unroll 4
+    for (uint32_t i = threadIdx.x; i < full; i += 256) put(8 * i, *reinterpret_cast<const Vec8<T>*>(in + 8 * i));
     const uint32_t i = 8 * full + threadIdx.x;
     if (i < n) out[i] = T(float(in[i]) * f);
 }
@@ -113,9 +141,13 @@ __global__ __launch_bounds__(256) void clip_scale_kernel(List l, const double* _
     const double q = double(max_norm) / (norm + double(eps));
     const float f = q > 1.0 ? 1.0f : float(q);
     if (out_norm && blockIdx.x == 0 && threadIdx.x == 0) *out_norm = float(norm);
-    for (uint32_t i = blockIdx.x; i < l.chunks; i += gridDim.x) {
-        const uint32_t c = l.chunks - 1 - i;
-        const Entry& e = entry_of(l, c);
+    if (!l.n) return;
+    const uint32_t b = gridDim.x - 1 - blockIdx.x;
+    const uint32_t c0 = uint32_t(uint64_t(l.chunks) * b / gridDim.x), c1 = uint32_t(uint64_t(l.chunks) * (b + 1) / gridDim.x);
+    uint32_t i = tensor_of(l, c0);
+    for (uint32_t c = c0; c < c1; ++c) {
+        if (i + 1 < l.n && l.e[i + 1].chunk0 <= c) ++i;
+        const Entry& e = l.e[i];
         if (f == 1.0f && e.in == e.out) continue;  // in place, and nothing changes
         const uint64_t at = uint64_t(c - e.chunk0) * kChunk;
         const uint32_t n = uint32_t(min(uint64_t(kChunk), e.count - at));
@@ -182,7 +214,7 @@ va_status va_grad_clip(va_context* ctx, const va_tensor_list* t, float max_norm,
     for (uint32_t i = 0; i < t->count || !told;) {
         VA_CHECK_STATUS(take(ctx, t, i, l, i));
         if (!l.n && told) break;
-        clip_scale_kernel<<<dim3(std::min(std::max(l.chunks, 1u), 2048u)), dim3(256), 0, ctx->stream>>>(l, sums, n, max_norm, epsilon, told ? nullptr : out_norm);
+        clip_scale_kernel<<<dim3(std::min(std::max(l.chunks, 1u), kMaxSums)), dim3(256), 0, ctx->stream>>>(l, sums, n, max_norm, epsilon, told ? nullptr : out_norm);
         VA_CHECK_LAUNCH(ctx);
         told = true;
     }

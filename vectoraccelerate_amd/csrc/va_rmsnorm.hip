@@ -6,7 +6,7 @@
 //   dx = i (w dy - n mean_d(w dy n)) + dresidual,  dw = sum_t dy n,  n = r i
 //
 // Bound by memory: every operand is read once and every result written once.  A row is held in
-// registers by one wave (D <= 2048) or one workgroup (D <= 8192): 8 consecutive values a lane and
+// registers by one wave (D <= 2048) or one workgroup (D <= 8192): 16 bytes (8-bit outputs: 8 values) a lane and
 // chunk, so a group's largest value is a few lane exchanges away.  Longer rows are read twice, the
 // second time from cache.  Values are loaded 16 bytes at a time whatever their alignment (global
 // loads on gfx950 need none beyond the element's); a row's last, partial 8 values element by element.
@@ -19,7 +19,9 @@
 namespace va {
 namespace {
 
-typedef float f32x8 __attribute__((ext_vector_type(8)));
+template <int E>
+using F = float __attribute__((ext_vector_type(E)));  // E consecutive values of a row
+using f32x8 = F<8>;
 
 enum Out : int { OUT_SAME = 0, OUT_INT8 = 1, OUT_FP8 = 2 };
 
@@ -40,31 +42,32 @@ struct Elem<VA_DTYPE_BF16> {
 template <int DT>
 using ElemT = typename Elem<DT>::T;
 
-// 8 consecutive values with no alignment beyond the element's
-template <class T>
-using Vec8 = T __attribute__((ext_vector_type(8), aligned(sizeof(T))));
+// E consecutive values with no alignment beyond the element's
+template <class T, int E>
+using Vec = T __attribute__((ext_vector_type(E), aligned(sizeof(T))));
 
-// values [d, d + 8) of a row as fp32, zeros from D on
-template <class T>
-__device__ __forceinline__ f32x8 load8(const T* row, uint32_t d, uint32_t D) {
-    f32x8 o;
-    if (d + 8 <= D) {
-        const Vec8<T> v = *reinterpret_cast<const Vec8<T>*>(row + d);
-        o = __builtin_convertvector(v, f32x8);
+// values [d, d + E) of a row as fp32, zeros from D on
+template <int E, class T>
+__device__ __forceinline__ F<E> load(const T* row, uint32_t d, uint32_t D) {
+    F<E> o;
+    if (d + E <= D) {
+        const Vec<T, E> v = *reinterpret_cast<const Vec<T, E>*>(row + d);
+        o = __builtin_convertvector(v, F<E>);
     } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) o[e] = d + e < D ? float(row[d + e]) : 0.0f;
+        for (int e = 0; e < E; ++e) o[e] = d + e < D ? float(row[d + e]) : 0.0f;
     }
     return o;
 }
-template <class T>
-__device__ __forceinline__ void store8(T* row, uint32_t d, uint32_t D, f32x8 v) {
-    const auto o = __builtin_convertvector(v, Vec8<T>);
-    if (d + 8 <= D) {
-        *reinterpret_cast<Vec8<T>*>(row + d) = o;
+template <int E, class T>
+__device__ __forceinline__ void store(T* row, uint32_t d, uint32_t D, F<E> v) {
+    typedef Vec<T, E> V;
+    const V o = __builtin_convertvector(v, V);
+    if (d + E <= D) {
+        *reinterpret_cast<V*>(row + d) = o;
     } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
+        for (int e = 0; e < E; ++e)
             if (d + e < D) row[d + e] = o[e];
     }
 }
@@ -148,11 +151,11 @@ __device__ __forceinline__ void store_codes(uint8_t* row, uint32_t d, uint32_t D
     }
 }
 
-// WPR waves a row; C chunks of 8 values a lane in registers, or (C == 0) any number, read again
+// WPR waves a row; C chunks of E values a lane in registers, or (C == 0) any number, read again
 template <int DT, int OUT, int WPR, int C>
 __global__ __launch_bounds__(256) void rms_norm_kernel(RmsArgs a) {
     using T = ElemT<DT>;
-    constexpr int NT = 64 * WPR;
+    constexpr int NT = 64 * WPR, E = OUT == OUT_SAME ? 16 / int(sizeof(T)) : 8;
     __shared__ float part[4];
     const uint32_t t = WPR == 1 ? blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
     if (t >= a.T) return;  // (a whole wave, or the workgroup)
@@ -161,26 +164,26 @@ __global__ __launch_bounds__(256) void rms_norm_kernel(RmsArgs a) {
     const T* res = a.residual ? static_cast<const T*>(a.residual) + t * a.ldr : nullptr;
     const T* w = static_cast<const T*>(a.weight);
     T* ro = a.out_residual ? static_cast<T*>(a.out_residual) + t * a.ldro : nullptr;
-    const uint32_t D = a.D, chunks = C ? C : (D + 8 * NT - 1) / (8 * NT);
-    auto sum8 = [&](uint32_t d) {
-        f32x8 v = load8(x, d, D);
-        if (res) v += load8(res, d, D);
+    const uint32_t D = a.D, chunks = C ? C : (D + E * NT - 1) / (E * NT);
+    auto sum_of = [&](uint32_t d) {
+        F<E> v = load<E>(x, d, D);
+        if (res) v += load<E>(res, d, D);
         return v;
     };
-    f32x8 r[C ? C : 1];
+    F<E> r[C ? C : 1];
     float ss = 0.0f;
     if constexpr (C > 0) {
 #pragma unroll
-        for (int c = 0; c < C; ++c) r[c] = sum8((c * NT + tid) * 8);
+        for (int c = 0; c < C; ++c) r[c] = sum_of((c * NT + tid) * E);
 #pragma unroll
         for (int c = 0; c < C; ++c)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) ss = fmaf(r[c][e], r[c][e], ss);
+            for (int e = 0; e < E; ++e) ss = fmaf(r[c][e], r[c][e], ss);
     } else {
         for (uint32_t c = 0; c < chunks; ++c) {
-            const f32x8 v = sum8((c * NT + tid) * 8);
+            const F<E> v = sum_of((c * NT + tid) * E);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) ss = fmaf(v[e], v[e], ss);
+            for (int e = 0; e < E; ++e) ss = fmaf(v[e], v[e], ss);
         }
     }
     ss = row_sum<WPR>(ss, part);
@@ -188,32 +191,32 @@ __global__ __launch_bounds__(256) void rms_norm_kernel(RmsArgs a) {
     if (a.inverse && tid == 0) a.inverse[t] = inv;
 
     // y of a chunk, the new residual stored on the way (once)
-    auto y_of = [&](uint32_t d, f32x8 v, bool keep) {
-        if (ro && keep) store8(ro, d, D, v);
-        return v * inv * load8(w, d, D);
+    auto y_of = [&](uint32_t d, F<E> v, bool keep) {
+        if (ro && keep) store<E>(ro, d, D, v);
+        return v * inv * load<E>(w, d, D);
     };
     if constexpr (OUT == OUT_SAME) {
         T* o = static_cast<T*>(a.out) + t * a.ldo;
         if constexpr (C > 0) {
 #pragma unroll
             for (int c = 0; c < C; ++c) {
-                const uint32_t d = (c * NT + tid) * 8;
-                store8(o, d, D, y_of(d, r[c], true));
+                const uint32_t d = (c * NT + tid) * E;
+                store<E>(o, d, D, y_of(d, r[c], true));
             }
         } else {
             for (uint32_t c = 0; c < chunks; ++c) {
-                const uint32_t d = (c * NT + tid) * 8;
-                store8(o, d, D, y_of(d, sum8(d), true));
+                const uint32_t d = (c * NT + tid) * E;
+                store<E>(o, d, D, y_of(d, sum_of(d), true));
             }
         }
     } else {
         constexpr bool fp8 = OUT == OUT_FP8;
         constexpr float most = fp8 ? 448.0f : 127.0f;
         uint8_t* o = static_cast<uint8_t*>(a.out) + t * a.ldo;
-        auto biggest = [&](f32x8 y) {
+        auto biggest = [&](F<E> y) {
             float m = fabsf(y[0]);
 #pragma unroll
-            for (int e = 1; e < 8; ++e) m = top(m, fabsf(y[e]));
+            for (int e = 1; e < E; ++e) m = top(m, fabsf(y[e]));
             return m;
         };
         // the scale of a whole row: one pass over y first
@@ -223,20 +226,20 @@ __global__ __launch_bounds__(256) void rms_norm_kernel(RmsArgs a) {
             if constexpr (C > 0) {
 #pragma unroll
                 for (int c = 0; c < C; ++c) {
-                    const uint32_t d = (c * NT + tid) * 8;
+                    const uint32_t d = (c * NT + tid) * E;
                     r[c] = y_of(d, r[c], true);
                     m = top(m, biggest(r[c]));
                 }
             } else {
                 for (uint32_t c = 0; c < chunks; ++c) {
-                    const uint32_t d = (c * NT + tid) * 8;
-                    m = top(m, biggest(y_of(d, sum8(d), false)));
+                    const uint32_t d = (c * NT + tid) * E;
+                    m = top(m, biggest(y_of(d, sum_of(d), false)));
                 }
             }
             s = row_top<WPR>(m, part) / most;
             if (tid == 0) a.scales[t] = s;
         }
-        auto emit = [&](uint32_t d, f32x8 y) {
+        auto emit = [&](uint32_t d, F<E> y) {
             float sc = s;
             if (a.group) {
                 float m = biggest(y);
@@ -250,13 +253,13 @@ __global__ __launch_bounds__(256) void rms_norm_kernel(RmsArgs a) {
             const bool have = a.group == 0 && !(a.given > 0.0f);  // r holds y
 #pragma unroll
             for (int c = 0; c < C; ++c) {
-                const uint32_t d = (c * NT + tid) * 8;
+                const uint32_t d = (c * NT + tid) * E;
                 emit(d, have ? r[c] : y_of(d, r[c], true));
             }
         } else {
             for (uint32_t c = 0; c < chunks; ++c) {
-                const uint32_t d = (c * NT + tid) * 8;
-                emit(d, y_of(d, sum8(d), true));
+                const uint32_t d = (c * NT + tid) * E;
+                emit(d, y_of(d, sum_of(d), true));
             }
         }
     }
@@ -293,7 +296,7 @@ __global__ __launch_bounds__(256) void rms_dequantize_kernel(const uint8_t* __re
             for (int e = 0; e < 4; ++e) v[4 * h + e] = float(int8_t(w[h] >> (8 * e)));
         }
     }
-    store8(out + t * ldo, d, D, v * s);
+    store<8>(out + t * ldo, d, D, f32x8(v * s));
 }
 
 // ---- backward ------------------------------------------------------------------------------------
@@ -313,18 +316,18 @@ struct RmsGradArgs {
 template <int DT, int WPR, int C>
 __global__ __launch_bounds__(256) void rms_grad_kernel(RmsGradArgs a) {
     using T = ElemT<DT>;
-    constexpr int NT = 64 * WPR, CC = C ? C : 1;
+    constexpr int NT = 64 * WPR, CC = C ? C : 1, E = 16 / int(sizeof(T));
     constexpr int ROWS = 4 / WPR;
     __shared__ float part[4];
-    __shared__ f32x8 join[WPR == 1 && C > 0 ? 256 : 1];
+    __shared__ F<E> join[WPR == 1 && C > 0 ? 256 : 1];
     const uint32_t tid = WPR == 1 ? threadIdx.x & 63 : threadIdx.x;
-    const uint32_t D = a.D, chunks = C ? C : (D + 8 * NT - 1) / (8 * NT);
+    const uint32_t D = a.D, chunks = C ? C : (D + E * NT - 1) / (E * NT);
     const T* w = static_cast<const T*>(a.weight);
-    f32x8 dw[CC], wv[CC];
+    F<E> dw[CC], wv[CC];
 #pragma unroll
     for (int c = 0; c < CC; ++c) {
-        dw[c] = f32x8(0.0f);
-        if constexpr (C > 0) wv[c] = load8(w, (c * NT + tid) * 8, D);
+        dw[c] = F<E>(0.0f);
+        if constexpr (C > 0) wv[c] = load<E>(w, (c * NT + tid) * E, D);
     }
     for (uint32_t t = blockIdx.x * ROWS + (WPR == 1 ? threadIdx.x >> 6 : 0); t < a.T; t += gridDim.x * ROWS) {
         const T* g = static_cast<const T*>(a.grad) + t * a.ldg;
@@ -332,42 +335,42 @@ __global__ __launch_bounds__(256) void rms_grad_kernel(RmsGradArgs a) {
         const T* gr = a.grad_residual ? static_cast<const T*>(a.grad_residual) + t * a.ldgr : nullptr;
         const float inv = a.inverse[t];
         float along = 0.0f;
-        f32x8 gv[CC], nv[CC];
-        auto chunk = [&](uint32_t d, f32x8 wc, f32x8& gg, f32x8& nn) {
-            gg = load8(g, d, D);
-            nn = load8(r, d, D) * inv;
+        F<E> gv[CC], nv[CC];
+        auto chunk = [&](uint32_t d, F<E> wc, F<E>& gg, F<E>& nn) {
+            gg = load<E>(g, d, D);
+            nn = load<E>(r, d, D) * inv;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) along = fmaf(gg[e] * wc[e], nn[e], along);
+            for (int e = 0; e < E; ++e) along = fmaf(gg[e] * wc[e], nn[e], along);
         };
         if constexpr (C > 0) {
 #pragma unroll
             for (int c = 0; c < C; ++c) {
-                chunk((c * NT + tid) * 8, wv[c], gv[c], nv[c]);
+                chunk((c * NT + tid) * E, wv[c], gv[c], nv[c]);
                 dw[c] += gv[c] * nv[c];
             }
         } else {
             for (uint32_t c = 0; c < chunks; ++c) {
-                const uint32_t d = (c * NT + tid) * 8;
-                f32x8 gg, nn;
-                chunk(d, load8(w, d, D), gg, nn);
+                const uint32_t d = (c * NT + tid) * E;
+                F<E> gg, nn;
+                chunk(d, load<E>(w, d, D), gg, nn);
             }
         }
         along = row_sum<WPR>(along, part) / float(D);
         if (!a.out) continue;
         T* o = static_cast<T*>(a.out) + t * a.ldo;
-        auto finish = [&](uint32_t d, f32x8 wc, f32x8 gg, f32x8 nn) {
-            f32x8 v = (gg * wc - nn * along) * inv;
-            if (gr) v += load8(gr, d, D);
-            store8(o, d, D, v);
+        auto finish = [&](uint32_t d, F<E> wc, F<E> gg, F<E> nn) {
+            F<E> v = (gg * wc - nn * along) * inv;
+            if (gr) v += load<E>(gr, d, D);
+            store<E>(o, d, D, v);
         };
         if constexpr (C > 0) {
 #pragma unroll
-            for (int c = 0; c < C; ++c) finish((c * NT + tid) * 8, wv[c], gv[c], nv[c]);
+            for (int c = 0; c < C; ++c) finish((c * NT + tid) * E, wv[c], gv[c], nv[c]);
         } else {
             for (uint32_t c = 0; c < chunks; ++c) {
-                const uint32_t d = (c * NT + tid) * 8;
-                f32x8 gg = load8(g, d, D), nn = load8(r, d, D) * inv;
-                finish(d, load8(w, d, D), gg, nn);
+                const uint32_t d = (c * NT + tid) * E;
+                F<E> gg = load<E>(g, d, D), nn = load<E>(r, d, D) * inv;
+                finish(d, load<E>(w, d, D), gg, nn);
             }
         }
     }
@@ -376,8 +379,8 @@ __global__ __launch_bounds__(256) void rms_grad_kernel(RmsGradArgs a) {
         float* o = a.part + uint64_t(blockIdx.x) * D;
 #pragma unroll
         for (int c = 0; c < C; ++c) {
-            const uint32_t d = (c * NT + tid) * 8;
-            f32x8 v = dw[c];
+            const uint32_t d = (c * NT + tid) * E;
+            F<E> v = dw[c];
             if constexpr (WPR == 1) {
                 __syncthreads();
                 join[threadIdx.x] = v;
@@ -386,7 +389,7 @@ __global__ __launch_bounds__(256) void rms_grad_kernel(RmsGradArgs a) {
                 v = (join[tid] + join[tid + 64]) + (join[tid + 128] + join[tid + 192]);
             }
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
+            for (int e = 0; e < E; ++e)
                 if (d + e < D) o[d + e] = v[e];
         }
     }
@@ -399,7 +402,7 @@ __global__ __launch_bounds__(256) void rms_weight_grad_kernel(RmsGradArgs a) {
     const uint32_t d = (blockIdx.x * 256 + threadIdx.x) * 8;
     f32x8 dw(0.0f);
     for (uint32_t t = blockIdx.y; t < a.T; t += gridDim.y)
-        dw += load8(static_cast<const T*>(a.grad) + t * a.ldg, d, a.D) * (load8(static_cast<const T*>(a.r) + t * a.ldr, d, a.D) * a.inverse[t]);
+        dw += load<8>(static_cast<const T*>(a.grad) + t * a.ldg, d, a.D) * (load<8>(static_cast<const T*>(a.r) + t * a.ldr, d, a.D) * a.inverse[t]);
     for (int e = 0; e < 8; ++e)
         if (d + e < a.D) a.part[uint64_t(blockIdx.y) * a.D + d + e] = dw[e];
 }
@@ -421,20 +424,31 @@ __global__ __launch_bounds__(1024) void rms_weight_sum_kernel(const float* __res
 }
 
 // ---- host ------------------------------------------------------------------------------------------
-template <class F>
-va_status by_shape(uint32_t D, F&& f) {
+// f(waves a row, chunks) for rows of D values, E a lane and chunk
+template <int E, class Fn>
+va_status by_shape(uint32_t D, Fn&& f) {
     using std::integral_constant;
-    const uint32_t c1 = ceil_div(D, 512), c4 = ceil_div(D, 2048);
-    if (c1 <= 1) return f(integral_constant<int, 1>(), integral_constant<int, 1>());
-    if (c1 == 2) return f(integral_constant<int, 1>(), integral_constant<int, 2>());
-    if (c1 == 3) return f(integral_constant<int, 1>(), integral_constant<int, 3>());
-    if (c1 == 4) return f(integral_constant<int, 1>(), integral_constant<int, 4>());
-    if (c4 == 2) return f(integral_constant<int, 4>(), integral_constant<int, 2>());
-    if (c4 <= 4) return f(integral_constant<int, 4>(), integral_constant<int, 4>());
-    return f(integral_constant<int, 4>(), integral_constant<int, 0>());
+    const integral_constant<int, 1> wave{};
+    const integral_constant<int, 4> group{};
+    switch (ceil_div(D, 64 * E)) {
+        case 1: return f(wave, integral_constant<int, 1>());
+        case 2: return f(wave, integral_constant<int, 2>());
+        case 3: return f(wave, integral_constant<int, 3>());
+        case 4: return f(wave, integral_constant<int, 4>());
+        default: break;
+    }
+    if constexpr (E == 4) {
+        if (D <= 64 * E * 6) return f(wave, integral_constant<int, 6>());
+        if (D <= 64 * E * 8) return f(wave, integral_constant<int, 8>());
+    }
+    const uint32_t c = ceil_div(D, 256 * E);
+    if (c <= 2) return f(group, integral_constant<int, 2>());
+    if (c <= 4) return f(group, integral_constant<int, 4>());
+    if (E == 4 && c <= 8) return f(group, integral_constant<int, 8>());
+    return f(group, integral_constant<int, 0>());
 }
-template <class F>
-va_status by_dtype(va_dtype t, F&& f) {
+template <class Fn>
+va_status by_dtype(va_dtype t, Fn&& f) {
     if (t == VA_DTYPE_F32) return f(std::integral_constant<int, VA_DTYPE_F32>());
     if (t == VA_DTYPE_F16) return f(std::integral_constant<int, VA_DTYPE_F16>());
     return f(std::integral_constant<int, VA_DTYPE_BF16>());
@@ -461,7 +475,8 @@ va_status forward(va_context* ctx, const va_rms_desc* d, void* out, uint64_t ldo
     RmsArgs a{d->x, d->residual, d->weight, d->out_residual, d->out_inverse_rms, out, scales, d->x_stride, d->residual_stride,
               d->out_residual_stride, ldo, d->rows, d->dim, group, group ? ceil_div(d->dim, group) : 1u, d->epsilon, given};
     return by_dtype(d->dtype, [&](auto dt) {
-        return by_shape(d->dim, [&](auto wpr, auto c) {
+        constexpr int E = OUT == OUT_SAME ? 16 / int(sizeof(ElemT<decltype(dt)::value>)) : 8;
+        return by_shape<E>(d->dim, [&](auto wpr, auto c) {
             const uint32_t grid = decltype(wpr)::value == 1 ? ceil_div(a.T, 4) : a.T;
             rms_norm_kernel<decltype(dt)::value, OUT, decltype(wpr)::value, decltype(c)::value><<<dim3(grid), dim3(256), 0, ctx->stream>>>(a);
             VA_CHECK_LAUNCH(ctx);
@@ -541,7 +556,7 @@ va_status va_rms_norm_backward(va_context* ctx, const va_rms_desc* d, const void
                   grad_x_stride, d->rows, d->dim};
     return by_dtype(d->dtype, [&](auto dt) {
         constexpr int DT = decltype(dt)::value;
-        return by_shape(d->dim, [&](auto wpr, auto c) {
+        return by_shape<16 / int(sizeof(ElemT<DT>))>(d->dim, [&](auto wpr, auto c) {
             constexpr int WPR = decltype(wpr)::value, C = decltype(c)::value;
             // two workgroups a CU; fewer where their shares of dw would be more than the rows
             const uint32_t grid = std::min(ceil_div(a.T, 4 / WPR), 2u * uint32_t(ctx->num_cus));
