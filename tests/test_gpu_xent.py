@@ -277,7 +277,7 @@ def test_torch_stream_context(ctx):
         pass
 
     c = Borrowed()
-    c.lib, c.handle = lib, handle
+    c.lib, c.handle, c.device = lib, handle, 0
     c.check = lambda st, what: (_ for _ in ()).throw(RuntimeError(what)) if st else None
     torch.cuda.synchronize()
     with torch.cuda.stream(stream):

@@ -40,36 +40,41 @@ def _dtype(t, name: str) -> int:
     return d
 
 
-def _rows(t, name: str, like=None, shape=None) -> tuple[int, int]:
-    """(device pointer, elements between rows) of a device matrix whose rows are contiguous; checked
-    against `like`'s type and device and against `shape`."""
-    if not t.is_cuda:
-        raise VectorError.invalidInput(f"{name}: expected a device (CUDA) tensor")
-    if t.dim() != 2:
-        raise VectorError.invalidInput(f"{name}: expected a matrix, got {t.dim()} dimensions")
-    if shape is not None and tuple(t.shape) != tuple(shape):
-        if t.shape[1] != shape[1]:
-            raise VectorError.dimensionMismatch(shape[1], t.shape[1])
-        raise VectorError.invalidInput(f"{name}: expected {shape[0]} rows, got {t.shape[0]}")
-    if like is not None:
-        if t.dtype != like.dtype:
-            raise VectorError.invalidInput(f"{name}: expected {like.dtype}, got {t.dtype}")
-        if t.device != like.device:
-            raise VectorError.invalidInput(f"{name}: on {t.device}, expected {like.device}")
-    rows, dim = t.shape
+def _place(t, name: str, device: int) -> None:
+    got = t.get_device()  # -1 on the CPU
+    if got != device:
+        raise VectorError.invalidInput(f"{name}: expected a device (CUDA) tensor" if got < 0 else f"{name}: on {t.device}, expected cuda:{device}")
+
+
+def _rows(t, name: str, device: int, dtype=None, shape=None) -> tuple[int, int]:
+    """(device pointer, elements between rows) of a matrix on the context's device whose rows are
+    contiguous; checked against `dtype` and `shape`."""
+    _place(t, name, device)
+    got = t.shape
+    if len(got) != 2:
+        raise VectorError.invalidInput(f"{name}: expected a matrix, got {len(got)} dimensions")
+    rows, dim = got
+    if shape is not None and got != shape:
+        if dim != shape[1]:
+            raise VectorError.dimensionMismatch(shape[1], dim)
+        raise VectorError.invalidInput(f"{name}: expected {shape[0]} rows, got {rows}")
+    if dtype is not None and t.dtype != dtype:
+        raise VectorError.invalidInput(f"{name}: expected {dtype}, got {t.dtype}")
     sr, sd = t.stride()
-    if dim > 1 and sd != 1:
+    if sd != 1 and dim > 1:
         raise VectorError.invalidInput(f"{name}: the values of a row must be contiguous")
-    if rows > 1 and sr < dim:
+    if rows < 2:
+        return t.data_ptr(), max(sr, dim)
+    if sr < dim:
         raise VectorError.invalidInput(f"{name}: rows overlap")
-    return t.data_ptr(), sr if rows > 1 else max(sr, dim)
+    return t.data_ptr(), sr
 
 
-def _vector(t, name: str, dtype, count: int, like) -> int:
-    """Device pointer of a contiguous vector of `count` values of `dtype` on `like`'s device."""
-    if t.dtype != dtype or t.numel() != count or t.device != like.device or not t.is_contiguous():
+def _vector(t, name: str, dtype, count: int, device: int) -> int:
+    """Device pointer of a contiguous vector of `count` values of `dtype` on the context's device."""
+    if t.dtype != dtype or t.numel() != count or t.get_device() != device or not t.is_contiguous():
         raise VectorError.invalidInput(
-            f"{name}: expected {count} contiguous values of {dtype} on {like.device}, got {tuple(t.shape)} of {t.dtype} on {t.device}")
+            f"{name}: expected {count} contiguous values of {dtype} on cuda:{device}, got {tuple(t.shape)} of {t.dtype} on {t.device}")
     return t.data_ptr()
 
 
@@ -99,14 +104,16 @@ class SoftmaxCrossEntropyKernel:
         self.context = context
 
     def _describe(self, hidden, items, targets, scale, offsets, ignoreIndex):
-        torch = _torch()
+        torch, device = _torch(), self.context.device
         dtype = _dtype(hidden, "hidden")
-        hp, hs = _rows(hidden, "hidden")
-        ip, is_ = _rows(items, "items", hidden, (items.shape[0], hidden.shape[1]))
+        hp, hs = _rows(hidden, "hidden", device)
         T, D = hidden.shape
-        V = items.shape[0]
-        return _lib.XentDesc(hp, ip, _vector(targets, "targets", torch.int64, T, hidden),
-                             _vector(offsets, "offsets", torch.float32, V, hidden) if offsets is not None else None,
+        ip, is_ = _rows(items, "items", device, hidden.dtype)
+        V, width = items.shape
+        if width != D:
+            raise VectorError.dimensionMismatch(D, width)
+        return _lib.XentDesc(hp, ip, _vector(targets, "targets", torch.int64, T, device),
+                             _vector(offsets, "offsets", torch.float32, V, device) if offsets is not None else None,
                              hs, is_, int(ignoreIndex), T, V, D, dtype, float(scale))
 
     def encodeForward(self, hidden, items, targets, outLoss, outLogSumExp, outReduced=None, reduction: str = "mean",
@@ -117,9 +124,9 @@ class SoftmaxCrossEntropyKernel:
         mode = _reduction(reduction) if outReduced is not None else _lib.VA_REDUCE_NONE
         if outReduced is not None and mode == _lib.VA_REDUCE_NONE:
             raise VectorError.invalidInput("a reduced loss needs a reduction")
-        c.check(c.lib.va_xent_forward(c.handle, C.byref(d), _vector(outLoss, "outLoss", f32, d.rows, hidden),
-                                      _vector(outLogSumExp, "outLogSumExp", f32, d.rows, hidden), mode,
-                                      _vector(outReduced, "outReduced", f32, 1, hidden) if outReduced is not None else None),
+        c.check(c.lib.va_xent_forward(c.handle, C.byref(d), _vector(outLoss, "outLoss", f32, d.rows, c.device),
+                                      _vector(outLogSumExp, "outLogSumExp", f32, d.rows, c.device), mode,
+                                      _vector(outReduced, "outReduced", f32, 1, c.device) if outReduced is not None else None),
                 "va_xent_forward")
 
     def encodeBackward(self, hidden, items, targets, logSumExp, outGradHidden=None, outGradItems=None, grad=None,
@@ -133,10 +140,10 @@ class SoftmaxCrossEntropyKernel:
         if mode == _lib.VA_REDUCE_NONE and grad is None:
             raise VectorError.invalidInput("without a reduction the rows' gradients are needed")
         count = d.rows if mode == _lib.VA_REDUCE_NONE else 1
-        hp, hs = _rows(outGradHidden, "outGradHidden", hidden, hidden.shape) if outGradHidden is not None else (None, 0)
-        ip, is_ = _rows(outGradItems, "outGradItems", hidden, items.shape) if outGradItems is not None else (None, 0)
-        c.check(c.lib.va_xent_backward(c.handle, C.byref(d), _vector(logSumExp, "logSumExp", f32, d.rows, hidden), mode,
-                                       _vector(grad, "grad", f32, count, hidden) if grad is not None else None, hp, hs, ip, is_),
+        hp, hs = _rows(outGradHidden, "outGradHidden", c.device, hidden.dtype, hidden.shape) if outGradHidden is not None else (None, 0)
+        ip, is_ = _rows(outGradItems, "outGradItems", c.device, hidden.dtype, items.shape) if outGradItems is not None else (None, 0)
+        c.check(c.lib.va_xent_backward(c.handle, C.byref(d), _vector(logSumExp, "logSumExp", f32, d.rows, c.device), mode,
+                                       _vector(grad, "grad", f32, count, c.device) if grad is not None else None, hp, hs, ip, is_),
                 "va_xent_backward")
 
     def forward(self, hidden, items, targets, reduction: str = "mean", scale: float = 1.0, offsets=None,
@@ -181,32 +188,27 @@ class RMSNormKernel:
     def __init__(self, context: GPUContext):
         self.context = context
 
-    @staticmethod
-    def _describe(x, weight, residual, outResidual, outInverseRms, epsilon):
-        torch = _torch()
+    def _describe(self, x, weight, residual, outResidual, outInverseRms, epsilon):
+        torch, device = _torch(), self.context.device
         dtype = _dtype(x, "x")
-        xp, xs = _rows(x, "x")
-        T, D = x.shape
-        rp, rs = _rows(residual, "residual", x, x.shape) if residual is not None else (None, 0)
-        op, os_ = _rows(outResidual, "outResidual", x, x.shape) if outResidual is not None else (None, 0)
-        ip = _vector(outInverseRms, "outInverseRms", torch.float32, T, x) if outInverseRms is not None else None
+        xp, xs = _rows(x, "x", device)
+        T, D = shape = x.shape
+        rp, rs = _rows(residual, "residual", device, x.dtype, shape) if residual is not None else (None, 0)
+        op, os_ = _rows(outResidual, "outResidual", device, x.dtype, shape) if outResidual is not None else (None, 0)
+        ip = _vector(outInverseRms, "outInverseRms", torch.float32, T, device) if outInverseRms is not None else None
         if weight.numel() != D:
             raise VectorError.dimensionMismatch(D, weight.numel())
-        return _lib.RmsDesc(xp, rp, _vector(weight, "weight", x.dtype, D, x), op, ip, xs, rs, os_, T, D, dtype, float(epsilon))
+        return _lib.RmsDesc(xp, rp, _vector(weight, "weight", x.dtype, D, device), op, ip, xs, rs, os_, T, D, dtype, float(epsilon))
 
-    @staticmethod
-    def _codes(codes, x_shape, like):
+    def _codes(self, codes, shape):
         _torch()
         code = _CODES.get(codes.dtype)
         if code is None:
             raise VectorError.invalidInput(f"codes: unsupported type {codes.dtype} (int8 or float8_e4m3fn)")
-        p, s = _rows(codes, "codes", None, x_shape)
-        if codes.device != like.device:
-            raise VectorError.invalidInput(f"codes: on {codes.device}, expected {like.device}")
+        p, s = _rows(codes, "codes", self.context.device, None, shape)
         return code, p, s
 
-    @staticmethod
-    def _scales(scales, givenScale, groupSize, T, D, like):
+    def _scales(self, scales, givenScale, groupSize, T, D):
         if (scales is None) == (givenScale is None):
             raise VectorError.invalidInput("either scales or a given scale")
         if givenScale is not None:
@@ -214,20 +216,20 @@ class RMSNormKernel:
                 raise VectorError.invalidInput(f"a given scale must be positive, got {givenScale}")
             return None
         groups = -(-D // groupSize) if groupSize else 1
-        return _vector(scales, "scales", _torch().float32, T * groups, like)
+        return _vector(scales, "scales", _torch().float32, T * groups, self.context.device)
 
     def encode(self, x, weight, out, residual=None, outResidual=None, outInverseRms=None, epsilon: float = 1e-6) -> None:
         c = self.context
         d = self._describe(x, weight, residual, outResidual, outInverseRms, epsilon)
-        op, os_ = _rows(out, "out", x, x.shape)
+        op, os_ = _rows(out, "out", c.device, x.dtype, x.shape)
         c.check(c.lib.va_rms_norm(c.handle, C.byref(d), op, os_), "va_rms_norm")
 
     def encodeQuantized(self, x, weight, outCodes, outScales=None, residual=None, outResidual=None, outInverseRms=None,
                         groupSize: int = 0, givenScale: float | None = None, epsilon: float = 1e-6) -> None:
         c = self.context
         d = self._describe(x, weight, residual, outResidual, outInverseRms, epsilon)
-        code, cp, cs = self._codes(outCodes, x.shape, x)
-        sp = self._scales(outScales, givenScale, groupSize, d.rows, d.dim, x)
+        code, cp, cs = self._codes(outCodes, x.shape)
+        sp = self._scales(outScales, givenScale, groupSize, d.rows, d.dim)
         c.check(c.lib.va_rms_norm_quantized(c.handle, C.byref(d), code, int(groupSize), float(givenScale or 0.0), cp, cs, sp),
                 "va_rms_norm_quantized")
 
@@ -235,10 +237,10 @@ class RMSNormKernel:
         """out = code * scale in out's type."""
         c = self.context
         dtype = _dtype(out, "out")
-        op, os_ = _rows(out, "out")
+        op, os_ = _rows(out, "out", c.device)
         T, D = out.shape
-        code, cp, cs = self._codes(codes, out.shape, out)
-        sp = self._scales(scales, givenScale, groupSize, T, D, out)
+        code, cp, cs = self._codes(codes, out.shape)
+        sp = self._scales(scales, givenScale, groupSize, T, D)
         c.check(c.lib.va_rms_dequantize(c.handle, cp, cs, code, sp, float(givenScale or 0.0), T, D, int(groupSize), dtype, op, os_),
                 "va_rms_dequantize")
 
@@ -248,12 +250,13 @@ class RMSNormKernel:
         gradient of x and of the residual alike."""
         c = self.context
         d = self._describe(summed, weight, None, None, None, 0.0)
-        gp, gs = _rows(grad, "grad", summed, summed.shape)
-        rp, rs = _rows(gradResidual, "gradResidual", summed, summed.shape) if gradResidual is not None else (None, 0)
-        xp, xs = _rows(outGradX, "outGradX", summed, summed.shape) if outGradX is not None else (None, 0)
-        wp = _vector(outGradWeight, "outGradWeight", summed.dtype, d.dim, summed) if outGradWeight is not None else None
+        dtype, shape = summed.dtype, summed.shape
+        gp, gs = _rows(grad, "grad", c.device, dtype, shape)
+        rp, rs = _rows(gradResidual, "gradResidual", c.device, dtype, shape) if gradResidual is not None else (None, 0)
+        xp, xs = _rows(outGradX, "outGradX", c.device, dtype, shape) if outGradX is not None else (None, 0)
+        wp = _vector(outGradWeight, "outGradWeight", dtype, d.dim, c.device) if outGradWeight is not None else None
         c.check(c.lib.va_rms_norm_backward(c.handle, C.byref(d), gp, gs, rp, rs,
-                                           _vector(inverseRms, "inverseRms", _torch().float32, d.rows, summed), xp, xs, wp),
+                                           _vector(inverseRms, "inverseRms", _torch().float32, d.rows, c.device), xp, xs, wp),
                 "va_rms_norm_backward")
 
     def forward(self, x, weight, residual=None, epsilon: float = 1e-6):
@@ -332,9 +335,10 @@ class GradientClipKernel:
     def encode(self, tensors: TensorList, maxNorm: float, outNorm=None, epsilon: float = 1e-6) -> None:
         """outNorm: one fp32 value on the device, or None."""
         c = self.context
-        if outNorm is not None and (outNorm.dtype != _torch().float32 or outNorm.numel() != 1 or not outNorm.is_cuda):
-            raise VectorError.invalidInput("outNorm: expected one float32 value on the device")
-        c.check(c.lib.va_grad_clip(c.handle, C.byref(tensors.desc), float(maxNorm), float(epsilon), dptr(outNorm) or None), "va_grad_clip")
+        if tensors.tensors:
+            _place(tensors.tensors[0], "tensors", c.device)  # (the list has checked that they are together)
+        norm = _vector(outNorm, "outNorm", _torch().float32, 1, c.device) if outNorm is not None else None
+        c.check(c.lib.va_grad_clip(c.handle, C.byref(tensors.desc), float(maxNorm), float(epsilon), norm), "va_grad_clip")
 
     def clip(self, tensors, maxNorm: float, epsilon: float = 1e-6) -> float:
         """Clips the tensors in place and returns their norm before."""
