@@ -218,3 +218,32 @@ def test_refusals(ctx):
               lambda: k.encodeBackward(x, x, w, torch.empty(3, device="cuda"), x), lambda: k.encodeBackward(x, x, w, torch.empty(4, device="cuda"))):
         with pytest.raises(VectorError):
             f()
+
+
+@pytest.mark.parametrize("code", [None, torch.int8])
+def test_more_rows_than_a_launch_holds(ctx, code):
+    """Rows past what one launch's 2^23 workgroups take (and a launch's 2^32 threads would)."""
+    from vectoraccelerate_amd import RMSNormKernel
+
+    k = RMSNormKernel(ctx)
+    T, D = (1 << 26) + 77, 3
+    x = torch.randn(T, D, device="cuda", dtype=torch.bfloat16, generator=torch.Generator("cuda").manual_seed(5))
+    w = torch.tensor([1.0, -0.5, 2.0], device="cuda", dtype=torch.bfloat16)
+    parts = [slice(0, 500), *(slice((i << 25) - 500, (i << 25) + 500) for i in (1, 2)), slice(T - 300, T)]
+    if code is None:
+        y, _, inv = k.forward(x, w, None, EPS)
+        for p in parts:
+            _, ii, yy, e = oracle.rms(x[p], None, w, EPS)
+            oracle.close(inv[p], ii, e * ii, "inverse rms")
+            oracle.close(y[p], yy, (e + U[torch.bfloat16]) * yy.abs() + TINY[torch.bfloat16], "y")
+        return
+    codes, scales, _ = k.quantize(x, w)
+    y = torch.empty(T, D, device="cuda", dtype=torch.float32)
+    k.encodeDequantize(codes, scales, y)
+    ctx.synchronize()
+    for p in parts:
+        _, ii, yy, e = oracle.rms(x[p], None, w, EPS)
+        want = yy.abs().amax(1) / 127.0
+        oracle.close(scales[p].squeeze(1), want, (e + 2 * U32) * want, "scales")
+        # (half a step of the code and what the arithmetic moves y / s by; the product's own rounding)
+        oracle.close(y[p], yy, want[:, None] * (0.5 + 127.0 * (2 * e + 8 * U32)), "codes")

@@ -325,3 +325,42 @@ def test_refusals(ctx):
                {"logSumExp": lse[:2]}):
         with pytest.raises(VectorError):
             k.encodeBackward(**({"hidden": h, "items": w, "targets": y, "logSumExp": lse, "outGradHidden": gh, "outGradItems": gw} | kw))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_more_rows_than_a_launch_holds(ctx, dtype):
+    """Rows past what 2^23 workgroups of one launch take: a wave a row in the copies and at the loss's end."""
+    from vectoraccelerate_amd import SoftmaxCrossEntropyKernel
+
+    k = SoftmaxCrossEntropyKernel(ctx)
+    T, V, D = (1 << 25) + 301, 3, 2
+    g = torch.Generator("cuda").manual_seed(53)
+    h = torch.randn(T, D, device="cuda", generator=g).to(dtype)
+    w = torch.randn(V, D, device="cuda", generator=g).to(dtype)
+    y = torch.randint(0, V, (T,), device="cuda", generator=g)
+    res = k.forward(h, w, y, "none")
+    for p in (slice(0, 400), slice((1 << 25) - 300, T)):
+        want = oracle.xent(h[p], w, y[p], 1.0, None, IGNORE, torch.zeros(h[p].shape[0], dtype=torch.float64))
+        oracle.close(res.logSumExp[p], *want["lse"], "lse")
+        oracle.close(res.loss[p], *want["loss"], "loss")
+
+
+def test_long_gradients_of_shares(ctx):
+    """The hidden rows' gradient in shares of more values than a launch has threads."""
+    from vectoraccelerate_amd import SoftmaxCrossEntropyKernel
+
+    k = SoftmaxCrossEntropyKernel(ctx)
+    T, V, D = (1 << 21) + 67, 700, 1028
+    g = torch.Generator("cuda").manual_seed(59)
+    h = torch.randn(T, D, device="cuda", dtype=torch.bfloat16, generator=g)
+    w = torch.randn(V, D, device="cuda", dtype=torch.bfloat16, generator=g) * D**-0.5
+    y = torch.randint(0, V, (T,), device="cuda", generator=g)
+    res = k.forward(h, w, y, "sum")
+    gh = torch.full_like(h, torch.nan)
+    ctx.order_after_torch()
+    k.encodeBackward(h, w, y, res.logSumExp, gh, None, None, "sum")
+    ctx.synchronize()
+    for p in (slice(0, 70), slice(T // 2, T // 2 + 70), slice(T - 70, T)):
+        want = oracle.xent(h[p], w, y[p], 1.0, None, IGNORE, torch.ones(h[p].shape[0], dtype=torch.float64))
+        oracle.close(gh[p], *want["grad_hidden"], "grad_hidden")
+    assert not bool(torch.isnan(gh).any())

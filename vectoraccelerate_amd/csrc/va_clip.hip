@@ -20,10 +20,12 @@ namespace {
 constexpr uint32_t kChunk = 16384;
 constexpr uint32_t kListMax = 166;    // just under 4 KiB of arguments
 constexpr uint32_t kChunk0Max = 1u << 22;
-constexpr uint32_t kMaxSums = 2048;   // workgroups of the first pass, all launches together: eight a CU
+// Workgroups of 256 threads a CU, all of them resident (72 registers): the two passes over 468 MB in bf16 take 289 us
+// with 7, 291 with 6, 294 with 8 (64 registers); over 94 MB in 290 tensors 66, 68 and 67.
+constexpr uint32_t kPerCu = 7;
 
-// A tensor in 24 bytes: the more of them a launch holds, the fewer launches (290 tensors: 124 a launch 81 us, 166 a
-// launch 72 us).
+// A tensor in 24 bytes: the more of them a launch holds, the fewer launches (290 tensors of 94 MB: 124 a launch
+// 81 us, 166 a launch 72 us, before the grid above).
 struct Entry {
     const void* in;
     void* out;
@@ -92,7 +94,7 @@ __device__ __forceinline__ double square_sum(const T* p, uint32_t n) {
     return s[0] + s[1];
 }
 
-__global__ __launch_bounds__(256) void clip_norm_kernel(List l, double* sums) {
+__global__ __launch_bounds__(256, kPerCu) void clip_norm_kernel(List l, double* sums) {
     __shared__ double part[4];
     double s = 0.0;
     const uint32_t c0 = uint32_t(uint64_t(l.chunks) * blockIdx.x / gridDim.x), c1 = uint32_t(uint64_t(l.chunks) * (blockIdx.x + 1) / gridDim.x);
@@ -135,7 +137,7 @@ __device__ __forceinline__ void scale_chunk(const T* in, T* out, uint32_t n, flo
     if (i < n) out[i] = T(float(in[i]) * f);
 }
 
-__global__ __launch_bounds__(256) void clip_scale_kernel(List l, const double* __restrict__ sums, uint32_t nsums, float max_norm, float eps,
+__global__ __launch_bounds__(256, kPerCu) void clip_scale_kernel(List l, const double* __restrict__ sums, uint32_t nsums, float max_norm, float eps,
                                                          float* out_norm) {
     __shared__ double part[4];
     double s = 0.0;
@@ -197,9 +199,11 @@ va_status va_grad_clip(va_context* ctx, const va_tensor_list* t, float max_norm,
         total += (t->sizes[i] + kChunk - 1) / kChunk;
     }
     DeviceGuard guard(ctx->device);
+    // the launches are at most so many: each is closed by its tensors, or by its chunks
+    const uint32_t most = kPerCu * uint32_t(ctx->num_cus);
+    const uint64_t launches = ceil_div(t->count, kListMax) + total / kChunk0Max;
     Scratch sc(ctx);
-    // each launch has one sum at least: at most so many launches are closed by their tensors, or by their chunks
-    const uint64_t slots = kMaxSums + ceil_div(t->count, kListMax) + total / kChunk0Max;
+    const uint64_t slots = std::min<uint64_t>(uint64_t(launches) * most, total);
     VA_CHECK_STATUS(sc.reserve(Scratch::round(slots * sizeof(double))));
     double* sums = sc.carve<double>(slots);
     uint32_t n = 0;
@@ -207,8 +211,7 @@ va_status va_grad_clip(va_context* ctx, const va_tensor_list* t, float max_norm,
     for (uint32_t i = 0; i < t->count;) {
         i = take(t, i, l);
         if (!l.n) break;
-        // the launch's share of the sums, by its share of the chunks
-        const uint32_t grid = uint32_t(std::max<uint64_t>(std::min<uint64_t>(l.chunks, uint64_t(kMaxSums) * l.chunks / std::max<uint64_t>(total, kMaxSums)), 1));
+        const uint32_t grid = std::min(l.chunks, most);
         clip_norm_kernel<<<dim3(grid), dim3(256), 0, ctx->stream>>>(l, sums + n);
         VA_CHECK_LAUNCH(ctx);
         n += grid;
@@ -217,7 +220,7 @@ va_status va_grad_clip(va_context* ctx, const va_tensor_list* t, float max_norm,
     for (uint32_t i = 0; i < t->count || !told;) {
         i = take(t, i, l);
         if (!l.n && told) break;
-        clip_scale_kernel<<<dim3(std::min(std::max(l.chunks, 1u), kMaxSums)), dim3(256), 0, ctx->stream>>>(l, sums, n, max_norm, epsilon, told ? nullptr : out_norm);
+        clip_scale_kernel<<<dim3(std::min(std::max(l.chunks, 1u), most)), dim3(256), 0, ctx->stream>>>(l, sums, n, max_norm, epsilon, told ? nullptr : out_norm);
         VA_CHECK_LAUNCH(ctx);
         told = true;
     }

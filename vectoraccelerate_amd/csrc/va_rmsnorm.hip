@@ -46,18 +46,18 @@ using ElemT = typename Elem<DT>::T;
 template <class T, int E>
 using Vec = T __attribute__((ext_vector_type(E), aligned(sizeof(T))));
 
-// values [d, d + E) of a row as fp32, zeros from D on
+// values [d, d + E) of a row, zeros from D on
+template <int E, class T>
+__device__ __forceinline__ Vec<T, E> raw(const T* row, uint32_t d, uint32_t D) {
+    if (d + E <= D) return *reinterpret_cast<const Vec<T, E>*>(row + d);
+    Vec<T, E> v;
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] = d + e < D ? row[d + e] : T(0.0f);
+    return v;
+}
 template <int E, class T>
 __device__ __forceinline__ F<E> load(const T* row, uint32_t d, uint32_t D) {
-    F<E> o;
-    if (d + E <= D) {
-        const Vec<T, E> v = *reinterpret_cast<const Vec<T, E>*>(row + d);
-        o = __builtin_convertvector(v, F<E>);
-    } else {
-#pragma unroll
-        for (int e = 0; e < E; ++e) o[e] = d + e < D ? float(row[d + e]) : 0.0f;
-    }
-    return o;
+    return __builtin_convertvector(raw<E>(row, d, D), F<E>);
 }
 template <int E, class T>
 __device__ __forceinline__ void store(T* row, uint32_t d, uint32_t D, F<E> v) {
@@ -115,7 +115,7 @@ struct RmsArgs {
     void* out;
     float* scales;  // 8-bit outputs without a given scale
     uint64_t ldx, ldr, ldro, ldo;
-    uint32_t T, D, group, groups;  // group 0: the row
+    uint32_t t0, T, D, group, groups;  // the launch's first row; group 0: the row
     float eps, given;              // given > 0: the scale
 };
 
@@ -157,7 +157,7 @@ __global__ __launch_bounds__(256) void rms_norm_kernel(RmsArgs a) {
     using T = ElemT<DT>;
     constexpr int NT = 64 * WPR, E = OUT == OUT_SAME ? 16 / int(sizeof(T)) : 8;
     __shared__ float part[4];
-    const uint32_t t = WPR == 1 ? blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
+    const uint32_t t = a.t0 + (WPR == 1 ? blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x);
     if (t >= a.T) return;  // (a whole wave, or the workgroup)
     const uint32_t tid = WPR == 1 ? threadIdx.x & 63 : threadIdx.x;
     const T* x = static_cast<const T*>(a.x) + t * a.ldx;
@@ -268,10 +268,10 @@ __global__ __launch_bounds__(256) void rms_norm_kernel(RmsArgs a) {
 // out = code scale, 8 values a thread
 template <int DT>
 __global__ __launch_bounds__(256) void rms_dequantize_kernel(const uint8_t* __restrict__ codes, const float* __restrict__ scales, uint64_t ldc,
-                                                             uint32_t T, uint32_t D, uint32_t group, uint32_t groups, float given, bool fp8,
+                                                             uint64_t i0, uint32_t T, uint32_t D, uint32_t group, uint32_t groups, float given, bool fp8,
                                                              ElemT<DT>* __restrict__ out, uint64_t ldo) {
     const uint32_t per = (D + 7) / 8;
-    const uint64_t i = uint64_t(blockIdx.x) * 256 + threadIdx.x;
+    const uint64_t i = i0 + uint64_t(blockIdx.x) * 256 + threadIdx.x;
     if (i >= uint64_t(T) * per) return;
     const uint32_t t = uint32_t(i / per), d = uint32_t(i % per) * 8;
     const float s = given > 0.0f ? given : scales[uint64_t(t) * groups + (group ? d / group : 0)];
@@ -312,85 +312,114 @@ struct RmsGradArgs {
     uint32_t T, D;
 };
 
-// A wave (or workgroup) takes rows in turn; dw's shares stay in registers (C > 0).
+// A wave (or workgroup) takes rows in turn; the next row's loads are in flight while a row is worked on, and dw's
+// shares stay in registers.  Rows of up to 64 E C WPR values.
 template <int DT, int WPR, int C>
 __global__ __launch_bounds__(256) void rms_grad_kernel(RmsGradArgs a) {
     using T = ElemT<DT>;
-    constexpr int NT = 64 * WPR, CC = C ? C : 1, E = 16 / int(sizeof(T));
+    constexpr int NT = 64 * WPR, E = 16 / int(sizeof(T));
     constexpr int ROWS = 4 / WPR;
+    using V = Vec<T, E>;
     __shared__ float part[4];
-    __shared__ F<E> join[WPR == 1 && C > 0 ? 256 : 1];
+    __shared__ F<E> join[WPR == 1 ? 256 : 1];
     const uint32_t tid = WPR == 1 ? threadIdx.x & 63 : threadIdx.x;
-    const uint32_t D = a.D, chunks = C ? C : (D + E * NT - 1) / (E * NT);
+    const uint32_t D = a.D, step = gridDim.x * ROWS;
     const T* w = static_cast<const T*>(a.weight);
-    F<E> dw[CC], wv[CC];
+    F<E> dw[C], wv[C];
 #pragma unroll
-    for (int c = 0; c < CC; ++c) {
+    for (int c = 0; c < C; ++c) {
         dw[c] = F<E>(0.0f);
-        if constexpr (C > 0) wv[c] = load<E>(w, (c * NT + tid) * E, D);
+        wv[c] = load<E>(w, (c * NT + tid) * E, D);
     }
-    for (uint32_t t = blockIdx.x * ROWS + (WPR == 1 ? threadIdx.x >> 6 : 0); t < a.T; t += gridDim.x * ROWS) {
+    struct Row {
+        V g[C], r[C], gr[C];
+        float inv;
+    } next;
+    auto fetch = [&](uint32_t t) {
         const T* g = static_cast<const T*>(a.grad) + t * a.ldg;
         const T* r = static_cast<const T*>(a.r) + t * a.ldr;
-        const T* gr = a.grad_residual ? static_cast<const T*>(a.grad_residual) + t * a.ldgr : nullptr;
-        const float inv = a.inverse[t];
-        float along = 0.0f;
-        F<E> gv[CC], nv[CC];
-        auto chunk = [&](uint32_t d, F<E> wc, F<E>& gg, F<E>& nn) {
-            gg = load<E>(g, d, D);
-            nn = load<E>(r, d, D) * inv;
-#pragma unroll
-            for (int e = 0; e < E; ++e) along = fmaf(gg[e] * wc[e], nn[e], along);
-        };
-        if constexpr (C > 0) {
-#pragma unroll
-            for (int c = 0; c < C; ++c) {
-                chunk((c * NT + tid) * E, wv[c], gv[c], nv[c]);
-                dw[c] += gv[c] * nv[c];
-            }
-        } else {
-            for (uint32_t c = 0; c < chunks; ++c) {
-                const uint32_t d = (c * NT + tid) * E;
-                F<E> gg, nn;
-                chunk(d, load<E>(w, d, D), gg, nn);
-            }
-        }
-        along = row_sum<WPR>(along, part) / float(D);
-        if (!a.out) continue;
-        T* o = static_cast<T*>(a.out) + t * a.ldo;
-        auto finish = [&](uint32_t d, F<E> wc, F<E> gg, F<E> nn) {
-            F<E> v = (gg * wc - nn * along) * inv;
-            if (gr) v += load<E>(gr, d, D);
-            store<E>(o, d, D, v);
-        };
-        if constexpr (C > 0) {
-#pragma unroll
-            for (int c = 0; c < C; ++c) finish((c * NT + tid) * E, wv[c], gv[c], nv[c]);
-        } else {
-            for (uint32_t c = 0; c < chunks; ++c) {
-                const uint32_t d = (c * NT + tid) * E;
-                F<E> gg = load<E>(g, d, D), nn = load<E>(r, d, D) * inv;
-                finish(d, load<E>(w, d, D), gg, nn);
-            }
-        }
-    }
-    if constexpr (C > 0) {
-        if (!a.part) return;
-        float* o = a.part + uint64_t(blockIdx.x) * D;
+        const T* gr = static_cast<const T*>(a.grad_residual) + t * a.ldgr;
 #pragma unroll
         for (int c = 0; c < C; ++c) {
             const uint32_t d = (c * NT + tid) * E;
-            F<E> v = dw[c];
-            if constexpr (WPR == 1) {
-                __syncthreads();
-                join[threadIdx.x] = v;
-                __syncthreads();
-                if (threadIdx.x >= 64) continue;
-                v = (join[tid] + join[tid + 64]) + (join[tid + 128] + join[tid + 192]);
-            }
+            next.g[c] = raw<E>(g, d, D);
+            next.r[c] = raw<E>(r, d, D);
+            if (a.grad_residual) next.gr[c] = raw<E>(gr, d, D);
+        }
+        next.inv = a.inverse[t];
+    };
+    uint32_t t = blockIdx.x * ROWS + (WPR == 1 ? threadIdx.x >> 6 : 0);
+    if (t < a.T) fetch(t);
+    while (t < a.T) {
+        const Row now = next;
+        const uint32_t row = t;
+        t += step;
+        if (t < a.T) fetch(t);
+        float along = 0.0f;
+        F<E> gv[C], nv[C];
 #pragma unroll
-            for (int e = 0; e < E; ++e)
-                if (d + e < D) o[d + e] = v[e];
+        for (int c = 0; c < C; ++c) {
+            gv[c] = __builtin_convertvector(now.g[c], F<E>);
+            nv[c] = __builtin_convertvector(now.r[c], F<E>) * now.inv;
+#pragma unroll
+            for (int e = 0; e < E; ++e) along = fmaf(gv[c][e] * wv[c][e], nv[c][e], along);
+            dw[c] += gv[c] * nv[c];
+        }
+        along = row_sum<WPR>(along, part) / float(D);
+        if (!a.out) continue;
+        T* o = static_cast<T*>(a.out) + row * a.ldo;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            F<E> v = (gv[c] * wv[c] - nv[c] * along) * now.inv;
+            if (a.grad_residual) v += __builtin_convertvector(now.gr[c], F<E>);
+            store<E>(o, (c * NT + tid) * E, D, v);
+        }
+    }
+    if (!a.part) return;
+    float* o = a.part + uint64_t(blockIdx.x) * D;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        const uint32_t d = (c * NT + tid) * E;
+        F<E> v = dw[c];
+        if constexpr (WPR == 1) {
+            __syncthreads();
+            join[threadIdx.x] = v;
+            __syncthreads();
+            if (threadIdx.x >= 64) continue;
+            v = (join[tid] + join[tid + 64]) + (join[tid + 128] + join[tid + 192]);
+        }
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+            if (d + e < D) o[d + e] = v[e];
+    }
+}
+
+// dx of longer rows: a workgroup takes rows in turn and reads each twice, the second time from cache
+template <int DT>
+__global__ __launch_bounds__(256) void rms_long_grad_kernel(RmsGradArgs a) {
+    using T = ElemT<DT>;
+    constexpr int E = 16 / int(sizeof(T));
+    __shared__ float part[4];
+    const uint32_t D = a.D;
+    const T* w = static_cast<const T*>(a.weight);
+    for (uint32_t t = blockIdx.x; t < a.T; t += gridDim.x) {
+        const T* g = static_cast<const T*>(a.grad) + t * a.ldg;
+        const T* r = static_cast<const T*>(a.r) + t * a.ldr;
+        const T* gr = a.grad_residual ? static_cast<const T*>(a.grad_residual) + t * a.ldgr : nullptr;
+        T* o = static_cast<T*>(a.out) + t * a.ldo;
+        const float inv = a.inverse[t];
+        float along = 0.0f;
+        for (uint32_t d = threadIdx.x * E; d < D; d += 256 * E) {
+            const F<E> gg = load<E>(g, d, D), nn = load<E>(r, d, D) * inv, wc = load<E>(w, d, D);
+#pragma unroll
+            for (int e = 0; e < E; ++e) along = fmaf(gg[e] * wc[e], nn[e], along);
+        }
+        along = row_sum<4>(along, part) / float(D);
+        for (uint32_t d = threadIdx.x * E; d < D; d += 256 * E) {
+            const F<E> gg = load<E>(g, d, D), nn = load<E>(r, d, D) * inv;
+            F<E> v = (gg * load<E>(w, d, D) - nn * along) * inv;
+            if (gr) v += load<E>(gr, d, D);
+            store<E>(o, d, D, v);
         }
     }
 }
@@ -444,7 +473,9 @@ va_status by_shape(uint32_t D, Fn&& f) {
     const uint32_t c = ceil_div(D, 256 * E);
     if (c <= 2) return f(group, integral_constant<int, 2>());
     if (c <= 4) return f(group, integral_constant<int, 4>());
-    if (E == 4 && c <= 8) return f(group, integral_constant<int, 8>());
+    if constexpr (E == 4) {
+        if (c <= 8) return f(group, integral_constant<int, 8>());
+    }
     return f(group, integral_constant<int, 0>());
 }
 template <class Fn>
@@ -466,20 +497,25 @@ va_status check(va_context* ctx, const va_rms_desc* d, const char* who) {
     VA_REQUIRE(ctx, aligned(d->x, d->dtype) && aligned(d->residual, d->dtype) && aligned(d->weight, d->dtype) && aligned(d->out_residual, d->dtype),
                "%s: an operand is not aligned to its type", who);
     VA_REQUIRE(ctx, std::isfinite(d->epsilon) && d->epsilon >= 0.0f, "%s: epsilon must be finite and not negative", who);
-    VA_REQUIRE(ctx, d->dim <= 0x7FFFFFFFu - 16384u, "%s: %u dimensions", who, d->dim);
+    VA_REQUIRE(ctx, d->rows <= 0x7FFFFFFFu && d->dim <= 0x7FFFFFFFu - 16384u, "%s: too many rows or dimensions (%u, %u)", who, d->rows, d->dim);
     return VA_OK;
 }
 
 template <int OUT>
 va_status forward(va_context* ctx, const va_rms_desc* d, void* out, uint64_t ldo, uint32_t group, float given, float* scales) {
     RmsArgs a{d->x, d->residual, d->weight, d->out_residual, d->out_inverse_rms, out, scales, d->x_stride, d->residual_stride,
-              d->out_residual_stride, ldo, d->rows, d->dim, group, group ? ceil_div(d->dim, group) : 1u, d->epsilon, given};
+              d->out_residual_stride, ldo, 0, d->rows, d->dim, group, group ? ceil_div(d->dim, group) : 1u, d->epsilon, given};
     return by_dtype(d->dtype, [&](auto dt) {
         constexpr int E = OUT == OUT_SAME ? 16 / int(sizeof(ElemT<decltype(dt)::value>)) : 8;
         return by_shape<E>(d->dim, [&](auto wpr, auto c) {
-            const uint32_t grid = decltype(wpr)::value == 1 ? ceil_div(a.T, 4) : a.T;
-            rms_norm_kernel<decltype(dt)::value, OUT, decltype(wpr)::value, decltype(c)::value><<<dim3(grid), dim3(256), 0, ctx->stream>>>(a);
-            VA_CHECK_LAUNCH(ctx);
+            constexpr uint32_t rows = decltype(wpr)::value == 1 ? 4 : 1;  // a workgroup's
+            for (a.t0 = 0; a.t0 < a.T;) {
+                const uint32_t grid = std::min(ceil_div(a.T - a.t0, rows), kGridMax);
+                rms_norm_kernel<decltype(dt)::value, OUT, decltype(wpr)::value, decltype(c)::value><<<dim3(grid), dim3(256), 0, ctx->stream>>>(a);
+                VA_CHECK_LAUNCH(ctx);
+                if (a.T - a.t0 <= grid * rows) break;
+                a.t0 += grid * rows;
+            }
             return VA_OK;
         });
     });
@@ -529,13 +565,14 @@ va_status va_rms_dequantize(va_context* ctx, const void* codes, uint64_t codes_s
     VA_REQUIRE(ctx, known(dtype) && aligned(out, dtype), "va_rms_dequantize: unknown type or misaligned output");
     VA_REQUIRE(ctx, codes_stride >= dim && out_stride >= dim, "va_rms_dequantize: a row stride is below the dimension");
     const uint64_t blocks = (uint64_t(rows) * ((uint64_t(dim) + 7) / 8) + 255) / 256;
-    VA_REQUIRE(ctx, blocks <= 0x7FFFFFFFull, "va_rms_dequantize: too many values");
     DeviceGuard guard(ctx->device);
     return by_dtype(dtype, [&](auto dt) {
-        rms_dequantize_kernel<decltype(dt)::value><<<dim3(uint32_t(blocks)), dim3(256), 0, ctx->stream>>>(
-            static_cast<const uint8_t*>(codes), scales, codes_stride, rows, dim, group, group ? ceil_div(dim, group) : 1u, given_scale,
-            code == VA_CODE_FP8_E4M3, static_cast<ElemT<decltype(dt)::value>*>(out), out_stride);
-        VA_CHECK_LAUNCH(ctx);
+        for (uint64_t b = 0; b < blocks; b += kGridMax) {
+            rms_dequantize_kernel<decltype(dt)::value><<<dim3(uint32_t(std::min<uint64_t>(blocks - b, kGridMax))), dim3(256), 0, ctx->stream>>>(
+                static_cast<const uint8_t*>(codes), scales, codes_stride, b * 256, rows, dim, group, group ? ceil_div(dim, group) : 1u, given_scale,
+                code == VA_CODE_FP8_E4M3, static_cast<ElemT<decltype(dt)::value>*>(out), out_stride);
+            VA_CHECK_LAUNCH(ctx);
+        }
         return VA_OK;
     });
 }
@@ -558,16 +595,20 @@ va_status va_rms_norm_backward(va_context* ctx, const va_rms_desc* d, const void
         constexpr int DT = decltype(dt)::value;
         return by_shape<16 / int(sizeof(ElemT<DT>))>(d->dim, [&](auto wpr, auto c) {
             constexpr int WPR = decltype(wpr)::value, C = decltype(c)::value;
-            // two workgroups a CU; fewer where their shares of dw would be more than the rows
-            const uint32_t grid = std::min(ceil_div(a.T, 4 / WPR), 2u * uint32_t(ctx->num_cus));
+            // Workgroups a CU: 2-byte rows need more of them for as many bytes in flight.  37,289 x 768 bf16, forward and
+            // backward: two 118 us, four 96; 30,000 x 512 fp32: 88 and 92.
+            const uint32_t grid = std::min(ceil_div(a.T, 4 / WPR), (DT == VA_DTYPE_F32 ? 2u : 4u) * uint32_t(ctx->num_cus));
             const uint32_t shares = C ? grid : std::min(a.T, 256u);
             Scratch sc(ctx);
             if (out_grad_weight) {
                 VA_CHECK_STATUS(sc.reserve(Scratch::round(uint64_t(shares) * a.D * 4)));
                 a.part = sc.carve<float>(uint64_t(shares) * a.D);
             }
-            if (C || a.out) {
+            if constexpr (C > 0) {
                 rms_grad_kernel<DT, WPR, C><<<dim3(grid), dim3(256), 0, ctx->stream>>>(a);
+                VA_CHECK_LAUNCH(ctx);
+            } else if (a.out) {
+                rms_long_grad_kernel<DT><<<dim3(grid), dim3(256), 0, ctx->stream>>>(a);
                 VA_CHECK_LAUNCH(ctx);
             }
             if (out_grad_weight) {

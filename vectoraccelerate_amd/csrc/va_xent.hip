@@ -330,8 +330,12 @@ va_status make_copy(va_context* ctx, int kind, const void* src, uint64_t ld, uin
                     float* inv, const uint32_t* run_if) {
     const uint32_t bytes = copy_bytes(kind, D);
     if (kind == g16::PLANES) {
-        planes_kernel<<<dim3(ceil_div(R, 4)), dim3(256), 0, ctx->stream>>>(static_cast<const float*>(src), ld, R, D, bytes / 4, absmax, drop,
-                                                                           static_cast<uint16_t*>(dst), inv);
+        for (uint32_t r = 0; r < R; r += 4 * kGridMax) {
+            const uint32_t n = std::min(R - r, 4 * kGridMax);
+            const Drop rest{drop.value ? drop.value + r : nullptr, drop.is};
+            planes_kernel<<<dim3(ceil_div(n, 4)), dim3(256), 0, ctx->stream>>>(static_cast<const float*>(src) + r * ld, ld, n, D, bytes / 4, absmax, rest,
+                                                                               static_cast<uint16_t*>(dst) + uint64_t(r) * (bytes / 2), inv + r);
+        }
     } else {
         const uint64_t n = uint64_t(R) * (bytes / 16);
         const dim3 grid(uint32_t(std::min<uint64_t>((n + 255) / 256, 16384)));
@@ -362,7 +366,7 @@ va_status check_desc(va_context* ctx, const va_xent_desc* d, const char* who) {
                d->num_items, d->dim);
     VA_REQUIRE(ctx, d->dtype == VA_DTYPE_F32 || d->dtype == VA_DTYPE_F16 || d->dtype == VA_DTYPE_BF16, "%s: unknown type %d", who, int(d->dtype));
     VA_REQUIRE(ctx, d->dim <= VA_XENT_MAX_DIM, "%s: %u dimensions (at most %u)", who, d->dim, VA_XENT_MAX_DIM);
-    VA_REQUIRE(ctx, d->num_items < 0xFFFFFF00u && d->rows < 0xFFFFFF00u, "%s: too many rows or items", who);
+    VA_REQUIRE(ctx, d->num_items <= 0x7FFFFFFFu && d->rows <= 0x7FFFFFFFu, "%s: too many rows or items", who);
     VA_REQUIRE(ctx, d->hidden_stride >= d->dim && d->items_stride >= d->dim, "%s: a row stride is below the dimension", who);
     VA_REQUIRE(ctx, std::isfinite(d->scale), "%s: the scale is not finite", who);
     const size_t es = elem_size(d->dtype);
@@ -457,7 +461,7 @@ va_status va_xent_forward(va_context* ctx, const va_xent_desc* d, float* out_los
     if (T <= kFinishRows) {
         xent_finish_kernel<<<dim3(1), dim3(1024), 0, ctx->stream>>>(d->targets, T, V, d->ignore_index, part, picked, slots, out_loss, out_lse, mean, out_reduced);
     } else {
-        xent_finish_kernel<<<dim3(ceil_div(T, 4)), dim3(256), 0, ctx->stream>>>(d->targets, T, V, d->ignore_index, part, picked, slots, out_loss, out_lse, mean, nullptr);
+        xent_finish_kernel<<<dim3(std::min(ceil_div(T, 4), kGridMax)), dim3(256), 0, ctx->stream>>>(d->targets, T, V, d->ignore_index, part, picked, slots, out_loss, out_lse, mean, nullptr);
         VA_CHECK_LAUNCH(ctx);
         if (out_reduced) xent_reduce_kernel<<<dim3(1), dim3(1024), 0, ctx->stream>>>(out_loss, d->targets, T, d->ignore_index, mean, out_reduced);
     }

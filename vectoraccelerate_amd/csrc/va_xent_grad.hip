@@ -373,19 +373,24 @@ __global__ __launch_bounds__(256) void share_sum_kernel(const float* __restrict_
                                                         const uint32_t* __restrict__ absmax, ElemT<dtype_of(KIND)>* __restrict__ out, uint64_t ld) {
     __shared__ f32x4 part[4][64];
     const uint32_t per = Dp / 4, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const uint64_t i = uint64_t(blockIdx.x) * 64 + lane, n = uint64_t(T) * per;
-    f32x4 v{0.0f, 0.0f, 0.0f, 0.0f};
-    if (i < n)
+    const uint64_t n = uint64_t(T) * per;
+    for (uint64_t i0 = uint64_t(blockIdx.x) * 64; i0 < n; i0 += uint64_t(gridDim.x) * 64) {
+        const uint64_t i = i0 + lane;
+        f32x4 v{0.0f, 0.0f, 0.0f, 0.0f};
+        if (i < n)
 #pragma unroll 8
-        for (uint32_t s = w; s < parts; s += 4) v += *reinterpret_cast<const f32x4*>(share + (uint64_t(s) * n + i) * 4);
-    part[w][lane] = v;
-    __syncthreads();
-    if (w || i >= n) return;
-    v = (v + part[1][lane]) + (part[2][lane] + part[3][lane]);
-    const uint32_t t = uint32_t(i / per), d = uint32_t(i % per) * 4;
-    const float m = *mul / (KIND == g16::PLANES ? scale_to_2p14(__builtin_bit_cast(float, *absmax)) : 1.0f);
-    const bool none = gk && gk[t] == 0.0f;
-    for (int e = 0; e < 4 && d + e < D; ++e) out[t * ld + d + e] = Elem<dtype_of(KIND)>::from_f(none ? 0.0f : v[e] * m);
+            for (uint32_t s = w; s < parts; s += 4) v += *reinterpret_cast<const f32x4*>(share + (uint64_t(s) * n + i) * 4);
+        part[w][lane] = v;
+        __syncthreads();
+        if (!w && i < n) {
+            v = (v + part[1][lane]) + (part[2][lane] + part[3][lane]);
+            const uint32_t t = uint32_t(i / per), d = uint32_t(i % per) * 4;
+            const float m = *mul / (KIND == g16::PLANES ? scale_to_2p14(__builtin_bit_cast(float, *absmax)) : 1.0f);
+            const bool none = gk && gk[t] == 0.0f;
+            for (int e = 0; e < 4 && d + e < D; ++e) out[t * ld + d + e] = Elem<dtype_of(KIND)>::from_f(none ? 0.0f : v[e] * m);
+        }
+        __syncthreads();  // the quarters are read
+    }
 }
 
 constexpr size_t kGradBudget = size_t(512) << 20;  // dl of one piece
@@ -499,7 +504,7 @@ va_status va_xent_backward(va_context* ctx, const va_xent_desc* d, const float* 
     auto sum_shares = [&](const float* from, uint32_t parts, uint32_t rows, const float* zero, const uint32_t* top, uintptr_t o, uint64_t ld) {
         return by_kind(kind, [&](auto k) {
             constexpr int kKind = decltype(k)::value;
-            share_sum_kernel<kKind><<<dim3(ceil_div(uint64_t(rows) * (Dp / 4), 64)), dim3(256), 0, ctx->stream>>>(
+            share_sum_kernel<kKind><<<dim3(uint32_t(std::min<uint64_t>((uint64_t(rows) * (Dp / 4) + 63) / 64, kGridMax))), dim3(256), 0, ctx->stream>>>(
                 from, parts, rows, D, Dp, zero, mul, top, reinterpret_cast<ElemT<dtype_of(kKind)>*>(o), ld);
             VA_CHECK_LAUNCH(ctx);
             return VA_OK;
