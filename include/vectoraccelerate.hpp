@@ -16,6 +16,8 @@
  *   MetalComputeProvider       Integration/MetalComputeProvider.swift (batchDistance, findNearest)
  *   KMeansPipeline             Index/Kernels/Clustering/KMeansPipeline.swift
  *   ProductQuantizationKernel  Kernels/Metal4/ProductQuantizationKernel.swift
+ * Without a counterpart there: SoftmaxCrossEntropyKernel, RMSNormKernel, GradientClipKernel (training
+ * and serving of the embeddings a collection holds).
  * Every call checks the status and throws VectorError with the library's message.
  */
 #ifndef VECTORACCELERATE_HPP
@@ -515,6 +517,70 @@ class ProductQuantizationKernel {
    private:
     const Context& ctx_;
     Config cfg_;
+};
+
+// Softmax cross entropy of rows [T x D] over all items of a collection, and its gradients; the
+// description's pointers are device memory (va_xent_desc).
+class SoftmaxCrossEntropyKernel {
+   public:
+    explicit SoftmaxCrossEntropyKernel(const Context& c) : ctx_(c) {}
+    struct Result {
+        DeviceBuffer<float> loss, logSumExp, reduced;
+    };
+    Result forward(const va_xent_desc& d, va_reduction reduction = VA_REDUCE_MEAN) const {
+        Result r{DeviceBuffer<float>(ctx_, d.rows), DeviceBuffer<float>(ctx_, d.rows), DeviceBuffer<float>(ctx_, 1)};
+        ctx_.check(va_xent_forward(ctx_.handle(), &d, r.loss.data(), r.logSumExp.data(), reduction,
+                                   reduction == VA_REDUCE_NONE ? nullptr : r.reduced.data()),
+                   "va_xent_forward");
+        return r;
+    }
+    // contiguous gradients of the hidden rows and of the items (either may be nullptr)
+    void backward(const va_xent_desc& d, const DeviceBuffer<float>& logSumExp, void* gradHidden, void* gradItems,
+                  va_reduction reduction = VA_REDUCE_MEAN, const float* grad = nullptr) const {
+        ctx_.check(va_xent_backward(ctx_.handle(), &d, logSumExp.data(), reduction, grad, gradHidden, d.dim, gradItems, d.dim),
+                   "va_xent_backward");
+    }
+
+   private:
+    const Context& ctx_;
+};
+
+// y = r / sqrt(mean r^2 + epsilon) * weight, r = x + residual, in the rows' type or in 8 bits.
+class RMSNormKernel {
+   public:
+    explicit RMSNormKernel(const Context& c) : ctx_(c) {}
+    void encode(const va_rms_desc& d, void* out) const { ctx_.check(va_rms_norm(ctx_.handle(), &d, out, d.dim), "va_rms_norm"); }
+    // givenScale > 0: codes on one grid and no scales
+    void quantize(const va_rms_desc& d, va_code code, void* outCodes, float* outScales, uint32_t group = 0, float givenScale = 0.0f) const {
+        ctx_.check(va_rms_norm_quantized(ctx_.handle(), &d, code, group, givenScale, outCodes, d.dim, outScales),
+                   "va_rms_norm_quantized");
+    }
+    void dequantize(const void* codes, va_code code, const float* scales, uint32_t rows, uint32_t dim, va_dtype dtype, void* out,
+                    uint32_t group = 0, float givenScale = 0.0f) const {
+        ctx_.check(va_rms_dequantize(ctx_.handle(), codes, dim, code, scales, givenScale, rows, dim, group, dtype, out, dim),
+                   "va_rms_dequantize");
+    }
+    // d.x: the summed rows; contiguous outputs, either may be nullptr
+    void backward(const va_rms_desc& d, const void* grad, const float* inverseRms, void* gradX, void* gradWeight,
+                  const void* gradResidual = nullptr) const {
+        ctx_.check(va_rms_norm_backward(ctx_.handle(), &d, grad, d.dim, gradResidual, d.dim, inverseRms, gradX, d.dim, gradWeight),
+                   "va_rms_norm_backward");
+    }
+
+   private:
+    const Context& ctx_;
+};
+
+// The global norm of a list of gradients, and the gradients clipped by it.
+class GradientClipKernel {
+   public:
+    explicit GradientClipKernel(const Context& c) : ctx_(c) {}
+    void encode(const va_tensor_list& list, float maxNorm, float* outNorm = nullptr, float epsilon = 1e-6f) const {
+        ctx_.check(va_grad_clip(ctx_.handle(), &list, maxNorm, epsilon, outNorm), "va_grad_clip");
+    }
+
+   private:
+    const Context& ctx_;
 };
 
 }  // namespace vectoraccelerate

@@ -124,6 +124,42 @@ int main(int argc, char** argv) {
         save(dir + "/ivx_ids.bin", lists.second);
         std::ofstream(dir + "/ivx_state.txt") << ivx.isTrained() << " " << ivx.info().ivf_routed << " " << ivx.count();
 
+        // the loss of the queries over the collection (target of query i: row i), its gradients clipped
+        // together, the norm of the queries in fp32 and in 8 bits
+        {
+            std::vector<int64_t> targets(Q);
+            for (uint32_t i = 0; i < Q; ++i) targets[i] = i;
+            va::DeviceBuffer<float> dq(ctx, load<float>(dir + "/q.bin", size_t(Q) * D)), dx(ctx, load<float>(dir + "/x.bin", size_t(N) * D));
+            va::DeviceBuffer<int64_t> dt(ctx, targets);
+            const va_xent_desc d{dq.data(), dx.data(), dt.data(), nullptr, D, D, -100, Q, N, D, VA_DTYPE_F32, 0.25f};
+            va::SoftmaxCrossEntropyKernel entropy(ctx);
+            auto r = entropy.forward(d);
+            va::DeviceBuffer<float> gq(ctx, size_t(Q) * D), gx(ctx, size_t(N) * D), norm(ctx, 1);
+            entropy.backward(d, r.logSumExp, gq.data(), gx.data());
+            save(dir + "/xent_loss.bin", r.loss.download());
+            save(dir + "/xent_mean.bin", r.reduced.download());
+            void* const tensors[2] = {gq.data(), gx.data()};
+            const uint64_t sizes[2] = {gq.size(), gx.size()};
+            const int32_t types[2] = {VA_DTYPE_F32, VA_DTYPE_F32};
+            va::GradientClipKernel(ctx).encode(va_tensor_list{tensors, nullptr, sizes, types, 2}, 0.01f, norm.data());
+            save(dir + "/clip_norm.bin", norm.download());
+            save(dir + "/clip_gq.bin", gq.download());
+            save(dir + "/clip_gx.bin", gx.download());
+            va::RMSNormKernel rms(ctx);
+            va::DeviceBuffer<float> weight(ctx, std::vector<float>(D, 0.5f)), inverse(ctx, Q), y(ctx, size_t(Q) * D), back(ctx, size_t(Q) * D),
+                scales(ctx, Q), gr(ctx, size_t(Q) * D);
+            va::DeviceBuffer<int8_t> codes(ctx, size_t(Q) * D);
+            va_rms_desc n{dq.data(), nullptr, weight.data(), nullptr, inverse.data(), D, D, D, Q, D, VA_DTYPE_F32, 1e-6f};
+            rms.encode(n, y.data());
+            rms.quantize(n, VA_CODE_INT8, codes.data(), scales.data());
+            rms.dequantize(codes.data(), VA_CODE_INT8, scales.data(), Q, D, VA_DTYPE_F32, back.data());
+            n.out_inverse_rms = nullptr;
+            rms.backward(n, y.data(), inverse.data(), gr.data(), nullptr);
+            save(dir + "/rms_y.bin", y.download());
+            save(dir + "/rms_back.bin", back.download());
+            save(dir + "/rms_gr.bin", gr.download());
+        }
+
         std::string kind = "none";
         try {
             topk.findNearestNeighbors(q, x, 0);

@@ -149,9 +149,9 @@ class SoftmaxCrossEntropyKernel:
     def forward(self, hidden, items, targets, reduction: str = "mean", scale: float = 1.0, offsets=None,
                 ignoreIndex: int = -100) -> SoftmaxCrossEntropyResult:
         c, torch = self.context, _torch()
-        T = hidden.shape[0]
+        T, mode = hidden.shape[0], _reduction(reduction)
         loss, lse = c.empty((T,), torch.float32), c.empty((T,), torch.float32)
-        reduced = c.empty((1,), torch.float32) if _reduction(reduction) != _lib.VA_REDUCE_NONE else None
+        reduced = c.empty((1,), torch.float32) if mode != _lib.VA_REDUCE_NONE else None
         c.order_after_torch()
         self.encodeForward(hidden, items, targets, loss, lse, reduced, reduction, scale, offsets, ignoreIndex)
         c.synchronize()
