@@ -56,15 +56,17 @@ __global__ __launch_bounds__(256) void copy_kernel(const U* __restrict__ src, ui
 // One wave per fp32 row: its planes dst[r] = {hi, lo} (Kp values each, zeros past D), scaled by the
 // power of two that puts the row's largest entry, or the tensor's (absmax), near 2^14; inv[r] = the
 // inverse.  Dropped rows are zeros.
-__global__ __launch_bounds__(256) void planes_kernel(const float* __restrict__ src, uint64_t ld, uint32_t R, uint32_t D, uint32_t Kp,
-                                                     const uint32_t* __restrict__ absmax, Drop drop,
-                                                     uint16_t* __restrict__ dst, float* __restrict__ inv) {
+// Rows of `a` in the first na workgroups, then of `b`.
+__global__ __launch_bounds__(256) void planes_kernel(Planes a, Planes b, uint32_t na, uint32_t D, uint32_t Kp) {
     typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
     const int lane = threadIdx.x & 63;
-    const uint32_t r = blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (r >= R) return;
-    const float* s = src + r * ld;
-    const bool none = drop.value && drop.value[r] == drop.is;
+    const bool second = blockIdx.x >= na;
+    const uint32_t r = (second ? blockIdx.x - na : blockIdx.x) * 4 + (threadIdx.x >> 6);
+    if (r >= (second ? b.R : a.R)) return;
+    const float* s = static_cast<const float*>(second ? b.src : a.src) + r * (second ? b.ld : a.ld);
+    const float* drop = second ? b.drop.value : a.drop.value;
+    const bool none = drop && drop[r] == (second ? b.drop.is : a.drop.is);
+    const uint32_t* absmax = second ? b.absmax : a.absmax;
     auto load4 = [&](uint32_t k) {
         f32x4 v{0.0f, 0.0f, 0.0f, 0.0f};
         if (none) return v;
@@ -93,8 +95,8 @@ __global__ __launch_bounds__(256) void planes_kernel(const float* __restrict__ s
         }
         sc = scale_to_2p14(wave_max(m));
     }
-    if (lane == 0) inv[r] = 1.0f / sc;
-    uint16_t* o = dst + uint64_t(r) * 2 * Kp;
+    if (lane == 0) (second ? b.inv : a.inv)[r] = 1.0f / sc;
+    uint16_t* o = static_cast<uint16_t*>(second ? b.dst : a.dst) + uint64_t(r) * 2 * Kp;
     auto put = [&](uint32_t k, f32x4 v) {
         uint16_t h[4], l[4];
 #pragma unroll
@@ -326,25 +328,34 @@ namespace xent {
 // Up to so many rows one workgroup finishes and reduces them (one launch instead of two).
 constexpr uint32_t kFinishRows = 64;
 
-va_status make_copy(va_context* ctx, int kind, const void* src, uint64_t ld, uint32_t R, uint32_t D, const uint32_t* absmax, Drop drop, void* dst,
-                    float* inv, const uint32_t* run_if) {
+va_status make_copy(va_context* ctx, int kind, const void* src, uint64_t ld, uint32_t R, uint32_t D, Drop drop, void* dst, const uint32_t* run_if) {
     const uint32_t bytes = copy_bytes(kind, D);
-    if (kind == g16::PLANES) {
-        for (uint32_t r = 0; r < R; r += 4 * kGridMax) {
-            const uint32_t n = std::min(R - r, 4 * kGridMax);
-            const Drop rest{drop.value ? drop.value + r : nullptr, drop.is};
-            planes_kernel<<<dim3(ceil_div(n, 4)), dim3(256), 0, ctx->stream>>>(static_cast<const float*>(src) + r * ld, ld, n, D, bytes / 4, absmax, rest,
-                                                                               static_cast<uint16_t*>(dst) + uint64_t(r) * (bytes / 2), inv + r);
-        }
-    } else {
-        const uint64_t n = uint64_t(R) * (bytes / 16);
-        const dim3 grid(uint32_t(std::min<uint64_t>((n + 255) / 256, 16384)));
-        if (kind == g16::F32)
-            copy_kernel<uint32_t><<<grid, dim3(256), 0, ctx->stream>>>(static_cast<const uint32_t*>(src), ld, D, bytes / 4, drop, run_if, static_cast<uint32_t*>(dst), n);
-        else
-            copy_kernel<uint16_t><<<grid, dim3(256), 0, ctx->stream>>>(static_cast<const uint16_t*>(src), ld, D, bytes / 2, drop, run_if, static_cast<uint16_t*>(dst), n);
-    }
+    const uint64_t n = uint64_t(R) * (bytes / 16);
+    const dim3 grid(uint32_t(std::min<uint64_t>((n + 255) / 256, 16384)));
+    if (kind == g16::F32)
+        copy_kernel<uint32_t><<<grid, dim3(256), 0, ctx->stream>>>(static_cast<const uint32_t*>(src), ld, D, bytes / 4, drop, run_if, static_cast<uint32_t*>(dst), n);
+    else
+        copy_kernel<uint16_t><<<grid, dim3(256), 0, ctx->stream>>>(static_cast<const uint16_t*>(src), ld, D, bytes / 2, drop, run_if, static_cast<uint16_t*>(dst), n);
     VA_CHECK_LAUNCH(ctx);
+    return VA_OK;
+}
+
+va_status make_planes(va_context* ctx, uint32_t D, Planes a, Planes b) {
+    const uint32_t bytes = copy_bytes(g16::PLANES, D);
+    auto rest = [&](Planes& p, uint32_t n) {  // what is left behind the first n rows
+        p.src = static_cast<const float*>(p.src) + n * p.ld;
+        p.dst = static_cast<char*>(p.dst) + uint64_t(n) * bytes;
+        p.inv += n;
+        if (p.drop.value) p.drop.value += n;
+        p.R -= n;
+    };
+    while (a.R || b.R) {
+        const uint32_t na = std::min(ceil_div(a.R, 4), kGridMax), nb = std::min(ceil_div(b.R, 4), kGridMax - na);
+        planes_kernel<<<dim3(na + nb), dim3(256), 0, ctx->stream>>>(a, b, na, D, bytes / 4);
+        VA_CHECK_LAUNCH(ctx);
+        rest(a, std::min(a.R, 4 * na));
+        rest(b, std::min(b.R, 4 * nb));
+    }
     return VA_OK;
 }
 
@@ -429,11 +440,16 @@ va_status va_xent_forward(va_context* ctx, const va_xent_desc* d, float* out_los
         VA_CHECK_STATUS(fill_u32(ctx, odd, 1, 0));
         VA_CHECK_STATUS(find_odd(ctx, d, odd));
     }
-    if (!qd) VA_CHECK_STATUS(make_copy(ctx, kind, d->hidden, d->hidden_stride, T, D, nullptr, Drop{}, qp, qinv));
+    const bool planes = kind == g16::PLANES;
+    if (!qd && !planes) VA_CHECK_STATUS(make_copy(ctx, kind, d->hidden, d->hidden_stride, T, D, Drop{}, qp));
     for (uint32_t c = 0; c < pieces; ++c) {
         const uint32_t v0 = c * piece, n = std::min(piece, V - v0);
         const char* items = row_at(d->items, d->items_stride, v0, dt);
-        if (!xd) VA_CHECK_STATUS(make_copy(ctx, kind, items, d->items_stride, n, D, nullptr, Drop{}, xp, xinv));
+        if (planes)
+            VA_CHECK_STATUS(make_planes(ctx, D, Planes{d->hidden, d->hidden_stride, c ? 0 : T, nullptr, Drop{}, qp, qinv},
+                                        Planes{items, d->items_stride, n, nullptr, Drop{}, xp, xinv}));
+        else if (!xd)
+            VA_CHECK_STATUS(make_copy(ctx, kind, items, d->items_stride, n, D, Drop{}, xp));
         g16::Args a;
         a.q = qd ? in_place(dt, d->hidden, d->hidden_stride, T, D) : copied(kind, qp, T, D);
         a.x = xd ? in_place(dt, items, d->items_stride, n, D) : copied(kind, xp, n, D);

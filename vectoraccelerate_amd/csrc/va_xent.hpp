@@ -180,10 +180,22 @@ struct Drop {
     const float* value = nullptr;
     float is = 0.0f;
 };
-// A copy of R rows as `kind` wants them.  PLANES: scaled by the power of two that puts the row's largest entry, or
-// the tensor's (absmax), near 2^14, and its inverse to inv[row].  Nothing where *run_if is zero (not PLANES).
-va_status make_copy(va_context* ctx, int kind, const void* src, uint64_t ld, uint32_t R, uint32_t D, const uint32_t* absmax, Drop drop, void* dst,
-                    float* inv, const uint32_t* run_if = nullptr);
+// A copy of R rows as `kind` (not PLANES) wants them; nothing where *run_if is zero.
+va_status make_copy(va_context* ctx, int kind, const void* src, uint64_t ld, uint32_t R, uint32_t D, Drop drop, void* dst,
+                    const uint32_t* run_if = nullptr);
+// The planes of R fp32 rows: scaled by the power of two that puts the row's largest entry, or the tensor's
+// (absmax), near 2^14, and its inverse to inv[row].
+struct Planes {
+    const void* src = nullptr;
+    uint64_t ld = 0;
+    uint32_t R = 0;
+    const uint32_t* absmax = nullptr;
+    Drop drop;
+    void* dst = nullptr;
+    float* inv = nullptr;
+};
+// Of one matrix, or of two in one launch (b.R = 0: none).
+va_status make_planes(va_context* ctx, uint32_t D, Planes a, Planes b = {});
 // *odd = 1 (0 before) if a masked item holds NaN or inf, or an offset is finite and near fp32's limits
 va_status find_odd(va_context* ctx, const va_xent_desc* d, uint32_t* odd);
 

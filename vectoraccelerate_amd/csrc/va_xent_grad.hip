@@ -87,14 +87,19 @@ __global__ __launch_bounds__(256) void xent_prepare_kernel(PrepareArgs a, uint32
     }
 }
 
-// out = the bits of the largest |src| (0 before the launch); dropped rows are left out
-__global__ __launch_bounds__(256) void absmax_kernel(const float* __restrict__ src, uint64_t ld, uint32_t R, uint32_t D,
-                                                     Drop drop, uint32_t* out) {
+// *absmax = the bits of the largest |src| (0 before the launch) of two matrices, `a` in the first na workgroups;
+// dropped rows are left out
+__global__ __launch_bounds__(256) void absmax_kernel(Planes a, Planes b, uint32_t na, uint32_t D, uint32_t* top) {
     typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
     __shared__ float part[4];
+    const bool second = blockIdx.x >= na;
+    const uint32_t R = second ? b.R : a.R, block = second ? blockIdx.x - na : blockIdx.x, blocks = second ? gridDim.x - na : na;
+    const float* src = static_cast<const float*>(second ? b.src : a.src);
+    const uint64_t ld = second ? b.ld : a.ld;
+    const Drop drop{second ? b.drop.value : a.drop.value, second ? b.drop.is : a.drop.is};
     float m = 0.0f;
     const int lane = threadIdx.x & 63;
-    for (uint32_t r = blockIdx.x * 4 + (threadIdx.x >> 6); r < R; r += gridDim.x * 4) {
+    for (uint32_t r = block * 4 + (threadIdx.x >> 6); r < R; r += blocks * 4) {
         if (drop.value && drop.value[r] == drop.is) continue;
         const float* s = src + r * ld;
         const uint32_t full = D / 4 * 4;
@@ -109,7 +114,7 @@ __global__ __launch_bounds__(256) void absmax_kernel(const float* __restrict__ s
     if (lane == 0) part[threadIdx.x >> 6] = m;
     __syncthreads();
     if (threadIdx.x == 0)
-        atomicMax(out, __builtin_bit_cast(uint32_t, fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]))));
+        atomicMax(top + second, __builtin_bit_cast(uint32_t, fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]))));
 }
 
 // dl of the piece's items, p[t][j]: Vp values a plane and row, zeros past the last item, rows `pitch` bytes
@@ -483,16 +488,17 @@ va_status va_xent_backward(va_context* ctx, const va_xent_desc* d, const float* 
             pa, rows_per, together ? static_cast<const uint16_t*>(d->hidden) : nullptr, d->hidden_stride, D, one / 2, reinterpret_cast<uint16_t*>(qp));
     VA_CHECK_LAUNCH(ctx);
     const Drop no_gradient{gk, 0.0f};
+    Planes hidden_planes{d->hidden, d->hidden_stride, T, absmax, no_gradient, qp, qinv};
+    auto item_planes = [&](const void* items, uint32_t n, const float* offsets) {
+        return Planes{items, d->items_stride, n, absmax + 1, Drop{offsets, -INFINITY}, xp, xinv};
+    };
     if (planes) {
         // one scale a tensor: both tensors are summed over in the second products
-        auto top = [&](const void* src, uint64_t ld, uint32_t R, Drop drop, uint32_t* out) {
-            absmax_kernel<<<dim3(std::min<uint32_t>(ceil_div(R, 16), 512)), dim3(256), 0, ctx->stream>>>(static_cast<const float*>(src), ld, R, D, drop, out);
-        };
-        top(d->hidden, d->hidden_stride, T, no_gradient, absmax);
-        top(d->items, d->items_stride, V, Drop{d->offsets, -INFINITY}, absmax + 1);
+        const uint32_t na = std::min(ceil_div(T, 16), 512u), nb = std::min(ceil_div(V, 16), 512u);
+        absmax_kernel<<<dim3(na + nb), dim3(256), 0, ctx->stream>>>(hidden_planes, item_planes(d->items, V, d->offsets), na, D, absmax);
         VA_CHECK_LAUNCH(ctx);
     }
-    if (!together) VA_CHECK_STATUS(make_copy(ctx, kind, d->hidden, d->hidden_stride, T, D, planes ? absmax : nullptr, no_gradient, qp, qinv));
+    if (!together && !planes) VA_CHECK_STATUS(make_copy(ctx, kind, d->hidden, d->hidden_stride, T, D, no_gradient, qp));
     if (checks) VA_CHECK_STATUS(find_odd(ctx, d, odd));
 
     auto rows_out = [&](auto sh, auto k, auto qk, const g16::Args& b, uintptr_t o, uint64_t ld, uint32_t rows, const uint32_t* top, const float* zero) {
@@ -514,8 +520,12 @@ va_status va_xent_backward(va_context* ctx, const va_xent_desc* d, const float* 
         const uint32_t v0 = c * piece, n = std::min(piece, V - v0), Vp = round_up(n, 64);
         const char* items = row_at(d->items, d->items_stride, v0, dt);
         const float* offsets = d->offsets ? d->offsets + v0 : nullptr;
-        if (copies)
-            VA_CHECK_STATUS(make_copy(ctx, kind, items, d->items_stride, n, D, planes ? absmax + 1 : nullptr, Drop{offsets, -INFINITY}, xp, xinv, checks ? odd : nullptr));
+        if (planes) {
+            VA_CHECK_STATUS(make_planes(ctx, D, hidden_planes, item_planes(items, n, offsets)));
+            hidden_planes.R = 0;  // (once)
+        } else if (copies) {
+            VA_CHECK_STATUS(make_copy(ctx, kind, items, d->items_stride, n, D, Drop{offsets, -INFINITY}, xp, checks ? odd : nullptr));
+        }
         const g16::Operand rows = copied(kind, qp, T, D);
         g16::Operand cols = xd ? in_place(dt, items, d->items_stride, n, D) : copied(kind, xp, n, D);
         if (checks) {
