@@ -364,3 +364,14 @@ def test_long_gradients_of_shares(ctx):
         want = oracle.xent(h[p], w, y[p], 1.0, None, IGNORE, torch.ones(h[p].shape[0], dtype=torch.float64))
         oracle.close(gh[p], *want["grad_hidden"], "grad_hidden")
     assert not bool(torch.isnan(gh).any())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("T,V,D", [(1, 1000, 768), (65, 129, 833), (64, 64, 1536), (30, 700, 2050), (130, 1900, 900), (5, 66, 5000)])
+def test_few_tiles_with_many_stages(ctx, T, V, D, dtype):
+    """Tiles whose stages are shared among waves, also when they do not divide evenly; with masks and both directions."""
+    h, w, y, g = _inputs(T, V, D, dtype, T + V + D)
+    off = torch.randn(V, generator=g)
+    off[torch.rand(V, generator=g) < 0.1] = -torch.inf
+    _check(ctx, h, w, y)
+    _check(ctx, h, w, y, scale=0.5, offsets=off.cuda())

@@ -8,14 +8,21 @@
 // A wave computes 64 queries x 64 rows (2 x 2 blocks of v_mfma_f32_32x32x16, 64 fp32 accumulators a
 // lane; NB = 1: 32 queries), a workgroup WQ x WR such waves: 4 x 4 for large products (256 x 256, four waves per
 // SIMD, one workgroup a CU), fewer where tiles of that size would leave CUs without work.  128 bytes of k (a stage)
-// of both operands move global -> LDS by direct loads into one of two slots while the
-// other is computed on (four slots where a launch does not fill the chip and waits for each stage); LDS rows are 128 bytes with their 16-byte chunks swizzled by the row, so
+// of both operands move global -> LDS by direct loads into one of two slots while the other is computed on (four
+// slots where a launch does not fill the chip and waits for each stage).  Where there are few tiles with many
+// stages, SLICES groups of waves take a share of a tile's stages each, with slots of their own, and the sums
+// join in the first one's registers.  LDS rows are 128 bytes with their 16-byte chunks swizzled by the row, so
 // fragment reads are conflict-free.  An operand stored across k is staged as it lies, the stage's k-rows of the
 // tile's width, and ds_read_tr16 turns it on the way into the fragments (a lane receives four k of one
 // column); its 64-byte segments are swizzled by k, so that four k-rows meet in no bank.  Rows need no
 // alignment but a dword's, and k may end anywhere: behind the end the row operand's values are cleared in its
 // fragments, and the query operand's are zeros in memory.  The launch is persistent: a workgroup walks its tiles, and the
 // next tile's first stage streams in during the epilogue.
+//
+// Bound by the matrix cores at the clock that the card's power leaves them: 8192^3 in bf16 runs at 1.3 PFLOP/s,
+// 4096 x 262,144 x 768 with the loss's epilogue at 1.03 (the vendor library's plain products of those shapes: 1.56 and 1.02).
+// Eight waves of 128 x 64 reach 1.30 and 1.05, four of 128 x 128 1.20 and 0.88, slots of half a stage 1.13
+// and 0.97: MFMA busy times clock is nearly the same for all.
 //
 // fp32 operands come in two ways.  As they are, on v_mfma_f32_32x32x2: a fragment's 16 bytes are four k-values
 // instead of eight, everything else is alike; a sixteenth of the 16-bit rate, which is enough while the
@@ -49,16 +56,19 @@ enum Kind : int { F16 = 0, BF16 = 1, PLANES = 2, F32 = 3 };
 constexpr int size_of(int kind) { return kind == F32 ? 4 : 2; }
 constexpr int stage_of(int kind) { return ROWB / size_of(kind); }  // k-values of a stage (of one plane)
 
-template <int WQ_, int WR_, int NB_ = 2, int SLOTS_ = 2>
+template <int WQ_, int WR_, int NB_ = 2, int SLOTS_ = 2, int SLICES_ = 1>
 struct Shape {
     static constexpr int SLOTS = SLOTS_;  // a power of two
-    static constexpr int WQ = WQ_, WR = WR_, NB = NB_, WAVES = WQ * WR, THREADS = 64 * WAVES;
+    static constexpr int WQ = WQ_, WR = WR_, NB = NB_, SLICES = SLICES_;
+    static constexpr int WPS = WQ * WR;  // waves of a slice
+    static constexpr int WAVES = WPS * SLICES, THREADS = 64 * WAVES;
     static constexpr int TQ = 32 * NB * WQ, TR = 64 * WR;
-    static constexpr int QB = TQ * ROWB, XB = TR * ROWB, STAGE = QB + XB, LDS = SLOTS * STAGE;
+    static constexpr int QB = TQ * ROWB, XB = TR * ROWB, STAGE = QB + XB, LDS = SLICES * SLOTS * STAGE;
     // waves per SIMD that the registers allow for: all of a CU's (16 waves), or two workgroups' and more
-    static constexpr int PER_SIMD = WAVES == 16 ? 4 : SLOTS == 2 ? 2 : 1;
+    static constexpr int PER_SIMD = WAVES == 16 ? 4 : LDS <= 80 * 1024 ? 2 : 1;
     static_assert(THREADS >= TQ && THREADS >= TR, "one thread per query and row");
-    static_assert(WAVES * 4096 <= STAGE, "the epilogue's LDS fits in one slot");
+    static_assert(WPS * 4096 <= STAGE, "the epilogue's LDS fits in one slot");
+    static_assert(SLICES == 1 || WPS * NB * 8192 <= STAGE, "a slice's sums fit in one slot");
 };
 using Large = Shape<4, 4>;
 
@@ -294,7 +304,8 @@ struct Feed {
 //   publish(State&, smem, tid)  after the main loop, before the barrier
 //   tile(State&, smem, lane, acc, tile, spare, settle)  spare: 4 KiB of LDS of the wave's own; with kStores,
 //                               settle() before the first store to memory
-//   end(State&, smem, lane, tile)  after an item's last tile
+//   end(State&, smem, lane, tile, mine)  after an item's last tile; mine: the wave's state has the item's tiles
+// With several slices, tile() runs in the first one's waves alone.
 template <int KIND, bool QK, bool XK, class Epi>
 __global__ __launch_bounds__(Epi::Shape::THREADS, Epi::Shape::PER_SIMD) void gemm16_kernel(Args a, Epi epi) {
     using Sh = typename Epi::Shape;
@@ -303,7 +314,8 @@ __global__ __launch_bounds__(Epi::Shape::THREADS, Epi::Shape::PER_SIMD) void gem
     __shared__ typename Epi::Shared smem;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const Lane<Sh::NB> ln{wave % Sh::WQ, wave / Sh::WQ, lane & 31, lane >> 5};
+    const int slice = wave / Sh::WPS, ws = wave % Sh::WPS;  // (uniform)
+    const Lane<Sh::NB> ln{ws % Sh::WQ, ws / Sh::WQ, lane & 31, lane >> 5};
     constexpr int NB = Sh::NB;
 
     Tiles<Epi::kWalk> tile;
@@ -311,12 +323,13 @@ __global__ __launch_bounds__(Epi::Shape::THREADS, Epi::Shape::PER_SIMD) void gem
     if (!tile.ok) return;
 
     const uint32_t total_stages = KIND == PLANES ? 3 * a.kstages : a.kstages;
-    const uint32_t lds0 = lds_addr_of(lds);
-    Feed<QK, KIND, Sh::WQ, Sh::WAVES, Sh::NB> fq_;
-    Feed<XK, KIND, Sh::WR, Sh::WAVES> fx_;
-    fq_.init(a.q, wave, lane, 0, ln.wq);
-    fx_.init(a.x, wave, lane, Sh::QB, ln.wr);
-    uint32_t s0, s1;  // the tile's stages
+    char* const mine = lds + slice * (Sh::SLOTS * STAGE);  // the slice's slots
+    const uint32_t lds0 = lds_addr_of(mine);
+    Feed<QK, KIND, Sh::WQ, Sh::WPS, Sh::NB> fq_;
+    Feed<XK, KIND, Sh::WR, Sh::WPS> fx_;
+    fq_.init(a.q, ws, lane, 0, ln.wq);
+    fx_.init(a.x, ws, lane, Sh::QB, ln.wr);
+    uint32_t s0, s1, ns;  // the slice's stages of the tile, and how many each slice takes
     auto open = [&]() {
         fq_.open(a.q, tile.qb);
         fx_.open(a.x, tile.rb);
@@ -326,6 +339,12 @@ __global__ __launch_bounds__(Epi::Shape::THREADS, Epi::Shape::PER_SIMD) void gem
         } else {
             s0 = uint32_t(uint64_t(total_stages) * tile.part / a.parts);
             s1 = uint32_t(uint64_t(total_stages) * (tile.part + 1) / a.parts);
+        }
+        ns = s1 - s0;
+        if constexpr (Sh::SLICES > 1) {  // (the last slices' may lie past the tile's: zeros)
+            ns = (ns + Sh::SLICES - 1) / Sh::SLICES;
+            s0 += uint32_t(slice) * ns;
+            s1 = min(s1, s0 + ns);
         }
     };
     // load i of the tile's stage s into slot `slot` (past the last stage: zeros)
@@ -345,7 +364,7 @@ __global__ __launch_bounds__(Epi::Shape::THREADS, Epi::Shape::PER_SIMD) void gem
     f32x16 acc[2][NB];
     u32x4 fx[2][2], fq[2][NB];
     auto read_one = [&](int buf, uint32_t slot, int t, int i) {
-        const char* base = lds + slot * STAGE;
+        const char* base = mine + slot * STAGE;
         if (i < 2) fx[buf][i] = fx_.read(base, i, t);
         else fq[buf][i - 2] = fq_.read(base, i - 2, t);
     };
@@ -406,7 +425,7 @@ __global__ __launch_bounds__(Epi::Shape::THREADS, Epi::Shape::PER_SIMD) void gem
     // the first tile's stages before anything that waits for memory; later tiles' first ones during the epilogues
 #pragma unroll
     for (int k = 0; k < SLOTS; ++k)
-        if (k == 0 || uint32_t(k) < s1 - s0) issue(s0 + k, k);
+        if (k == 0 || uint32_t(k) < ns) issue(s0 + k, k);
     epi.begin(st, smem, tile);
     bool settled = false, first = true;
     for (;;) {
@@ -417,25 +436,49 @@ __global__ __launch_bounds__(Epi::Shape::THREADS, Epi::Shape::PER_SIMD) void gem
             for (int n = 0; n < NB; ++n)
 #pragma unroll
                 for (int v = 0; v < 16; ++v) acc[m][n][v] = 0.0f;
-        const uint32_t ns = s1 - s0;
+        const uint32_t todo = ns;
         if (!first) {
             barrier();  // every wave is past the previous tile's epilogue: the other slots are free
 #pragma unroll
             for (int k = 1; k < SLOTS; ++k)
-                if (uint32_t(k) < ns) issue(s0 + k, k);
+                if (uint32_t(k) < todo) issue(s0 + k, k);
         }
         first = false;
         if (!settled) {
-            wait_but(min(SLOTS, int(ns)) - 1);  // stage 0 (older than the others' loads)
+            wait_but(min(SLOTS, int(todo)) - 1);  // stage 0 (older than the others' loads)
             barrier();
         }
 #pragma unroll
         for (int i = 0; i < 2 + NB; ++i) read_one(0, 0, 0, i);
         uint32_t i = 0;
-        for (; i + SLOTS < ns; ++i) stage(i, ns, std::true_type(), false);
-        for (; i < ns; ++i) stage(i, ns, std::false_type(), !XK && a.tail && s0 + i + 1 == total_stages);
+        for (; i + SLOTS < todo; ++i) stage(i, todo, std::true_type(), false);
+        for (; i < todo; ++i) stage(i, todo, std::false_type(), !XK && a.tail && s0 + i + 1 == total_stages);
         epi.publish(st, smem, tid);
         __syncthreads();  // every wave is past the main loop: slot 0 is free
+        if constexpr (Sh::SLICES > 1) {
+            // the slices' sums join in the first one's registers
+            char* const at = mine + STAGE + ws * (NB * 8192) + lane * 16;
+            if (slice) {
+#pragma unroll
+                for (int c = 0; c < 8 * NB; ++c) {
+                    f32x4 v;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[e] = acc[c & 1][c / 8][4 * ((c >> 1) & 3) + e];
+                    *reinterpret_cast<f32x4*>(at + 1024 * c) = v;
+                }
+            }
+            __syncthreads();
+            if (!slice) {
+#pragma unroll
+                for (int p = 1; p < Sh::SLICES; ++p)
+#pragma unroll
+                    for (int c = 0; c < 8 * NB; ++c) {
+                        const f32x4 v = *reinterpret_cast<const f32x4*>(at + p * (Sh::SLOTS * STAGE) + 1024 * c);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) acc[c & 1][c / 8][4 * ((c >> 1) & 3) + e] += v[e];
+                    }
+            }
+        }
         const Tiles<Epi::kWalk> here = tile;
         const bool last = tile.next(a);
         if (tile.ok) {
@@ -449,9 +492,10 @@ __global__ __launch_bounds__(Epi::Shape::THREADS, Epi::Shape::PER_SIMD) void gem
         // An epilogue that stores much waits for the next tile's first stage before its first store: behind the
         // stores, that wait would be for all of them.
         settled = Epi::kStores;
-        epi.tile(st, smem, le, acc, here, lds + STAGE + wave * 4096, [] { wait_vmcnt<0>(); });
+        if (Sh::SLICES == 1 || !slice) epi.tile(st, smem, le, acc, here, lds + STAGE + ws * 4096, [] { wait_vmcnt<0>(); });
+        else if (Epi::kStores) wait_vmcnt<0>();
         if (last) {
-            epi.end(st, smem, ln, here);
+            epi.end(st, smem, ln, here, Sh::SLICES == 1 || !slice);
             if (!tile.ok) break;
             epi.begin(st, smem, tile);
         }

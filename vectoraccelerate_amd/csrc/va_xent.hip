@@ -231,13 +231,13 @@ struct LseEpi {
         }
     }
     template <class Tile>
-    __device__ void end(State& s, Shared& sm, const g16::Lane<Sh::NB>& ln, const Tile& t) {
+    __device__ void end(State& s, Shared& sm, const g16::Lane<Sh::NB>& ln, const Tile& t, bool mine) {
 #pragma unroll
         for (int n = 0; n < Sh::NB; ++n) {
             // (natural units from here; a row's largest logit and its target's are scaled alike)
             float m = s.natural ? s.m[n] : s.m[n] * kLn2;
             join(m, s.z[n], __shfl_xor(m, 32), __shfl_xor(s.z[n], 32));
-            if (ln.hh == 0) sm.red[ln.wr][ln.q(n)] = make_float2(m, s.z[n]);
+            if (mine && ln.hh == 0) sm.red[ln.wr][ln.q(n)] = make_float2(m, s.z[n]);
         }
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
         const uint32_t q = threadIdx.x;
@@ -411,7 +411,7 @@ va_status va_xent_forward(va_context* ctx, const va_xent_desc* d, float* out_los
     const size_t q_bytes = qd ? 0 : uint64_t(T) * copy_bytes(kind, D), x_row = copy_bytes(kind, D);
     const uint32_t piece = xd ? round_up(V, 256) : piece_items(V, x_row, kCopyBudget), most = std::min(piece, V);
     const uint32_t pieces = ceil_div(V, piece);
-    const Blocks bl = blocks_for(ctx, T, most, 1, kind == g16::F32 && T <= 32);
+    const Blocks bl = blocks_for(ctx, T, most, 1, kind == g16::F32 && T <= 32, stages_of(kind, D));
     // Offsets are looked over first where the shorter epilogue counts: 16-bit products on the matrix cores'
     // time (4096 rows x 262,144 items of 768: the check takes 15 us and saves 100; a product that streams its
     // items hides the longer epilogue).
@@ -459,7 +459,7 @@ va_status va_xent_forward(va_context* ctx, const va_xent_desc* d, float* out_los
         a.nr = bl.nr(n);
         a.parts = c + 1 < pieces ? parts : last_parts;
         VA_CHECK_STATUS(by_kind(kind, d->offsets || wild, n % bl.tr, [&](auto k, auto off) {
-            return by_shape_of<decltype(k)::value>(bl.shape, [&](auto sh) {
+            return by_logit_shape<decltype(k)::value>(bl.shape, [&](auto sh) {
                 using Sh = decltype(sh);
                 LseEpi<Sh, decltype(k)::value, decltype(off)::value> e;
                 e.a = LogitArgs{d->offsets ? d->offsets + v0 : nullptr, checks ? odd : nullptr, qinv, xinv, d->scale, T, n};

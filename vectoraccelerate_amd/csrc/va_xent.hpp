@@ -203,15 +203,20 @@ va_status check_desc(va_context* ctx, const va_xent_desc* d, const char* who);
 // A scale at which the logits' other unit might overflow: natural units (as with odd offsets).
 inline bool wild_scale(const va_xent_desc* d) { return fabsf(d->scale) > 1e18f; }
 
+// Stages of a product along rows of D values.
+inline uint32_t stages_of(int kind, uint32_t D) { return (D * uint32_t(g16::size_of(kind)) + g16::ROWB - 1) / g16::ROWB * (kind == g16::PLANES ? 3 : 1); }
+
 // The shapes of a product's workgroups.  Deep ones have four slots: alone on their CU, three stages in flight.
+// Sliced ones (logits) have smaller tiles, with the stages of each shared among four waves.
 using Medium = g16::Shape<2, 2>;
 using Small = g16::Shape<1, 2>;
 using DeepMedium = g16::Shape<2, 2, 2, 4>;
 using DeepSmall = g16::Shape<1, 2, 2, 4>;
+using Sliced = g16::Shape<1, 1, 2, 2, 4>;
 // 32 queries, along k: fp32 products as they are, which 64 padded ones would bind to the matrix cores.
 using Narrow = g16::Shape<1, 2, 1>;
-using DeepNarrow = g16::Shape<1, 2, 1, 4>;
-enum ShapeId : int { LARGE = 0, MEDIUM = 1, SMALL = 2, NARROW = 3, DEEP_MEDIUM = 4, DEEP_SMALL = 5, DEEP_NARROW = 6 };
+using SlicedNarrow = g16::Shape<1, 1, 1, 2, 4>;
+enum ShapeId : int { LARGE = 0, MEDIUM = 1, SMALL = 2, NARROW = 3, DEEP_MEDIUM = 4, DEEP_SMALL = 5, SLICED = 6, SLICED_NARROW = 7 };
 template <class F>
 va_status by_shape(int shape, F&& f) {
     switch (shape) {
@@ -224,11 +229,16 @@ va_status by_shape(int shape, F&& f) {
 }
 template <int KIND, class F>
 va_status by_shape_of(int shape, F&& f) {
-    if constexpr (KIND == g16::F32) {
+    if constexpr (KIND == g16::F32)
         if (shape == NARROW) return f(Narrow());
-        if (shape == DEEP_NARROW) return f(DeepNarrow());
-    }
     return by_shape(shape, f);
+}
+template <int KIND, class F>
+va_status by_logit_shape(int shape, F&& f) {
+    if constexpr (KIND == g16::F32)
+        if (shape == SLICED_NARROW) return f(SlicedNarrow());
+    if (shape == SLICED) return f(Sliced());
+    return by_shape_of<KIND>(shape, f);
 }
 struct Blocks {
     int shape;              // ShapeId
@@ -241,8 +251,14 @@ struct Blocks {
 // the fewest operand bytes, but a small or ragged product fills few of them: with as many stages each, a round of
 // 128 x 128 tiles (two a CU) takes 0.50 to 0.56 of one of 256 x 256 in short products (0.61 to 0.75 in long ones
 // of whole rounds, which the rule gives to the large tiles), one of 64 x 128 (three a CU) 0.48 to 0.59; measured on
-// 1023 x 49,999 x 300 and 4096 x 262,144 x 768.  `shares`: how many shares of the sum the caller can make.
-inline Blocks blocks_for(const va_context* ctx, uint64_t Q, uint64_t R, uint32_t shares = 1, bool narrow = false) {
+// 1023 x 49,999 x 300 and 4096 x 262,144 x 768.  `shares`: how many shares of the sum the caller can make.  `stages`:
+// those of a tile, where it may be sliced (logits; a sum shared among workgroups has short chains already: dh of
+// 32 x 6979 x 1536 took 14 us sliced, 8 as it is).  Sliced pays where stages are many and tiles few.  64-query
+// tiles, scoring, sliced and as they are: 1 x 10,000 x 768 (157 tiles, 12 stages) 12.6 and 14.3 us, 37 x 5510 x 1024 in
+// fp32 (87, 48) 35.6 and 42.6; 1 x 10,000 x 512 (157, 8) 12.9 and 12.7, 64 x 16,000 x 640 (250, 10) 25.8 and 20.3.
+// 32-query ones: 4 x 36,909 x 768 (577, 24) 38 and 58, 10 x 10,000 x 100 (157, 4) 15.0 and 16.4; 30 x 200,000 x 256
+// (3125, 8) 70 and 63.
+inline Blocks blocks_for(const va_context* ctx, uint64_t Q, uint64_t R, uint32_t shares = 1, bool narrow = false, uint32_t stages = 0) {
     Blocks all[4] = {{LARGE, 256, 256, g16::grid_max<g16::Large>(ctx), 1},
                      {MEDIUM, 128, 128, g16::grid_max<Medium>(ctx), 1},
                      {SMALL, 64, 128, g16::grid_max<Small>(ctx), 1},
@@ -260,14 +276,21 @@ inline Blocks blocks_for(const va_context* ctx, uint64_t Q, uint64_t R, uint32_t
         }
     }
     Blocks b = all[best];
-    // one workgroup a CU, or fewer: the time is that of a tile's loads
-    if (b.shape != LARGE && uint64_t(b.nq(Q)) * b.nr(R) * b.parts <= uint64_t(ctx->num_cus)) {
+    // Fewer tiles than CUs: the time is that of one tile's loads, and of a wave's chain through its stages.
+    const uint64_t cus = uint64_t(ctx->num_cus);
+    if (narrow) {
+        const Blocks f{SLICED_NARROW, 32, 64, g16::grid_max<SlicedNarrow>(ctx), 1};
+        if (stages >= 4 && f.nr(R) * uint64_t(f.nq(Q)) <= 4 * cus) return f;
+        return b;
+    }
+    const Blocks f{SLICED, 64, 64, g16::grid_max<Sliced>(ctx), 1};
+    if (stages >= 12 && uint64_t(f.nq(Q)) * f.nr(R) <= cus * 5 / 8) return f;
+    if (b.shape != LARGE && uint64_t(b.nq(Q)) * b.nr(R) * b.parts <= cus) {
         b.shape += DEEP_MEDIUM - MEDIUM;
         b.grid = g16::grid_max<DeepSmall>(ctx);
     }
     return b;
 }
-static_assert(DEEP_SMALL - SMALL == DEEP_MEDIUM - MEDIUM && DEEP_NARROW - NARROW == DEEP_MEDIUM - MEDIUM, "deep shapes follow the others");
 
 // f(kind, offsets) of a launch; edge: the last tile is not whole
 template <class F>

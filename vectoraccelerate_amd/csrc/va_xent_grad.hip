@@ -262,7 +262,7 @@ struct GradEpi {
         }
     }
     template <class Tile>
-    __device__ void end(State&, Shared&, const g16::Lane<Sh::NB>&, const Tile&) {}
+    __device__ void end(State&, Shared&, const g16::Lane<Sh::NB>&, const Tile&, bool) {}
 };
 
 // A product's rows as fp32 shares [part][row][Dp], dh's added to over the pieces (first: written)
@@ -304,7 +304,7 @@ struct ShareEpi {
         }
     }
     template <class Tile>
-    __device__ void end(State&, Shared&, const g16::Lane<Sh::NB>&, const Tile&) {}
+    __device__ void end(State&, Shared&, const g16::Lane<Sh::NB>&, const Tile&, bool) {}
 };
 
 // A product's rows, final: dw's, or dh's where its sum is not shared (gk: rows whose gradient is zero)
@@ -367,7 +367,7 @@ struct RowsEpi {
         }
     }
     template <class Tile>
-    __device__ void end(State&, Shared&, const g16::Lane<Sh::NB>&, const Tile&) {}
+    __device__ void end(State&, Shared&, const g16::Lane<Sh::NB>&, const Tile&, bool) {}
 };
 
 // out[t][d] = mul sum over the shares (zero for a row without a gradient, gk not NULL).  64 groups of four values a
@@ -452,7 +452,7 @@ va_status va_xent_backward(va_context* ctx, const va_xent_desc* d, const float* 
         return stages <= 24 && once ? 1u : std::max(stages / 8, 1u);
     };
     const bool narrow = kind == g16::F32 && T <= 32;
-    const Blocks lb = blocks_for(ctx, T, most, 1, narrow), hb = blocks_for(ctx, T, D, shares_of(Vpmax, pieces == 1), narrow),
+    const Blocks lb = blocks_for(ctx, T, most, 1, narrow, stages_of(kind, D)), hb = blocks_for(ctx, T, D, shares_of(Vpmax, pieces == 1), narrow),
                  wb = blocks_for(ctx, most, D, shares_of(T, true));
     const bool h_shared = out_grad_hidden && (hb.parts > 1 || pieces > 1), w_shared = out_grad_items && wb.parts > 1;
 
@@ -547,7 +547,7 @@ va_status va_xent_backward(va_context* ctx, const va_xent_desc* d, const float* 
         a.nq = lb.nq(T);
         a.nr = lb.nr(n);
         VA_CHECK_STATUS(by_kind(kind, offsets || wild, n % lb.tr, [&](auto k, auto off) {
-            return by_shape_of<decltype(k)::value>(lb.shape, [&](auto sh) {
+            return by_logit_shape<decltype(k)::value>(lb.shape, [&](auto sh) {
                 using Sh = decltype(sh);
                 GradEpi<Sh, decltype(k)::value, decltype(off)::value> e;
                 e.a = LogitArgs{offsets, checks && !wild ? odd : nullptr, qinv, xinv, d->scale, T, n};
