@@ -9,6 +9,9 @@
 // fp64 from the first product on (gradients of any magnitude, no overflow) and joined in a fixed order by every
 // workgroup of the second pass, so results do not depend on the order in which workgroups run.  The second pass
 // starts where the first one ended: what is left of it in the caches is read from there.
+//
+// Measured: 468 MB in bf16 110 us to read (4.2 TB/s, the cache writing back what a pass before left in it) and
+// 165 us to scale (5.7 TB/s); 94 MB in 290 tensors 22 and 41 us; a few small tensors 4 and 5 us, the launches.
 #include <algorithm>
 #include <cmath>
 

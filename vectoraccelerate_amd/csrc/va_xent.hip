@@ -12,7 +12,7 @@
 // of them the recomputation), and the memory is that of one piece.
 //
 // Precision: fp16 / bf16 operands enter the matrix cores as they are, sums are fp32.  dl is rounded
-// once to the operands' type for the second products (relative 2^-12 / 2^-9 a value, like the
+// once to the operands' type for the second products (relative 2^-11 / 2^-8 a value, like the
 // rounding of the result), after a scale that takes the largest |g| to 2^14: fp16's range then holds
 // probabilities down to 2^-38 of it, and with one g for all rows the target's -g is exact.  fp32 operands, and dl with them, are
 // multiplied as fp32 for few rows and as two fp16 planes for many (va_gemm16.hpp).
@@ -20,6 +20,12 @@
 // Masks: an item whose offset is -inf has no probability whatever its vector holds (NaN and inf
 // included) and gets a zero gradient; a row without a target has loss 0 and a zero gradient whatever
 // it holds.  When every item is masked, lse = -inf, the losses are 0 and so are the gradients.
+//
+// What bounds it: few rows, the stream of the items (10 x 1M x 768 in fp16 258 us, 5.9 TB/s); many, the matrix cores and
+// after them the exp of every logit, which share a SIMD's waves (4096 x 262,144 x 768 in bf16 1.60 ms, 1.03
+// PFLOP/s; 1023 x 49,999 x 300 in fp16 53 us, 0.58 PFLOP/s with five stages a tile); fp32 rows in planes, three
+// times the products and the copies (512 x 100,003 x 384: 131 + 54 us); a small collection, latency
+// (1 x 10,000 x 768 in bf16: 9 + 5 us).
 #include "va_xent.hpp"
 
 namespace va {

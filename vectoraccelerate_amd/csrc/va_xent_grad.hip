@@ -5,6 +5,10 @@
 // dw = dl^T h; at the end the shares of dh summed, where there are several.  dl is bounded by
 // kGradBudget: a piece of 65,536 items for 4096 rows (pieces of 8,192 to 32,768, whose dl stays in the last
 // level cache, ran 35 to 6 % slower: each product then ends in a round of half-idle CUs).
+//
+// What bounds it: the matrix cores.  A piece of 65,536 items by 4096 rows of 768 in bf16 takes 0.47 ms for the logits and dl
+// (0.87 PFLOP/s; dl's 0.5 GB leave during the products), 0.39 for dh and 0.35 for dw (1.05 and 1.17); 1023 x 49,999 x
+// 300 in fp16 63, 47 and 50 us.
 #include "va_xent.hpp"
 
 namespace va {
