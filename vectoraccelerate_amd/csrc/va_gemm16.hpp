@@ -27,9 +27,10 @@
 // fp32 operands come in two ways.  As they are, on v_mfma_f32_32x32x2: a fragment's 16 bytes are four k-values
 // instead of eight, everything else is alike; a sixteenth of the 16-bit rate, which is enough while the
 // operands' bytes are what takes the time.  Or as two fp16 planes (value = (hi + lo) 2^-e with one
-// exponent a row or tensor): a product is then hi hi + hi lo + lo hi, three passes over k with the same
-// accumulators.  lo lo is below 2^-22 of the product and is left out; what remains is exact to about 2^-22 a
-// term, the same as an fp32 fma chain of a few terms.
+// exponent a row or tensor): a product is then hi hi + hi lo + lo hi, into the same accumulators.  The planes
+// alternate in memory, 16 values of hi and the same 16 of lo, so a stage holds both of 32 values and each
+// fragment is read once for its two products.  lo lo is below 2^-22 of the product and is left out; what
+// remains is exact to about 2^-22 a term, the same as an fp32 fma chain of a few terms.
 #pragma once
 
 #include <algorithm>
@@ -53,8 +54,8 @@ constexpr int ROWB = 128;  // bytes of an LDS row (k along the rows)
 
 // What the operands are made of.
 enum Kind : int { F16 = 0, BF16 = 1, PLANES = 2, F32 = 3 };
-constexpr int size_of(int kind) { return kind == F32 ? 4 : 2; }
-constexpr int stage_of(int kind) { return ROWB / size_of(kind); }  // k-values of a stage (of one plane)
+constexpr int size_of(int kind) { return kind >= PLANES ? 4 : 2; }  // bytes of a value in memory
+constexpr int stage_of(int kind) { return ROWB / size_of(kind); }     // k-values of a stage
 
 template <int WQ_, int WR_, int NB_ = 2, int SLOTS_ = 2, int SLICES_ = 1>
 struct Shape {
@@ -76,8 +77,7 @@ struct Operand {
     const void* p = nullptr;   // row 0
     uint64_t pitch = 0;        // bytes between rows (a multiple of 16)
     uint32_t rows = 0;         // k along the rows: queries (rows) of the product; across: values of k
-    uint32_t width = 0;        // bytes of a row that may be read (of one plane; whole dwords)
-    uint32_t plane = 0;        // bytes from a row's hi plane to its lo plane (PLANES)
+    uint32_t width = 0;        // bytes of a row that may be read (whole dwords)
     // read instead when *choose is not zero: a copy with rows of other_pitch bytes
     const void* other = nullptr;
     uint64_t other_pitch = 0;
@@ -86,7 +86,7 @@ struct Operand {
 
 struct Args {
     Operand q, x;
-    uint32_t kstages = 0;  // stages of k of one plane
+    uint32_t kstages = 0;  // stages of k
     uint32_t tail = 0;     // bytes of k in the last stage (0: all of it); x along the rows only
     uint32_t nq = 0, nr = 0;  // blocks of the shape's queries and rows
     uint32_t parts = 1;  // walk: workgroups per query block; tiles: shares of the k-stages
@@ -179,9 +179,10 @@ struct Lane {
 template <bool KM, int KIND, int W, int WAVES, int N = 2>
 struct Feed {
     static_assert(N == 2 || !KM, "narrow waves only along k");
-    static constexpr int ES = size_of(KIND), KV = stage_of(KIND);
+    static constexpr int ES = KIND == F32 ? 4 : 2, KV = stage_of(KIND);  // bytes of a value in LDS
     static constexpr int LPW = 4 * N * W / WAVES;   // 1 KiB direct loads per wave and stage
-    static constexpr int KROW = 64 * ES * W;        // bytes of a k-row (KM)
+    static constexpr int KROW = 64 * ES * W;        // bytes of a k-row of one plane (KM)
+    static constexpr int KMEM = 64 * size_of(KIND) * W;  // of the columns of a tile in memory
     // the place of a k-row's 16-byte chunk c: 16-bit values, its segment (four chunks) xored by k; fp32, its half
     // of 256 bytes by bit 2 of k (the two k-rows that a fragment reads at once are four apart)
     static __device__ uint32_t placed(uint32_t k, uint32_t c) {
@@ -192,7 +193,7 @@ struct Feed {
     const char* base;  // of the tile
     uint32_t records;  // bytes behind it (k along the rows)
     uint64_t left;     // (KM)
-    uint32_t pitch, plane;
+    uint32_t pitch;
     uint32_t voff[LPW];
     uint32_t lds_at;   // of the wave's first load, within a stage
     uint32_t frag[KM ? 2 : 1];  // fragment addresses within a stage
@@ -209,7 +210,6 @@ struct Feed {
         const bool copy = choose && *choose;
         p = static_cast<const char*>(copy ? two : one);
         pitch = uint32_t(copy ? pitch2 : pitch1);
-        plane = KIND == PLANES ? o.plane : 0;
         lds_at = at + uint32_t(wave) * 1024u;
         const int l32 = lane & 31;
         hh = lane >> 5;
@@ -218,7 +218,10 @@ struct Feed {
             for (int i = 0; i < LPW; ++i) {
                 const uint32_t byte = uint32_t(1024 * (wave + WAVES * i) + 16 * lane);
                 const uint32_t k = byte / KROW, c = byte % KROW / 16;
-                voff[i] = k * pitch + 16u * placed(k, c);
+                const uint32_t at_c = placed(k, c);
+                // PLANES: 16 k-rows of hi, the same of lo, and so on
+                if constexpr (KIND == PLANES) voff[i] = ((k >> 5) * 16u + (k & 15u)) * pitch + (at_c >> 1) * 64u + ((k >> 4) & 1u) * 32u + (at_c & 1u) * 16u;
+                else voff[i] = k * pitch + 16u * at_c;
             }
             const int e = (lane & 15) >> 2;
 #pragma unroll
@@ -242,23 +245,22 @@ struct Feed {
     // the operand's block b of 32 N W queries (rows)
     __device__ void open(const Operand& o, uint32_t b) {
         if constexpr (KM) {
-            base = p + b * uint32_t(KROW);
-            left = uint64_t(o.rows - 1) * pitch + o.width - b * uint32_t(KROW);
+            base = p + uint64_t(b) * uint32_t(KMEM);
+            left = uint64_t(o.rows - 1) * pitch + o.width - uint64_t(b) * uint32_t(KMEM);
         } else {
             base = p + uint64_t(b) * (32u * N * W) * pitch;
-            records = (min(32u * N * W, o.rows - b * (32u * N * W)) - 1u) * pitch + o.width + plane;
+            records = (min(32u * N * W, o.rows - b * (32u * N * W)) - 1u) * pitch + o.width;
         }
     }
-    // load i of stage k (of the plane `lo`) into the slot at LDS address `slot`; !ok: zeros
-    __device__ void issue(uint32_t k, bool lo, bool ok, uint32_t slot, int i) const {
+    // load i of stage k into the slot at LDS address `slot`; !ok: zeros
+    __device__ void issue(uint32_t k, bool ok, uint32_t slot, int i) const {
         if constexpr (KM) {
             const uint64_t skip = uint64_t(k) * KV * pitch;
-            const dma_rsrc r = make_dma_rsrc(base + skip + (lo ? plane : 0u),
-                                             ok && skip < left ? uint32_t(min(left - skip, uint64_t(kDmaMaxBytes))) : 0u);
+            const dma_rsrc r = make_dma_rsrc(base + skip, ok && skip < left ? uint32_t(min(left - skip, uint64_t(kDmaMaxBytes))) : 0u);
             lds_dma16(r, voff[i], slot + lds_at + uint32_t(1024 * WAVES * i));
         } else {
             const dma_rsrc r = make_dma_rsrc(base, records);
-            lds_dma16_so(r, ok ? voff[i] : kDmaSkip, ok ? k * uint32_t(ROWB) + (lo ? plane : 0u) : 0u, slot + lds_at + uint32_t(1024 * WAVES * i));
+            lds_dma16_so(r, ok ? voff[i] : kDmaSkip, ok ? k * uint32_t(ROWB) : 0u, slot + lds_at + uint32_t(1024 * WAVES * i));
         }
     }
     // the fragment of the wave's 32-query (row) block n, k-step t of the slot (32 bytes of k: this lane's half)
@@ -322,7 +324,7 @@ __global__ __launch_bounds__(Epi::Shape::THREADS, Epi::Shape::PER_SIMD) void gem
     tile.first(a);
     if (!tile.ok) return;
 
-    const uint32_t total_stages = KIND == PLANES ? 3 * a.kstages : a.kstages;
+    const uint32_t total_stages = a.kstages;
     char* const mine = lds + slice * (Sh::SLOTS * STAGE);  // the slice's slots
     const uint32_t lds0 = lds_addr_of(mine);
     Feed<QK, KIND, Sh::WQ, Sh::WPS, Sh::NB> fq_;
@@ -351,10 +353,9 @@ __global__ __launch_bounds__(Epi::Shape::THREADS, Epi::Shape::PER_SIMD) void gem
     constexpr int LQ = decltype(fq_)::LPW, LX = decltype(fx_)::LPW;
     auto issue_one = [&](uint32_t s, uint32_t slot, int i) {
         const bool ok = s < s1;
-        const uint32_t k = KIND == PLANES ? s / 3u : s, seg = KIND == PLANES ? s - 3u * k : 0u;  // (a k's planes are read together)
         const uint32_t sb = lds0 + slot * uint32_t(STAGE);
-        if (i < LQ) fq_.issue(k, seg == 2, ok, sb, i);
-        else fx_.issue(k, seg == 1, ok, sb, i - LQ);
+        if (i < LQ) fq_.issue(s, ok, sb, i);
+        else fx_.issue(s, ok, sb, i - LQ);
     };
     auto issue = [&](uint32_t s, uint32_t slot) {
 #pragma unroll
@@ -362,7 +363,8 @@ __global__ __launch_bounds__(Epi::Shape::THREADS, Epi::Shape::PER_SIMD) void gem
     };
 
     f32x16 acc[2][NB];
-    u32x4 fx[2][2], fq[2][NB];
+    constexpr int BUFS = KIND == PLANES ? 3 : 2;
+    u32x4 fx[BUFS][2], fq[BUFS][NB];
     auto read_one = [&](int buf, uint32_t slot, int t, int i) {
         const char* base = mine + slot * STAGE;
         if (i < 2) fx[buf][i] = fx_.read(base, i, t);
@@ -396,6 +398,31 @@ __global__ __launch_bounds__(Epi::Shape::THREADS, Epi::Shape::PER_SIMD) void gem
             __builtin_amdgcn_sched_barrier(0);
         }
     };
+    // The same of planes.  T even: hi hi, and the reads of the lo fragments (buffer 1); odd: lo hi and hi lo, and the reads
+    // of the next hi ones (buffers 0 and 2 in turn).
+    auto step_planes = [&](auto t, uint32_t slot_next, auto more, uint32_t s_load, uint32_t slot_load) {
+        constexpr int T = decltype(t)::value, HI = T < 2 ? 0 : 2, NEXT = T & 1 ? 2 - HI : 1, N = T & 1 ? 4 * NB : 2 * NB;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int m = i & 1, n = (i >> 1) % NB;
+            const bool second = i >= 2 * NB;
+            acc[m][n] = mfma<KIND>(fx[T & 1 && !second ? 1 : HI][m], fq[second ? 1 : HI][n], acc[m][n]);
+            __builtin_amdgcn_sched_barrier(0);
+            if (i < 2 + NB) {
+                if (NB == 2) {
+                    read_one(NEXT, slot_next, (T + 1) & 3, (i & 1) * 2 + (i >> 1));
+                } else if (i < 2) {
+                    read_one(NEXT, slot_next, (T + 1) & 3, i);
+                    if (i) read_one(NEXT, slot_next, (T + 1) & 3, 2);
+                }
+            }
+            if constexpr (decltype(more)::value) {
+#pragma unroll
+                for (int l = i * (LQ + LX) / N; l < (i + 1) * (LQ + LX) / N; ++l) issue_one(s_load, slot_load, l);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
     // a workgroup barrier that leaves the direct loads in flight; this wave's LDS reads are done
     auto barrier = [&]() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
     // waits for all but the youngest `stages` stages of direct loads
@@ -410,14 +437,22 @@ __global__ __launch_bounds__(Epi::Shape::THREADS, Epi::Shape::PER_SIMD) void gem
     // stage i of the tile's ns; more: stage i + SLOTS follows; ends: k ends within it
     auto stage = [&](uint32_t i, uint32_t ns, auto more, bool ends) {
         const uint32_t slot = i & (SLOTS - 1);
+        const std::integral_constant<bool, false> none{};
+        if constexpr (KIND == PLANES) {
+            step_planes(std::integral_constant<int, 0>(), slot, none, 0, 0);
+            step_planes(std::integral_constant<int, 1>(), slot, none, 0, 0);
+            step_planes(std::integral_constant<int, 2>(), slot, none, 0, 0);
+        } else {
 #pragma unroll
-        for (int t = 0; t < 3; ++t) step(t & 1, slot, t + 1, std::integral_constant<bool, false>(), 0, 0, ends && !decltype(more)::value);
+            for (int t = 0; t < 3; ++t) step(t & 1, slot, t + 1, none, 0, 0, ends && !decltype(more)::value);
+        }
         // the last k-step's fragments are in registers: publish the next stage, free this slot
         if (decltype(more)::value) wait_but(SLOTS - 2);
         else wait_but(min(SLOTS - 2, int(ns) - 2 - int(i)));
         barrier();
         __builtin_amdgcn_sched_barrier(0);
-        step(1, (slot + 1) & (SLOTS - 1), 0, more, s0 + i + SLOTS, slot, ends);
+        if constexpr (KIND == PLANES) step_planes(std::integral_constant<int, 3>(), (slot + 1) & (SLOTS - 1), more, s0 + i + SLOTS, slot);
+        else step(1, (slot + 1) & (SLOTS - 1), 0, more, s0 + i + SLOTS, slot, ends);
     };
 
     typename Epi::State st;

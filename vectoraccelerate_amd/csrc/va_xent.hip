@@ -59,7 +59,7 @@ __global__ __launch_bounds__(256) void copy_kernel(const U* __restrict__ src, ui
     }
 }
 
-// One wave per fp32 row: its planes dst[r] = {hi, lo} (Kp values each, zeros past D), scaled by the
+// One wave per fp32 row: its planes dst[r] (16 values of hi, the same of lo, and so on; Kp values, zeros past D), scaled by the
 // power of two that puts the row's largest entry, or the tensor's (absmax), near 2^14; inv[r] = the
 // inverse.  Dropped rows are zeros.
 // Rows of `a` in the first na workgroups, then of `b`.
@@ -107,8 +107,9 @@ __global__ __launch_bounds__(256) void planes_kernel(Planes a, Planes b, uint32_
         uint16_t h[4], l[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) split16(v[e] * sc, h[e], l[e]);
-        *reinterpret_cast<uint2*>(o + k) = make_uint2(h[0] | uint32_t(h[1]) << 16, h[2] | uint32_t(h[3]) << 16);
-        *reinterpret_cast<uint2*>(o + Kp + k) = make_uint2(l[0] | uint32_t(l[1]) << 16, l[2] | uint32_t(l[3]) << 16);
+        uint16_t* at = o + k / 16 * 32 + k % 16;
+        *reinterpret_cast<uint2*>(at) = make_uint2(h[0] | uint32_t(h[1]) << 16, h[2] | uint32_t(h[3]) << 16);
+        *reinterpret_cast<uint2*>(at + 16) = make_uint2(l[0] | uint32_t(l[1]) << 16, l[2] | uint32_t(l[3]) << 16);
     };
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -410,14 +411,14 @@ va_status va_xent_forward(va_context* ctx, const va_xent_desc* d, float* out_los
     const uint32_t T = d->rows, V = d->num_items, D = d->dim;
     const va_dtype dt = d->dtype;
     const int kind = kind_of(dt, T, V);
-    const uint32_t one = round_up(D * uint32_t(g16::size_of(kind)), g16::ROWB), tail = kind == g16::PLANES ? 0 : D * uint32_t(elem_size(dt)) % g16::ROWB;
+    const uint32_t one = copy_bytes(kind, D), tail = kind == g16::PLANES ? 0 : D * uint32_t(elem_size(dt)) % g16::ROWB;
     // the hidden rows end in zeros, the items are cut in their fragments
     const bool qd = kind != g16::PLANES && tail == 0 && in_dwords(dt, d->hidden, d->hidden_stride);
     const bool xd = kind != g16::PLANES && in_dwords(dt, d->items, d->items_stride);
     const size_t q_bytes = qd ? 0 : uint64_t(T) * copy_bytes(kind, D), x_row = copy_bytes(kind, D);
     const uint32_t piece = xd ? round_up(V, 256) : piece_items(V, x_row, kCopyBudget), most = std::min(piece, V);
     const uint32_t pieces = ceil_div(V, piece);
-    const Blocks bl = blocks_for(ctx, T, most, 1, kind == g16::F32 && T <= 32, stages_of(kind, D));
+    const Blocks bl = blocks_for(ctx, kind, T, most, 1, kind == g16::F32 && T <= 32, stages_of(kind, D));
     // Offsets are looked over first where the shorter epilogue counts: 16-bit products on the matrix cores'
     // time (4096 rows x 262,144 items of 768: the check takes 15 us and saves 100; a product that streams its
     // items hides the longer epilogue).

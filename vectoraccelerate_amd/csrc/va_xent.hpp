@@ -140,12 +140,9 @@ inline const char* row_at(const void* p, uint64_t ld, uint64_t row, va_dtype dt)
 
 // Rows that a product can read where they are: dwords.
 inline bool in_dwords(va_dtype dt, const void* p, uint64_t ld) { return ld * elem_size(dt) % 4 == 0 && reinterpret_cast<uintptr_t>(p) % 4 == 0; }
-// Bytes of a row of D values in place, and of one of a copy: whole stages, both planes of PLANES.
+// Bytes of a row of D values in place, and of one of a copy: whole stages.
 inline uint32_t row_bytes(va_dtype dt, uint32_t D) { return round_up(D * uint32_t(elem_size(dt)), 4); }
-inline uint32_t copy_bytes(int kind, uint32_t D) {
-    const uint32_t one = round_up(D * uint32_t(g16::size_of(kind)), g16::ROWB);
-    return kind == g16::PLANES ? 2 * one : one;
-}
+inline uint32_t copy_bytes(int kind, uint32_t D) { return round_up(D * uint32_t(g16::size_of(kind)), g16::ROWB); }
 // Operands over rows in place and over copies.
 inline g16::Operand in_place(va_dtype dt, const void* p, uint64_t ld, uint32_t rows, uint32_t D) {
     g16::Operand o;
@@ -160,8 +157,7 @@ inline g16::Operand copied(int kind, const void* p, uint32_t rows, uint32_t D) {
     o.p = p;
     o.pitch = copy_bytes(kind, D);
     o.rows = rows;
-    o.width = uint32_t(o.pitch) / (kind == g16::PLANES ? 2 : 1);
-    o.plane = kind == g16::PLANES ? o.width : 0;
+    o.width = uint32_t(o.pitch);
     return o;
 }
 
@@ -204,7 +200,7 @@ va_status check_desc(va_context* ctx, const va_xent_desc* d, const char* who);
 inline bool wild_scale(const va_xent_desc* d) { return fabsf(d->scale) > 1e18f; }
 
 // Stages of a product along rows of D values.
-inline uint32_t stages_of(int kind, uint32_t D) { return (D * uint32_t(g16::size_of(kind)) + g16::ROWB - 1) / g16::ROWB * (kind == g16::PLANES ? 3 : 1); }
+inline uint32_t stages_of(int kind, uint32_t D) { return copy_bytes(kind, D) / g16::ROWB; }
 
 // The shapes of a product's workgroups.  Deep ones have four slots: alone on their CU, three stages in flight.
 // Sliced ones (logits) have smaller tiles, with the stages of each shared among four waves.
@@ -217,10 +213,11 @@ using Sliced = g16::Shape<1, 1, 2, 2, 4>;
 using Narrow = g16::Shape<1, 2, 1>;
 using SlicedNarrow = g16::Shape<1, 1, 1, 2, 4>;
 enum ShapeId : int { LARGE = 0, MEDIUM = 1, SMALL = 2, NARROW = 3, DEEP_MEDIUM = 4, DEEP_SMALL = 5, SLICED = 6, SLICED_NARROW = 7 };
-template <class F>
+template <int KIND, class F>
 va_status by_shape(int shape, F&& f) {
+    if constexpr (KIND != g16::PLANES)
+        if (shape == LARGE) return f(g16::Large());
     switch (shape) {
-        case LARGE: return f(g16::Large());
         case MEDIUM: return f(Medium());
         case SMALL: return f(Small());
         case DEEP_MEDIUM: return f(DeepMedium());
@@ -231,7 +228,7 @@ template <int KIND, class F>
 va_status by_shape_of(int shape, F&& f) {
     if constexpr (KIND == g16::F32)
         if (shape == NARROW) return f(Narrow());
-    return by_shape(shape, f);
+    return by_shape<KIND>(shape, f);
 }
 template <int KIND, class F>
 va_status by_logit_shape(int shape, F&& f) {
@@ -258,7 +255,7 @@ struct Blocks {
 // fp32 (87, 48) 35.6 and 42.6; 1 x 10,000 x 512 (157, 8) 12.9 and 12.7, 64 x 16,000 x 640 (250, 10) 25.8 and 20.3.
 // 32-query ones: 4 x 36,909 x 768 (577, 24) 38 and 58, 10 x 10,000 x 100 (157, 4) 15.0 and 16.4; 30 x 200,000 x 256
 // (3125, 8) 70 and 63.
-inline Blocks blocks_for(const va_context* ctx, uint64_t Q, uint64_t R, uint32_t shares = 1, bool narrow = false, uint32_t stages = 0) {
+inline Blocks blocks_for(const va_context* ctx, int kind, uint64_t Q, uint64_t R, uint32_t shares = 1, bool narrow = false, uint32_t stages = 0) {
     Blocks all[4] = {{LARGE, 256, 256, g16::grid_max<g16::Large>(ctx), 1},
                      {MEDIUM, 128, 128, g16::grid_max<Medium>(ctx), 1},
                      {SMALL, 64, 128, g16::grid_max<Small>(ctx), 1},
@@ -266,7 +263,7 @@ inline Blocks blocks_for(const va_context* ctx, uint64_t Q, uint64_t R, uint32_t
     const double round[4] = {1.0, 0.56, 0.5, 0.5};
     int best = -1;
     double least = 0.0;
-    for (int i = narrow ? 3 : 0; i < (narrow ? 4 : 3); ++i) {
+    for (int i = narrow ? 3 : kind == g16::PLANES ? 1 : 0; i < (narrow ? 4 : 3); ++i) {
         const uint64_t tiles = uint64_t(all[i].nq(Q)) * all[i].nr(R);
         all[i].parts = uint32_t(std::min<uint64_t>(std::max<uint64_t>(all[i].grid / tiles, 1), shares));
         const double t = double((tiles * all[i].parts + all[i].grid - 1) / all[i].grid) / all[i].parts * round[i];

@@ -121,8 +121,7 @@ __global__ __launch_bounds__(256) void absmax_kernel(Planes a, Planes b, uint32_
         atomicMax(top + second, __builtin_bit_cast(uint32_t, fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]))));
 }
 
-// dl of the piece's items, p[t][j]: Vp values a plane and row, zeros past the last item, rows `pitch` bytes
-// apart.
+// dl of the piece's items, p[t][j]: Vp values a row, zeros past the last item, rows `pitch` bytes apart.
 template <class Sh, int KIND, int OFF>
 struct GradEpi {
     using Shape = Sh;
@@ -181,7 +180,7 @@ struct GradEpi {
         sm.lse[tid] = s.lse;
         sm.target[tid] = s.target;
     }
-    // The wave's 4 KiB of LDS hold 32 rows of 128 bytes of dl (64 items of one plane, or 32 in fp32), 16-byte chunks
+    // The wave's 4 KiB of LDS hold 32 rows of 128 bytes of dl (64 items in 16 bits, 32 in fp32 or planes), 16-byte chunks
     // swizzled by t & 7 (the writes and the reads then touch every bank equally); whole 128-byte lines go
     // out.  (Stored straight from the accumulators, 8 bytes a lane, a tile took three times as long.)
     __device__ void put(const char* spare, const g16::Lane<Sh::NB>& ln, const uint32_t q0, uint64_t at) {
@@ -195,11 +194,12 @@ struct GradEpi {
         }
         asm volatile("" ::: "memory");  // and the reads before what is written next
     }
-    static __device__ void write16(char* spare, const g16::Lane<Sh::NB>& ln, int m, int j, const uint16_t (&v)[4]) {
-        *reinterpret_cast<uint2*>(spare + ln.l32 * 128 + 16 * ((4 * m + j) ^ (ln.l32 & 7)) + 8 * ln.hh) =
+    // four 16-bit values of the lane into chunk c of its row
+    static __device__ void write16(char* spare, const g16::Lane<Sh::NB>& ln, int c, const uint16_t (&v)[4]) {
+        *reinterpret_cast<uint2*>(spare + ln.l32 * 128 + 16 * (c ^ (ln.l32 & 7)) + 8 * ln.hh) =
             make_uint2(v[0] | uint32_t(v[1]) << 16, v[2] | uint32_t(v[3]) << 16);
     }
-    // dl of the lane's 16 items of one block (m), 16-bit to LDS or fp32 in place.  TARGETS: one of the wave's rows
+    // dl of the lane's 16 items of one block (m) to LDS.  TARGETS: one of the wave's rows
     // has its target among the block's items
     template <bool NATURAL, bool TARGETS>
     __device__ void block(Shared& sm, const g16::Lane<Sh::NB>& ln, f32x16 (&acc)[2][Sh::NB], uint32_t y, int m, int n, char* spare) {
@@ -215,7 +215,7 @@ struct GradEpi {
                 float d = exp_diff<NATURAL>(v[e], ref);
                 if (TARGETS && y == uint32_t(r + e) && v[e] != -INFINITY) d -= 1.0f;
                 d *= g;
-                if constexpr (KIND >= g16::PLANES) acc[m][n][4 * j + e] = d;
+                if constexpr (KIND == g16::F32) acc[m][n][4 * j + e] = d;
                 if constexpr (KIND == g16::PLANES) split16(d, hi[e], lo[e]);
                 else if constexpr (KIND != g16::F32) hi[e] = bits16<KIND == g16::BF16>(d);
             }
@@ -224,8 +224,11 @@ struct GradEpi {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) d[e] = acc[m][n][4 * j + e];
                 *reinterpret_cast<f32x4*>(spare + ln.l32 * 128 + 16 * ((2 * j + ln.hh) ^ (ln.l32 & 7))) = d;
+            } else if constexpr (KIND == g16::PLANES) {
+                write16(spare, ln, 4 * (j >> 1) + (j & 1), hi);
+                write16(spare, ln, 4 * (j >> 1) + (j & 1) + 2, lo);
             } else {
-                write16(spare, ln, m, j, hi);
+                write16(spare, ln, 4 * m + j, hi);
             }
         }
     }
@@ -246,23 +249,11 @@ struct GradEpi {
                     else if (hit) block<false, true>(sm, ln, acc, y, m, n, spare);
                     else block<false, false>(sm, ln, acc, y, m, n, spare);
                 }
-                if (n == 0 && m == (KIND == g16::F32 ? 0 : 1)) settle();
+                if (n == 0 && m == (ES == 4 ? 0 : 1)) settle();
                 // (dl's rows hold whole groups of 64 items: a wave's are inside or outside)
-                if (KIND == g16::F32 && rw < Vp) put(spare, ln, q0, uint64_t(rw + 32 * m) * ES);
+                if (ES == 4 && rw < Vp) put(spare, ln, q0, uint64_t(rw + 32 * m) * ES);
             }
-            if (KIND != g16::F32 && rw < Vp) put(spare, ln, q0, uint64_t(rw) * ES);
-            if constexpr (KIND == g16::PLANES) {
-#pragma unroll
-                for (int m = 0; m < 2; ++m)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        uint16_t hi[4], lo[4];
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) split16(acc[m][n][4 * j + e], hi[e], lo[e]);
-                        write16(spare, ln, m, j, lo);
-                    }
-                if (rw < Vp) put(spare, ln, q0, uint64_t(Vp + rw) * ES);
-            }
+            if (ES == 2 && rw < Vp) put(spare, ln, q0, uint64_t(rw) * ES);
         }
     }
     template <class Tile>
@@ -437,30 +428,29 @@ va_status va_xent_backward(va_context* ctx, const va_xent_desc* d, const float* 
     const int kind = kind_of(dt, T, V);
     const bool planes = kind == g16::PLANES, wild = wild_scale(d);
     const uint32_t ks = uint32_t(g16::size_of(kind)), kv = uint32_t(g16::stage_of(kind));
-    const uint32_t one = round_up(D * ks, g16::ROWB), tail = planes ? 0 : D * ks % g16::ROWB;
+    const uint32_t one = copy_bytes(kind, D), tail = planes ? 0 : D * ks % g16::ROWB;
     // Masked items may hold anything, and dh sums over them: unless they are found to be finite, a copy is read in
     // which they are zeros.
     const bool xd = !planes && in_dwords(dt, d->items, d->items_stride), checks = xd && d->offsets, copies = !xd || checks;
     const uint32_t x_row = copy_bytes(kind, D);
 
     // the piece: dl and the copied items within their budgets, dl's rows within the products' 32-bit offsets
-    const uint32_t per_item = planes ? 2 * ks : ks;  // bytes of dl
-    uint32_t piece = piece_items(V, uint64_t(T) * per_item, kGradBudget);
+    uint32_t piece = piece_items(V, uint64_t(T) * ks, kGradBudget);
     if (copies) piece = std::min(piece, piece_items(V, x_row, kCopyBudget));
-    piece = std::min<uint32_t>(piece, (uint32_t(kDmaMaxBytes / 256) - kRowPad) / per_item / 256 * 256);
+    piece = std::min<uint32_t>(piece, (uint32_t(kDmaMaxBytes / 256) - kRowPad) / ks / 256 * 256);
     const uint32_t pieces = ceil_div(V, piece), most = std::min(piece, V), Vpmax = round_up(most, 64);
     // dh has few tiles and a long sum, and so has dw of many rows and few items: shares of it until the chip is
     // filled once, eight stages at least each.  A short sum in one piece is not shared, its rows are final.
     const auto shares_of = [&](uint32_t k, bool once) {
-        const uint32_t stages = ceil_div(k, kv) * (planes ? 3 : 1);
+        const uint32_t stages = ceil_div(k, kv);
         return stages <= 24 && once ? 1u : std::max(stages / 8, 1u);
     };
     const bool narrow = kind == g16::F32 && T <= 32;
-    const Blocks lb = blocks_for(ctx, T, most, 1, narrow, stages_of(kind, D)), hb = blocks_for(ctx, T, D, shares_of(Vpmax, pieces == 1), narrow),
-                 wb = blocks_for(ctx, most, D, shares_of(T, true));
+    const Blocks lb = blocks_for(ctx, kind, T, most, 1, narrow, stages_of(kind, D)), hb = blocks_for(ctx, kind, T, D, shares_of(Vpmax, pieces == 1), narrow),
+                 wb = blocks_for(ctx, kind, most, D, shares_of(T, true));
     const bool h_shared = out_grad_hidden && (hb.parts > 1 || pieces > 1), w_shared = out_grad_items && wb.parts > 1;
 
-    const size_t p_bytes = uint64_t(T) * (uint64_t(Vpmax) * per_item + kRowPad);
+    const size_t p_bytes = uint64_t(T) * (uint64_t(Vpmax) * ks + kRowPad);
     const size_t share_n = h_shared ? uint64_t(hb.parts) * T * Dp : 0, w_share_n = w_shared ? uint64_t(wb.parts) * most * Dp : 0;
     const size_t q_bytes = uint64_t(T) * copy_bytes(kind, D), x_bytes = copies ? uint64_t(most) * x_row : 0;
     Scratch sc(ctx);
@@ -539,10 +529,9 @@ va_status va_xent_backward(va_context* ctx, const va_xent_desc* d, const float* 
         }
         g16::Operand dl;
         dl.p = p;
-        dl.pitch = uint64_t(Vp) * per_item + kRowPad;
+        dl.pitch = uint64_t(Vp) * ks + kRowPad;
         dl.rows = T;
         dl.width = Vp * ks;
-        dl.plane = planes ? Vp * ks : 0;
         g16::Args a;
         a.q = rows;
         a.x = cols;
@@ -593,7 +582,7 @@ va_status va_xent_backward(va_context* ctx, const va_xent_desc* d, const float* 
             b.parts = wb.parts;
             const uintptr_t o = reinterpret_cast<uintptr_t>(out_grad_items) + uint64_t(v0) * grad_items_stride * es;
             VA_CHECK_STATUS(by_kind(kind, [&](auto k) {
-                return by_shape(wb.shape, [&](auto sh) {
+                return by_shape<decltype(k)::value>(wb.shape, [&](auto sh) {
                     if (!w_shared) return rows_out(sh, k, std::true_type(), b, o, grad_items_stride, n, absmax, nullptr);
                     const ShareEpi<decltype(sh)> e{w_share, n, D, Dp, true};
                     return g16::launch<decltype(k)::value, true, true>(ctx, b, e);
