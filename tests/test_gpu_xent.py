@@ -375,3 +375,13 @@ def test_few_tiles_with_many_stages(ctx, T, V, D, dtype):
     off[torch.rand(V, generator=g) < 0.1] = -torch.inf
     _check(ctx, h, w, y)
     _check(ctx, h, w, y, scale=0.5, offsets=off.cuda())
+
+
+@pytest.mark.parametrize("T,V,D", [(1500, 12_000, 130), (1281, 30_001, 40)])
+def test_large_tiles_of_planes(ctx, T, V, D):
+    """fp32 rows and items that fill the chip with the largest tiles."""
+    h, w, y, g = _inputs(T, V, D, torch.float32, T + V)
+    off = torch.randn(V, generator=g)
+    off[torch.rand(V, generator=g) < 0.05] = -torch.inf
+    _check(ctx, h, w, y)
+    _check(ctx, h, w, y, scale=0.7, offsets=off.cuda())

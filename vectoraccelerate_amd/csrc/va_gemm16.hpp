@@ -6,7 +6,7 @@
 // Either operand is stored with k along its rows (Q[q] is a row) or across them (k is the row: QK, XK).
 //
 // A wave computes 64 queries x 64 rows (2 x 2 blocks of v_mfma_f32_32x32x16, 64 fp32 accumulators a
-// lane; NB = 1: 32 queries), a workgroup WQ x WR such waves: 4 x 4 for large products (256 x 256, four waves per
+// lane; NB = 1: 32 queries, 4: 128), a workgroup WQ x WR such waves: 4 x 4 for large products (256 x 256, four waves per
 // SIMD, one workgroup a CU), fewer where tiles of that size would leave CUs without work.  128 bytes of k (a stage)
 // of both operands move global -> LDS by direct loads into one of two slots while the other is computed on (four
 // slots where a launch does not fill the chip and waits for each stage).  Where there are few tiles with many
@@ -34,8 +34,7 @@
 #pragma once
 
 #include <algorithm>
-#include <mutex>
-#include <set>
+#include <atomic>
 #include <type_traits>
 #include <utility>
 
@@ -409,7 +408,9 @@ __global__ __launch_bounds__(Epi::Shape::THREADS, Epi::Shape::PER_SIMD) void gem
             acc[m][n] = mfma<KIND>(fx[T & 1 && !second ? 1 : HI][m], fq[second ? 1 : HI][n], acc[m][n]);
             __builtin_amdgcn_sched_barrier(0);
             if (i < 2 + NB) {
-                if (NB == 2) {
+                if (NB == 4) {
+                    read_one(NEXT, slot_next, (T + 1) & 3, i);
+                } else if (NB == 2) {
                     read_one(NEXT, slot_next, (T + 1) & 3, (i & 1) * 2 + (i >> 1));
                 } else if (i < 2) {
                     read_one(NEXT, slot_next, (T + 1) & 3, i);
@@ -550,16 +551,6 @@ template <class Sh>
 uint32_t grid_max(const va_context* ctx) {
     return std::max(uint32_t(ctx->num_cus), kXcds) / kXcds * kXcds * per_cu<Sh>();
 }
-// Lets a kernel take `bytes` of dynamic LDS on the device; the runtime is asked once per kernel and device.
-inline hipError_t allow_lds(const void* kern, int bytes, int device) {
-    static std::mutex lock;
-    static std::set<std::pair<const void*, int>> done;
-    std::lock_guard<std::mutex> hold(lock);
-    if (done.count({kern, device})) return hipSuccess;
-    const hipError_t e = hipFuncSetAttribute(kern, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e == hipSuccess) done.insert({kern, device});
-    return e;
-}
 template <int KIND, bool QK, bool XK, class Epi>
 va_status launch(va_context* ctx, const Args& a, const Epi& epi) {
     using Sh = typename Epi::Shape;
@@ -572,7 +563,13 @@ va_status launch(va_context* ctx, const Args& a, const Epi& epi) {
                     (unsigned long long)pitch);
     const uint64_t grid = std::min<uint64_t>((tiles + kXcds - 1) / kXcds * kXcds, grid_max<Sh>(ctx));
     auto kern = &gemm16_kernel<KIND, QK, XK, Epi>;
-    VA_CHECK_HIP(ctx, allow_lds(reinterpret_cast<const void*>(kern), Sh::LDS, ctx->device));
+    // the kernel may take its dynamic LDS: asked once per device
+    static std::atomic<uint64_t> allowed{0};
+    const uint64_t bit = ctx->device < 64 ? 1ull << ctx->device : 0;
+    if (!(allowed.load(std::memory_order_relaxed) & bit)) {
+        VA_CHECK_HIP(ctx, hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, Sh::LDS));
+        allowed.fetch_or(bit, std::memory_order_relaxed);
+    }
     kern<<<dim3(uint32_t(grid)), dim3(Sh::THREADS), Sh::LDS, ctx->stream>>>(a, epi);
     VA_CHECK_LAUNCH(ctx);
     return VA_OK;

@@ -161,8 +161,8 @@ inline g16::Operand copied(int kind, const void* p, uint32_t rows, uint32_t D) {
     return o;
 }
 
-// fp32 operands as they are or as planes.  Planes cost passes over the items that write copies, and products that
-// read them one and a half times (42 bytes a value of a training step, where fp32 as it is takes 16), and save
+// fp32 operands as they are or as planes.  Planes cost passes over the items that write copies
+// (36 bytes a value of a training step, where fp32 as it is takes 16), and save
 // 9/10 of the matrix cores' time: they win as soon as that counts, which for a short collection is the time of
 // one tile (10,000 items of 768 by 100 rows, logits alone: 27 us against 55).
 inline int kind_of(va_dtype dt, uint32_t rows, uint32_t items) {
@@ -209,6 +209,10 @@ using Small = g16::Shape<1, 2>;
 using DeepMedium = g16::Shape<2, 2, 2, 4>;
 using DeepSmall = g16::Shape<1, 2, 2, 4>;
 using Sliced = g16::Shape<1, 1, 2, 2, 4>;
+// Planes' 256 x 256, for logits: eight waves of 128 x 64, whose registers hold both planes' fragments beside the sums.
+// 4096 x 50,000 x 1024, loss: 1.03 ms, with 128 x 128 tiles 1.18; 2808 x 21,283 x 512 with gradients 846 and 860 us.
+// (For dh too, 400 x 10,000 x 768 took 188 us instead of 182, the 2808 rows 833 instead of 846.)
+using Wide = g16::Shape<2, 4, 4>;
 // 32 queries, along k: fp32 products as they are, which 64 padded ones would bind to the matrix cores.
 using Narrow = g16::Shape<1, 2, 1>;
 using SlicedNarrow = g16::Shape<1, 1, 1, 2, 4>;
@@ -234,6 +238,8 @@ template <int KIND, class F>
 va_status by_logit_shape(int shape, F&& f) {
     if constexpr (KIND == g16::F32)
         if (shape == SLICED_NARROW) return f(SlicedNarrow());
+    if constexpr (KIND == g16::PLANES)
+        if (shape == LARGE) return f(Wide());
     if (shape == SLICED) return f(Sliced());
     return by_shape_of<KIND>(shape, f);
 }
@@ -263,7 +269,7 @@ inline Blocks blocks_for(const va_context* ctx, int kind, uint64_t Q, uint64_t R
     const double round[4] = {1.0, 0.56, 0.5, 0.5};
     int best = -1;
     double least = 0.0;
-    for (int i = narrow ? 3 : kind == g16::PLANES ? 1 : 0; i < (narrow ? 4 : 3); ++i) {
+    for (int i = narrow ? 3 : kind == g16::PLANES && !stages ? 1 : 0; i < (narrow ? 4 : 3); ++i) {
         const uint64_t tiles = uint64_t(all[i].nq(Q)) * all[i].nr(R);
         all[i].parts = uint32_t(std::min<uint64_t>(std::max<uint64_t>(all[i].grid / tiles, 1), shares));
         const double t = double((tiles * all[i].parts + all[i].grid - 1) / all[i].grid) / all[i].parts * round[i];
