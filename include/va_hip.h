@@ -535,14 +535,15 @@ va_status va_rms_dequantize(va_context* ctx, const void* codes, uint64_t codes_s
                             va_dtype dtype, void* out, uint64_t out_stride);
 /* desc: x is r (va_rms_norm's out_residual, or x where there was no residual), no residual and no
  * outputs.  grad: of y; grad_residual (may be NULL): what reaches r past the norm.  out_grad_x is the
- * gradient of x and of the residual alike; either output may be NULL. */
+ * gradient of x and of the residual alike, and may be written over grad, grad_residual or x; either output
+ * may be NULL. */
 va_status va_rms_norm_backward(va_context* ctx, const va_rms_desc* desc, const void* grad, uint64_t grad_stride,
                                const void* grad_residual, uint64_t grad_residual_stride, const float* inverse_rms,
                                void* out_grad_x, uint64_t grad_x_stride, void* out_grad_weight);
 
 /* The 2-norm n of all values of a list of tensors (out_norm, one float; may be NULL), and every
  * tensor times min(1, max_norm / (n + epsilon)), into `outputs` or in place (outputs NULL).  The
- * arrays are host memory, read before the call returns; tensors may be empty. */
+ * arrays are host memory, read before the call returns; tensors may be empty, and none overlaps another. */
 typedef struct {
     void* const* tensors;    /* device, contiguous */
     void* const* outputs;    /* device, or NULL: in place */

@@ -247,3 +247,23 @@ def test_more_rows_than_a_launch_holds(ctx, code):
         oracle.close(scales[p].squeeze(1), want, (e + 2 * U32) * want, "scales")
         # (half a step of the code and what the arithmetic moves y / s by; the product's own rounding)
         oracle.close(y[p], yy, want[:, None] * (0.5 + 127.0 * (2 * e + 8 * U32)), "codes")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("D", [700, 3000, 9000])
+@pytest.mark.parametrize("over", ["grad", "residual", "x"])
+def test_backward_in_place(ctx, D, dtype, over):
+    """The gradient of x written over one of the operands."""
+    from vectoraccelerate_amd import RMSNormKernel
+
+    k = RMSNormKernel(ctx)
+    T = 40
+    x, r, w, g = _inputs(T, D, dtype, 29)
+    dy, dr = (torch.randn(T, D, generator=g).to(dtype).cuda() for _ in range(2))
+    _, s, inv = k.forward(x, w, r)
+    gx, gw = k.backward(dy, s, w, inv, dr)
+    out, weight = {"grad": dy, "residual": dr, "x": s}[over], torch.empty_like(gw)
+    ctx.order_after_torch()
+    k.encodeBackward(dy, s, w, inv, out, weight, dr)
+    ctx.synchronize()
+    assert torch.equal(out, gx) and torch.equal(weight, gw)

@@ -610,15 +610,18 @@ va_status va_rms_norm_backward(va_context* ctx, const va_rms_desc* d, const void
             if constexpr (C > 0) {
                 rms_grad_kernel<DT, WPR, C><<<dim3(grid), dim3(256), 0, ctx->stream>>>(a);
                 VA_CHECK_LAUNCH(ctx);
-            } else if (a.out) {
-                rms_long_grad_kernel<DT><<<dim3(grid), dim3(256), 0, ctx->stream>>>(a);
-                VA_CHECK_LAUNCH(ctx);
-            }
-            if (out_grad_weight) {
-                if (!C) {
+            } else {
+                // (dw first: dx may be written over what it is the sum of)
+                if (out_grad_weight) {
                     rms_weight_grad_kernel<DT><<<dim3(ceil_div(a.D, 2048), shares), dim3(256), 0, ctx->stream>>>(a);
                     VA_CHECK_LAUNCH(ctx);
                 }
+                if (a.out) {
+                    rms_long_grad_kernel<DT><<<dim3(grid), dim3(256), 0, ctx->stream>>>(a);
+                    VA_CHECK_LAUNCH(ctx);
+                }
+            }
+            if (out_grad_weight) {
                 rms_weight_sum_kernel<DT><<<dim3(ceil_div(a.D, 64)), dim3(1024), 0, ctx->stream>>>(a.part, shares, a.D, static_cast<ElemT<DT>*>(out_grad_weight));
                 VA_CHECK_LAUNCH(ctx);
             }

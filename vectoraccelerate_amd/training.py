@@ -322,7 +322,8 @@ class TensorList:
 
 class GradientClipKernel:
     """norm = sqrt(sum of the squares of all values of a list of tensors); every tensor times
-    min(1, maxNorm / (norm + epsilon)), in place or into the list's outputs.  Types may be mixed."""
+    min(1, maxNorm / (norm + epsilon)), in place or into the list's outputs.  Types may be mixed; a tensor is
+    listed once."""
 
     name = "GradientClipKernel"
 
