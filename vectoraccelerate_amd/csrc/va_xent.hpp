@@ -257,8 +257,8 @@ struct Blocks {
 // 1023 x 49,999 x 300 and 4096 x 262,144 x 768.  `shares`: how many shares of the sum the caller can make.  `stages`:
 // those of a tile, where it may be sliced (logits; a sum shared among workgroups has short chains already: dh of
 // 32 x 6979 x 1536 took 14 us sliced, 8 as it is).  Sliced pays where stages are many and tiles few.  64-query
-// tiles, scoring, sliced and as they are: 1 x 10,000 x 768 (157 tiles, 12 stages) 12.6 and 14.3 us, 37 x 5510 x 1024 in
-// fp32 (87, 48) 35.6 and 42.6; 1 x 10,000 x 512 (157, 8) 12.9 and 12.7, 64 x 16,000 x 640 (250, 10) 25.8 and 20.3.
+// tiles, scoring, sliced and as they are: 1 x 10,000 x 768 (157 tiles, 12 stages) 12.6 and 14.3 us, 32 x 6979 x 1536
+// (110, 24; the logits alone) 12.6 and 16.4; 1 x 10,000 x 512 (157, 8) 12.9 and 12.7, 64 x 16,000 x 640 (250, 10) 25.8 and 20.3.
 // 32-query ones: 4 x 36,909 x 768 (577, 24) 38 and 58, 10 x 10,000 x 100 (157, 4) 15.0 and 16.4; 30 x 200,000 x 256
 // (3125, 8) 70 and 63.
 inline Blocks blocks_for(const va_context* ctx, int kind, uint64_t Q, uint64_t R, uint32_t shares = 1, bool narrow = false, uint32_t stages = 0) {
