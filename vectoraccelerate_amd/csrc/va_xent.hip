@@ -424,10 +424,10 @@ va_status va_xent_forward(va_context* ctx, const va_xent_desc* d, float* out_los
     // items hides the longer epilogue).
     const bool wild = wild_scale(d), checks = d->offsets && kind < g16::PLANES && !wild && bl.shape == LARGE;
     const uint32_t nq = bl.nq(T);
-    // parts per query block: whole multiples of the XCDs when there are that many
-    uint32_t parts = std::max(bl.grid / nq, 1u);
-    if (parts > kXcds) parts = parts / kXcds * kXcds;
-    parts = std::min(parts, bl.nr(most));
+    // parts per query block: whole multiples of the XCDs where that costs no round of tiles
+    uint32_t parts = std::min(std::max(bl.grid / nq, 1u), bl.nr(most));
+    const uint32_t even = parts / kXcds * kXcds;
+    if (even && ceil_div(bl.nr(most), even) == ceil_div(bl.nr(most), parts)) parts = even;
     const uint32_t last_parts = std::min(parts, bl.nr(V - (pieces - 1) * piece));  // (of the last piece)
     const uint32_t slots = parts * (pieces - 1) + last_parts;
 

@@ -257,8 +257,9 @@ struct Blocks {
 // 1023 x 49,999 x 300 and 4096 x 262,144 x 768.  `shares`: how many shares of the sum the caller can make.  `stages`:
 // those of a tile, where it may be sliced (logits; a sum shared among workgroups has short chains already: dh of
 // 32 x 6979 x 1536 took 14 us sliced, 8 as it is).  Sliced pays where stages are many and tiles few.  64-query
-// tiles, scoring, sliced and as they are: 1 x 10,000 x 768 (157 tiles, 12 stages) 12.6 and 14.3 us, 32 x 6979 x 1536
-// (110, 24; the logits alone) 12.6 and 16.4; 1 x 10,000 x 512 (157, 8) 12.9 and 12.7, 64 x 16,000 x 640 (250, 10) 25.8 and 20.3.
+// tiles, scoring, sliced and as they are: 32 x 6979 x 1536 (110 tiles, 24 stages; the
+// logits alone) 12.6 and 16.4 us, 37 x 5510 x 1024 in fp32 (87, 32) 34 and 43; 64 x 9000 x 1024 (141, 16) 22.7 and 22.3,
+// 64 x 16,000 x 640 (250, 10) 25.8 and 20.3, 1 x 10,000 x 512 (157, 8) 12.9 and 12.7 (but x 768 13.1 and 14.3).
 // 32-query ones: 4 x 36,909 x 768 (577, 24) 38 and 58, 10 x 10,000 x 100 (157, 4) 15.0 and 16.4; 30 x 200,000 x 256
 // (3125, 8) 70 and 63.
 inline Blocks blocks_for(const va_context* ctx, int kind, uint64_t Q, uint64_t R, uint32_t shares = 1, bool narrow = false, uint32_t stages = 0) {
@@ -287,7 +288,7 @@ inline Blocks blocks_for(const va_context* ctx, int kind, uint64_t Q, uint64_t R
         return b;
     }
     const Blocks f{SLICED, 64, 64, g16::grid_max<Sliced>(ctx), 1};
-    if (stages >= 12 && uint64_t(f.nq(Q)) * f.nr(R) <= cus * 5 / 8) return f;
+    if (stages >= 12 && uint64_t(f.nq(Q)) * f.nr(R) <= cus / 2) return f;
     if (b.shape != LARGE && uint64_t(b.nq(Q)) * b.nr(R) * b.parts <= cus) {
         b.shape += DEEP_MEDIUM - MEDIUM;
         b.grid = g16::grid_max<DeepSmall>(ctx);

@@ -302,20 +302,22 @@ struct ShareEpi {
     __device__ void end(State&, Shared&, const g16::Lane<Sh::NB>&, const Tile&, bool) {}
 };
 
-// A product's rows, final: dw's, or dh's where its sum is not shared (gk: rows whose gradient is zero)
+// A product's rows, final: dw's, or dh's where its sum is not shared (gk: rows whose gradient is zero).  They leave
+// through the wave's LDS as dl does, 128 bytes of a row at once (stored straight from the accumulators, 16 bytes
+// of a row, a step of 11 rows, 155,134 items of 1536 in bf16 took 472 us, so 408; 40, 15,787 of 513 100 and 75).
 template <class Sh, int KIND>
 struct RowsEpi {
     static constexpr int DT = dtype_of(KIND);
     using Shape = Sh;
+    using T = ElemT<DT>;
     static constexpr int TQ = Sh::TQ, TR = Sh::TR;
     static constexpr bool kWalk = false, kStores = true;
-    ElemT<DT>* out;
+    T* out;
     uint64_t ld;
     uint32_t rows, D;
     const float* mul;        // scale over dl's factor
     const uint32_t* absmax;  // PLANES: of the row operand (its scale)
     const float* gk;         // nullptr: no such rows
-    bool vec;                // rows of four values are aligned
     struct Shared {
         float mul;
     };
@@ -327,8 +329,33 @@ struct RowsEpi {
     __device__ void publish(State&, Shared& sm, int tid) {
         if (tid == 0) sm.mul = *mul / (KIND == g16::PLANES ? scale_to_2p14(__builtin_bit_cast(float, *absmax)) : 1.0f);
     }
+    // 32 rows from q0, 128 bytes each from column d0
+    __device__ void put(const char* spare, const g16::Lane<Sh::NB>& ln, uint32_t q0, uint32_t d0) {
+        constexpr int E = 16 / int(sizeof(T));
+        typedef T V __attribute__((ext_vector_type(E)));
+        typedef T Vu __attribute__((ext_vector_type(E), aligned(sizeof(T))));  // (rows of any alignment)
+        const int lane = ln.hh * 32 + ln.l32;
+        asm volatile("" ::: "memory");  // the writes come first (a wave's LDS accesses execute in order)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int t = 8 * i + (lane >> 3), c = lane & 7;
+            const u32x4 w = *reinterpret_cast<const u32x4*>(spare + t * 128 + 16 * (c ^ (t & 7)));
+            const V v = __builtin_bit_cast(V, w);
+            const uint32_t d = d0 + uint32_t(c * E);
+            if (q0 + t >= rows || d >= D) continue;
+            T* o = out + (q0 + t) * ld + d;
+            if (d + E <= D) {
+                *reinterpret_cast<Vu*>(o) = v;
+            } else {
+#pragma unroll
+                for (int e = 0; e < E - 1; ++e)
+                    if (d + e < D) o[e] = v[e];
+            }
+        }
+        asm volatile("" ::: "memory");  // and the reads before what is written next
+    }
     template <class Tile, class Settle>
-    __device__ void tile(State&, Shared& sm, const g16::Lane<Sh::NB>& ln, f32x16 (&acc)[2][Sh::NB], const Tile& t, char*, Settle settle) {
+    __device__ void tile(State&, Shared& sm, const g16::Lane<Sh::NB>& ln, f32x16 (&acc)[2][Sh::NB], const Tile& t, char* spare, Settle settle) {
         bool none[Sh::NB];
 #pragma unroll
         for (int n = 0; n < Sh::NB; ++n) {
@@ -337,28 +364,27 @@ struct RowsEpi {
         }
         settle();
         const float s = sm.mul;
+        const uint32_t d0 = t.rb * TR + uint32_t(ln.wr * 64);
+        if (d0 >= D) return;
 #pragma unroll
         for (int n = 0; n < Sh::NB; ++n) {
-            const uint32_t q = t.qb * TQ + uint32_t(ln.q(n));
-            if (q >= rows) continue;
-            ElemT<DT>* o = out + q * ld;
+            const uint32_t q0 = t.qb * TQ + uint32_t(ln.wq * 32 * Sh::NB + 32 * n);
+            if (q0 >= rows) break;
 #pragma unroll
-            for (int m = 0; m < 2; ++m)
+            for (int m = 0; m < 2; ++m) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const uint32_t d = t.rb * TR + uint32_t(ln.r(m, j));
-                    if (d >= D) continue;
-                    struct alignas(4 * sizeof(ElemT<DT>)) V4 {
-                        ElemT<DT> v[4];
+                    struct alignas(4 * sizeof(T)) V4 {
+                        T v[4];
                     } v;
 #pragma unroll
                     for (int e = 0; e < 4; ++e) v.v[e] = Elem<DT>::from_f(none[n] ? 0.0f : acc[m][n][4 * j + e] * s);
-                    if (vec && d + 4 <= D) *reinterpret_cast<V4*>(o + d) = v;
-                    else
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            if (d + e < D) o[d + e] = v.v[e];
+                    const int c = sizeof(T) == 4 ? 2 * j + ln.hh : 4 * m + j;  // the four values' chunk of the row
+                    *reinterpret_cast<V4*>(spare + ln.l32 * 128 + 16 * (c ^ (ln.l32 & 7)) + (sizeof(T) == 4 ? 0 : 8 * ln.hh)) = v;
                 }
+                if (sizeof(T) == 4) put(spare, ln, q0, d0 + 32 * m);
+            }
+            if (sizeof(T) == 2) put(spare, ln, q0, d0);
         }
     }
     template <class Tile>
@@ -498,7 +524,7 @@ va_status va_xent_backward(va_context* ctx, const va_xent_desc* d, const float* 
     auto rows_out = [&](auto sh, auto k, auto qk, const g16::Args& b, uintptr_t o, uint64_t ld, uint32_t rows, const uint32_t* top, const float* zero) {
         constexpr int kKind = decltype(k)::value;
         using E = ElemT<dtype_of(kKind)>;
-        const RowsEpi<decltype(sh), kKind> e{reinterpret_cast<E*>(o), ld, rows, D, mul, top, zero, o % (4 * sizeof(E)) == 0 && ld % 4 == 0};
+        const RowsEpi<decltype(sh), kKind> e{reinterpret_cast<E*>(o), ld, rows, D, mul, top, zero};
         return g16::launch<kKind, decltype(qk)::value, true>(ctx, b, e);
     };
     auto sum_shares = [&](const float* from, uint32_t parts, uint32_t rows, const float* zero, const uint32_t* top, uintptr_t o, uint64_t ld) {
