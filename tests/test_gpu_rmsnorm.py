@@ -95,6 +95,35 @@ def test_given_scale_saturates(ctx, D, code, dtype):
     assert ((got - val).abs() <= step + 1e-5 * val.abs())[inside].all()
 
 
+@pytest.mark.parametrize("code", [torch.int8, torch.float8_e4m3fn])
+@pytest.mark.parametrize("group", [0, 32])
+@pytest.mark.parametrize("D", [64, 8300])
+def test_tiny_scales(ctx, D, group, code):
+    """Scales below 2^-128, whose reciprocals are no fp32 values: zeros stay zeros, the others keep their codes."""
+    from vectoraccelerate_amd import RMSNormKernel
+
+    g = torch.Generator().manual_seed(D + group)
+    x = torch.randn(3, D, generator=g) * 2e-37
+    x[:, ::5] = 0.0
+    w = torch.full((D,), 1e-4)
+    codes, scales, _ = RMSNormKernel(ctx).quantize(x.cuda(), w.cuda(), None, code, group, None, EPS)
+    _, _, yy, e = oracle.rms(x.cuda(), None, w.cuda(), EPS)
+    most = 127.0 if code == torch.int8 else 448.0
+    size = group or D
+    groups = -(-D // size)
+    z = torch.nn.functional.pad(yy, (0, groups * size - D)).view(3, groups, size)
+    want = z.abs().amax(2) / most
+    assert (want < 2.0**-128).all() and (want > 2.0**-140).all()
+    # y and the scale are fp32 values below its normal ones: half of 2^-149 on top of the usual errors
+    oracle.close(scales, want, (e + 2 * U32) * want + 2.0**-149, "scales")
+    val = (z / want.unsqueeze(2)).view(3, -1)[:, :D]
+    off = (2.0**-148 / want).repeat_interleave(size, 1)[:, :D]
+    got = codes.cpu().float().double()
+    assert torch.isfinite(got).all() and (got[:, ::5] == 0).all()
+    step = torch.full_like(val, 0.5) if code == torch.int8 else torch.maximum(val.abs() * 2.0**-4, torch.tensor(2.0**-10))
+    assert ((got - val).abs() <= step + (2 * e + 8 * U32 + off) * val.abs() + off).all()
+
+
 @pytest.mark.parametrize("code", [None, torch.int8, torch.float8_e4m3fn])
 @pytest.mark.parametrize("D", [40, 3000, 9000])
 def test_non_finite_rows_stay_alone(ctx, D, code):

@@ -250,7 +250,9 @@ __global__ __launch_bounds__(256) void rms_norm_kernel(RmsArgs a) {
                 sc = m / most;
                 if (d < D && d % a.group == 0) a.scales[uint64_t(t) * a.groups + d / a.group] = sc;
             }
-            store_codes(o, d, D, codes8(y, sc == 0.0f ? 0.0f : 1.0f / sc, fp8));
+            // (a tiny scale's reciprocal would overflow: both are raised by a power of two)
+            const float up = sc < 0x1p-100f ? 0x1p64f : 1.0f;
+            store_codes(o, d, D, codes8(y * up, sc == 0.0f ? 0.0f : 1.0f / (sc * up), fp8));
         };
         if constexpr (C > 0) {
             const bool have = a.group == 0 && !(a.given > 0.0f);  // r holds y

@@ -64,7 +64,7 @@ def _rows(t, name: str, device: int, dtype=None, shape=None) -> tuple[int, int]:
     if sd != 1 and dim > 1:
         raise VectorError.invalidInput(f"{name}: the values of a row must be contiguous")
     if rows < 2:
-        return t.data_ptr(), max(sr, dim)
+        return t.data_ptr(), dim  # (one row has no stride, whatever the tensor's view says)
     if sr < dim:
         raise VectorError.invalidInput(f"{name}: rows overlap")
     return t.data_ptr(), sr
