@@ -385,3 +385,12 @@ def test_large_tiles_of_planes(ctx, T, V, D):
     off[torch.rand(V, generator=g) < 0.05] = -torch.inf
     _check(ctx, h, w, y)
     _check(ctx, h, w, y, scale=0.7, offsets=off.cuda())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_one_row_of_any_stride(ctx, dtype):
+    """The stride of a single row is never walked: a view whose stride passes every limit is a row like any other."""
+    h, w, y, _ = _inputs(1, 300, 96, dtype, 5)
+    apart = h.as_strided((1, 96), (1 << 40, 1))
+    _check(ctx, apart, w, y)
+    _check(ctx, h.expand(1, 96).as_strided((1, 96), (0, 1)), w, y)
