@@ -119,17 +119,34 @@ __global__ __launch_bounds__(256) void planes_kernel(Planes a, Planes b, uint32_
     for (uint32_t k = 1024 + 4 * lane; k < Kp; k += 256) put(k, load4(k));
 }
 
-// *odd = 1 (0 before the launch) if a masked item holds NaN or inf, or if an offset is finite and beyond
-// 1e37 (log2 e times it may not be).  One wave per 64 items; masked rows are read.
+// *odd = 1 (0 before the launch) if a masked item holds a value of magnitude `most` or more (bits; NaN and inf are), if
+// an offset is finite and beyond 1e37 (log2 e times it may not be), or if a hidden value from `wide` to inf is among
+// `hidden` (or nullptr).  One wave per 64 items, whose masked rows are read; then the workgroups behind the first
+// `blocks`, a wave a hidden row in turn.
 template <class U>
 __global__ __launch_bounds__(256) void xent_odd_kernel(const U* __restrict__ items, uint64_t ld, const float* __restrict__ offsets, uint32_t V,
-                                                       uint32_t D, U exponent, uint32_t* odd) {
-    const uint32_t lane = threadIdx.x & 63, j0 = (blockIdx.x * 4 + (threadIdx.x >> 6)) * 64;
-    const float o = j0 + lane < V ? offsets[j0 + lane] : 0.0f;
-    bool bad = fabsf(o) > 1e37f && fabsf(o) < INFINITY;
-    for (uint64_t masked = __ballot(o == -INFINITY); masked; masked &= masked - 1) {
-        const U* row = items + (j0 + uint32_t(__builtin_ctzll(masked))) * ld;
-        for (uint32_t d = lane; d < D; d += 64) bad |= (row[d] & exponent) == exponent;
+                                                       uint32_t D, U most, uint32_t blocks, const U* __restrict__ hidden, uint64_t ldh, uint32_t T,
+                                                       U wide, U inf, uint32_t* odd) {
+    constexpr U kSign = U(U(1) << (8 * sizeof(U) - 1));
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    bool bad = false;
+    if (blockIdx.x < blocks) {
+        const uint32_t j0 = (blockIdx.x * 4 + wave) * 64;
+        const float o = j0 + lane < V ? offsets[j0 + lane] : 0.0f;
+        bad = fabsf(o) > 1e37f && fabsf(o) < INFINITY;
+        for (uint64_t masked = __ballot(o == -INFINITY); masked; masked &= masked - 1) {
+            const U* row = items + (j0 + uint32_t(__builtin_ctzll(masked))) * ld;
+            for (uint32_t d = lane; d < D; d += 64) bad |= U(row[d] & U(~kSign)) >= most;
+        }
+    } else {
+        for (uint32_t t = (blockIdx.x - blocks) * 4 + wave; t < T; t += (gridDim.x - blocks) * 4) {
+            const U* row = hidden + t * ldh;
+#pragma unroll 4
+            for (uint32_t d = lane; d < D; d += 64) {
+                const U v = U(row[d] & U(~kSign));
+                bad |= v >= wide && v <= inf;
+            }
+        }
     }
     if (__any(bad) && lane == 0) *odd = 1;
 }
@@ -367,12 +384,22 @@ va_status make_planes(va_context* ctx, uint32_t D, Planes a, Planes b) {
 }
 
 va_status find_odd(va_context* ctx, const va_xent_desc* d, uint32_t* odd) {
-    const dim3 grid(ceil_div(d->num_items, 256));
-    if (d->dtype == VA_DTYPE_F32)
-        xent_odd_kernel<uint32_t><<<grid, dim3(256), 0, ctx->stream>>>(static_cast<const uint32_t*>(d->items), d->items_stride, d->offsets, d->num_items, d->dim, 0x7F800000u, odd);
-    else
-        xent_odd_kernel<uint16_t><<<grid, dim3(256), 0, ctx->stream>>>(static_cast<const uint16_t*>(d->items), d->items_stride, d->offsets, d->num_items, d->dim,
-                                                                       d->dtype == VA_DTYPE_F16 ? uint16_t(0x7C00) : uint16_t(0x7F80), odd);
+    const uint32_t blocks = ceil_div(d->num_items, 256);
+    if (d->dtype == VA_DTYPE_F32) {
+        xent_odd_kernel<uint32_t><<<dim3(blocks), dim3(256), 0, ctx->stream>>>(static_cast<const uint32_t*>(d->items), d->items_stride, d->offsets, d->num_items,
+                                                                               d->dim, 0x7F800000u, blocks, nullptr, 0, 0, 0u, 0u, odd);
+    } else {
+        // A masked bf16 item's finite values may overflow its logits, which an offset of -inf then turns into NaN.  Items
+        // below 2^64 and hidden values below 2^46 cannot: 2^16 products (VA_XENT_MAX_DIM) of less than 2^110 each.  Nor
+        // can fp16's, 2^16 products of 2^32.
+        static_assert(VA_XENT_MAX_DIM <= 1u << 16, "the bound on a logit's sum");
+        const bool bf16 = d->dtype == VA_DTYPE_BF16;
+        const uint16_t most = bf16 ? (127 + 64) << 7 : 0x7C00, wide = (127 + 46) << 7, inf = 0x7F80;
+        const uint32_t more = bf16 ? std::min(ceil_div(d->rows, 4), 1024u) : 0u;
+        xent_odd_kernel<uint16_t><<<dim3(blocks + more), dim3(256), 0, ctx->stream>>>(static_cast<const uint16_t*>(d->items), d->items_stride, d->offsets,
+                                                                                      d->num_items, d->dim, most, blocks, static_cast<const uint16_t*>(d->hidden),
+                                                                                      d->hidden_stride, d->rows, wide, inf, odd);
+    }
     VA_CHECK_LAUNCH(ctx);
     return VA_OK;
 }

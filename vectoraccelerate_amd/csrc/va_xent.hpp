@@ -81,7 +81,7 @@ enum Offsets : int { OFF_NONE = 0, OFF_EDGE = 1, OFF_ANY = 2 };
 
 struct LogitArgs {
     const float* offsets;  // of the launch's first item (nullptr: zeros)
-    const uint32_t* odd;   // OFF_ANY: zero if no masked item holds NaN or inf and no offset is near fp32's
+    const uint32_t* odd;   // OFF_ANY: zero if no masked item's logit can be NaN or inf and no offset is near fp32's
                            // limits (nullptr: not known)
     const float* qinv;     // fp32 operands: the rows' and the items' inverse scales
     const float* xinv;
@@ -192,7 +192,8 @@ struct Planes {
 };
 // Of one matrix, or of two in one launch (b.R = 0: none).
 va_status make_planes(va_context* ctx, uint32_t D, Planes a, Planes b = {});
-// *odd = 1 (0 before) if a masked item holds NaN or inf, or an offset is finite and near fp32's limits
+// *odd = 1 (0 before) if a masked item holds NaN, inf or values whose products with the hidden rows may overflow, or an
+// offset is finite and near fp32's limits
 va_status find_odd(va_context* ctx, const va_xent_desc* d, uint32_t* odd);
 
 va_status check_desc(va_context* ctx, const va_xent_desc* d, const char* who);
