@@ -469,7 +469,7 @@ va_status va_probe_mfma(va_context* ctx, va_probe_kind kind, int random_operands
  * collection, the norm and 8-bit coding of an encoder's output, and the clipping of its gradients.
  * Device pointers and the context's stream as everywhere; nothing here waits on the host except to
  * grow the scratch arena.  Rows are row-major with a stride in elements; sums, softmax statistics
- * and norms are fp32 or wider whatever the type. */
+ * and norms are fp32 or wider whatever the type (what is rounded to fewer bits is said below). */
 typedef enum { VA_DTYPE_F32 = 0, VA_DTYPE_F16 = 1, VA_DTYPE_BF16 = 2 } va_dtype;
 typedef enum { VA_REDUCE_MEAN = 0, VA_REDUCE_SUM = 1, VA_REDUCE_NONE = 2 } va_reduction;
 
@@ -482,7 +482,12 @@ typedef enum { VA_REDUCE_MEAN = 0, VA_REDUCE_SUM = 1, VA_REDUCE_NONE = 2 } va_re
  *    that are deleted, which have probability and gradient 0 whatever their vector holds.  With
  *    every item masked, lse is -inf and losses and gradients are 0.  A masked target's loss is +inf.
  *  - a row whose target is ignore_index has loss 0 and gradient 0; a target outside
- *    [0, num_items) gives that row a NaN loss and gradient 0. */
+ *    [0, num_items) gives that row a NaN loss and gradient 0.
+ *  - fp32: for more than 32 rows (64 over 65,536 items and more) each value enters the logits as two fp16
+ *    values, exact to 2^-22 of it or to 2^-39 of the largest of its row, whichever is more; few rows are
+ *    multiplied as fp32, and the gradients' sums always have fp32's digits and range.
+ *  - fp16, bf16: the logits' gradients dl are rounded once to the type before they are summed into those of the
+ *    rows and items; in fp16 those below 2^-38 of the largest row gradient are zero. */
 typedef struct {
     const void* hidden;      /* [rows x dim] */
     const void* items;       /* [num_items x dim] */

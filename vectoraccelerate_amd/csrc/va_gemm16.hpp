@@ -24,13 +24,18 @@
 // Eight waves of 128 x 64 reach 1.30 and 1.05, four of 128 x 128 1.20 and 0.88, slots of half a stage 1.13
 // and 0.97: MFMA busy times clock is nearly the same for all.
 //
-// fp32 operands come in two ways.  As they are, on v_mfma_f32_32x32x2: a fragment's 16 bytes are four k-values
+// fp32 operands come in three ways.  F32: as they are, on v_mfma_f32_32x32x2: a fragment's 16 bytes are four k-values
 // instead of eight, everything else is alike; a sixteenth of the 16-bit rate, which is enough while the
-// operands' bytes are what takes the time.  Or as two fp16 planes (value = (hi + lo) 2^-e with one
-// exponent a row or tensor): a product is then hi hi + hi lo + lo hi, into the same accumulators.  The planes
+// operands' bytes are what takes the time.  PLANES: as two fp16 planes (value = (hi + lo) 2^-e with one
+// exponent a row): a product is then hi hi + hi lo + lo hi, into the same accumulators.  The planes
 // alternate in memory, 16 values of hi and the same 16 of lo, so a stage holds both of 32 values and each
-// fragment is read once for its two products.  lo lo is below 2^-22 of the product and is left out; what
-// remains is exact to about 2^-22 a term, the same as an fp32 fma chain of a few terms.
+// fragment is read once for its two products.  lo lo is below 2^-22 of the product and is left out; a value is exact to
+// 2^-22 of it, or, where that is more, to 2^-39 of its row's largest: fp32's exactness for rows whose values are
+// within 17 binary orders of each other, and not its range.  So planes are for sums over a row's values alone.
+// SPLIT: as they are in memory and LDS, and split in the fragments into three bf16 values, which have fp32's range and
+// together all its digits; six products of 16-bit rate.  For the sums across rows, whose terms may be of any size.
+// Loss and gradients of 4096 x 20,000 x 768 with these sums in SPLIT 2.29 ms, in F32 2.78; 100 x 10,000 x 768
+// 118 and 137 us.
 #pragma once
 
 #include <algorithm>
@@ -52,7 +57,7 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 constexpr int ROWB = 128;  // bytes of an LDS row (k along the rows)
 
 // What the operands are made of.
-enum Kind : int { F16 = 0, BF16 = 1, PLANES = 2, F32 = 3 };
+enum Kind : int { F16 = 0, BF16 = 1, PLANES = 2, F32 = 3, SPLIT = 4 };
 constexpr int size_of(int kind) { return kind >= PLANES ? 4 : 2; }  // bytes of a value in memory
 constexpr int stage_of(int kind) { return ROWB / size_of(kind); }     // k-values of a stage
 
@@ -151,6 +156,24 @@ struct Tiles {
     }
 };
 
+// Eight fp32 values of a fragment as three bf16 ones each, v = o[0] + o[1] + o[2] exactly: the upper 8 binary digits cut off
+// (a rounding could overflow), the next 8 rounded, the rest.
+__device__ __forceinline__ void split3(const u32x4 (&v)[2], u32x4 (&o)[3]) {
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    const auto as_f = [](uint32_t b) { return __builtin_bit_cast(float, b); };
+    const auto pack = [](float a, float b) { return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, bf16x2)); };
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t a = v[i >> 1][2 * i & 3], b = v[i >> 1][(2 * i + 1) & 3];
+        o[0][i] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+        const float ra = as_f(a) - as_f(a & 0xFFFF0000u), rb = as_f(b) - as_f(b & 0xFFFF0000u);
+        const uint32_t mid = pack(ra, rb);
+        o[1][i] = mid;
+        o[2][i] = pack(ra - as_f(mid << 16), rb - as_f(mid & 0xFFFF0000u));
+    }
+}
+
 template <int KIND>
 __device__ __forceinline__ f32x16 mfma(u32x4 x, u32x4 q, f32x16 c) {
     if constexpr (KIND == F32) {
@@ -158,7 +181,7 @@ __device__ __forceinline__ f32x16 mfma(u32x4 x, u32x4 q, f32x16 c) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(__builtin_bit_cast(f32x4, x)[e], __builtin_bit_cast(f32x4, q)[e], c, 0, 0, 0);
         return c;
-    } else if constexpr (KIND == BF16) {
+    } else if constexpr (KIND == BF16 || KIND == SPLIT) {
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, q), c, 0, 0, 0);
     } else {
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, x), __builtin_bit_cast(f16x8, q), c, 0, 0, 0);
@@ -177,11 +200,10 @@ struct Lane {
 // KM: stored across k (N = 2).
 template <bool KM, int KIND, int W, int WAVES, int N = 2>
 struct Feed {
-    static_assert(N == 2 || !KM, "narrow waves only along k");
-    static constexpr int ES = KIND == F32 ? 4 : 2, KV = stage_of(KIND);  // bytes of a value in LDS
+    static_assert((N == 2 && KIND != PLANES) || !KM, "narrow waves and planes only along k");
+    static constexpr int ES = KIND >= F32 ? 4 : 2, KV = stage_of(KIND);  // bytes of a value in LDS
     static constexpr int LPW = 4 * N * W / WAVES;   // 1 KiB direct loads per wave and stage
-    static constexpr int KROW = 64 * ES * W;        // bytes of a k-row of one plane (KM)
-    static constexpr int KMEM = 64 * size_of(KIND) * W;  // of the columns of a tile in memory
+    static constexpr int KROW = 64 * ES * W;        // bytes of a k-row, the columns of a tile (KM)
     // the place of a k-row's 16-byte chunk c: 16-bit values, its segment (four chunks) xored by k; fp32, its half
     // of 256 bytes by bit 2 of k (the two k-rows that a fragment reads at once are four apart)
     static __device__ uint32_t placed(uint32_t k, uint32_t c) {
@@ -218,9 +240,7 @@ struct Feed {
                 const uint32_t byte = uint32_t(1024 * (wave + WAVES * i) + 16 * lane);
                 const uint32_t k = byte / KROW, c = byte % KROW / 16;
                 const uint32_t at_c = placed(k, c);
-                // PLANES: 16 k-rows of hi, the same of lo, and so on
-                if constexpr (KIND == PLANES) voff[i] = ((k >> 5) * 16u + (k & 15u)) * pitch + (at_c >> 1) * 64u + ((k >> 4) & 1u) * 32u + (at_c & 1u) * 16u;
-                else voff[i] = k * pitch + 16u * at_c;
+                voff[i] = k * pitch + 16u * at_c;
             }
             const int e = (lane & 15) >> 2;
 #pragma unroll
@@ -244,8 +264,8 @@ struct Feed {
     // the operand's block b of 32 N W queries (rows)
     __device__ void open(const Operand& o, uint32_t b) {
         if constexpr (KM) {
-            base = p + uint64_t(b) * uint32_t(KMEM);
-            left = uint64_t(o.rows - 1) * pitch + o.width - uint64_t(b) * uint32_t(KMEM);
+            base = p + uint64_t(b) * uint32_t(KROW);
+            left = uint64_t(o.rows - 1) * pitch + o.width - uint64_t(b) * uint32_t(KROW);
         } else {
             base = p + uint64_t(b) * (32u * N * W) * pitch;
             records = (min(32u * N * W, o.rows - b * (32u * N * W)) - 1u) * pitch + o.width;
@@ -362,7 +382,7 @@ __global__ __launch_bounds__(Epi::Shape::THREADS, Epi::Shape::PER_SIMD) void gem
     };
 
     f32x16 acc[2][NB];
-    constexpr int BUFS = KIND == PLANES ? 3 : 2;
+    constexpr int BUFS = KIND == PLANES ? 3 : 2;  // (SPLIT: the two halves of a k-step)
     u32x4 fx[BUFS][2], fq[BUFS][NB];
     auto read_one = [&](int buf, uint32_t slot, int t, int i) {
         const char* base = mine + slot * STAGE;
@@ -424,6 +444,35 @@ __global__ __launch_bounds__(Epi::Shape::THREADS, Epi::Shape::PER_SIMD) void gem
             __builtin_amdgcn_sched_barrier(0);
         }
     };
+    // The same of fp32 values split into three bf16 ones: k-steps of 16 values, two fragments as they lie in LDS (any 16
+    // values of k will do, as long as both operands' are the same).  Six of the nine products: the others are below
+    // 2^-21 of the value, 2^-25 as a rule.  The fragments are split first, then the next ones read into their place.
+    auto step_split = [&](uint32_t slot_next, int t_next, auto more, uint32_t s_load, uint32_t slot_load) {
+        static_assert(KIND != SPLIT || XK, "k does not end within a stage");
+        u32x4 px[2][3], pq[NB][3];
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+            const u32x4 v[2] = {fx[0][m], fx[1][m]};
+            split3(v, px[m]);
+        }
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+            const u32x4 v[2] = {fq[0][n], fq[1][n]};
+            split3(v, pq[n]);
+        }
+#pragma unroll
+        for (int i = 0; i < 2 * (2 + NB); ++i) read_one(i / (2 + NB), slot_next, t_next + i / (2 + NB), i % (2 + NB));
+        constexpr int PX[6] = {2, 0, 1, 1, 0, 0}, PQ[6] = {0, 2, 1, 0, 1, 0};  // the smallest products first
+#pragma unroll
+        for (int p = 0; p < 6; ++p) {
+#pragma unroll
+            for (int i = 0; i < 2 * NB; ++i) acc[i & 1][i >> 1] = mfma<KIND>(px[i & 1][PX[p]], pq[i >> 1][PQ[p]], acc[i & 1][i >> 1]);
+            if constexpr (decltype(more)::value) {
+#pragma unroll
+                for (int l = p * (LQ + LX) / 6; l < (p + 1) * (LQ + LX) / 6; ++l) issue_one(s_load, slot_load, l);
+            }
+        }
+    };
     // a workgroup barrier that leaves the direct loads in flight; this wave's LDS reads are done
     auto barrier = [&]() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
     // waits for all but the youngest `stages` stages of direct loads
@@ -443,6 +492,8 @@ __global__ __launch_bounds__(Epi::Shape::THREADS, Epi::Shape::PER_SIMD) void gem
             step_planes(std::integral_constant<int, 0>(), slot, none, 0, 0);
             step_planes(std::integral_constant<int, 1>(), slot, none, 0, 0);
             step_planes(std::integral_constant<int, 2>(), slot, none, 0, 0);
+        } else if constexpr (KIND == SPLIT) {
+            step_split(slot, 2, none, 0, 0);
         } else {
 #pragma unroll
             for (int t = 0; t < 3; ++t) step(t & 1, slot, t + 1, none, 0, 0, ends && !decltype(more)::value);
@@ -453,6 +504,7 @@ __global__ __launch_bounds__(Epi::Shape::THREADS, Epi::Shape::PER_SIMD) void gem
         barrier();
         __builtin_amdgcn_sched_barrier(0);
         if constexpr (KIND == PLANES) step_planes(std::integral_constant<int, 3>(), (slot + 1) & (SLOTS - 1), more, s0 + i + SLOTS, slot);
+        else if constexpr (KIND == SPLIT) step_split((slot + 1) & (SLOTS - 1), 0, more, s0 + i + SLOTS, slot);
         else step(1, (slot + 1) & (SLOTS - 1), 0, more, s0 + i + SLOTS, slot, ends);
     };
 
@@ -485,7 +537,7 @@ __global__ __launch_bounds__(Epi::Shape::THREADS, Epi::Shape::PER_SIMD) void gem
             barrier();
         }
 #pragma unroll
-        for (int i = 0; i < 2 + NB; ++i) read_one(0, 0, 0, i);
+        for (int i = 0; i < (KIND == SPLIT ? 2 : 1) * (2 + NB); ++i) read_one(i / (2 + NB), 0, i / (2 + NB), i % (2 + NB));
         uint32_t i = 0;
         for (; i + SLOTS < todo; ++i) stage(i, todo, std::true_type(), false);
         for (; i < todo; ++i) stage(i, todo, std::false_type(), !XK && a.tail && s0 + i + 1 == total_stages);

@@ -14,8 +14,11 @@
 // Precision: fp16 / bf16 operands enter the matrix cores as they are, sums are fp32.  dl is rounded
 // once to the operands' type for the second products (relative 2^-11 / 2^-8 a value, like the
 // rounding of the result), after a scale that takes the largest |g| to 2^14: fp16's range then holds
-// probabilities down to 2^-38 of it, and with one g for all rows the target's -g is exact.  fp32 operands, and dl with them, are
-// multiplied as fp32 for few rows and as two fp16 planes for many (va_gemm16.hpp).
+// probabilities down to 2^-38 of it, and with one g for all rows the target's -g is exact.  What falls below would
+// be below fp16's smallest gradient too, unless the largest is near its end: dl w scale of the largest |g| is at most
+// 2^16, what is lost of it 2^-39, fp16's step 2^-24.  fp32 operands are
+// multiplied as fp32 for few rows; for many, in the logits as two fp16 planes of each row, and in the second
+// products split into three bf16 values (va_gemm16.hpp), dl being fp32 in both.
 //
 // Masks: an item whose offset is -inf has no probability whatever its vector holds (NaN and inf
 // included) and gets a zero gradient; a row without a target has loss 0 and a zero gradient whatever
@@ -60,8 +63,7 @@ __global__ __launch_bounds__(256) void copy_kernel(const U* __restrict__ src, ui
 }
 
 // One wave per fp32 row: its planes dst[r] (16 values of hi, the same of lo, and so on; Kp values, zeros past D), scaled by the
-// power of two that puts the row's largest entry, or the tensor's (absmax), near 2^14; inv[r] = the
-// inverse.  Dropped rows are zeros.
+// power of two that puts the row's largest entry near 2^14; inv[r] = the inverse.  Dropped rows are zeros.
 // Rows of `a` in the first na workgroups, then of `b`.
 __global__ __launch_bounds__(256) void planes_kernel(Planes a, Planes b, uint32_t na, uint32_t D, uint32_t Kp) {
     typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
@@ -72,7 +74,6 @@ __global__ __launch_bounds__(256) void planes_kernel(Planes a, Planes b, uint32_
     const float* s = static_cast<const float*>(second ? b.src : a.src) + r * (second ? b.ld : a.ld);
     const float* drop = second ? b.drop.value : a.drop.value;
     const bool none = drop && drop[r] == (second ? b.drop.is : a.drop.is);
-    const uint32_t* absmax = second ? b.absmax : a.absmax;
     auto load4 = [&](uint32_t k) {
         f32x4 v{0.0f, 0.0f, 0.0f, 0.0f};
         if (none) return v;
@@ -85,22 +86,17 @@ __global__ __launch_bounds__(256) void planes_kernel(Planes a, Planes b, uint32_
     f32x4 held[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) held[i] = load4(256 * i + 4 * lane);
-    float sc;
-    if (absmax) {
-        sc = scale_to_2p14(__builtin_bit_cast(float, *absmax));
-    } else {
-        float m = 0.0f;
+    float m = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) m = fmaxf(m, fabsf(held[i][e]));
-        for (uint32_t k = 1024 + 4 * lane; k < D; k += 256) {
-            const f32x4 v = load4(k);
+        for (int e = 0; e < 4; ++e) m = fmaxf(m, fabsf(held[i][e]));
+    for (uint32_t k = 1024 + 4 * lane; k < D; k += 256) {
+        const f32x4 v = load4(k);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) m = fmaxf(m, fabsf(v[e]));
-        }
-        sc = scale_to_2p14(wave_max(m));
+        for (int e = 0; e < 4; ++e) m = fmaxf(m, fabsf(v[e]));
     }
+    const float sc = scale_to_2p14(wave_max(m));
     if (lane == 0) (second ? b.inv : a.inv)[r] = 1.0f / sc;
     uint16_t* o = static_cast<uint16_t*>(second ? b.dst : a.dst) + uint64_t(r) * 2 * Kp;
     auto put = [&](uint32_t k, f32x4 v) {
@@ -356,7 +352,7 @@ va_status make_copy(va_context* ctx, int kind, const void* src, uint64_t ld, uin
     const uint32_t bytes = copy_bytes(kind, D);
     const uint64_t n = uint64_t(R) * (bytes / 16);
     const dim3 grid(uint32_t(std::min<uint64_t>((n + 255) / 256, 16384)));
-    if (kind == g16::F32)
+    if (kind >= g16::F32)
         copy_kernel<uint32_t><<<grid, dim3(256), 0, ctx->stream>>>(static_cast<const uint32_t*>(src), ld, D, bytes / 4, drop, run_if, static_cast<uint32_t*>(dst), n);
     else
         copy_kernel<uint16_t><<<grid, dim3(256), 0, ctx->stream>>>(static_cast<const uint16_t*>(src), ld, D, bytes / 2, drop, run_if, static_cast<uint16_t*>(dst), n);
@@ -480,8 +476,8 @@ va_status va_xent_forward(va_context* ctx, const va_xent_desc* d, float* out_los
         const uint32_t v0 = c * piece, n = std::min(piece, V - v0);
         const char* items = row_at(d->items, d->items_stride, v0, dt);
         if (planes)
-            VA_CHECK_STATUS(make_planes(ctx, D, Planes{d->hidden, d->hidden_stride, c ? 0 : T, nullptr, Drop{}, qp, qinv},
-                                        Planes{items, d->items_stride, n, nullptr, Drop{}, xp, xinv}));
+            VA_CHECK_STATUS(make_planes(ctx, D, Planes{d->hidden, d->hidden_stride, c ? 0 : T, Drop{}, qp, qinv},
+                                        Planes{items, d->items_stride, n, Drop{}, xp, xinv}));
         else if (!xd)
             VA_CHECK_STATUS(make_copy(ctx, kind, items, d->items_stride, n, D, Drop{}, xp));
         g16::Args a;

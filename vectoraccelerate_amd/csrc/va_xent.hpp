@@ -162,9 +162,10 @@ inline g16::Operand copied(int kind, const void* p, uint32_t rows, uint32_t D) {
 }
 
 // fp32 operands as they are or as planes.  Planes cost passes over the items that write copies
-// (36 bytes a value of a training step, where fp32 as it is takes 16), and save
-// 9/10 of the matrix cores' time: they win as soon as that counts.  Loss and gradients, as it is and in planes: 10 x 5000 x
-// 512 56 and 74 us, 30 x 100,000 x 384 212 and 331, 48 x 100,000 x 768 566 and 677; 60 x 30,000 x 512 174 and 156.
+// (32 bytes a value of a training step, where fp32 as it is takes 16), and with the second products in SPLIT save
+// 7/10 of the matrix cores' time: they win as soon as that counts.  Loss and gradients, as it is and in planes: 10 x 5000 x
+// 512 56 and 75 us, 30 x 100,000 x 384 194 and 291, 48 x 100,000 x 768 546 and 614; 60 x 30,000 x 512 170 and 144,
+// 33 x 5000 x 512 84 and 82.
 inline int kind_of(va_dtype dt, uint32_t rows, uint32_t items) {
     if (dt == VA_DTYPE_F16) return g16::F16;
     if (dt == VA_DTYPE_BF16) return g16::BF16;
@@ -179,13 +180,12 @@ struct Drop {
 // A copy of R rows as `kind` (not PLANES) wants them; nothing where *run_if is zero.
 va_status make_copy(va_context* ctx, int kind, const void* src, uint64_t ld, uint32_t R, uint32_t D, Drop drop, void* dst,
                     const uint32_t* run_if = nullptr);
-// The planes of R fp32 rows: scaled by the power of two that puts the row's largest entry, or the tensor's
-// (absmax), near 2^14, and its inverse to inv[row].
+// The planes of R fp32 rows: scaled by the power of two that puts the row's largest entry near 2^14, and its
+// inverse to inv[row].
 struct Planes {
     const void* src = nullptr;
     uint64_t ld = 0;
     uint32_t R = 0;
-    const uint32_t* absmax = nullptr;
     Drop drop;
     void* dst = nullptr;
     float* inv = nullptr;
@@ -220,7 +220,7 @@ using SlicedNarrow = g16::Shape<1, 1, 1, 2, 4>;
 enum ShapeId : int { LARGE = 0, MEDIUM = 1, SMALL = 2, NARROW = 3, DEEP_MEDIUM = 4, DEEP_SMALL = 5, SLICED = 6, SLICED_NARROW = 7 };
 template <int KIND, class F>
 va_status by_shape(int shape, F&& f) {
-    if constexpr (KIND != g16::PLANES)
+    if constexpr (KIND != g16::PLANES && KIND != g16::SPLIT)
         if (shape == LARGE) return f(g16::Large());
     switch (shape) {
         case MEDIUM: return f(Medium());
@@ -271,7 +271,7 @@ inline Blocks blocks_for(const va_context* ctx, int kind, uint64_t Q, uint64_t R
     const double round[4] = {1.0, 0.56, 0.5, 0.5};
     int best = -1;
     double least = 0.0;
-    for (int i = narrow ? 3 : kind == g16::PLANES && !stages ? 1 : 0; i < (narrow ? 4 : 3); ++i) {
+    for (int i = narrow ? 3 : kind == g16::SPLIT ? 1 : 0; i < (narrow ? 4 : 3); ++i) {
         const uint64_t tiles = uint64_t(all[i].nq(Q)) * all[i].nr(R);
         all[i].parts = uint32_t(std::min<uint64_t>(std::max<uint64_t>(all[i].grid / tiles, 1), shares));
         const double t = double((tiles * all[i].parts + all[i].grid - 1) / all[i].grid) / all[i].parts * round[i];
@@ -311,11 +311,12 @@ va_status by_kind(int kind, bool offsets, bool edge, F&& f) {
     if (kind == g16::PLANES) return full(integral_constant<int, g16::PLANES>());
     return full(integral_constant<int, g16::F32>());
 }
+// f(kind) of a product with dl
 template <class F>
-va_status by_kind(int kind, F&& f) {
+va_status by_second(int kind, F&& f) {
     if (kind == g16::F16) return f(std::integral_constant<int, g16::F16>());
     if (kind == g16::BF16) return f(std::integral_constant<int, g16::BF16>());
-    if (kind == g16::PLANES) return f(std::integral_constant<int, g16::PLANES>());
+    if (kind == g16::SPLIT) return f(std::integral_constant<int, g16::SPLIT>());
     return f(std::integral_constant<int, g16::F32>());
 }
 // The element type of a kind's tensors.

@@ -1,7 +1,7 @@
 // va_xent_grad.hip — the gradient of the softmax cross entropy (va_xent.hip has the formulas).
 //
-// Launches of a call: the rows' factors and the hidden rows ended by zeros (fp32 planes: the tensors' scales
-// first), then per piece of the items the logits again with dl as their epilogue's result, dh += dl w,
+// Launches of a call: the rows' factors and the hidden rows ended by zeros, then per piece of the items (fp32 rows
+// for a product in planes: those first) the logits again with dl as their epilogue's result, dh += dl w,
 // dw = dl^T h; at the end the shares of dh summed, where there are several.  dl is bounded by
 // kGradBudget: a piece of 65,536 items for 4096 rows (pieces of 8,192 to 32,768, whose dl stays in the last
 // level cache, ran 35 to 6 % slower: each product then ends in a round of half-idle CUs).
@@ -26,7 +26,7 @@ struct PrepareArgs {
     float scale;
     float* gk;
     float* mul;
-    uint32_t* words;  // cleared: the largest |hidden| and |item|, odd offsets
+    uint32_t* odd;  // cleared
 };
 
 // gk[t] = g_t c, *mul = scale / c: g_t is the gradient that reaches the row's loss, 0 for a row without a
@@ -37,7 +37,7 @@ __global__ __launch_bounds__(256) void xent_prepare_kernel(PrepareArgs a, uint32
                                                            U* __restrict__ dst) {
     __shared__ float top[4];
     __shared__ uint32_t cnt[4];
-    if (blockIdx.x == 0 && threadIdx.x < 3) a.words[threadIdx.x] = 0;
+    if (blockIdx.x == 0 && threadIdx.x == 0) *a.odd = 0;
     float m = 0.0f;
     uint32_t c = 0;
     for (uint32_t t = threadIdx.x; t < a.T; t += 256) {
@@ -91,37 +91,8 @@ __global__ __launch_bounds__(256) void xent_prepare_kernel(PrepareArgs a, uint32
     }
 }
 
-// *absmax = the bits of the largest |src| (0 before the launch) of two matrices, `a` in the first na workgroups;
-// dropped rows are left out
-__global__ __launch_bounds__(256) void absmax_kernel(Planes a, Planes b, uint32_t na, uint32_t D, uint32_t* top) {
-    typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
-    __shared__ float part[4];
-    const bool second = blockIdx.x >= na;
-    const uint32_t R = second ? b.R : a.R, block = second ? blockIdx.x - na : blockIdx.x, blocks = second ? gridDim.x - na : na;
-    const float* src = static_cast<const float*>(second ? b.src : a.src);
-    const uint64_t ld = second ? b.ld : a.ld;
-    const Drop drop{second ? b.drop.value : a.drop.value, second ? b.drop.is : a.drop.is};
-    float m = 0.0f;
-    const int lane = threadIdx.x & 63;
-    for (uint32_t r = block * 4 + (threadIdx.x >> 6); r < R; r += blocks * 4) {
-        if (drop.value && drop.value[r] == drop.is) continue;
-        const float* s = src + r * ld;
-        const uint32_t full = D / 4 * 4;
-#pragma unroll 4
-        for (uint32_t k = 4 * lane; k < full; k += 256) {
-            const f32x4 v = *reinterpret_cast<const f32x4u*>(s + k);
-            m = fmaxf(fmaxf(m, fmaxf(fabsf(v[0]), fabsf(v[1]))), fmaxf(fabsf(v[2]), fabsf(v[3])));
-        }
-        if (full + lane < D) m = fmaxf(m, fabsf(s[full + lane]));
-    }
-    m = wave_max(m);
-    if (lane == 0) part[threadIdx.x >> 6] = m;
-    __syncthreads();
-    if (threadIdx.x == 0)
-        atomicMax(top + second, __builtin_bit_cast(uint32_t, fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]))));
-}
-
-// dl of the piece's items, p[t][j]: Vp values a row, zeros past the last item, rows `pitch` bytes apart.
+// dl of the piece's items, p[t][j]: Vp values a row in 16 bits (fp32 rows: fp32), zeros past the last item, rows `pitch`
+// bytes apart.
 template <class Sh, int KIND, int OFF>
 struct GradEpi {
     using Shape = Sh;
@@ -180,7 +151,7 @@ struct GradEpi {
         sm.lse[tid] = s.lse;
         sm.target[tid] = s.target;
     }
-    // The wave's 4 KiB of LDS hold 32 rows of 128 bytes of dl (64 items in 16 bits, 32 in fp32 or planes), 16-byte chunks
+    // The wave's 4 KiB of LDS hold 32 rows of 128 bytes of dl (64 items in 16 bits, 32 in fp32), 16-byte chunks
     // swizzled by t & 7 (the writes and the reads then touch every bank equally); whole 128-byte lines go
     // out.  (Stored straight from the accumulators, 8 bytes a lane, a tile took three times as long.)
     __device__ void put(const char* spare, const g16::Lane<Sh::NB>& ln, const uint32_t q0, uint64_t at) {
@@ -194,11 +165,6 @@ struct GradEpi {
         }
         asm volatile("" ::: "memory");  // and the reads before what is written next
     }
-    // four 16-bit values of the lane into chunk c of its row
-    static __device__ void write16(char* spare, const g16::Lane<Sh::NB>& ln, int c, const uint16_t (&v)[4]) {
-        *reinterpret_cast<uint2*>(spare + ln.l32 * 128 + 16 * (c ^ (ln.l32 & 7)) + 8 * ln.hh) =
-            make_uint2(v[0] | uint32_t(v[1]) << 16, v[2] | uint32_t(v[3]) << 16);
-    }
     // dl of the lane's 16 items of one block (m) to LDS.  TARGETS: one of the wave's rows
     // has its target among the block's items
     template <bool NATURAL, bool TARGETS>
@@ -209,26 +175,23 @@ struct GradEpi {
         for (int j = 0; j < 4; ++j) {
             const int r = ln.r(m, j);
             const f32x4 v = logits4<NATURAL, KIND, OFF, TR>(sm, acc[m][n], j, r, c);
-            uint16_t hi[4], lo[4];
+            uint16_t b[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 float d = exp_diff<NATURAL>(v[e], ref);
                 if (TARGETS && y == uint32_t(r + e) && v[e] != -INFINITY) d -= 1.0f;
                 d *= g;
-                if constexpr (KIND == g16::F32) acc[m][n][4 * j + e] = d;
-                if constexpr (KIND == g16::PLANES) split16(d, hi[e], lo[e]);
-                else if constexpr (KIND != g16::F32) hi[e] = bits16<KIND == g16::BF16>(d);
+                if constexpr (KIND >= g16::PLANES) acc[m][n][4 * j + e] = d;
+                else b[e] = bits16<KIND == g16::BF16>(d);
             }
-            if constexpr (KIND == g16::F32) {
+            if constexpr (KIND >= g16::PLANES) {
                 f32x4 d;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) d[e] = acc[m][n][4 * j + e];
                 *reinterpret_cast<f32x4*>(spare + ln.l32 * 128 + 16 * ((2 * j + ln.hh) ^ (ln.l32 & 7))) = d;
-            } else if constexpr (KIND == g16::PLANES) {
-                write16(spare, ln, 4 * (j >> 1) + (j & 1), hi);
-                write16(spare, ln, 4 * (j >> 1) + (j & 1) + 2, lo);
             } else {
-                write16(spare, ln, 4 * m + j, hi);
+                *reinterpret_cast<uint2*>(spare + ln.l32 * 128 + 16 * ((4 * m + j) ^ (ln.l32 & 7)) + 8 * ln.hh) =
+                    make_uint2(b[0] | uint32_t(b[1]) << 16, b[2] | uint32_t(b[3]) << 16);
             }
         }
     }
@@ -315,9 +278,8 @@ struct RowsEpi {
     T* out;
     uint64_t ld;
     uint32_t rows, D;
-    const float* mul;        // scale over dl's factor
-    const uint32_t* absmax;  // PLANES: of the row operand (its scale)
-    const float* gk;         // nullptr: no such rows
+    const float* mul;  // scale over dl's factor
+    const float* gk;   // nullptr: no such rows
     struct Shared {
         float mul;
     };
@@ -327,7 +289,7 @@ struct RowsEpi {
     template <class Tile>
     __device__ void load(State&, const Tile&, int) {}
     __device__ void publish(State&, Shared& sm, int tid) {
-        if (tid == 0) sm.mul = *mul / (KIND == g16::PLANES ? scale_to_2p14(__builtin_bit_cast(float, *absmax)) : 1.0f);
+        if (tid == 0) sm.mul = *mul;
     }
     // 32 rows from q0, 128 bytes each from column d0
     __device__ void put(const char* spare, const g16::Lane<Sh::NB>& ln, uint32_t q0, uint32_t d0) {
@@ -396,7 +358,7 @@ struct RowsEpi {
 template <int KIND>
 __global__ __launch_bounds__(256) void share_sum_kernel(const float* __restrict__ share, uint32_t parts, uint32_t T, uint32_t D,
                                                         uint32_t Dp, const float* __restrict__ gk, const float* __restrict__ mul,
-                                                        const uint32_t* __restrict__ absmax, ElemT<dtype_of(KIND)>* __restrict__ out, uint64_t ld) {
+                                                        ElemT<dtype_of(KIND)>* __restrict__ out, uint64_t ld) {
     __shared__ f32x4 part[4][64];
     const uint32_t per = Dp / 4, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     const uint64_t n = uint64_t(T) * per;
@@ -411,7 +373,7 @@ __global__ __launch_bounds__(256) void share_sum_kernel(const float* __restrict_
         if (!w && i < n) {
             v = (v + part[1][lane]) + (part[2][lane] + part[3][lane]);
             const uint32_t t = uint32_t(i / per), d = uint32_t(i % per) * 4;
-            const float m = *mul / (KIND == g16::PLANES ? scale_to_2p14(__builtin_bit_cast(float, *absmax)) : 1.0f);
+            const float m = *mul;
             const bool none = gk && gk[t] == 0.0f;
             for (int e = 0; e < 4 && d + e < D; ++e) out[t * ld + d + e] = Elem<dtype_of(KIND)>::from_f(none ? 0.0f : v[e] * m);
         }
@@ -451,18 +413,20 @@ va_status va_xent_backward(va_context* ctx, const va_xent_desc* d, const float* 
                "va_xent_backward: a gradient is not aligned to its type");
     DeviceGuard guard(ctx->device);
     const uint32_t T = d->rows, V = d->num_items, D = d->dim, Dp = round_up(D, 4);
-    const int kind = kind_of(dt, T, V);
+    // The logits' kind, and the second products': dl's values reach from g down to the smallest probability, and each of its
+    // columns is a sum of its own, so for fp32 rows it is fp32.  (Two fp16 planes of it would end 38 binary orders below
+    // the largest |g|: probabilities of exp(-27) of it would be zeros.)
+    const int kind = kind_of(dt, T, V), second = kind == g16::PLANES ? int(g16::SPLIT) : kind;
     const bool planes = kind == g16::PLANES, wild = wild_scale(d);
-    const uint32_t ks = uint32_t(g16::size_of(kind)), kv = uint32_t(g16::stage_of(kind));
-    const uint32_t one = copy_bytes(kind, D), tail = planes ? 0 : D * ks % g16::ROWB;
+    const uint32_t ks = uint32_t(g16::size_of(second)), kv = uint32_t(g16::stage_of(second));
+    const uint32_t row = copy_bytes(kind, D), tail = planes ? 0 : D * ks % g16::ROWB;
     // Masked items may hold anything, and dh sums over them: unless they are found to be finite, a copy is read in
     // which they are zeros.
-    const bool xd = !planes && in_dwords(dt, d->items, d->items_stride), checks = xd && d->offsets, copies = !xd || checks;
-    const uint32_t x_row = copy_bytes(kind, D);
+    const bool xd = in_dwords(dt, d->items, d->items_stride), checks = xd && d->offsets, copies = !xd || checks;
 
     // the piece: dl and the copied items within their budgets, dl's rows within the products' 32-bit offsets
     uint32_t piece = piece_items(V, uint64_t(T) * ks, kGradBudget);
-    if (copies) piece = std::min(piece, piece_items(V, x_row, kCopyBudget));
+    if (copies || planes) piece = std::min(piece, piece_items(V, row, kCopyBudget));
     piece = std::min<uint32_t>(piece, (uint32_t(kDmaMaxBytes / 256) - kRowPad) / ks / 256 * 256);
     const uint32_t pieces = ceil_div(V, piece), most = std::min(piece, V), Vpmax = round_up(most, 64);
     // dh has few tiles and a long sum, and so has dw of many rows and few items: shares of it until the chip is
@@ -472,66 +436,58 @@ va_status va_xent_backward(va_context* ctx, const va_xent_desc* d, const float* 
         return stages <= 24 && once ? 1u : std::max(stages / 8, 1u);
     };
     const bool narrow = kind == g16::F32 && T <= 32;
-    const Blocks lb = blocks_for(ctx, kind, T, most, 1, narrow, stages_of(kind, D)), hb = blocks_for(ctx, kind, T, D, shares_of(Vpmax, pieces == 1), narrow),
-                 wb = blocks_for(ctx, kind, most, D, shares_of(T, true));
+    const Blocks lb = blocks_for(ctx, kind, T, most, 1, narrow, stages_of(kind, D)), hb = blocks_for(ctx, second, T, D, shares_of(Vpmax, pieces == 1), narrow),
+                 wb = blocks_for(ctx, second, most, D, shares_of(T, true));
     const bool h_shared = out_grad_hidden && (hb.parts > 1 || pieces > 1), w_shared = out_grad_items && wb.parts > 1;
 
     const size_t p_bytes = uint64_t(T) * (uint64_t(Vpmax) * ks + kRowPad);
     const size_t share_n = h_shared ? uint64_t(hb.parts) * T * Dp : 0, w_share_n = w_shared ? uint64_t(wb.parts) * most * Dp : 0;
-    const size_t q_bytes = uint64_t(T) * copy_bytes(kind, D), x_bytes = copies ? uint64_t(most) * x_row : 0;
+    const size_t q_bytes = uint64_t(T) * row, x_bytes = copies ? uint64_t(most) * row : 0;
+    const size_t qs_bytes = planes ? q_bytes : 0, xs_bytes = planes ? uint64_t(most) * row : 0;
     Scratch sc(ctx);
     const size_t need = Scratch::round(p_bytes) + Scratch::round(share_n * 4) + Scratch::round(w_share_n * 4) + Scratch::round(q_bytes) + Scratch::round(x_bytes) +
-                        2 * Scratch::round(T * 4ull) + Scratch::round(most * 4ull) + Scratch::round(16);
+                        Scratch::round(qs_bytes) + Scratch::round(xs_bytes) + 2 * Scratch::round(T * 4ull) + Scratch::round(most * 4ull) + Scratch::round(8);
     VA_CHECK_STATUS(sc.reserve(need));
     char* p = sc.carve<char>(p_bytes);
     float* share = sc.carve<float>(share_n);
     float* w_share = sc.carve<float>(w_share_n);
     char* qp = sc.carve<char>(q_bytes);
     char* xp = sc.carve<char>(x_bytes);
+    char* qs = sc.carve<char>(qs_bytes);  // planes
+    char* xs = sc.carve<char>(xs_bytes);
     float* gk = sc.carve<float>(T);
     float* qinv = sc.carve<float>(T);
     float* xinv = sc.carve<float>(most);
-    float* mul = sc.carve<float>(4);
-    uint32_t* absmax = reinterpret_cast<uint32_t*>(mul + 1);  // of the hidden rows, of the items
-    uint32_t* odd = absmax + 2;
+    float* mul = sc.carve<float>(2);
+    uint32_t* odd = reinterpret_cast<uint32_t*>(mul + 1);
     VA_CHECK_STATUS(sc.verify(need));
 
     // gk, and the hidden rows ended by zeros
-    const PrepareArgs pa{grad, d->targets, T, V, d->ignore_index, int(reduction), d->scale, gk, mul, absmax};
-    const bool together = T <= kPrepareRows && !planes;
+    const PrepareArgs pa{grad, d->targets, T, V, d->ignore_index, int(reduction), d->scale, gk, mul, odd};
+    const bool together = T <= kPrepareRows;
     const uint32_t rows_per = together ? std::max(4u, ceil_div(T, 512)) : T;
-    if (kind == g16::F32)
+    if (dt == VA_DTYPE_F32)
         xent_prepare_kernel<uint32_t><<<dim3(ceil_div(T, rows_per)), dim3(256), 0, ctx->stream>>>(
-            pa, rows_per, together ? static_cast<const uint32_t*>(d->hidden) : nullptr, d->hidden_stride, D, one / 4, reinterpret_cast<uint32_t*>(qp));
+            pa, rows_per, together ? static_cast<const uint32_t*>(d->hidden) : nullptr, d->hidden_stride, D, row / 4, reinterpret_cast<uint32_t*>(qp));
     else
         xent_prepare_kernel<uint16_t><<<dim3(ceil_div(T, rows_per)), dim3(256), 0, ctx->stream>>>(
-            pa, rows_per, together ? static_cast<const uint16_t*>(d->hidden) : nullptr, d->hidden_stride, D, one / 2, reinterpret_cast<uint16_t*>(qp));
+            pa, rows_per, together ? static_cast<const uint16_t*>(d->hidden) : nullptr, d->hidden_stride, D, row / 2, reinterpret_cast<uint16_t*>(qp));
     VA_CHECK_LAUNCH(ctx);
     const Drop no_gradient{gk, 0.0f};
-    Planes hidden_planes{d->hidden, d->hidden_stride, T, absmax, no_gradient, qp, qinv};
-    auto item_planes = [&](const void* items, uint32_t n, const float* offsets) {
-        return Planes{items, d->items_stride, n, absmax + 1, Drop{offsets, -INFINITY}, xp, xinv};
-    };
-    if (planes) {
-        // one scale a tensor: both tensors are summed over in the second products
-        const uint32_t na = std::min(ceil_div(T, 16), 512u), nb = std::min(ceil_div(V, 16), 512u);
-        absmax_kernel<<<dim3(na + nb), dim3(256), 0, ctx->stream>>>(hidden_planes, item_planes(d->items, V, d->offsets), na, D, absmax);
-        VA_CHECK_LAUNCH(ctx);
-    }
-    if (!together && !planes) VA_CHECK_STATUS(make_copy(ctx, kind, d->hidden, d->hidden_stride, T, D, no_gradient, qp));
+    if (!together) VA_CHECK_STATUS(make_copy(ctx, second, d->hidden, d->hidden_stride, T, D, no_gradient, qp));
     if (checks) VA_CHECK_STATUS(find_odd(ctx, d, odd));
 
-    auto rows_out = [&](auto sh, auto k, auto qk, const g16::Args& b, uintptr_t o, uint64_t ld, uint32_t rows, const uint32_t* top, const float* zero) {
+    auto rows_out = [&](auto sh, auto k, auto qk, const g16::Args& b, uintptr_t o, uint64_t ld, uint32_t rows, const float* zero) {
         constexpr int kKind = decltype(k)::value;
         using E = ElemT<dtype_of(kKind)>;
-        const RowsEpi<decltype(sh), kKind> e{reinterpret_cast<E*>(o), ld, rows, D, mul, top, zero};
+        const RowsEpi<decltype(sh), kKind> e{reinterpret_cast<E*>(o), ld, rows, D, mul, zero};
         return g16::launch<kKind, decltype(qk)::value, true>(ctx, b, e);
     };
-    auto sum_shares = [&](const float* from, uint32_t parts, uint32_t rows, const float* zero, const uint32_t* top, uintptr_t o, uint64_t ld) {
-        return by_kind(kind, [&](auto k) {
+    auto sum_shares = [&](const float* from, uint32_t parts, uint32_t rows, const float* zero, uintptr_t o, uint64_t ld) {
+        return by_second(second, [&](auto k) {
             constexpr int kKind = decltype(k)::value;
             share_sum_kernel<kKind><<<dim3(uint32_t(std::min<uint64_t>((uint64_t(rows) * (Dp / 4) + 63) / 64, kGridMax))), dim3(256), 0, ctx->stream>>>(
-                from, parts, rows, D, Dp, zero, mul, top, reinterpret_cast<ElemT<dtype_of(kKind)>*>(o), ld);
+                from, parts, rows, D, Dp, zero, mul, reinterpret_cast<ElemT<dtype_of(kKind)>*>(o), ld);
             VA_CHECK_LAUNCH(ctx);
             return VA_OK;
         });
@@ -540,17 +496,16 @@ va_status va_xent_backward(va_context* ctx, const va_xent_desc* d, const float* 
         const uint32_t v0 = c * piece, n = std::min(piece, V - v0), Vp = round_up(n, 64);
         const char* items = row_at(d->items, d->items_stride, v0, dt);
         const float* offsets = d->offsets ? d->offsets + v0 : nullptr;
-        if (planes) {
-            VA_CHECK_STATUS(make_planes(ctx, D, hidden_planes, item_planes(items, n, offsets)));
-            hidden_planes.R = 0;  // (once)
-        } else if (copies) {
-            VA_CHECK_STATUS(make_copy(ctx, kind, items, d->items_stride, n, D, Drop{offsets, -INFINITY}, xp, checks ? odd : nullptr));
-        }
-        const g16::Operand rows = copied(kind, qp, T, D);
-        g16::Operand cols = xd ? in_place(dt, items, d->items_stride, n, D) : copied(kind, xp, n, D);
+        const Drop masked{offsets, -INFINITY};
+        if (planes)
+            VA_CHECK_STATUS(make_planes(ctx, D, Planes{d->hidden, d->hidden_stride, c ? 0 : T, no_gradient, qs, qinv},
+                                        Planes{items, d->items_stride, n, masked, xs, xinv}));
+        if (copies) VA_CHECK_STATUS(make_copy(ctx, second, items, d->items_stride, n, D, masked, xp, checks ? odd : nullptr));
+        const g16::Operand rows = copied(second, qp, T, D);
+        g16::Operand cols = xd ? in_place(dt, items, d->items_stride, n, D) : copied(second, xp, n, D);
         if (checks) {
             cols.other = xp;
-            cols.other_pitch = x_row;
+            cols.other_pitch = row;
             cols.choose = odd;
         }
         g16::Operand dl;
@@ -559,9 +514,9 @@ va_status va_xent_backward(va_context* ctx, const va_xent_desc* d, const float* 
         dl.rows = T;
         dl.width = Vp * ks;
         g16::Args a;
-        a.q = rows;
-        a.x = cols;
-        a.kstages = one / g16::ROWB;
+        a.q = planes ? copied(kind, qs, T, D) : rows;
+        a.x = planes ? copied(kind, xs, n, D) : cols;
+        a.kstages = row / g16::ROWB;
         a.tail = xd ? tail : 0;
         a.nq = lb.nq(T);
         a.nr = lb.nr(n);
@@ -589,9 +544,9 @@ va_status va_xent_backward(va_context* ctx, const va_xent_desc* d, const float* 
             b.nq = hb.nq(T);
             b.nr = hb.nr(D);
             b.parts = hb.parts;
-            VA_CHECK_STATUS(by_kind(kind, [&](auto k) {
+            VA_CHECK_STATUS(by_second(second, [&](auto k) {
                 return by_shape_of<decltype(k)::value>(hb.shape, [&](auto sh) {
-                    if (!h_shared) return rows_out(sh, k, std::false_type(), b, reinterpret_cast<uintptr_t>(out_grad_hidden), grad_hidden_stride, T, absmax + 1, gk);
+                    if (!h_shared) return rows_out(sh, k, std::false_type(), b, reinterpret_cast<uintptr_t>(out_grad_hidden), grad_hidden_stride, T, gk);
                     const ShareEpi<decltype(sh)> e{share, T, D, Dp, c == 0};
                     return g16::launch<decltype(k)::value, false, true>(ctx, b, e);
                 });
@@ -607,17 +562,17 @@ va_status va_xent_backward(va_context* ctx, const va_xent_desc* d, const float* 
             b.nr = wb.nr(D);
             b.parts = wb.parts;
             const uintptr_t o = reinterpret_cast<uintptr_t>(out_grad_items) + uint64_t(v0) * grad_items_stride * es;
-            VA_CHECK_STATUS(by_kind(kind, [&](auto k) {
+            VA_CHECK_STATUS(by_second(second, [&](auto k) {
                 return by_shape<decltype(k)::value>(wb.shape, [&](auto sh) {
-                    if (!w_shared) return rows_out(sh, k, std::true_type(), b, o, grad_items_stride, n, absmax, nullptr);
+                    if (!w_shared) return rows_out(sh, k, std::true_type(), b, o, grad_items_stride, n, nullptr);
                     const ShareEpi<decltype(sh)> e{w_share, n, D, Dp, true};
                     return g16::launch<decltype(k)::value, true, true>(ctx, b, e);
                 });
             }));
-            if (w_shared) VA_CHECK_STATUS(sum_shares(w_share, wb.parts, n, nullptr, absmax, o, grad_items_stride));
+            if (w_shared) VA_CHECK_STATUS(sum_shares(w_share, wb.parts, n, nullptr, o, grad_items_stride));
         }
     }
-    if (h_shared) VA_CHECK_STATUS(sum_shares(share, hb.parts, T, gk, absmax + 1, reinterpret_cast<uintptr_t>(out_grad_hidden), grad_hidden_stride));
+    if (h_shared) VA_CHECK_STATUS(sum_shares(share, hb.parts, T, gk, reinterpret_cast<uintptr_t>(out_grad_hidden), grad_hidden_stride));
     return VA_OK;
 }
 

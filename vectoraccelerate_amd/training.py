@@ -96,6 +96,10 @@ class SoftmaxCrossEntropyKernel:
     vectors hold.  Rows whose target is ``ignoreIndex`` have loss 0 and gradient 0; a target outside
     the collection gives a NaN loss and gradient 0.  Targets are int64.  hidden and items are float32,
     float16 or bfloat16 alike, their rows may be strided.
+
+    Sums are fp32.  In 16 bits the logits' gradients are rounded once to the type before they are summed
+    into the results.  In float32 more than 32 rows (64 over 65,536 items and more) enter the logits
+    as two float16 values each: exact to 2^-22 of the value or 2^-39 of the largest of its row.
     """
 
     name = "SoftmaxCrossEntropyKernel"
