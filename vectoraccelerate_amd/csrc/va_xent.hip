@@ -36,7 +36,7 @@ namespace {
 
 using namespace xent;
 
-// ---- copies: rows not in dwords, operands whose rows must end in zeros or may not be read, planes -------------
+// ---- copies: rows a product cannot read in place, operands whose rows must end in zeros or may not be read, planes -------------
 // dst[r][k] = src[r][k], zeros for k in [D, Kp) and in dropped rows.  Nothing if *run_if is zero.
 template <class U>
 __global__ __launch_bounds__(256) void copy_kernel(const U* __restrict__ src, uint64_t ld, uint32_t D, uint32_t Kp, Drop drop, const uint32_t* run_if,
@@ -436,8 +436,8 @@ va_status va_xent_forward(va_context* ctx, const va_xent_desc* d, float* out_los
     const int kind = kind_of(dt, T, V);
     const uint32_t one = copy_bytes(kind, D), tail = kind == g16::PLANES ? 0 : D * uint32_t(elem_size(dt)) % g16::ROWB;
     // the hidden rows end in zeros, the items are cut in their fragments
-    const bool qd = kind != g16::PLANES && tail == 0 && in_dwords(dt, d->hidden, d->hidden_stride);
-    const bool xd = kind != g16::PLANES && in_dwords(dt, d->items, d->items_stride);
+    const bool qd = kind != g16::PLANES && tail == 0 && in_place_rows(dt, d->hidden, d->hidden_stride);
+    const bool xd = kind != g16::PLANES && in_place_rows(dt, d->items, d->items_stride);
     const size_t q_bytes = qd ? 0 : uint64_t(T) * copy_bytes(kind, D), x_row = copy_bytes(kind, D);
     const uint32_t piece = xd ? round_up(V, 256) : piece_items(V, x_row, kCopyBudget), most = std::min(piece, V);
     const uint32_t pieces = ceil_div(V, piece);

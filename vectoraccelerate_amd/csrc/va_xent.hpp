@@ -138,8 +138,10 @@ inline size_t elem_size(va_dtype t) { return t == VA_DTYPE_F32 ? 4 : 2; }
 inline uint32_t round_up(uint32_t v, uint32_t m) { return (v + m - 1) / m * m; }
 inline const char* row_at(const void* p, uint64_t ld, uint64_t row, va_dtype dt) { return static_cast<const char*>(p) + row * ld * elem_size(dt); }
 
-// Rows that a product can read where they are: dwords.
-inline bool in_dwords(va_dtype dt, const void* p, uint64_t ld) { return ld * elem_size(dt) % 4 == 0 && reinterpret_cast<uintptr_t>(p) % 4 == 0; }
+// Rows that a product can read where they are: dwords, 256 of them (a tile's) within the reach of its loads' offsets.
+inline bool in_place_rows(va_dtype dt, const void* p, uint64_t ld) {
+    return ld * elem_size(dt) % 4 == 0 && reinterpret_cast<uintptr_t>(p) % 4 == 0 && ld <= kDmaMaxBytes / 256 / elem_size(dt);
+}
 // Bytes of a row of D values in place, and of one of a copy: whole stages.
 inline uint32_t row_bytes(va_dtype dt, uint32_t D) { return round_up(D * uint32_t(elem_size(dt)), 4); }
 inline uint32_t copy_bytes(int kind, uint32_t D) { return round_up(D * uint32_t(g16::size_of(kind)), g16::ROWB); }

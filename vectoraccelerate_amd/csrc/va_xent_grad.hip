@@ -422,7 +422,7 @@ va_status va_xent_backward(va_context* ctx, const va_xent_desc* d, const float* 
     const uint32_t row = copy_bytes(kind, D), tail = planes ? 0 : D * ks % g16::ROWB;
     // Masked items may hold anything, and dh sums over them: unless they are found to be finite, a copy is read in
     // which they are zeros.
-    const bool xd = in_dwords(dt, d->items, d->items_stride), checks = xd && d->offsets, copies = !xd || checks;
+    const bool xd = in_place_rows(dt, d->items, d->items_stride), checks = xd && d->offsets, copies = !xd || checks;
 
     // the piece: dl and the copied items within their budgets, dl's rows within the products' 32-bit offsets
     uint32_t piece = piece_items(V, uint64_t(T) * ks, kGradBudget);
