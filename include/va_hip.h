@@ -468,8 +468,9 @@ va_status va_probe_mfma(va_context* ctx, va_probe_kind kind, int random_operands
  * What a program needs around the search: the loss that trains queries against all items of a
  * collection, the norm and 8-bit coding of an encoder's output, and the clipping of its gradients.
  * Device pointers and the context's stream as everywhere; nothing here waits on the host except to
- * grow the scratch arena.  Rows are row-major with a stride in elements; sums, softmax statistics
- * and norms are fp32 or wider whatever the type (what is rounded to fewer bits is said below). */
+ * grow the scratch arena.  Rows are row-major with a stride in elements (a single row's is not looked
+ * at); sums, softmax statistics and norms are fp32 or wider whatever the type (what is rounded to fewer
+ * bits is said below). */
 typedef enum { VA_DTYPE_F32 = 0, VA_DTYPE_F16 = 1, VA_DTYPE_BF16 = 2 } va_dtype;
 typedef enum { VA_REDUCE_MEAN = 0, VA_REDUCE_SUM = 1, VA_REDUCE_NONE = 2 } va_reduction;
 

@@ -1,5 +1,7 @@
-"""Rows of the softmax cross entropy far apart in memory."""
+"""Rows of the softmax cross entropy far apart in memory, and single rows, whose stride is never walked."""
 from __future__ import annotations
+
+import ctypes as C
 
 import pytest
 import torch
@@ -40,5 +42,30 @@ def test_rows_megabytes_apart(ctx, T, D, which, dtype):
     k.encodeBackward(hh, ww, y, res.logSumExp, gh, gw, offsets=off.cuda())
     ctx.synchronize()
     want = oracle.xent(h, w, y, 1.0, off.cuda(), IGNORE, torch.full((T,), 1.0 / T, dtype=torch.float64))
+    oracle.close(gh, *want["grad_hidden"], "grad_hidden")
+    oracle.close(gw, *want["grad_items"], "grad_items")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("stride", [0, 5, 1 << 40])
+@pytest.mark.parametrize("T,V", [(1, 300), (40, 1), (1, 1)])
+def test_single_rows_of_a_description(ctx, T, V, stride, dtype):
+    """The C description of one row or one item takes any stride for it, and so do their gradients."""
+    from vectoraccelerate_amd import _lib
+
+    D = 96
+    h, w, y, _ = _inputs(T, V, D, dtype, T + V)
+    loss, lse, mean = (torch.empty(n, device="cuda") for n in (T, T, 1))
+    gh, gw = torch.empty_like(h), torch.empty_like(w)
+    kinds = {torch.float32: _lib.VA_DTYPE_F32, torch.float16: _lib.VA_DTYPE_F16, torch.bfloat16: _lib.VA_DTYPE_BF16}
+    hs, ws = stride if T == 1 else D, stride if V == 1 else D
+    d = _lib.XentDesc(h.data_ptr(), w.data_ptr(), y.data_ptr(), None, hs, ws, IGNORE, T, V, D, kinds[dtype], 1.0)
+    ctx.order_after_torch()
+    ctx.check(ctx.lib.va_xent_forward(ctx.handle, C.byref(d), loss.data_ptr(), lse.data_ptr(), _lib.VA_REDUCE_MEAN, mean.data_ptr()), "va_xent_forward")
+    ctx.check(ctx.lib.va_xent_backward(ctx.handle, C.byref(d), lse.data_ptr(), _lib.VA_REDUCE_MEAN, None, gh.data_ptr(), hs, gw.data_ptr(), ws),
+              "va_xent_backward")
+    ctx.synchronize()
+    want = oracle.xent(h, w, y, 1.0, None, IGNORE, torch.full((T,), 1.0 / T, dtype=torch.float64))
+    oracle.close(loss, *want["loss"], "loss")
     oracle.close(gh, *want["grad_hidden"], "grad_hidden")
     oracle.close(gw, *want["grad_items"], "grad_items")

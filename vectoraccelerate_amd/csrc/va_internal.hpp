@@ -168,6 +168,8 @@ constexpr uint32_t kSentinel = 0xFFFFFFFFu;
 constexpr uint32_t kXcds = 8;
 
 inline uint32_t ceil_div(uint64_t a, uint64_t b) { return uint32_t((a + b - 1) / b); }
+// The stride of `rows` rows of `dim` values: a single row has none, whatever its description says.
+inline uint64_t stride_of(uint32_t rows, uint64_t stride, uint32_t dim) { return rows == 1 ? dim : stride; }
 // Workgroups of 256 threads a launch at most: its threads are counted in 32 bits.
 constexpr uint32_t kGridMax = 1u << 23;
 

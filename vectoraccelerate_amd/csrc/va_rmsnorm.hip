@@ -492,8 +492,12 @@ va_status by_dtype(va_dtype t, Fn&& f) {
 bool known(va_dtype t) { return t == VA_DTYPE_F32 || t == VA_DTYPE_F16 || t == VA_DTYPE_BF16; }
 bool aligned(const void* p, va_dtype t) { return reinterpret_cast<uintptr_t>(p) % (t == VA_DTYPE_F32 ? 4 : 2) == 0; }
 
-va_status check(va_context* ctx, const va_rms_desc* d, const char* who) {
-    VA_REQUIRE(ctx, d, "%s: NULL description", who);
+// The description with the strides of a single row set, checked.
+va_status check(va_context* ctx, const va_rms_desc* desc, const char* who, va_rms_desc& own) {
+    VA_REQUIRE(ctx, desc, "%s: NULL description", who);
+    own = *desc;
+    for (uint64_t* stride : {&own.x_stride, &own.residual_stride, &own.out_residual_stride}) *stride = stride_of(own.rows, *stride, own.dim);
+    const va_rms_desc* d = &own;
     VA_REQUIRE(ctx, d->x && d->weight, "%s: NULL pointer", who);
     VA_REQUIRE(ctx, d->rows > 0 && d->dim > 0, "%s: empty input (%u rows, %u dimensions)", who, d->rows, d->dim);
     VA_REQUIRE(ctx, known(d->dtype), "%s: unknown type %d", who, int(d->dtype));
@@ -541,18 +545,24 @@ using namespace va;
 
 extern "C" {
 
-va_status va_rms_norm(va_context* ctx, const va_rms_desc* d, void* out, uint64_t out_stride) {
+va_status va_rms_norm(va_context* ctx, const va_rms_desc* desc, void* out, uint64_t out_stride) {
     if (!ctx) return VA_ERR_INVALID_ARG;
-    VA_CHECK_STATUS(check(ctx, d, "va_rms_norm"));
+    va_rms_desc own;
+    VA_CHECK_STATUS(check(ctx, desc, "va_rms_norm", own));
+    const va_rms_desc* d = &own;
+    out_stride = stride_of(d->rows, out_stride, d->dim);
     VA_REQUIRE(ctx, out && out_stride >= d->dim && aligned(out, d->dtype), "va_rms_norm: the output is NULL, misaligned or its stride below the dimension");
     DeviceGuard guard(ctx->device);
     return forward<OUT_SAME>(ctx, d, out, out_stride, 0, 0.0f, nullptr);
 }
 
-va_status va_rms_norm_quantized(va_context* ctx, const va_rms_desc* d, va_code code, uint32_t group, float given_scale, void* out_codes,
+va_status va_rms_norm_quantized(va_context* ctx, const va_rms_desc* desc, va_code code, uint32_t group, float given_scale, void* out_codes,
                                 uint64_t codes_stride, float* out_scales) {
     if (!ctx) return VA_ERR_INVALID_ARG;
-    VA_CHECK_STATUS(check(ctx, d, "va_rms_norm_quantized"));
+    va_rms_desc own;
+    VA_CHECK_STATUS(check(ctx, desc, "va_rms_norm_quantized", own));
+    const va_rms_desc* d = &own;
+    codes_stride = stride_of(d->rows, codes_stride, d->dim);
     VA_CHECK_STATUS(check_codes(ctx, code, group, given_scale, "va_rms_norm_quantized"));
     VA_REQUIRE(ctx, out_codes && codes_stride >= d->dim, "va_rms_norm_quantized: the codes are NULL or their stride below the dimension");
     VA_REQUIRE(ctx, (given_scale > 0.0f) == (out_scales == nullptr), "va_rms_norm_quantized: scales are written unless one is given");
@@ -568,6 +578,8 @@ va_status va_rms_dequantize(va_context* ctx, const void* codes, uint64_t codes_s
     VA_REQUIRE(ctx, codes && out && (given_scale > 0.0f) == (scales == nullptr), "va_rms_dequantize: NULL pointer, or scales beside a given scale");
     VA_REQUIRE(ctx, rows > 0 && dim > 0, "va_rms_dequantize: empty input (%u rows, %u dimensions)", rows, dim);
     VA_REQUIRE(ctx, known(dtype) && aligned(out, dtype), "va_rms_dequantize: unknown type or misaligned output");
+    codes_stride = stride_of(rows, codes_stride, dim);
+    out_stride = stride_of(rows, out_stride, dim);
     VA_REQUIRE(ctx, codes_stride >= dim && out_stride >= dim, "va_rms_dequantize: a row stride is below the dimension");
     const uint64_t blocks = (uint64_t(rows) * ((uint64_t(dim) + 7) / 8) + 255) / 256;
     DeviceGuard guard(ctx->device);
@@ -582,11 +594,14 @@ va_status va_rms_dequantize(va_context* ctx, const void* codes, uint64_t codes_s
     });
 }
 
-va_status va_rms_norm_backward(va_context* ctx, const va_rms_desc* d, const void* grad, uint64_t grad_stride, const void* grad_residual,
+va_status va_rms_norm_backward(va_context* ctx, const va_rms_desc* desc, const void* grad, uint64_t grad_stride, const void* grad_residual,
                                uint64_t grad_residual_stride, const float* inverse_rms, void* out_grad_x, uint64_t grad_x_stride,
                                void* out_grad_weight) {
     if (!ctx) return VA_ERR_INVALID_ARG;
-    VA_CHECK_STATUS(check(ctx, d, "va_rms_norm_backward"));
+    va_rms_desc own;
+    VA_CHECK_STATUS(check(ctx, desc, "va_rms_norm_backward", own));
+    const va_rms_desc* d = &own;
+    for (uint64_t* stride : {&grad_stride, &grad_residual_stride, &grad_x_stride}) *stride = stride_of(d->rows, *stride, d->dim);
     VA_REQUIRE(ctx, grad && inverse_rms && (out_grad_x || out_grad_weight), "va_rms_norm_backward: NULL pointer");
     VA_REQUIRE(ctx, !d->residual && !d->out_residual && !d->out_inverse_rms, "va_rms_norm_backward: x is the summed row; the description has no residual and no output");
     VA_REQUIRE(ctx, grad_stride >= d->dim && (!grad_residual || grad_residual_stride >= d->dim) && (!out_grad_x || grad_x_stride >= d->dim),

@@ -400,8 +400,12 @@ va_status find_odd(va_context* ctx, const va_xent_desc* d, uint32_t* odd) {
     return VA_OK;
 }
 
-va_status check_desc(va_context* ctx, const va_xent_desc* d, const char* who) {
-    VA_REQUIRE(ctx, d != nullptr, "%s: NULL description", who);
+va_status check_desc(va_context* ctx, const va_xent_desc* desc, const char* who, va_xent_desc& own) {
+    VA_REQUIRE(ctx, desc != nullptr, "%s: NULL description", who);
+    own = *desc;
+    own.hidden_stride = stride_of(own.rows, own.hidden_stride, own.dim);
+    own.items_stride = stride_of(own.num_items, own.items_stride, own.dim);
+    const va_xent_desc* d = &own;
     VA_REQUIRE(ctx, d->hidden && d->items && d->targets, "%s: NULL pointer", who);
     VA_REQUIRE(ctx, d->rows > 0 && d->num_items > 0 && d->dim > 0, "%s: empty input (%u rows, %u items, %u dimensions)", who, d->rows,
                d->num_items, d->dim);
@@ -424,9 +428,11 @@ using namespace va::xent;
 
 extern "C" {
 
-va_status va_xent_forward(va_context* ctx, const va_xent_desc* d, float* out_loss, float* out_lse, va_reduction reduction, float* out_reduced) {
+va_status va_xent_forward(va_context* ctx, const va_xent_desc* desc, float* out_loss, float* out_lse, va_reduction reduction, float* out_reduced) {
     if (!ctx) return VA_ERR_INVALID_ARG;
-    VA_CHECK_STATUS(check_desc(ctx, d, "va_xent_forward"));
+    va_xent_desc own;
+    VA_CHECK_STATUS(check_desc(ctx, desc, "va_xent_forward", own));
+    const va_xent_desc* d = &own;
     VA_REQUIRE(ctx, out_loss && out_lse, "va_xent_forward: NULL output");
     VA_REQUIRE(ctx, reduction == VA_REDUCE_MEAN || reduction == VA_REDUCE_SUM || reduction == VA_REDUCE_NONE, "va_xent_forward: unknown reduction %d", int(reduction));
     VA_REQUIRE(ctx, (reduction == VA_REDUCE_NONE) == (out_reduced == nullptr), "va_xent_forward: a reduced loss goes with a reduction");

@@ -198,7 +198,8 @@ va_status make_planes(va_context* ctx, uint32_t D, Planes a, Planes b = {});
 // offset is finite and near fp32's limits
 va_status find_odd(va_context* ctx, const va_xent_desc* d, uint32_t* odd);
 
-va_status check_desc(va_context* ctx, const va_xent_desc* d, const char* who);
+// The description with the strides of single rows set, checked.
+va_status check_desc(va_context* ctx, const va_xent_desc* desc, const char* who, va_xent_desc& d);
 // A scale at which the logits' other unit might overflow: natural units (as with odd offsets).
 inline bool wild_scale(const va_xent_desc* d) { return fabsf(d->scale) > 1e18f; }
 

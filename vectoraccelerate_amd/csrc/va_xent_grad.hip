@@ -396,10 +396,14 @@ using namespace va::xent;
 
 extern "C" {
 
-va_status va_xent_backward(va_context* ctx, const va_xent_desc* d, const float* lse, va_reduction reduction, const float* grad,
+va_status va_xent_backward(va_context* ctx, const va_xent_desc* desc, const float* lse, va_reduction reduction, const float* grad,
                            void* out_grad_hidden, uint64_t grad_hidden_stride, void* out_grad_items, uint64_t grad_items_stride) {
     if (!ctx) return VA_ERR_INVALID_ARG;
-    VA_CHECK_STATUS(check_desc(ctx, d, "va_xent_backward"));
+    va_xent_desc own;
+    VA_CHECK_STATUS(check_desc(ctx, desc, "va_xent_backward", own));
+    const va_xent_desc* d = &own;
+    grad_hidden_stride = stride_of(d->rows, grad_hidden_stride, d->dim);
+    grad_items_stride = stride_of(d->num_items, grad_items_stride, d->dim);
     VA_REQUIRE(ctx, lse, "va_xent_backward: NULL log-sum-exp");
     VA_REQUIRE(ctx, reduction == VA_REDUCE_MEAN || reduction == VA_REDUCE_SUM || reduction == VA_REDUCE_NONE, "va_xent_backward: unknown reduction %d", int(reduction));
     VA_REQUIRE(ctx, reduction != VA_REDUCE_NONE || grad, "va_xent_backward: without a reduction the rows' gradients are needed");
