@@ -514,8 +514,8 @@ va_status va_xent_backward(va_context* ctx, const va_xent_desc* desc, const floa
 /* Root-mean-square norm of rows, after the addition of a residual:
  *   r = x + residual,  i = 1 / sqrt(mean_d r_d^2 + epsilon),  y_d = r_d i w_d.
  * residual, out_residual (r in the rows' type) and out_inverse_rms (i, [rows] fp32) may be NULL;
- * outputs may be the inputs they replace.  8-bit outputs: code = round(y / s) (ties to even,
- * saturating) with s = max |y| / 127 (int8) or / 448 (fp8, e4m3 without infinities) over each group
+ * outputs may be the inputs they replace.  8-bit outputs: code = round(y / s) (y and the quotient
+ * in fp32, ties to even, saturating) with s = max |y| / 127 (int8) or / 448 (fp8, e4m3 without infinities) over each group
  * of `group` dimensions (0: the row; else a power of two from 8 to 512, the last one may be
  * shorter), written to out_scales [rows x groups]; or with one given scale > 0 and no out_scales
  * (codes on one grid, as va_i8_scan_topk compares them).  A group of zeros has scale 0; one that

@@ -11,7 +11,7 @@
 // alignment (global loads on gfx950 need none beyond the element's); a row's last, partial chunk element by
 // element.  Sums are fp32 (a lane's chain of at most 32 values, then a tree).
 //
-// Measured: 65,536 x 1536 bf16 with residual to int8 by groups 150 us = 4.7 TB/s, and back 53 us = 5.7 TB/s; 10,007
+// Measured: 65,536 x 1536 bf16 with residual to int8 by groups 156 us = 4.5 TB/s, and back 53 us = 5.7 TB/s; 10,007
 // x 513 fp32 forward 18 us and backward 18 + 4 us (4.6 TB/s each); 37,289 x 768 bf16 forward 44 us = 5.2 TB/s.  One
 // row: 5 us, the launch.
 #include <algorithm>
@@ -122,14 +122,17 @@ struct RmsArgs {
     float eps, given;              // given > 0: the scale
 };
 
-__device__ __forceinline__ uint2 codes8(f32x8 y, float inv, bool fp8) {
+// The codes of y / s (0 where s is), the quotient rounded to fp32 and then to the nearest code.  A division a value: by the
+// reciprocal, a quotient next to a midpoint may come out on its other side (65,536 x 1536 to int8 by groups of 128 144 us
+// that way and 156 divided, by rows 130 and 134).
+__device__ __forceinline__ uint2 codes8(f32x8 y, float s, bool fp8) {
     uint32_t w[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         float z[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            z[e] = y[4 * h + e] * inv;
+            z[e] = s == 0.0f ? 0.0f : y[4 * h + e] / s;
             const float most = fp8 ? 448.0f : 127.0f;
             z[e] = z[e] != z[e] ? z[e] : fminf(fmaxf(z[e], -most), most);
         }
@@ -250,9 +253,7 @@ __global__ __launch_bounds__(256) void rms_norm_kernel(RmsArgs a) {
                 sc = m / most;
                 if (d < D && d % a.group == 0) a.scales[uint64_t(t) * a.groups + d / a.group] = sc;
             }
-            // (a tiny scale's reciprocal would overflow: both are raised by a power of two)
-            const float up = sc < 0x1p-100f ? 0x1p64f : 1.0f;
-            store_codes(o, d, D, codes8(y * up, sc == 0.0f ? 0.0f : 1.0f / (sc * up), fp8));
+            store_codes(o, d, D, codes8(y, sc, fp8));
         };
         if constexpr (C > 0) {
             const bool have = a.group == 0 && !(a.given > 0.0f);  // r holds y
