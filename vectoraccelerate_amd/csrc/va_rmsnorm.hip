@@ -493,6 +493,12 @@ va_status by_dtype(va_dtype t, Fn&& f) {
 bool known(va_dtype t) { return t == VA_DTYPE_F32 || t == VA_DTYPE_F16 || t == VA_DTYPE_BF16; }
 bool aligned(const void* p, va_dtype t) { return reinterpret_cast<uintptr_t>(p) % (t == VA_DTYPE_F32 ? 4 : 2) == 0; }
 
+// Rows and dimensions that the kernels can count in 32 bits (a row's last chunk ends past it).
+va_status check_sizes(va_context* ctx, uint32_t rows, uint32_t dim, const char* who) {
+    VA_REQUIRE(ctx, rows <= 0x7FFFFFFFu && dim <= 0x7FFFFFFFu - 16384u, "%s: too many rows or dimensions (%u, %u)", who, rows, dim);
+    return VA_OK;
+}
+
 // The description with the strides of a single row set, checked.
 va_status check(va_context* ctx, const va_rms_desc* desc, const char* who, va_rms_desc& own) {
     VA_REQUIRE(ctx, desc, "%s: NULL description", who);
@@ -507,8 +513,7 @@ va_status check(va_context* ctx, const va_rms_desc* desc, const char* who, va_rm
     VA_REQUIRE(ctx, aligned(d->x, d->dtype) && aligned(d->residual, d->dtype) && aligned(d->weight, d->dtype) && aligned(d->out_residual, d->dtype),
                "%s: an operand is not aligned to its type", who);
     VA_REQUIRE(ctx, std::isfinite(d->epsilon) && d->epsilon >= 0.0f, "%s: epsilon must be finite and not negative", who);
-    VA_REQUIRE(ctx, d->rows <= 0x7FFFFFFFu && d->dim <= 0x7FFFFFFFu - 16384u, "%s: too many rows or dimensions (%u, %u)", who, d->rows, d->dim);
-    return VA_OK;
+    return check_sizes(ctx, d->rows, d->dim, who);
 }
 
 template <int OUT>
@@ -578,6 +583,7 @@ va_status va_rms_dequantize(va_context* ctx, const void* codes, uint64_t codes_s
     VA_CHECK_STATUS(check_codes(ctx, code, group, given_scale, "va_rms_dequantize"));
     VA_REQUIRE(ctx, codes && out && (given_scale > 0.0f) == (scales == nullptr), "va_rms_dequantize: NULL pointer, or scales beside a given scale");
     VA_REQUIRE(ctx, rows > 0 && dim > 0, "va_rms_dequantize: empty input (%u rows, %u dimensions)", rows, dim);
+    VA_CHECK_STATUS(check_sizes(ctx, rows, dim, "va_rms_dequantize"));
     VA_REQUIRE(ctx, known(dtype) && aligned(out, dtype), "va_rms_dequantize: unknown type or misaligned output");
     codes_stride = stride_of(rows, codes_stride, dim);
     out_stride = stride_of(rows, out_stride, dim);
