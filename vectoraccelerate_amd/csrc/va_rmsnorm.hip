@@ -9,13 +9,15 @@
 // wave (D <= 2048) or one workgroup (D <= 8192), 16 bytes a lane and chunk (8-bit outputs: 8 values, so that a
 // group's largest value is a few lane exchanges away).  Longer rows are read twice, the second time from cache.  Values are loaded 16 bytes at a time whatever their
 // alignment (global loads on gfx950 need none beyond the element's); a row's last, partial chunk element by
-// element.  Sums are fp32 (a lane's chain of at most 32 values, then a tree).
+// element.  A row's sums are fp32 where it is held in registers (a lane's chain of at most 32 values, then a tree) and fp64
+// in longer rows; the weight's gradient is a chain of fp32 over the rows of each share, then a tree.
 //
 // Measured: 65,536 x 1536 bf16 with residual to int8 by groups 156 us = 4.5 TB/s, and back 53 us = 5.7 TB/s; 10,007
 // x 513 fp32 forward 18 us and backward 18 + 4 us (4.6 TB/s each); 37,289 x 768 bf16 forward 44 us = 5.2 TB/s.  One
 // row: 5 us, the launch.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "va_internal.hpp"
 
@@ -75,8 +77,8 @@ __device__ __forceinline__ void store(T* row, uint32_t d, uint32_t D, F<E> v) {
     }
 }
 
-template <int N>
-__device__ __forceinline__ float lanes_sum(float v) {
+template <int N, class S>
+__device__ __forceinline__ S lanes_sum(S v) {
 #pragma unroll
     for (int d = 1; d < N; d <<= 1) v += __shfl_xor(v, d);
     return v;
@@ -85,8 +87,8 @@ __device__ __forceinline__ float lanes_sum(float v) {
 __device__ __forceinline__ float top(float a, float b) { return b > a || b != b ? b : a; }
 
 // a sum over the row's threads (one wave, or the workgroup's four)
-template <int WPR>
-__device__ __forceinline__ float row_sum(float v, float* part) {
+template <int WPR, class S>
+__device__ __forceinline__ S row_sum(S v, S* part) {
     v = lanes_sum<64>(v);
     if constexpr (WPR > 1) {
         __syncthreads();  // the previous row's sums are read
@@ -162,7 +164,9 @@ template <int DT, int OUT, int WPR, int C>
 __global__ __launch_bounds__(256) void rms_norm_kernel(RmsArgs a) {
     using T = ElemT<DT>;
     constexpr int NT = 64 * WPR, E = OUT == OUT_SAME ? 16 / int(sizeof(T)) : 8;
-    __shared__ float part[4];
+    using S = std::conditional_t<C == 0, double, float>;  // of the row's sum
+    __shared__ S part[4];
+    __shared__ float tops[4];
     const uint32_t t = a.t0 + (WPR == 1 ? blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x);
     if (t >= a.T) return;  // (a whole wave, or the workgroup)
     const uint32_t tid = WPR == 1 ? threadIdx.x & 63 : threadIdx.x;
@@ -177,7 +181,7 @@ __global__ __launch_bounds__(256) void rms_norm_kernel(RmsArgs a) {
         return v;
     };
     F<E> r[C ? C : 1];
-    float ss = 0.0f;
+    S ss = 0;
     if constexpr (C > 0) {
 #pragma unroll
         for (int c = 0; c < C; ++c) r[c] = sum_of((c * NT + tid) * E);
@@ -189,11 +193,11 @@ __global__ __launch_bounds__(256) void rms_norm_kernel(RmsArgs a) {
         for (uint32_t c = 0; c < chunks; ++c) {
             const F<E> v = sum_of((c * NT + tid) * E);
 #pragma unroll
-            for (int e = 0; e < E; ++e) ss = fmaf(v[e], v[e], ss);
+            for (int e = 0; e < E; ++e) ss = fma(double(v[e]), double(v[e]), ss);
         }
     }
     ss = row_sum<WPR>(ss, part);
-    const float inv = 1.0f / sqrtf(ss / float(D) + a.eps);
+    const float inv = 1.0f / sqrtf(float(ss / S(D)) + a.eps);
     if (a.inverse && tid == 0) a.inverse[t] = inv;
 
     // y of a chunk, the new residual stored on the way (once)
@@ -242,7 +246,7 @@ __global__ __launch_bounds__(256) void rms_norm_kernel(RmsArgs a) {
                     m = top(m, biggest(y_of(d, sum_of(d), false)));
                 }
             }
-            s = row_top<WPR>(m, part) / most;
+            s = row_top<WPR>(m, tops) / most;
             if (tid == 0) a.scales[t] = s;
         }
         auto emit = [&](uint32_t d, F<E> y) {
@@ -405,7 +409,7 @@ template <int DT>
 __global__ __launch_bounds__(256) void rms_long_grad_kernel(RmsGradArgs a) {
     using T = ElemT<DT>;
     constexpr int E = 16 / int(sizeof(T));
-    __shared__ float part[4];
+    __shared__ double part[4];
     const uint32_t D = a.D;
     const T* w = static_cast<const T*>(a.weight);
     for (uint32_t t = blockIdx.x; t < a.T; t += gridDim.x) {
@@ -414,13 +418,13 @@ __global__ __launch_bounds__(256) void rms_long_grad_kernel(RmsGradArgs a) {
         const T* gr = a.grad_residual ? static_cast<const T*>(a.grad_residual) + t * a.ldgr : nullptr;
         T* o = static_cast<T*>(a.out) + t * a.ldo;
         const float inv = a.inverse[t];
-        float along = 0.0f;
+        double sum = 0.0;
         for (uint32_t d = threadIdx.x * E; d < D; d += 256 * E) {
             const F<E> gg = load<E>(g, d, D), nn = load<E>(r, d, D) * inv, wc = load<E>(w, d, D);
 #pragma unroll
-            for (int e = 0; e < E; ++e) along = fmaf(gg[e] * wc[e], nn[e], along);
+            for (int e = 0; e < E; ++e) sum = fma(double(gg[e] * wc[e]), double(nn[e]), sum);
         }
-        along = row_sum<4>(along, part) / float(D);
+        const float along = float(row_sum<4>(sum, part) / double(D));
         for (uint32_t d = threadIdx.x * E; d < D; d += 256 * E) {
             const F<E> gg = load<E>(g, d, D), nn = load<E>(r, d, D) * inv;
             F<E> v = (gg * load<E>(w, d, D) - nn * along) * inv;
