@@ -48,3 +48,23 @@ def test_codes_of_long_rows(ctx):
     _, scales, _ = RMSNormKernel(ctx).quantize(x, w, None, torch.int8)
     want = oracle.rms(x, None, w, 1e-6)[2].abs().amax(1, keepdim=True) / 127.0
     oracle.close(scales, want, 8 * U32 * want, "scales")
+
+
+def test_weight_gradient_of_more_values_than_a_launch_has_threads(ctx):
+    """A row of so many values that the sum of its weight's gradient takes more threads than a launch can have."""
+    from vectoraccelerate_amd import RMSNormKernel
+
+    k = RMSNormKernel(ctx)
+    D = (1 << 28) + 1021
+    g = torch.Generator("cuda").manual_seed(3)
+    x, dy = (torch.randn(1, D, device="cuda", dtype=torch.bfloat16, generator=g) for _ in range(2))
+    w = torch.ones(D, device="cuda", dtype=torch.bfloat16)
+    inv = torch.full((1,), 0.75, device="cuda")
+    gw = torch.full_like(w, torch.nan)
+    ctx.order_after_torch()
+    k.encodeBackward(dy, x, w, inv, None, gw)
+    ctx.synchronize()
+    want = (dy.float() * (x.float() * 0.75))[0]
+    assert not bool(torch.isnan(gw).any())
+    # one product in fp32 before the rounding, in the kernel and here
+    assert bool(((gw.float() - want).abs() <= 2 * U[torch.bfloat16] * want.abs() + TINY[torch.bfloat16]).all())

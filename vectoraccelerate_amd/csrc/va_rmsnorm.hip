@@ -450,16 +450,21 @@ __global__ __launch_bounds__(256) void rms_weight_grad_kernel(RmsGradArgs a) {
 template <int DT>
 __global__ __launch_bounds__(1024) void rms_weight_sum_kernel(const float* __restrict__ part, uint32_t shares, uint32_t D, ElemT<DT>* __restrict__ out) {
     __shared__ float s[16][64];
-    const uint32_t c = threadIdx.x & 63, g = threadIdx.x >> 6, d = blockIdx.x * 64 + c;
-    float v = 0.0f;
-    if (d < D)
+    const uint32_t c = threadIdx.x & 63, g = threadIdx.x >> 6;
+    for (uint32_t d0 = blockIdx.x * 64; d0 < D; d0 += gridDim.x * 64) {
+        const uint32_t d = d0 + c;
+        float v = 0.0f;
+        if (d < D)
 #pragma unroll 8
-        for (uint32_t i = g; i < shares; i += 16) v += part[uint64_t(i) * D + d];
-    s[g][c] = v;
-    __syncthreads();
-    if (g || d >= D) return;
-    for (int i = 1; i < 16; ++i) v += s[i][c];
-    out[d] = ElemT<DT>(v);
+            for (uint32_t i = g; i < shares; i += 16) v += part[uint64_t(i) * D + d];
+        s[g][c] = v;
+        __syncthreads();
+        if (g == 0 && d < D) {
+            for (int i = 1; i < 16; ++i) v += s[i][c];
+            out[d] = ElemT<DT>(v);
+        }
+        __syncthreads();  // the groups' sums are read
+    }
 }
 
 // ---- host ------------------------------------------------------------------------------------------
@@ -650,7 +655,7 @@ va_status va_rms_norm_backward(va_context* ctx, const va_rms_desc* desc, const v
                 }
             }
             if (out_grad_weight) {
-                rms_weight_sum_kernel<DT><<<dim3(ceil_div(a.D, 64)), dim3(1024), 0, ctx->stream>>>(a.part, shares, a.D, static_cast<ElemT<DT>*>(out_grad_weight));
+                rms_weight_sum_kernel<DT><<<dim3(std::min(ceil_div(a.D, 64), kGridMax / 4)), dim3(1024), 0, ctx->stream>>>(a.part, shares, a.D, static_cast<ElemT<DT>*>(out_grad_weight));
                 VA_CHECK_LAUNCH(ctx);
             }
             return VA_OK;
