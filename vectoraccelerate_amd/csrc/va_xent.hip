@@ -13,7 +13,7 @@
 //
 // Precision: fp16 / bf16 operands enter the matrix cores as they are, sums are fp32.  dl is rounded
 // once to the operands' type for the second products (relative 2^-11 / 2^-8 a value, like the
-// rounding of the result), after a scale that takes the largest |g| to 2^14: fp16's range then holds
+// rounding of the result), after a scale that takes the largest |g| to 1, in fp16 to 2^14: its range then holds
 // probabilities down to 2^-38 of it, and with one g for all rows the target's -g is exact.  What falls below would
 // be below fp16's smallest gradient too, unless the largest is near its end: dl w scale of the largest |g| is at most
 // 2^16, what is lost of it 2^-39, fp16's step 2^-24.  fp32 operands are

@@ -23,19 +23,19 @@ struct PrepareArgs {
     uint32_t T, V;
     int64_t ignore;
     int reduction;
-    float scale;
+    float scale, top;
     float* gk;
     float* mul;
     uint32_t* odd;  // cleared
 };
 
 // gk[t] = g_t c, *mul = scale / c: g_t is the gradient that reaches the row's loss, 0 for a row without a
-// target, c takes the largest |g_t| to 2^14.  Every workgroup finds c for itself and takes rows_per rows; with
+// target, c takes the largest |g_t| to `top`.  Every workgroup finds c for itself and takes rows_per rows; with
 // src it also copies them, ended by zeros (rows without a gradient: zeros).
 template <class U>
 __global__ __launch_bounds__(256) void xent_prepare_kernel(PrepareArgs a, uint32_t rows_per, const U* __restrict__ src, uint64_t ld, uint32_t D, uint32_t Kp,
                                                            U* __restrict__ dst) {
-    __shared__ float top[4];
+    __shared__ float tops[4];
     __shared__ uint32_t cnt[4];
     if (blockIdx.x == 0 && threadIdx.x == 0) *a.odd = 0;
     float m = 0.0f;
@@ -51,11 +51,11 @@ __global__ __launch_bounds__(256) void xent_prepare_kernel(PrepareArgs a, uint32
         c += __shfl_xor(c, d);
     }
     if ((threadIdx.x & 63) == 0) {
-        top[threadIdx.x >> 6] = m;
+        tops[threadIdx.x >> 6] = m;
         cnt[threadIdx.x >> 6] = c;
     }
     __syncthreads();
-    m = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+    m = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
     c = (cnt[0] + cnt[1]) + (cnt[2] + cnt[3]);
     float g = 1.0f;
     if (a.reduction != VA_REDUCE_NONE) {
@@ -63,11 +63,11 @@ __global__ __launch_bounds__(256) void xent_prepare_kernel(PrepareArgs a, uint32
         if (a.reduction == VA_REDUCE_MEAN) g /= float(max(c, 1u));
         m = fabsf(g);
     }
-    if (!(m > 0.0f) || !(m < INFINITY)) m = 16384.0f;
-    if (blockIdx.x == 0 && threadIdx.x == 0) *a.mul = a.scale * (m / 16384.0f);
+    if (!(m > 0.0f) || !(m < INFINITY)) m = a.top;
+    if (blockIdx.x == 0 && threadIdx.x == 0) *a.mul = a.scale * (m / a.top);
     auto of_row = [&](uint32_t t) {
         const int64_t y = a.targets[t];
-        return y != a.ignore && y >= 0 && y < int64_t(a.V) ? (a.reduction == VA_REDUCE_NONE ? a.grad[t] : g) / m * 16384.0f : 0.0f;
+        return y != a.ignore && y >= 0 && y < int64_t(a.V) ? (a.reduction == VA_REDUCE_NONE ? a.grad[t] : g) / m * a.top : 0.0f;
     };
     const uint32_t t0 = blockIdx.x * rows_per, t1 = min(a.T, t0 + rows_per);
     for (uint32_t t = t0 + threadIdx.x; t < t1; t += 256) a.gk[t] = of_row(t);
@@ -467,7 +467,9 @@ va_status va_xent_backward(va_context* ctx, const va_xent_desc* desc, const floa
     VA_CHECK_STATUS(sc.verify(need));
 
     // gk, and the hidden rows ended by zeros
-    const PrepareArgs pa{grad, d->targets, T, V, d->ignore_index, int(reduction), d->scale, gk, mul, odd};
+    // (dl's largest values: 2^14 in fp16, whose range is short; in types of fp32's range 1, so that no sum of dl w or dl h
+    // passes fp32 where the gradient does not)
+    const PrepareArgs pa{grad, d->targets, T, V, d->ignore_index, int(reduction), d->scale, dt == VA_DTYPE_F16 ? 0x1p14f : 1.0f, gk, mul, odd};
     const bool together = T <= kPrepareRows;
     const uint32_t rows_per = together ? std::max(4u, ceil_div(T, 512)) : T;
     if (dt == VA_DTYPE_F32)
