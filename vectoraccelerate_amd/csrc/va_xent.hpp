@@ -110,10 +110,11 @@ __device__ __forceinline__ f32x4 logits4(const LogitShared<KIND, OFF, TR>& sm, c
     if constexpr (KIND == g16::PLANES) x = *reinterpret_cast<const f32x4*>(sm.inv + r);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-        float a = acc[4 * j + e];
-        if constexpr (KIND == g16::PLANES) a *= x[e];
-        if constexpr (OFF == OFF_NONE) v[e] = a * c;
-        else v[e] = NATURAL && o[e] == -INFINITY ? -INFINITY : fmaf(a, c, o[e]);
+        const float a = acc[4 * j + e];
+        // (the factors first: an item's alone may take the sum past fp32 where the row's brings it back)
+        const float f = KIND == g16::PLANES ? x[e] * c : c;
+        if constexpr (OFF == OFF_NONE) v[e] = a * f;
+        else v[e] = NATURAL && o[e] == -INFINITY ? -INFINITY : fmaf(a, f, o[e]);
     }
     return v;
 }
