@@ -10,7 +10,7 @@
 // group's largest value is a few lane exchanges away).  Longer rows are read twice, the second time from cache.  Values are loaded 16 bytes at a time whatever their
 // alignment (global loads on gfx950 need none beyond the element's); a row's last, partial chunk element by
 // element.  A row's sums are fp32 where it is held in registers (a lane's chain of at most 32 values, then a tree) and fp64
-// in longer rows; the weight's gradient is a chain of fp32 over the rows of each share, then a tree.
+// in longer rows and where the squares leave fp32's range; the weight's gradient is a chain of fp32 over the rows of each share, then a tree.
 //
 // Measured: 65,536 x 1536 bf16 with residual to int8 by groups 156 us = 4.5 TB/s, and back 53 us = 5.7 TB/s; 10,007
 // x 513 fp32 forward 18 us and backward 18 + 4 us (4.6 TB/s each); 37,289 x 768 bf16 forward 44 us = 5.2 TB/s.  One
@@ -164,9 +164,8 @@ template <int DT, int OUT, int WPR, int C>
 __global__ __launch_bounds__(256) void rms_norm_kernel(RmsArgs a) {
     using T = ElemT<DT>;
     constexpr int NT = 64 * WPR, E = OUT == OUT_SAME ? 16 / int(sizeof(T)) : 8;
-    using S = std::conditional_t<C == 0, double, float>;  // of the row's sum
-    __shared__ S part[4];
-    __shared__ float tops[4];
+    __shared__ float part[4];
+    __shared__ double wide[4];
     const uint32_t t = a.t0 + (WPR == 1 ? blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x);
     if (t >= a.T) return;  // (a whole wave, or the workgroup)
     const uint32_t tid = WPR == 1 ? threadIdx.x & 63 : threadIdx.x;
@@ -181,23 +180,33 @@ __global__ __launch_bounds__(256) void rms_norm_kernel(RmsArgs a) {
         return v;
     };
     F<E> r[C ? C : 1];
-    S ss = 0;
+    double ds = 0.0;
+    const auto add = [&](F<E> v) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) ds = fma(double(v[e]), double(v[e]), ds);
+    };
+    const auto inverse = [&] { return float(1.0 / sqrt(row_sum<WPR>(ds, wide) / double(D) + double(a.eps))); };
+    float inv;
     if constexpr (C > 0) {
+        float ss = 0.0f;
 #pragma unroll
         for (int c = 0; c < C; ++c) r[c] = sum_of((c * NT + tid) * E);
 #pragma unroll
         for (int c = 0; c < C; ++c)
 #pragma unroll
             for (int e = 0; e < E; ++e) ss = fmaf(r[c][e], r[c][e], ss);
-    } else {
-        for (uint32_t c = 0; c < chunks; ++c) {
-            const F<E> v = sum_of((c * NT + tid) * E);
+        ss = row_sum<WPR>(ss, part);
+        if (ss > 0x1p-100f && ss < 0x1p126f) {
+            inv = 1.0f / sqrtf(ss / float(D) + a.eps);
+        } else {  // (the whole row's threads) squares near or past the ends of fp32
 #pragma unroll
-            for (int e = 0; e < E; ++e) ss = fma(double(v[e]), double(v[e]), ss);
+            for (int c = 0; c < C; ++c) add(r[c]);
+            inv = inverse();
         }
+    } else {
+        for (uint32_t c = 0; c < chunks; ++c) add(sum_of((c * NT + tid) * E));
+        inv = inverse();
     }
-    ss = row_sum<WPR>(ss, part);
-    const float inv = 1.0f / sqrtf(float(ss / S(D)) + a.eps);
     if (a.inverse && tid == 0) a.inverse[t] = inv;
 
     // y of a chunk, the new residual stored on the way (once)
@@ -246,7 +255,7 @@ __global__ __launch_bounds__(256) void rms_norm_kernel(RmsArgs a) {
                     m = top(m, biggest(y_of(d, sum_of(d), false)));
                 }
             }
-            s = row_top<WPR>(m, tops) / most;
+            s = row_top<WPR>(m, part) / most;
             if (tid == 0) a.scales[t] = s;
         }
         auto emit = [&](uint32_t d, F<E> y) {
