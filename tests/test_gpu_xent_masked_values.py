@@ -43,3 +43,19 @@ def test_large_hidden_rows(ctx, T, V, D, size, dtype):
     h, w = h * 2.0**size, w * 2.0**-size
     w[masked.cuda()] = 2.0 ** (130 - size)
     _check(ctx, h, w, y, offsets=off)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("T,V", [(1, 60), (10, 900), (40, 300), (70, 130)])
+@pytest.mark.parametrize("stages", [5, 9, 10, 12, 13, 14, 15, 17, 18, 22, 25, 34])
+def test_rows_next_to_masked_ones(ctx, T, V, stages, dtype):
+    """Rows whose last 128 bytes are begun by a single dword and continued by the next item's, which is masked and holds NaN
+    or inf; tiles of so many stages that groups of waves share them, in any remainder."""
+    D = (stages - 1) * 32 + 1
+    if dtype != torch.float32:
+        D *= 2
+    h, w, y, g = _inputs(T, V, D, dtype, T + D)
+    masked, off = _masked(V, y, g)
+    w[masked.cuda()] = torch.inf
+    w[torch.nonzero(masked)[::2].flatten().cuda()] = torch.nan
+    _check(ctx, h, w, y, offsets=off)

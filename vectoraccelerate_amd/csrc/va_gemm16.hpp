@@ -362,10 +362,13 @@ __global__ __launch_bounds__(Epi::Shape::THREADS, Epi::Shape::PER_SIMD) void gem
             s1 = uint32_t(uint64_t(total_stages) * (tile.part + 1) / a.parts);
         }
         ns = s1 - s0;
-        if constexpr (Sh::SLICES > 1) {  // (the last slices' may lie past the tile's: zeros)
-            ns = (ns + Sh::SLICES - 1) / Sh::SLICES;
-            s0 += uint32_t(slice) * ns;
-            s1 = min(s1, s0 + ns);
+        if constexpr (Sh::SLICES > 1) {
+            // even shares: all of a slice's ns stages but one at most are the tile's (past its share: zeros), so k ends within
+            // the last two, where the loop below looks for it
+            const uint32_t n = ns, from = s0;
+            ns = (n + Sh::SLICES - 1) / Sh::SLICES;
+            s0 = from + n * uint32_t(slice) / Sh::SLICES;
+            s1 = from + n * uint32_t(slice + 1) / Sh::SLICES;
         }
     };
     // load i of the tile's stage s into slot `slot` (past the last stage: zeros)
