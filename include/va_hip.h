@@ -506,7 +506,10 @@ typedef struct {
 va_status va_xent_forward(va_context* ctx, const va_xent_desc* desc, float* out_loss, float* out_lse,
                           va_reduction reduction, float* out_reduced);
 /* Gradients of the reduced loss (times *grad, 1 when grad is NULL) or, without a reduction, of
- * sum_t grad[t] loss_t.  lse: va_xent_forward's.  Either output may be NULL. */
+ * sum_t grad[t] loss_t.  lse: va_xent_forward's.  Either output may be NULL.  Scratch: the logits'
+ * gradients of a piece of the items, up to 512 MB or, where the rows are more than that holds for 256
+ * items, 640 bytes a row (fp32 1152); copied rows and items, the latter up to 256 MB a form; and fp32
+ * shares of the hidden gradient, rows x dim each. */
 va_status va_xent_backward(va_context* ctx, const va_xent_desc* desc, const float* lse, va_reduction reduction,
                            const float* grad, void* out_grad_hidden, uint64_t grad_hidden_stride,
                            void* out_grad_items, uint64_t grad_items_stride);

@@ -9,7 +9,7 @@
 // pieces; for each piece the logits are computed again, dl leaves the product's epilogue as 16-bit
 // values in a bounded workspace, and two more products read it, along its rows and across them: dh accumulates over
 // the pieces in fp32, dw's rows of the piece are final.  So a training step is four products (one
-// of them the recomputation), and the memory is that of one piece.
+// of them the recomputation), and the memory is that of one piece and of dh's shares.
 //
 // Precision: fp16 / bf16 operands enter the matrix cores as they are, sums are fp32.  dl is rounded
 // once to the operands' type for the second products (relative 2^-11 / 2^-8 a value, like the

@@ -2,8 +2,8 @@
 //
 // Launches of a call: the rows' factors and the hidden rows ended by zeros, then per piece of the items (fp32 rows
 // for a product in planes: those first) the logits again with dl as their epilogue's result, dh += dl w,
-// dw = dl^T h; at the end the shares of dh summed, where there are several.  dl is bounded by
-// kGradBudget: a piece of 65,536 items for 4096 rows (pieces of 8,192 to 32,768, whose dl stays in the last
+// dw = dl^T h; at the end the shares of dh summed, where there are several.  dl of a piece stays within
+// kGradBudget, or is that of 256 items where the rows are too many for it: a piece of 65,536 items for 4096 rows (pieces of 8,192 to 32,768, whose dl stays in the last
 // level cache, ran 35 to 6 % slower: each product then ends in a round of half-idle CUs).
 //
 // What bounds it: the matrix cores.  A piece of 65,536 items by 4096 rows of 768 in bf16 takes 0.47 ms for the logits and dl
