@@ -27,8 +27,8 @@
 // What bounds it: few rows, the stream of the items (10 x 1M x 768 in fp16 258 us, 5.9 TB/s); many, the matrix cores and
 // after them the exp of every logit, which share a SIMD's waves (4096 x 262,144 x 768 in bf16 1.60 ms, 1.03
 // PFLOP/s; 1023 x 49,999 x 300 in fp16 53 us, 0.58 PFLOP/s with five stages a tile); fp32 rows in planes, three
-// times the products and the copies (512 x 100,003 x 384: 122 + 57 us); a small collection, latency
-// (1 x 10,000 x 768 in bf16: 9 + 5 us).
+// times the products and the copies (512 x 100,003 x 384: 111 + 52 us); a small collection, latency
+// (1 x 10,000 x 768 in bf16: 10 + 4 us).
 #include "va_xent.hpp"
 
 namespace va {
