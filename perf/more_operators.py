@@ -7,8 +7,7 @@ Three operators next to the loss, the norm and the clipping of perf/operators.py
   quant / score   rows in microscaled 4-bit floating point (e2m1 in blocks of 32 with a power of two each): coding
                   and reading back, and the product of queries with all items of a collection; the queries are
                   coded in the call ("mx") or stay in 16 bits ("plain")
-  sample          an item for each row of logits, by temperature, top-k, top-p and min-p, from a given random number (the first
-                  in the order of the items whose kept probability, added up, exceeds it)
+  sample          an item for each row of logits, by temperature, top-k, top-p and min-p, from a given random number
 
 Sizes: T rows, V items, D dimensions; "type" is the type of the parameters, rows or logits.
 """
@@ -354,16 +353,14 @@ def _run_plain(s):
     x, order = torch.sort(x.float(), dim=1, descending=True, stable=True)
     x = x.double()
     w = torch.exp((x - x[:, :1]) / torch.where(temperature == 0, 1, temperature))
-    before = torch.nn.functional.pad(w.cumsum(dim=1)[:, :-1], (1, 0))
+    upto = w.cumsum(dim=1)
+    before = torch.nn.functional.pad(upto[:, :-1], (1, 0))
     keep = torch.arange(V, device="cuda") < k
     total = (w * keep).sum(dim=1, keepdim=True)
     keep &= (before < p * total) & (w >= m)
-    # drawn in the order of the items
-    w = torch.zeros_like(w).scatter_(1, order, w * keep)
-    upto = w.cumsum(dim=1)
-    total = upto[:, -1:]
-    at = (upto <= u.double().view(T, 1) * total).sum(dim=1, keepdim=True).clamp(max=V - 1)
-    return {"items": at.view(T), "log_probability": torch.log(w.gather(1, at) / total).float().view(T)}
+    total = upto.gather(1, keep.sum(dim=1, keepdim=True) - 1)
+    at = ((upto <= u.double().view(T, 1) * total) & keep).sum(dim=1, keepdim=True).minimum(keep.sum(dim=1, keepdim=True) - 1)
+    return {"items": order.gather(1, at).view(T), "log_probability": torch.log(w.gather(1, at) / total).float().view(T)}
 
 
 # ---------------------------------------------------------------------------------------
@@ -435,12 +432,10 @@ def exact(case, seed):
         # the nucleus ends with the first item that brings the sum to p; min-p and top-k may end it before
         kept = torch.searchsorted(cumulated, setting[2][:, None] * all_k).squeeze(1) + 1
         kept = torch.where(setting[2] >= 1, V, kept).minimum(k).minimum((probability >= setting[3][:, None] * probability[:, :1]).sum(1))
-        probability[torch.arange(V, device="cuda") >= kept[:, None]] = 0.0
-        probability = torch.gather(probability, 1, torch.argsort(order, dim=1))
-        cumulated = torch.cumsum(probability, 1)
-        at = torch.searchsorted(cumulated, u[rows, None] * cumulated[:, -1:], right=True).minimum(torch.tensor(V - 1, device="cuda"))
-        items.append(at.squeeze(1))
-        logs.append((probability.gather(1, at) / cumulated[:, -1:]).log().squeeze(1))
+        all_kept = cumulated.gather(1, kept[:, None] - 1)
+        at = torch.searchsorted(cumulated, u[rows, None] * all_kept, right=True).squeeze(1).minimum(kept - 1)[:, None]
+        items.append(order.gather(1, at).squeeze(1))
+        logs.append((probability.gather(1, at) / all_kept).log().squeeze(1))
     return {"items": torch.cat(items), "log_probability": torch.cat(logs)}
 
 
