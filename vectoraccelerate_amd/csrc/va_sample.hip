@@ -1081,7 +1081,9 @@ constexpr uint32_t kSlices = 64;
 struct Joined {
     // cleared before the first pass
     uint32_t count[kBins + 4];
-    uint32_t tops, listed, failed, pad;
+    uint32_t tops, listed;
+    uint32_t failed;   // set by the first pass alone: the sample holds no value to refer to
+    uint32_t dropped;  // set by the second pass and read by the last kernel alone, so that a workgroup's waves see one `failed`
     // written by it and the second
     Mid mid;
     float top[kSlices];
@@ -1170,8 +1172,7 @@ __global__ __launch_bounds__(kThreads, 6) void sample_two_kernel(Row a, Joined* 
         good = between(x.n, s, q, m);
     }
     if (!good) {  // (every workgroup of the row finds the same)
-        // (others still read `failed`: they find what this one found)
-        if (blockIdx.x == 0 && tid == 0) atomicExch(&j.failed, 1u);
+        if (blockIdx.x == 0 && tid == 0) j.dropped = 1;
         return;
     }
     pass_two(x, s, part, q, m);
@@ -1213,7 +1214,7 @@ __global__ __launch_bounds__(kThreads, 4) void sample_three_kernel(Row a, Joined
     const Joined& j = joined[row];
     const Logits<T> x{static_cast<const T*>(a.logits) + row * a.stride, a.V};
     bool done = false;
-    if (!j.failed) {
+    if (!j.failed && !j.dropped) {
         const Settings s = settings_of(a, row);
         const Kind kind = kind_of(s, x.n);
         const Part part = whole_of(x.n);
