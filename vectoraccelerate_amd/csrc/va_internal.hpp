@@ -233,8 +233,7 @@ __device__ __forceinline__ void lds_dma16_so(const dma_rsrc& rsrc, uint32_t voff
                  : "memory");
 }
 
-// The one-dword form: lane i's 4 bytes land at lds_addr + 4*i (256 B per wave).  Used as an L2
-// prefetch whose data is not needed.
+// The one-dword form: lane i's 4 bytes land at lds_addr + 4*i (256 B per wave).
 __device__ __forceinline__ void lds_dma4(const dma_rsrc& rsrc, uint32_t voff, uint32_t lds_addr) {
     dma_rsrc r;
     r[0] = __builtin_amdgcn_readfirstlane(rsrc[0]);

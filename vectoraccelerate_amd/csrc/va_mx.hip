@@ -13,6 +13,7 @@
 #include <type_traits>
 
 #include "va_internal.hpp"
+#include "va_mx_tile.hpp"
 
 namespace va {
 namespace {
@@ -30,7 +31,7 @@ uint32_t size_of(va_dtype d) { return d == VA_DTYPE_F32 ? 4 : 2; }
 bool aligned(const void* p, uintptr_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
 
 constexpr uint32_t kGroup = 128;  // values of a group
-constexpr uint32_t kCodes = 64;   // bytes of its codes
+constexpr uint32_t kCodes = kMxCodes;  // bytes of its codes
 constexpr uint32_t groups_of(uint32_t dim) { return (dim + kGroup - 1) / kGroup; }
 
 // values [d, d + 8) of a row of dim; behind its end: zeros
@@ -257,39 +258,37 @@ __global__ __launch_bounds__(Sh::THREADS, Sh::PER_SIMD) void mx_tile_kernel(Prod
 
     // Codes: RL LDS rows a load, first the queries', then the items'; lane: row l / CH of them, physical chunk l % CH = logical chunk
     // (l % CH) ^ (the row's swizzle).  Scales: a dword of 64 rows a load, one group's rows behind the other's, first the items'.
-    const auto item_of = [](uint32_t r) { return r / 64u * 64u + r % 32u * 2u + r % 64u / 32u; };  // of an LDS row
-    const auto swizzle = [](uint32_t row) { return (GS == 1 ? row >> 2 : row >> 1) & uint32_t(CH - 1); };
     uint32_t code_off[LC], scale_off[LS];
 #pragma unroll
     for (int j = 0; j < LC; ++j) {
         const uint32_t row = uint32_t(wave + WAVES * (j < LQ ? j : j - LQ)) * RL + uint32_t(lane / CH);
-        code_off[j] = (j < LQ ? row * qp : item_of(row) * xp) + 16u * (uint32_t(lane % CH) ^ swizzle(row));
+        code_off[j] = j < LQ ? mx_code_offset<GS>(row, uint32_t(lane % CH), row, qp) : mx_code_offset<GS>(row, uint32_t(lane % CH), mx_item_of(row), xp);
     }
 #pragma unroll
     for (int j = 0; j < LS; ++j) {
         const uint32_t g = uint32_t(wave + WAVES * (j < LXS ? j : j - LXS)), blocks = uint32_t(j < LXS ? Sh::TI : Sh::TQ) / 64;
         const uint32_t row = g % blocks * 64 + uint32_t(lane);
         // (a wave without rows of its own loads zeros into a place of its own)
-        scale_off[j] = g < blocks * GS ? (j < LXS ? item_of(row) * xsp : row * qsp) + 4u * (g / blocks) : kDmaSkip;
+        scale_off[j] = g < blocks * GS ? (j < LXS ? mx_scale_offset(g / blocks, mx_item_of(row), xsp) : mx_scale_offset(g / blocks, row, qsp)) : kDmaSkip;
     }
     dma_rsrc from_q, from_x, from_qs, from_xs;
     const auto open = [&](uint32_t i) {
         uint32_t qb = 0, ib = 0;
         const bool there = tiles.at(i, qb, ib);
-        const uint32_t q0 = qb * Sh::TQ, i0 = ib * Sh::TI, nq = min(uint32_t(Sh::TQ), a.T - q0) - 1, ni = min(uint32_t(Sh::TI), a.V - i0) - 1;
+        const uint32_t q0 = qb * Sh::TQ, i0 = ib * Sh::TI, nq = min(uint32_t(Sh::TQ), a.T - q0), ni = min(uint32_t(Sh::TI), a.V - i0);
         // (where there is no tile more: nothing lies behind the descriptors, and zeros arrive)
-        from_q = make_dma_rsrc(static_cast<const char*>(a.queries) + uint64_t(q0) * qp, there ? nq * qp + groups * kCodes : 0);
-        from_x = make_dma_rsrc(a.codes + uint64_t(i0) * xp, there ? ni * xp + groups * kCodes : 0);
-        from_qs = make_dma_rsrc(a.query_scales + uint64_t(q0) * qsp, there ? nq * qsp + groups * 4 : 0);
-        from_xs = make_dma_rsrc(a.scales + uint64_t(i0) * xsp, there ? ni * xsp + groups * 4 : 0);
+        from_q = make_dma_rsrc(static_cast<const char*>(a.queries) + uint64_t(q0) * qp, there ? mx_records(nq, qp, groups, kMxCodes) : 0);
+        from_x = make_dma_rsrc(a.codes + uint64_t(i0) * xp, there ? mx_records(ni, xp, groups, kMxCodes) : 0);
+        from_qs = make_dma_rsrc(a.query_scales + uint64_t(q0) * qsp, there ? mx_records(nq, qsp, groups, kMxScales) : 0);
+        from_xs = make_dma_rsrc(a.scales + uint64_t(i0) * xsp, there ? mx_records(ni, xsp, groups, kMxScales) : 0);
         return there;
     };
     uint32_t ahead_tile = 0, ahead_stage = 0, ahead_slot = 0;
     // load j of the L of the stage that is three ahead
     const auto load = [&](int j) {
         const uint32_t to = lds0 + ahead_slot * uint32_t(Sh::SLOT) + uint32_t(wave) * (j < LC ? 1024u : 256u);
-        if (j < LC) lds_dma16_so(j < LQ ? from_q : from_x, code_off[j], ahead_stage * uint32_t(Sh::ROWB), to + uint32_t(j * WAVES * 1024));
-        else lds_dma4_so(j - LC < LXS ? from_xs : from_qs, scale_off[j - LC], ahead_stage * uint32_t(4 * GS), to + uint32_t(Sh::SCALES + (j - LC) * WAVES * 256));
+        if (j < LC) lds_dma16(j < LQ ? from_q : from_x, mx_stage_offset(code_off[j], ahead_stage, Sh::ROWB), to + uint32_t(j * WAVES * 1024));
+        else lds_dma4(j - LC < LXS ? from_xs : from_qs, mx_stage_offset(scale_off[j - LC], ahead_stage, kMxScales * GS), to + uint32_t(Sh::SCALES + (j - LC) * WAVES * 256));
     };
     const auto loaded = [&] {
         ahead_slot = ahead_slot == 2 ? 0 : ahead_slot + 1;
@@ -301,7 +300,7 @@ __global__ __launch_bounds__(Sh::THREADS, Sh::PER_SIMD) void mx_tile_kernel(Prod
     const auto barrier = [] { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
 
     // fragments: block b's lane reads row l32 of it, half hh of a step's 64 values
-    const int swz = int(swizzle(uint32_t(l32)));
+    const int swz = int(mx_swizzle<GS>(uint32_t(l32)));
     const char* const my_q = lds + (wq * 64 + l32) * Sh::ROWB;
     const char* const my_x = lds + (Sh::TQ + wi * 64 + l32) * Sh::ROWB;
     const char* const my_xs = lds + Sh::SCALES + (wi * 64 + l32) * 4;
