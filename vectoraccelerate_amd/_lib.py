@@ -321,6 +321,7 @@ class SampleDesc(C.Structure):
         ("top_k", C.c_int32),
         ("top_p", C.c_float),
         ("min_p", C.c_float),
+        ("order", C.c_int32),
         ("workspace", C.c_void_p),
         ("workspace_bytes", C.c_uint64),
     ]

@@ -3,8 +3,8 @@
 // With x_j the logits of a row, M their largest and T the temperature, item j weighs w_j = exp((x_j - M) / T).  Ordered by
 // (x descending, j ascending) every truncation keeps a prefix:
 //   top-k  the first k;        top-p  the fewest whose weights reach p of those that top-k keeps;        min-p  w_j >= m
-// and the drawn item is the first, in the order of the items, at which the kept weights added up exceed u times their sum.
-// NaN and -inf are no items.
+// and the drawn item is the first, in the order of the items or in that of the truncations, at which the kept weights added up exceed u
+// times their sum.  NaN and -inf are no items.
 //
 // Weights and their sums are fp64 throughout: an item next to a border has to fall on its side of it, and fp32's weights of
 // 100,000 items would move one draw in a hundred.  A sum's order is fixed, so results repeat bit for bit.
@@ -14,6 +14,9 @@
 // above the sample's largest.  From the counts follow the bins that hold the cut.  The second pass lists their items, some dozens
 // to some thousands, and adds up the weights above them by chunks of the row.  The list sorted gives the cut to the item, the
 // chunks' sums the chunk that u falls into, and that chunk the item.  Where nothing is cut one pass gives the chunks' sums.
+// Along falling logits (FALLING) the drawn item is the end of a prefix too, that whose weights exceed u times what is kept.  A list
+// from the top holds it beside the cut.  Of long prefixes the list near the cut, or a pass without a list, gives what is kept, and a further
+// pass, its bins chosen as before, lists the items around u times that; where nothing is cut the second pass does.
 // A long row's passes are divided among workgroups, with a launch for each pass; a row that the quick way cannot take (+inf, more
 // items of one value than a list holds) goes through as many passes as it needs.
 //
@@ -22,6 +25,7 @@
 // 15; 1 x 10,000, top 50: 23 us in one launch).
 #include <algorithm>
 #include <cmath>
+#include <cstddef>
 
 #include "va_internal.hpp"
 
@@ -39,6 +43,7 @@ struct Row {
     int64_t* items;
     float* log_probability;
     uint32_t rows, V;
+    bool falling;  // drawn along falling logits
 };
 
 // What a row is drawn by.  Values on the device that make no sense are taken as the nearest that does.
@@ -59,6 +64,9 @@ __device__ __forceinline__ Settings settings_of(const Row& a, uint32_t row) {
     s.m = m > 0.0f ? fmin(double(m), 1.0) : 0.0;
     return s;
 }
+
+// Along falling logits u is kept below 1, so that no rounding of what is kept takes the draw past its last item.
+__device__ __forceinline__ double inner(float u) { return fmin(fmax(double(u), 0.0), 0x1.fffffep-1); }
 
 // Larger logits have larger keys; 0: no item.
 constexpr uint32_t kLowest = 0x00800000u;  // the key of the lowest finite value
@@ -176,9 +184,9 @@ __device__ Cut cut_by_count(const Logits<T>& x, uint32_t k, Shared& sh) {
     return {known, left};
 }
 
-// The fewest items whose weights reach `target`, which those with keys of at least `least` do.
+// The fewest items whose weights reach `target` (past: exceed it), which those with keys of at least that of `most` do.
 template <class T>
-__device__ Cut cut_by_weight(const Logits<T>& x, double target, const Cut& most, double top, double c, Shared& sh) {
+__device__ Cut cut_by_weight(const Logits<T>& x, double target, bool past, const Cut& most, double top, double c, Shared& sh) {
     uint32_t known = 0;
     double before = 0.0;
     for (int shift = 30; shift >= 0; shift -= 2) {
@@ -198,27 +206,28 @@ __device__ Cut cut_by_weight(const Logits<T>& x, double target, const Cut& most,
                 found = d;
                 before = at;
                 at += sums[d];
-                if (at >= target) break;
+                if (past ? at > target : at >= target) break;
             }
         }
         if (found < 0) return most;  // nothing of these weighs anything
         known = known << 2 | uint32_t(found);
         __syncthreads();
     }
-    const double w = weight(value_of(known), top, c), n = ceil((target - before) / w);
+    const double w = weight(value_of(known), top, c), n = past ? floor((target - before) / w) + 1.0 : ceil((target - before) / w);
     return {known, n < 1.0 ? 1u : n < 4294967295.0 ? uint32_t(n) : 0xFFFFFFFFu};
 }
 
-// The index up to which items with the cut's key are kept.
+// The index up to which items with the cut's key are kept; of: that of the last of them.
 template <class T>
-__device__ uint32_t last_tie(const Logits<T>& x, const Cut& cut, Shared& sh) {
+__device__ uint32_t last_tie(const Logits<T>& x, const Cut& cut, bool of, Shared& sh) {
     uint32_t n = 0;
     for (uint32_t i = threadIdx.x; i < x.n; i += kThreads) n += key_of(x(i)) == cut.key;
-    if (block_count(n, sh) <= cut.ties) return x.n - 1;
+    n = block_count(n, sh);
+    if (!of && n <= cut.ties) return x.n - 1;
     // a wave goes through the row; the others wait
     __syncthreads();
     if (threadIdx.x < 64) {
-        uint32_t left = cut.ties;  // at least 1
+        uint32_t left = min(cut.ties, n);  // at least 1
         for (uint32_t b = 0; b < x.n; b += 64) {
             const uint32_t i = b + threadIdx.x;
             uint64_t m = __ballot(i < x.n && key_of(x(min(i, x.n - 1))) == cut.key);
@@ -266,7 +275,7 @@ __device__ __noinline__ void sample_slowly(Row a, uint32_t row, Logits<T> x, Sha
         }
         sum = block_sum(sum, sh);
         if (cut.ties != 0xFFFFFFFFu) sum += double(cut.ties) * weight(value_of(cut.key), top, s.c);
-        const Cut by = cut_by_weight(x, s.p * sum, cut, top, s.c, sh);
+        const Cut by = cut_by_weight(x, s.p * sum, false, cut, top, s.c, sh);
         if (by.shorter(cut)) cut = by;
     }
     if (s.m > 0.0) {
@@ -280,11 +289,26 @@ __device__ __noinline__ void sample_slowly(Row a, uint32_t row, Logits<T> x, Sha
         const Cut by{lo, 0xFFFFFFFFu};
         if (by.shorter(cut)) cut = by;
     }
-    const uint32_t last = cut.ties == 0xFFFFFFFFu ? x.n - 1 : last_tie(x, cut, sh);
+    const uint32_t last = cut.ties == 0xFFFFFFFFu ? x.n - 1 : last_tie(x, cut, false, sh);
     const auto kept = [&](uint32_t i, float v) {
         const uint32_t k = key_of(v);
         return k > cut.key || (k == cut.key && i <= last);
     };
+    if (a.falling) {
+        double sum = 0.0;
+        for (uint32_t i = threadIdx.x; i < x.n; i += kThreads) {
+            const float v = x(i);
+            if (kept(i, v)) sum += weight(v, top, s.c);
+        }
+        sum = block_sum(sum, sh);
+        const Cut by = cut_by_weight(x, inner(a.uniforms[row]) * sum, true, cut, top, s.c, sh);
+        const uint32_t item = last_tie(x, by, true, sh);
+        if (threadIdx.x == 0) {
+            a.items[row] = item;
+            if (a.log_probability) a.log_probability[row] = float(log(weight(value_of(by.key), top, s.c) / sum));
+        }
+        return;
+    }
     // the kept weights of chunks of the row, then of one of them item by item
     uint32_t size = 64;
     while (uint64_t(size) * kMostChunks < x.n) size *= 2;
@@ -661,6 +685,9 @@ struct Mid {
     uint32_t tops;         // items above ref
     int first, end;        // the bins whose items are listed (first -1: and what lies above them)
     uint32_t least;        // the least key that min-p keeps
+    // along falling logits
+    double kept, target;   // what is kept weighs (the second pass: that of it which lies above the listed items); the drawn item is the first past
+    bool whole;            // target, which is negative as long as it is not known; whether all that min-p keeps is listed
 };
 struct Kind {
     bool by_count, by_weight;
@@ -724,15 +751,15 @@ __device__ bool begin(const Logits<T>& x, Q& q, Mid& m) {
 }
 
 // The first pass.  Neither top-k nor top-p: the chunks' sums, or with min-p, which needs the row's largest value, that alone.  Else
-// the bins' counts, what lies above ref listed, and, where top-k does not cut, the sum of all weights.
-template <class T, class Q>
+// the bins' counts, what lies above ref listed, and, where top-k does not cut, the sum of all weights.  FALLING: these always.
+template <bool FALLING, class T, class Q>
 __device__ void pass_one(const Logits<T>& x, const Settings& s, const Part& part, Q& q, Mid& m) {
     const Kind kind = kind_of(s, x.n);
     const uint32_t lane = threadIdx.x & 63;
     float top = -__builtin_inff();
     m.all = 0.0;
     m.tops = 0;
-    if (kind.sums()) {
+    if (!FALLING && kind.sums()) {
         double sum = 0.0;
         through(x, part, [&](uint32_t, const float(&v)[8]) {
 #pragma unroll
@@ -785,80 +812,151 @@ __device__ void pass_one(const Logits<T>& x, const Settings& s, const Part& part
 // Whether weights that refer to ref have room in fp64, and the list held what lies above it.
 __device__ __forceinline__ bool fits(const Settings& s, const Mid& m) { return m.top < __builtin_inff() && m.tops <= kTops && (double(m.top) - double(m.ref)) * s.c < 900.0; }
 
+// The bins' counts added up: a thread's four sums (up to each bin and with it), what lies before them, the items of all bins and of the last.
+struct Counts {
+    uint32_t mine[4], before, items, last;
+};
+__device__ Counts counts_of(Quick& q) {
+    Counts c;
+    c.last = q.count[kBins - 1];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) c.mine[e] = q.count[4 * threadIdx.x + e];
+    c.before = quick_before(c.mine[0] + c.mine[1] + c.mine[2] + c.mine[3], c.items, q.word);
+    c.mine[0] += c.before;
+#pragma unroll
+    for (int e = 1; e < 4; ++e) c.mine[e] += c.mine[e - 1];
+    static_assert(kBins == 4 * kThreads, "four bins a thread");
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < 4; ++e) q.count[4 * threadIdx.x + e] = c.mine[e];
+    __syncthreads();
+    return c;
+}
+// items of the bins up to b, whose counts are added up
+__device__ __forceinline__ uint32_t upto(const Quick& q, int b) { return b < 0 ? 0u : q.count[min(b, int(kBins) - 1)]; }
+
+// The bin with the k-th item.
+__device__ void range_by_count(uint32_t k, const Counts& counts, Quick& q, Mid& m) {
+    uint32_t c = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) c += m.tops + counts.mine[e] < k;
+    m.end = int(quick_count(c, q));
+    if (k <= m.tops) m.end = -1;
+}
+// The bins in which what lies behind may come to weigh `need`, and the one where it likely does: from the least weights up, each item
+// taken for one in its bin's middle and so off by at most half a bin's width (in the last bin, which has no lower end, for too large).
+__device__ int range_by_weight(const Settings& s, double need, const Counts& counts, Quick& q, Mid& m) {
+    const Bins bins(m, s);
+    const double width = bins.per > 0.0f ? s.c / double(bins.per) : 0.0, off = exp2_of(0.501 * width);
+    const double open = double(counts.last) * exp2_of(-(double(kBins) - 0.5) * width);
+    double tail[4], sum;
+    uint32_t above = 0, each = 0, within = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const uint32_t c = counts.mine[e] - (e ? counts.mine[e - 1] : counts.before);
+        tail[e] = c ? double(c) * exp2_of(-(double(4 * threadIdx.x + e) + 0.5) * width) : 0.0;
+    }
+    double have = quick_before(tail[0] + tail[1] + tail[2] + tail[3], sum, q.part);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        have += tail[e];
+        const double behind = sum - have;
+        above += behind - open > need * off;
+        each += behind > need;
+        within += behind * off > need;
+    }
+    above = quick_count(above, q), each = quick_count(each, q), within = quick_count(within, q);
+    m.first = bins.per > 0.0f && sum - open > need * off ? int(above) : -1;
+    m.end = sum * off > need ? int(min(within, kBins - 1)) : -1;
+    return int(min(each, kBins - 1));
+}
+// As many of these bins as a list holds: from the top if that is few; of many items those in the middle, where errors cancel out.
+__device__ bool narrow(int at, const Quick& q, Mid& m) {
+    for (;;) {
+        if (m.first <= 0 || m.tops + upto(q, m.end) <= kFew) m.first = -1;
+        if ((m.first < 0 ? m.tops + upto(q, m.end) : upto(q, m.end) - upto(q, m.first - 1)) <= kListed) return true;
+        const int first = m.first < 0 ? 0 : m.first;
+        if (m.end <= at && first >= at && m.first >= 0) return false;
+        m.first = min(first + max((at - first + 1) / 2, 1), max(at, 1));
+        m.end = max(m.end - max((m.end - at + 1) / 2, 0), at);
+    }
+}
+
 // From the counts, which bins' items are listed.
 __device__ bool between(uint32_t n, const Settings& s, Quick& q, Mid& m) {
     const Kind kind = kind_of(s, n);
     m.above = 0.0;
     m.first = m.end = -1;
-    int at = -1;  // the bin that likely holds the cut
     if (kind.sums()) {
         if (s.m > 0.0) m.ref = m.top;
         m.least = s.m > 0.0 ? least_key(s.m, m.top, s.c) : kLowest;
         return true;
     }
-    // the bins' counts added up
-    uint32_t mine[4], items;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) mine[e] = q.count[4 * threadIdx.x + e];
-    const uint32_t before = quick_before(mine[0] + mine[1] + mine[2] + mine[3], items, q.word);
-    mine[0] += before;
-#pragma unroll
-    for (int e = 1; e < 4; ++e) mine[e] += mine[e - 1];
-    static_assert(kBins == 4 * kThreads, "four bins a thread");
+    const Counts counts = counts_of(q);
     if (kind.by_count) {
-        if (s.k > m.tops + items) return false;
-        uint32_t c = 0;  // the bin with the k-th item
-#pragma unroll
-        for (int e = 0; e < 4; ++e) c += m.tops + mine[e] < s.k;
-        m.end = int(quick_count(c, q));
-        if (s.k <= m.tops) m.end = -1;
-    } else {
-        // from the least weights up: the bins that may leave 1 - p behind them, each item taken for one in its bin's middle and so off by
-        // at most half a bin's width (in the last bin, which has no lower end, for too large)
-        const Bins bins(m, s);
-        const double width = bins.per > 0.0f ? s.c / double(bins.per) : 0.0, off = exp2_of(0.501 * width), need = (1.0 - s.p) * m.all;
-        const double open = double(q.count[kBins - 1]) * exp2_of(-(double(kBins) - 0.5) * width);
-        double tail[4], sum;
-        uint32_t above = 0, each = 0, within = 0;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const uint32_t c = mine[e] - (e ? mine[e - 1] : before);
-            tail[e] = c ? double(c) * exp2_of(-(double(4 * threadIdx.x + e) + 0.5) * width) : 0.0;
-        }
-        double have = quick_before(tail[0] + tail[1] + tail[2] + tail[3], sum, q.part);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            have += tail[e];
-            const double behind = sum - have;
-            above += behind - open > need * off;
-            each += behind > need;
-            within += behind * off > need;
-        }
-        above = quick_count(above, q), each = quick_count(each, q), within = quick_count(within, q);
-        at = int(min(each, kBins - 1));
-        m.first = bins.per > 0.0f && sum - open > need * off ? int(above) : -1;
-        m.end = sum * off > need ? int(min(within, kBins - 1)) : -1;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int e = 0; e < 4; ++e) q.count[4 * threadIdx.x + e] = mine[e];
-    __syncthreads();
-    const auto upto = [&](int b) { return b < 0 ? 0u : q.count[min(b, int(kBins) - 1)]; };
-    if (kind.by_count) {
-        if (m.tops + upto(m.end) > kListed) return false;
-    } else {
-        // from the top if that is few; of many items those in the middle, where errors cancel out
-        for (;;) {
-            if (m.first <= 0 || m.tops + upto(m.end) <= kFew) m.first = -1;
-            if ((m.first < 0 ? m.tops + upto(m.end) : upto(m.end) - upto(m.first - 1)) <= kListed) break;
-            const int first = m.first < 0 ? 0 : m.first;
-            if (m.end <= at && first >= at && m.first >= 0) return false;
-            m.first = min(first + max((at - first + 1) / 2, 1), max(at, 1));
-            m.end = max(m.end - max((m.end - at + 1) / 2, 0), at);
-        }
+        if (s.k > m.tops + counts.items) return false;
+        range_by_count(s.k, counts, q, m);
+        if (m.tops + upto(q, m.end) > kListed) return false;
+    } else if (!narrow(range_by_weight(s, (1.0 - s.p) * m.all, counts, q, m), q, m)) {
+        return false;
     }
     m.least = s.m > 0.0 ? least_key(s.m, m.top, s.c) : kLowest;
     return true;
+}
+
+// The same along falling logits.  First: what the cut needs, or, where nothing is cut, what the draw does; -2 for the end: the second pass
+// lists nothing and adds up what min-p keeps.
+constexpr int kNoList = -2;
+__device__ bool between_falling(uint32_t n, const Settings& s, double u, Quick& q, Mid& m) {
+    const Kind kind = kind_of(s, n);
+    m.above = m.kept = 0.0;
+    m.target = -1.0;
+    m.whole = false;
+    m.first = m.end = -1;
+    m.least = s.m > 0.0 ? least_key(s.m, m.top, s.c) : kLowest;
+    const Counts counts = counts_of(q);
+    if (kind.by_count) {
+        if (s.k > m.tops + counts.items) return false;
+        range_by_count(s.k, counts, q, m);
+        return m.tops + upto(q, m.end) <= kListed;
+    }
+    if (s.m == 0.0 && !kind.by_weight) {
+        m.kept = m.all;
+        m.target = u * m.all;
+        return narrow(range_by_weight(s, m.all - m.target, counts, q, m), q, m);
+    }
+    int at = 0;
+    m.end = int(kBins);
+    if (kind.by_weight) at = range_by_weight(s, (1.0 - s.p) * m.all, counts, q, m);
+    if (s.m > 0.0) {
+        // what min-p keeps, if that is few, from the top, unless top-p's cut lies above its end
+        const float least = value_of(m.least);
+        const int end = least > m.ref ? -1 : min(int(Bins(m, s).of(least)), int(kBins) - 1);
+        if (m.tops + upto(q, end) <= kListed && (m.first > 0 || end <= m.end)) {
+            m.first = -1;
+            m.end = end;
+            m.whole = true;
+            return true;
+        }
+    }
+    if (kind.by_weight) return narrow(at, q, m);
+    m.end = kNoList;
+    return true;
+}
+// Again: the bins around the target.  summed: whether the counts are added up.
+__device__ bool between_again(const Settings& s, bool summed, Quick& q, Mid& m) {
+    Counts counts;
+    if (!summed) {
+        counts = counts_of(q);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) counts.mine[e] = q.count[4 * threadIdx.x + e];
+        counts.before = threadIdx.x ? q.count[4 * threadIdx.x - 1] : 0u;
+        counts.items = q.count[kBins - 1];
+        counts.last = counts.items - q.count[kBins - 2];
+    }
+    m.above = 0.0;
+    return narrow(range_by_weight(s, m.all - m.target, counts, q, m), q, m);
 }
 
 // The second pass: the items of the chosen bins are listed, and the sums of what lies above them and min-p keeps go to the chunks.
@@ -933,6 +1031,144 @@ __device__ void pass_two(const Logits<T>& x, const Settings& s, const Part& part
         }
     });
     m.above = quick_sum(above, q);
+}
+
+// The same along falling logits: the items of the chosen bins are listed, what lies above them is added up, and that of it which min-p keeps.
+// again: the list is for the draw, and what is kept is known.
+template <class T>
+__device__ void pass_two_falling(const Logits<T>& x, const Settings& s, const Part& part, bool again, Quick& q, Mid& m) {
+    if (!again && m.first < 0 && m.end == -1) {  // what lies above ref, listed already
+        if (threadIdx.x == 0) q.listed = m.tops;
+        __syncthreads();
+        return;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) q.listed = 0;
+    __syncthreads();
+    const float least = value_of(m.least);
+    double above = 0.0, kept = 0.0;
+    if (m.end == kNoList) {
+        through(x, part, [&](uint32_t, const float(&v)[8]) {
+            bool any = false;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) any |= v[e] >= least;
+            if (__any(any)) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const double w = exp2_of((double(v[e]) - double(m.ref)) * s.c);
+                    kept += v[e] >= least ? w : 0.0;
+                }
+            }
+        }, [](uint32_t) {});
+        m.kept = quick_sum(kept, q);
+        return;
+    }
+    const Bins bins(m, s);
+    const float past = nextafterf(m.ref, __builtin_inff());
+    const float up = m.first < 0 ? __builtin_inff() : m.first == 0 ? past : edge_of(bins, m.first - 1), down = m.end < 0 ? past : edge_of(bins, m.end);
+    through(x, part, [&](uint32_t i, const float(&v)[8]) {
+        bool high = false, in = false;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            high |= v[e] >= up;
+            in |= v[e] >= down && v[e] < up;
+        }
+        if (__any(high)) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const double w = exp2_of((double(v[e]) - double(m.ref)) * s.c);
+                above += v[e] >= up ? w : 0.0;
+                kept += v[e] >= up && v[e] >= least ? w : 0.0;
+            }
+        }
+        if (__any(in)) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (v[e] >= down && v[e] < up) {
+                    const uint32_t at = atomicAdd(&q.listed, 1u);
+                    if (at < kListed) q.list[at] = entry_of(key_of(v[e]), i + e);
+                }
+        }
+    }, [](uint32_t) {});
+    m.above = quick_sum(above, q);
+    if (!again && m.target < 0.0) m.kept = quick_sum(kept, q);
+}
+
+// From the list, and from what lies above it, the cut and the item.
+enum class Found { nothing, item, target };  // the row is one for the other way; it is drawn; what is kept is known, the item not listed
+template <class T>
+__device__ Found finish_falling(const Row& a, uint32_t row, const Logits<T>& x, const Settings& s, Quick& q, Mid& m) {
+    const Kind kind = kind_of(s, x.n);
+    const double u = inner(a.uniforms[row]);
+    if (m.target < 0.0 && m.end == kNoList) {
+        m.target = u * m.kept;
+        return Found::target;
+    }
+    const uint32_t listed = q.listed;
+    if (listed > kListed || !listed) return Found::nothing;
+    quick_sort(q.list, listed);
+    // their weights added up, eight neighbours a thread
+    double w[8], sum = 0.0, total;
+    const uint32_t from = 8 * threadIdx.x, held = kind.by_count ? min(listed, s.k) : listed;
+    static_assert(kListed == 8 * kThreads, "eight entries a thread");
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        w[e] = from + e < held ? weight(value_of(entry_key(q.list[from + e])), double(m.ref), s.c) : 0.0;
+        sum += w[e];
+    }
+    const double before = m.above + quick_before(sum, total, q.part);
+    uint32_t n = held;  // entries among which the item is
+    if (m.target < 0.0) {
+        if (kind.by_weight) {
+            const double enough = s.p * (kind.by_count ? total : m.all);
+            double run = before;
+            n = 0;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                n += from + e < held && run < enough;
+                run += w[e];
+            }
+            n = quick_count(n, q);
+            if (!kind.by_count && m.above >= enough && m.above > 0.0) return Found::nothing;  // the cut lies above the list, or below it
+            if (!kind.by_count && !m.whole && n == listed && m.above + total < enough && m.end < int(kBins) - 1) return Found::nothing;
+            n = max(n, 1u);
+        }
+        uint32_t keep = 0;
+        sum = 0.0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (from + e < n && entry_key(q.list[from + e]) >= m.least) {
+                ++keep;
+                sum += w[e];
+            }
+        n = quick_count(keep, q);
+        m.kept += quick_sum(sum, q);
+        m.target = u * m.kept;
+        if (m.first >= 0 && (!n || m.target < m.above)) return Found::target;
+    } else {
+        if (m.first >= 0 && m.above > m.target) return Found::nothing;  // the item lies above the list, or below it
+        if (m.above + total <= m.target && m.end < int(kBins) - 1) return Found::nothing;
+    }
+    // the first that brings the sum past the target, or the last that weighs something
+    uint32_t short_of = 0, some = 0;
+    double run = before;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        run += w[e];
+        const bool there = from + e < n && w[e] > 0.0;
+        some += there;
+        short_of += there && run <= m.target;
+    }
+    short_of = quick_count(short_of, q), some = quick_count(some, q);
+    if (!some) return Found::nothing;
+    const uint32_t at = min(short_of, some - 1);
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        if (from + e == at) {
+            a.items[row] = int64_t(uint32_t(q.list[at]));
+            if (a.log_probability) a.log_probability[row] = float(log(w[e] / m.kept));
+        }
+    return Found::item;
 }
 
 // From the list and the chunks' sums: the cut, and the item.
@@ -1041,7 +1277,7 @@ __device__ __forceinline__ Part whole_of(uint32_t n) {
 }
 
 // A row in one workgroup.  False: nothing is written, the row is one for the other way.
-template <class T>
+template <bool FALLING, class T>
 __device__ bool sample_quickly(const Row& a, uint32_t row, const Logits<T>& x, Quick& q) {
     const Settings s = settings_of(a, row);
     const Part part = whole_of(x.n);
@@ -1049,22 +1285,32 @@ __device__ bool sample_quickly(const Row& a, uint32_t row, const Logits<T>& x, Q
     if (!begin(x, q, m)) return false;
 #pragma nounroll
     for (int tries = 0;; ++tries) {
-        pass_one(x, s, part, q, m);
+        pass_one<FALLING>(x, s, part, q, m);
         if (fits(s, m)) break;
         if (tries || !(m.top < __builtin_inff())) return false;
         m.ref = m.top;  // the sample was too far below
     }
-    if (!between(x.n, s, q, m)) return false;
-    pass_two(x, s, part, q, m);
-    return finish(a, row, x, s, part, q, m);
+    if constexpr (FALLING) {
+#pragma nounroll
+        for (bool again = false;; again = true) {
+            if (!(again ? between_again(s, true, q, m) : between_falling(x.n, s, inner(a.uniforms[row]), q, m))) return false;
+            pass_two_falling(x, s, part, again, q, m);
+            const Found found = finish_falling(a, row, x, s, q, m);
+            if (found != Found::target) return found == Found::item;
+        }
+    } else {
+        if (!between(x.n, s, q, m)) return false;
+        pass_two(x, s, part, q, m);
+        return finish(a, row, x, s, part, q, m);
+    }
 }
 
-template <class T>
+template <class T, bool FALLING>
 __global__ __launch_bounds__(kThreads, 4) void sample_kernel(Row a) {
     __shared__ Both sh;
     for (uint32_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
         const Logits<T> x{static_cast<const T*>(a.logits) + row * a.stride, a.V};
-        if (!sample_quickly(a, row, x, sh.quick)) {
+        if (!sample_quickly<FALLING>(a, row, x, sh.quick)) {
             __syncthreads();
             sample_slowly(a, row, x, sh.slow);
         }
@@ -1084,14 +1330,17 @@ struct Joined {
     uint32_t tops, listed;
     uint32_t failed;   // set by the first pass alone: the sample holds no value to refer to
     uint32_t dropped;  // set by the second pass and read by the last kernel alone, so that a workgroup's waves see one `failed`
+    uint32_t again;    // set by the kernel that ends a row: its draw needs a list of its own
+    uint32_t pad[3];
     // written by it and the second
     Mid mid;
     float top[kSlices];
-    double all[kSlices], above[kSlices];
+    double all[kSlices], above[kSlices], kept[kSlices];
     double chunk[kMostChunks];
     uint64_t top_list[kTops], list[kListed];
 };
-constexpr uint32_t kCleared = kBins + 8;  // words
+constexpr uint32_t kCleared = kBins + 12;  // words
+static_assert(offsetof(Joined, mid) == 4 * kCleared, "what lies before it is cleared");
 
 __global__ __launch_bounds__(256) void sample_clear_kernel(Joined* j) {
     uint32_t* const p = reinterpret_cast<uint32_t*>(j + blockIdx.y);
@@ -1105,7 +1354,7 @@ __device__ __forceinline__ Part slice_of(uint32_t n) {
     return p;
 }
 
-template <class T>
+template <class T, bool FALLING>
 __global__ __launch_bounds__(kThreads, 8) void sample_one_kernel(Row a, Joined* joined) {
     __shared__ Brief q;
     __shared__ uint32_t base;
@@ -1122,14 +1371,14 @@ __global__ __launch_bounds__(kThreads, 8) void sample_one_kernel(Row a, Joined* 
         }
         return;
     }
-    pass_one(x, s, part, q, m);
+    pass_one<FALLING>(x, s, part, q, m);
     if (tid == 0) {
         j.top[blockIdx.x] = m.top;
         j.all[blockIdx.x] = m.all;
         if (blockIdx.x == 0) j.mid = m;
     }
     __syncthreads();
-    if (kind_of(s, x.n).sums()) {
+    if (!FALLING && kind_of(s, x.n).sums()) {
         if (s.m == 0.0)
             for (uint32_t i = part.from + tid; i < part.to; i += kThreads) j.chunk[i] = q.chunk[i];
         return;
@@ -1240,6 +1489,106 @@ __global__ __launch_bounds__(kThreads, 4) void sample_three_kernel(Row a, Joined
     }
 }
 
+// The second pass and the end of a row along falling logits; again: of the rows whose draw needs a list of its own.
+template <class T>
+__global__ __launch_bounds__(kThreads, 6) void sample_two_falling_kernel(Row a, Joined* joined, bool again) {
+    __shared__ Quick q;
+    __shared__ uint32_t base;
+    const uint32_t row = blockIdx.y, tid = threadIdx.x;
+    Joined& j = joined[row];
+    if (again ? !j.again : j.failed) return;
+    const Logits<T> x{static_cast<const T*>(a.logits) + row * a.stride, a.V};
+    const Settings s = settings_of(a, row);
+    const Part part = slice_of(x.n);
+    Mid m = j.mid;
+    m.top = -__builtin_inff();
+    m.all = 0.0;
+    for (uint32_t i = 0; i < gridDim.x; ++i) {
+        m.top = fmaxf(m.top, j.top[i]);
+        m.all += j.all[i];
+    }
+    m.tops = j.tops;
+    bool good = fits(s, m);
+    if (good) {
+        for (uint32_t i = tid; i < kBins; i += kThreads) q.count[i] = j.count[i];
+        __syncthreads();
+        good = again ? between_again(s, false, q, m) : between_falling(x.n, s, inner(a.uniforms[row]), q, m);
+    }
+    if (!good) {  // (every workgroup of the row finds the same)
+        if (blockIdx.x == 0 && tid == 0) j.dropped = 1;
+        return;
+    }
+    // (of what this kernel's other workgroups read of `mid` nothing changes: ref and low, and again also least, kept and target)
+    if (blockIdx.x == 0 && tid == 0) {
+        j.mid.top = m.top;
+        j.mid.all = m.all;
+        j.mid.first = m.first;
+        j.mid.end = m.end;
+        if (!again) {
+            j.mid.least = m.least;
+            j.mid.kept = m.kept;
+            j.mid.target = m.target;
+            j.mid.whole = m.whole;
+        }
+    }
+    pass_two_falling(x, s, part, again, q, m);
+    __syncthreads();
+    if (tid == 0) {
+        j.above[blockIdx.x] = m.above;
+        j.kept[blockIdx.x] = m.kept;
+    }
+    if (!again && m.first < 0 && m.end == -1) return;
+    const uint32_t n = q.listed;
+    if (n) {
+        if (tid == 0) base = atomicAdd(&j.listed, n);
+        __syncthreads();
+        for (uint32_t i = tid; i < min(n, kListed); i += kThreads)
+            if (base + i < kListed) j.list[base + i] = q.list[i];
+    }
+}
+
+template <class T>
+__global__ __launch_bounds__(kThreads, 4) void sample_three_falling_kernel(Row a, Joined* joined, uint32_t slices, bool again) {
+    __shared__ Both sh;
+    Quick& q = sh.quick;
+    const uint32_t row = blockIdx.x, tid = threadIdx.x;
+    Joined& j = joined[row];
+    if (again && !j.again) return;
+    const Logits<T> x{static_cast<const T*>(a.logits) + row * a.stride, a.V};
+    Found found = Found::nothing;
+    if (!j.failed && !j.dropped) {
+        const Settings s = settings_of(a, row);
+        Mid m = j.mid;
+        m.above = 0.0;
+        if (m.first >= 0)
+            for (uint32_t i = 0; i < slices; ++i) m.above += j.above[i];
+        if (m.target < 0.0) {
+            m.kept = 0.0;
+            if (m.first >= 0 || m.end == kNoList)
+                for (uint32_t i = 0; i < slices; ++i) m.kept += j.kept[i];
+        }
+        const bool listed = again || m.first >= 0 || m.end != -1;
+        const uint32_t n = listed ? j.listed : j.tops;
+        for (uint32_t i = tid; i < min(n, kListed); i += kThreads) q.list[i] = listed ? j.list[i] : j.top_list[i];
+        if (tid == 0) q.listed = n;
+        __syncthreads();
+        found = finish_falling(a, row, x, s, q, m);
+        if (found == Found::target) {
+            __syncthreads();
+            if (tid == 0) {
+                j.mid.kept = m.kept;
+                j.mid.target = m.target;
+                j.listed = 0;
+                j.again = 1;
+            }
+        }
+    }
+    if (found == Found::nothing) {
+        __syncthreads();
+        sample_slowly(a, row, x, sh.slow);
+    }
+}
+
 // Rows that are drawn from whole: after the first pass a wave each, eight a workgroup, which takes those together that the quick way does
 // not.
 template <class T>
@@ -1277,10 +1626,10 @@ uint32_t slices_of(const va_context* ctx, uint32_t rows, uint32_t V, bool whole)
 }
 constexpr uint32_t kBatch = 1024;  // rows that share a launch, and a workspace
 
-template <class T>
+template <class T, bool FALLING>
 va_status run(va_context* ctx, const Row& all, bool whole, Joined* joined, uint32_t slices) {
     if (!slices) {
-        sample_kernel<T><<<dim3(std::min<uint32_t>(all.rows, 1u << 20)), dim3(kThreads), 0, ctx->stream>>>(all);
+        sample_kernel<T, FALLING><<<dim3(std::min<uint32_t>(all.rows, 1u << 20)), dim3(kThreads), 0, ctx->stream>>>(all);
         VA_CHECK_LAUNCH(ctx);
         return VA_OK;
     }
@@ -1294,8 +1643,8 @@ va_status run(va_context* ctx, const Row& all, bool whole, Joined* joined, uint3
         if (a.top_ps) a.top_ps += r;
         if (a.min_ps) a.min_ps += r;
         if (a.top_ks) a.top_ks += r;
-        if (whole) {
-            sample_one_kernel<T><<<dim3(slices, a.rows), dim3(kThreads), 0, ctx->stream>>>(a, joined);
+        if (whole && !FALLING) {
+            sample_one_kernel<T, false><<<dim3(slices, a.rows), dim3(kThreads), 0, ctx->stream>>>(a, joined);
             VA_CHECK_LAUNCH(ctx);
             sample_whole_kernel<T><<<dim3(ceil_div(a.rows, kWaves)), dim3(kThreads), 0, ctx->stream>>>(a, joined, slices);
             VA_CHECK_LAUNCH(ctx);
@@ -1303,8 +1652,19 @@ va_status run(va_context* ctx, const Row& all, bool whole, Joined* joined, uint3
         }
         sample_clear_kernel<<<dim3((kCleared + 255) / 256, a.rows), dim3(256), 0, ctx->stream>>>(joined);
         VA_CHECK_LAUNCH(ctx);
-        sample_one_kernel<T><<<dim3(slices, a.rows), dim3(kThreads), 0, ctx->stream>>>(a, joined);
+        sample_one_kernel<T, FALLING><<<dim3(slices, a.rows), dim3(kThreads), 0, ctx->stream>>>(a, joined);
         VA_CHECK_LAUNCH(ctx);
+        if constexpr (FALLING) {
+            // (top-k's list holds the item, and of whole rows the first list does)
+            const bool by_count = !a.top_ks && ((a.top_k > 0 && a.top_k < a.V) || (!a.temperatures && a.temperature == 0.0f));
+            for (int again = 0; again < (whole || by_count ? 1 : 2); ++again) {
+                sample_two_falling_kernel<T><<<dim3(slices, a.rows), dim3(kThreads), 0, ctx->stream>>>(a, joined, again != 0);
+                VA_CHECK_LAUNCH(ctx);
+                sample_three_falling_kernel<T><<<dim3(a.rows), dim3(kThreads), 0, ctx->stream>>>(a, joined, slices, again != 0);
+                VA_CHECK_LAUNCH(ctx);
+            }
+            continue;
+        }
         sample_two_kernel<T><<<dim3(slices, a.rows), dim3(kThreads), 0, ctx->stream>>>(a, joined);
         VA_CHECK_LAUNCH(ctx);
         sample_three_kernel<T><<<dim3(a.rows), dim3(kThreads), 0, ctx->stream>>>(a, joined, slices);
@@ -1328,6 +1688,7 @@ va_status va_sample(va_context* ctx, const va_sample_desc* d, int64_t* out_items
     VA_REQUIRE(ctx, d->temperatures || (std::isfinite(d->temperature) && d->temperature >= 0.0f), "va_sample: the temperature must be finite and not negative");
     VA_REQUIRE(ctx, d->top_ks || d->top_k >= 0, "va_sample: top_k must not be negative");
     VA_REQUIRE(ctx, d->top_ps || (d->top_p > 0.0f && d->top_p <= 1.0f), "va_sample: top_p must lie in (0, 1]");
+    VA_REQUIRE(ctx, d->order == VA_SAMPLE_BY_ITEM || d->order == VA_SAMPLE_BY_LOGIT, "va_sample: unknown order %d", int(d->order));
     VA_REQUIRE(ctx, d->min_ps || (d->min_p >= 0.0f && d->min_p <= 1.0f), "va_sample: min_p must lie in [0, 1]");
     if (!d->rows) return VA_OK;
     VA_REQUIRE(ctx, d->logits && d->uniforms && out_items, "va_sample: NULL pointer");
@@ -1341,9 +1702,10 @@ va_status va_sample(va_context* ctx, const va_sample_desc* d, int64_t* out_items
     a.temperatures = d->temperatures, a.top_ps = d->top_ps, a.min_ps = d->min_ps, a.top_ks = d->top_ks;
     a.temperature = d->temperature, a.top_p = d->top_p, a.min_p = d->min_p, a.top_k = uint32_t(d->top_k);
     a.items = out_items, a.log_probability = out_log_probability, a.rows = d->rows, a.V = d->num_items;
+    a.falling = d->order == VA_SAMPLE_BY_LOGIT;
     // no row is cut, as the host can tell
     const bool whole = !a.temperatures && !a.top_ps && !a.min_ps && !a.top_ks && a.temperature > 0.0f && a.top_p >= 1.0f && a.min_p == 0.0f && (a.top_k == 0 || a.top_k >= a.V);
-    uint32_t slices = slices_of(ctx, d->rows, d->num_items, whole);
+    uint32_t slices = slices_of(ctx, d->rows, d->num_items, whole && !a.falling);
     Joined* joined = nullptr;
     if (slices) {
         const uint64_t need = uint64_t(std::min(d->rows, kBatch)) * sizeof(Joined);
@@ -1364,9 +1726,13 @@ va_status va_sample(va_context* ctx, const va_sample_desc* d, int64_t* out_items
             }
         }
     }
-    if (d->dtype == VA_DTYPE_F32) return run<float>(ctx, a, whole, joined, slices);
-    if (d->dtype == VA_DTYPE_F16) return run<_Float16>(ctx, a, whole, joined, slices);
-    return run<__bf16>(ctx, a, whole, joined, slices);
+    const auto go = [&](auto t) {
+        using T = decltype(t);
+        return a.falling ? run<T, true>(ctx, a, whole, joined, slices) : run<T, false>(ctx, a, whole, joined, slices);
+    };
+    if (d->dtype == VA_DTYPE_F32) return go(0.0f);
+    if (d->dtype == VA_DTYPE_F16) return go(_Float16(0));
+    return go(__bf16(0));
 }
 
 uint64_t va_sample_workspace(va_context* ctx, uint32_t rows, uint32_t num_items) {

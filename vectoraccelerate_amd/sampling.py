@@ -18,7 +18,8 @@ class SoftmaxSamplingKernel:
     With M a row's largest logit, item j weighs exp((x_j - M) / temperature).  Ordered by (logit descending, index ascending)
     topK keeps the first k items (0: all), topP the fewest whose weights add up to p of those that topK keeps, minP
     those that weigh at least minP.  The drawn item is the first, in the order of the items, at which the kept weights added up
-    exceed u times their sum; u in [0, 1) is given.  A temperature of 0 draws the most likely item, the first of those as
+    exceed u times their sum; u in [0, 1) is given.  With order "logits" it is the first in the order of the truncations: a smaller u draws
+    a more likely item, wherever it lies.  A temperature of 0 draws the most likely item, the first of those as
     likely.  NaN and -inf (a masked item) are never drawn; a row without an item gives -1 and a log probability of -inf.
     Weights and sums are fp64; the same inputs give the same items.
 
@@ -27,6 +28,7 @@ class SoftmaxSamplingKernel:
     """
 
     name = "SoftmaxSamplingKernel"
+    orders = {"items": 0, "logits": 1}
 
     def __init__(self, context: GPUContext):
         self.context = context
@@ -35,16 +37,18 @@ class SoftmaxSamplingKernel:
         """Bytes of a workspace for logits of that shape (0: none is used)."""
         return int(self.context.lib.va_sample_workspace(self.context.handle, rows, items))
 
-    def encode(self, logits, uniforms, outItems, outLogProbability=None, temperature=1.0, topK=0, topP=1.0, minP=0.0, workspace=None) -> None:
+    def encode(self, logits, uniforms, outItems, outLogProbability=None, temperature=1.0, topK=0, topP=1.0, minP=0.0, workspace=None, order: str = "items") -> None:
         """uniforms: float32 [T]; outItems: int64 [T]; outLogProbability (float32 [T] or None): of the drawn item among those
         that were kept.  workspace (uint8, or None): memory of the call's own in place of the context's scratch arena; a call that is
         captured into a graph without one takes a slower way, and no other call may use it meanwhile."""
         c, torch = self.context, _torch()
+        if order not in self.orders:
+            raise VectorError.invalidInput(f"order: {order!r} (one of {', '.join(self.orders)})")
         dtype = _dtype(logits, "logits")
         p, stride = _rows(logits, "logits", c.device)
         T, V = logits.shape
         d = _lib.SampleDesc(logits=p, uniforms=_vector(uniforms, "uniforms", torch.float32, T, c.device), stride=stride, rows=T, num_items=V, dtype=dtype,
-                            temperature=1.0, top_p=1.0)
+                            temperature=1.0, top_p=1.0, order=self.orders[order])
         for name, value, one, many, of in (("temperature", temperature, "temperature", "temperatures", torch.float32), ("topK", topK, "top_k", "top_ks", torch.int32),
                                            ("topP", topP, "top_p", "top_ps", torch.float32), ("minP", minP, "min_p", "min_ps", torch.float32)):
             if isinstance(value, torch.Tensor):
@@ -61,11 +65,11 @@ class SoftmaxSamplingKernel:
                                 _vector(outLogProbability, "outLogProbability", torch.float32, T, c.device) if outLogProbability is not None else None),
                 "va_sample")
 
-    def sample(self, logits, uniforms, temperature=1.0, topK=0, topP=1.0, minP=0.0):
+    def sample(self, logits, uniforms, temperature=1.0, topK=0, topP=1.0, minP=0.0, order: str = "items"):
         """(items, log probabilities)."""
         c, torch = self.context, _torch()
         items, logs = c.empty((logits.shape[0],), torch.int64), c.empty((logits.shape[0],), torch.float32)
         c.order_after_torch()
-        self.encode(logits, uniforms, items, logs, temperature, topK, topP, minP)
+        self.encode(logits, uniforms, items, logs, temperature, topK, topP, minP, order=order)
         c.synchronize()
         return items, logs
