@@ -261,7 +261,7 @@ def _run_own(s):
             microscaled.encodeQuantize(s["x"], queries)
         microscaled.encodeProduct(queries, MicroscaledRows(s["codes"], s["scales"], D), s["out"], scale=s["scale"], offsets=s["offsets"])
         return s["out"]
-    sampling.encode(s["logits"], s["uniforms"], s["out"]["items"], s["out"]["log_probability"], **s["set"])
+    sampling.encode(s["logits"], s["uniforms"], s["out"]["items"], s["out"]["log_probability"], **s["set"], order="logits")
     return s["out"]
 
 
