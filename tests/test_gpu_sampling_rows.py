@@ -2,6 +2,7 @@
 workgroups (va_sample.hip); against the definition in 64 bits."""
 from __future__ import annotations
 
+import numpy as np
 import pytest
 import torch
 
@@ -35,3 +36,48 @@ def test_rows_that_the_second_pass_gives_up_on(ctx, V, s):
     for _ in range(10):
         got = k.sample(x, u, **s)
         assert torch.equal(got[0], want[0]) and torch.equal(got[1].view(torch.int32), want[1].view(torch.int32))
+
+
+def _first_kept(x, temperature, topK, topP, minP):
+    """The first kept item that weighs anything in fp64, of one row: what u = 0 draws in the order of the items; and its share."""
+    x = np.asarray(x, np.float64)
+    items = np.nonzero(x > -np.inf)[0]
+    items = items[np.lexsort((items, -x[items]))]
+    w = np.exp((x[items] - x[items[0]]) / temperature)
+    upto = np.cumsum(w)
+    n = min(topK or len(items), len(items))
+    if topP < 1:
+        n = min(n, int(np.searchsorted(upto, topP * upto[n - 1])) + 1)
+    n = min(n, int((w >= minP).sum()))
+    first = int(items[:n][w[:n] > 0].min())
+    return first, float(np.exp((x[first] - x[items[0]]) / temperature) / upto[n - 1])
+
+
+@pytest.mark.parametrize("V", [1500, 9000, 40_000, 300_000])
+@pytest.mark.parametrize("s", [dict(), dict(temperature=0.5), dict(topK=1000), dict(topK=3000), dict(topK=200, topP=0.9999), dict(topP=0.9), dict(topP=1 - 2.0**-24), dict(minP=1e-30), dict(topK=100, minP=1e-20)])
+def test_nothing_random_draws_the_first_kept_item(ctx, V, s):
+    """u = 0 draws the first kept item, little as it may weigh: 2^-701 of the largest, items that do so together where none does alone,
+    below 2^-51 of a list's largest, and behind masked ones."""
+    g = torch.Generator().manual_seed(V)
+    x = torch.full((7, V), -torch.inf)
+    x[0, 1:512] = -486.0
+    x[0, 700] = 0.0
+    x[1, 5] = -486.1
+    x[1, 1400:] = torch.randn(V - 1400, generator=g)
+    x[2, 9:] = torch.randn(V - 9, generator=g) - 40.0
+    x[2, 1300:1340] = torch.randn(40, generator=g)
+    x[3] = torch.randn(V, generator=g)
+    x[3, :3] = -torch.inf
+    x[4, 7:600] = -480.0 - torch.rand(593, generator=g) * 30
+    x[4, V - 1] = 3.0
+    x[5, 3:] = -36.0
+    x[5, 600:900] = torch.rand(300, generator=g)
+    x[6, 100:] = -300.0
+    x[6, V - 300 :] = 1.0
+    settings = dict(temperature=1.0, topK=0, topP=1.0, minP=0.0) | s
+    items, logs = (t.cpu().tolist() for t in _kernel(ctx).sample(x.cuda(), torch.zeros(7, device="cuda"), **s))
+    settings["topP"], settings["minP"] = float(np.float32(settings["topP"])), float(np.float32(settings["minP"]))
+    for t in range(7):
+        want, share = _first_kept(x[t].double().numpy(), **settings)
+        assert items[t] == want, f"row {t}: item {items[t]} where {want} is right"
+        assert abs(logs[t] - np.log(share)) <= 2.0**-22 * abs(np.log(share)) + 1e-10, f"row {t}"

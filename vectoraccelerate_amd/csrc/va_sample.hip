@@ -599,8 +599,8 @@ __device__ uint32_t least_key(double m, float top, double c) {
     return lo;
 }
 
-// The item that u draws from those that the cut keeps, whose weights the chunks' sums hold; by one wave.  (Sums of 2^-700 of the
-// whole and less are nothing.)
+// The item that u draws from those that the cut keeps, whose weights the chunks' sums hold; by one wave.  A chunk's sum is zero only
+// where none of its kept items weighs anything, so that an item is found within.
 template <class T>
 __device__ void draw(const Row& a, uint32_t row, const Logits<T>& x, const Part& part, uint32_t cut_key, uint32_t last, float ref, double c, const double* chunk) {
     const uint32_t lane = threadIdx.x & 63, per = (part.chunks + 63) / 64, from = lane * per, to = min(from + per, part.chunks);
@@ -612,13 +612,13 @@ __device__ void draw(const Row& a, uint32_t row, const Logits<T>& x, const Part&
         const double o = __shfl_up(upto, d);
         if (int(lane) >= d) upto += o;
     }
-    const double total = __shfl(upto, 63), least = total * 0x1p-700, target = fmax(double(a.uniforms[row]) * total, least);
+    const double total = __shfl(upto, 63), target = double(a.uniforms[row]) * total;
     // the first chunk that brings the sum past the target, or the last that holds something
     double run = upto - mine, start = 0.0;
     uint32_t found = 0, some = 0;
     for (uint32_t j = from; j < to && !found; ++j) {
         const double v = chunk[j];
-        if (v > least) {
+        if (v > 0.0) {
             some = j + 1;
             start = run;
             if (run + v > target) found = j + 1;
@@ -650,7 +650,7 @@ __device__ void draw(const Row& a, uint32_t row, const Logits<T>& x, const Part&
             const double o = __shfl_up(within, d);
             if (int(lane) >= d) within += o;
         }
-        const uint64_t holds = __ballot(sum > least), over = __ballot(sum > least && start + within > target);
+        const uint64_t holds = __ballot(sum > 0.0), over = __ballot(sum > 0.0 && start + within > target);
         if (holds) {
             const int l = over ? __ffsll((unsigned long long)over) - 1 : 63 - __clzll((long long)holds);
             // within the lane: the first past the target, or the last that weighs something
@@ -660,7 +660,7 @@ __device__ void draw(const Row& a, uint32_t row, const Logits<T>& x, const Part&
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 here += ws[e];
-                if (!done && ws[e] > least) {
+                if (!done && ws[e] > 0.0) {
                     im = int(i) + e;
                     wm = ws[e];
                     done = here > target;
@@ -1256,14 +1256,23 @@ __device__ bool finish(const Row& a, uint32_t row, const Logits<T>& x, const Set
         }
         return true;
     }
-    // the kept ones' weights go to their chunks as whole numbers: no order of the additions changes those
+    // the kept ones' weights go to their chunks as whole numbers of 2^-50 of the largest: no order of the additions changes those; the
+    // upmost bit, which 4096 of them do not reach, tells a chunk whose items all round to zero from one without an item
     int order;
     (void)frexp(weight(value_of(entry_key(q.list[0])), double(m.ref), s.c), &order);
 #pragma unroll
     for (int e = 0; e < 8; ++e)
-        if (from + e < n && entry_key(q.list[from + e]) >= m.least) atomicAdd(&q.fixed[uint32_t(q.list[from + e]) / part.size], (unsigned long long)(ldexp(w[e], 50 - order) + 0.5));
+        if (from + e < n && w[e] > 0.0 && entry_key(q.list[from + e]) >= m.least) {
+            unsigned long long* const to = &q.fixed[uint32_t(q.list[from + e]) / part.size];
+            atomicOr(to, 1ull << 63);
+            atomicAdd(to, (unsigned long long)(ldexp(w[e], 50 - order) + 0.5));
+        }
     __syncthreads();
-    for (uint32_t i = threadIdx.x; i < part.chunks; i += kThreads) q.chunk[i] = (m.first >= 0 ? q.chunk[i] : 0.0) + ldexp(double(q.fixed[i]), order - 50);
+    for (uint32_t i = threadIdx.x; i < part.chunks; i += kThreads) {
+        const unsigned long long f = q.fixed[i];
+        const double v = (m.first >= 0 ? q.chunk[i] : 0.0) + ldexp(double(f & ~(1ull << 63)), order - 50);
+        q.chunk[i] = f && v == 0.0 ? 0x1p-1022 : v;
+    }
     __syncthreads();
     if (threadIdx.x < 64) draw(a, row, x, part, cut, last, m.ref, s.c, q.chunk);
     return true;
