@@ -519,3 +519,28 @@ def test_refusals(ctx):
     lst.close()
     with pytest.raises(VectorError):
         k.encode(lst, 1, 0.1)
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+@pytest.mark.parametrize("kind", [0, 2, 6])
+def test_the_least_epsilons(ctx, bits, kind):
+    """Divisors below fp32's normal values: epsilon alone, where v is zero; and m = v = 0, which moves nothing."""
+    k = _kernel(ctx)
+    n, rate, step = 700, 1e-3, 3
+    for epsilon in (1e-45, 1e-40, 1.1754e-38, 1.2e-38, 1e-30, 1e30, 2e30, 3e38):
+        p = [torch.randn(n, generator=torch.Generator().manual_seed(1)).to(KINDS[kind][0]).cuda()]
+        g = [torch.zeros(n, dtype=KINDS[kind][1], device="cuda")]
+        state = k.state(p, bits, masters=KINDS[kind][2])
+        if bits == 32:
+            state.first[0][::2] = 1e-37
+        out = _like(p, state)
+        k.step(k.tensorList(p, g, state, outputs=out), step, rate, beta1=0.9, beta2=0.99, epsilon=epsilon, weightDecay=0.0)
+        m = 0.9 * state.first[0].cpu().double() if bits == 32 else torch.zeros(n, dtype=torch.float64)
+        eps = float(torch.tensor(epsilon, dtype=F32))  # (what the step has of it)
+        want = (state.masters[0] if KINDS[kind][2] else p[0]).cpu().double().view(-1) - rate / (1 - 0.9**step) * m / eps
+        got = out[0][0].cpu().double()
+        assert bool(torch.isfinite(got).all())
+        # m is off by a half of the least fp32 value and 3 u, the quotient and the product by an u each, the sum by its own rounding
+        loose = (5 * U32 * m.abs() + 2.0**-149) * (rate / (1 - 0.9**step) / eps) + 2 * U32 * want.abs() + U[p[0].dtype] * want.abs() + TINY[p[0].dtype]
+        assert bool(((got - want).abs() <= loose).all()), f"epsilon {epsilon}"
+        assert torch.equal(got[1::2], p[0].cpu().double()[1::2])
