@@ -592,10 +592,11 @@ typedef struct {
     float rate_factor, decay_factor; /* of the step's rate and weight decay for this tensor */
 } va_adamw_tensor;
 typedef struct va_adamw_list va_adamw_list;
-/* The list laid out in device memory, once (allocates and waits; not while the stream is captured).  The tensors must
+/* The list laid out in device memory, once (allocates and waits; refused while the context's stream is captured).  The tensors must
  * live, where they are, as long as it is used, and no two of its arrays that are written may overlap. */
 va_status va_adamw_list_create(va_context* ctx, const va_adamw_tensor* tensors, uint32_t count, uint32_t moment_bits,
                                va_adamw_list** out);
+/* Frees it and waits for the device (not while a stream is captured). */
 va_status va_adamw_list_destroy(va_adamw_list* list);
 typedef struct {
     const int64_t* device_step; /* read on the device instead of step (a captured step), or NULL */

@@ -3,6 +3,7 @@ boundary, and what the Python classes check before they call.  No kernel is laun
 from __future__ import annotations
 
 import ctypes as C
+import subprocess
 
 import pytest
 import torch
@@ -91,3 +92,15 @@ def test_dimensions_and_counts_are_checked():
               lambda: sampling.encode(torch.zeros(4), torch.zeros(4), torch.zeros(4, dtype=torch.int64))):
         with pytest.raises(VectorError):
             f()
+
+
+def test_a_list_is_not_made_while_its_stream_is_captured(lib, tmp_path):
+    """tests/cpp/capture_host.cpp, whose runtime is host memory: a refusal before anything is allocated or copied."""
+    root = _lib.LIB_PATH.parent.parent
+    exe = tmp_path / "capture_host"
+    cmd = ["g++", "-std=c++17", "-O1", "-rdynamic", f"-I{root / 'include'}", "-I/opt/rocm/include", str(root / "tests" / "cpp" / "capture_host.cpp"), f"-L{_lib.LIB_PATH.parent}",
+           "-lva_hip", f"-Wl,-rpath,{_lib.LIB_PATH.parent}", "-Wl,-rpath-link,/opt/rocm/lib", "-o", str(exe)]
+    proc = subprocess.run(cmd, capture_output=True, text=True)
+    assert proc.returncode == 0, proc.stderr
+    run = subprocess.run([str(exe)], capture_output=True, text=True, timeout=60)
+    assert run.returncode == 0 and "ok" in run.stdout, run.stdout + run.stderr

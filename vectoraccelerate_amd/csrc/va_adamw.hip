@@ -447,6 +447,10 @@ va_status va_adamw_list_create(va_context* ctx, const va_adamw_tensor* tensors, 
     *out = nullptr;
     VA_REQUIRE(ctx, moment_bits == 8 || moment_bits == 32, "va_adamw_list_create: moments of %u bits (8 or 32)", moment_bits);
     DeviceGuard guard(ctx->device);
+    // (before anything is allocated: what a capture forbids would end it, and be an error of the caller's next calls)
+    hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+    VA_CHECK_HIP(ctx, hipStreamIsCapturing(ctx->stream, &capture));
+    VA_REQUIRE(ctx, capture == hipStreamCaptureStatusNone, "va_adamw_list_create: the context's stream is being captured");
     try {
         return create(ctx, tensors, count, moment_bits, out);
     } catch (const std::bad_alloc&) {

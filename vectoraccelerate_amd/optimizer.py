@@ -160,7 +160,7 @@ class AdamWKernel:
 
     def tensorList(self, parameters, gradients, state: AdamWState, outputs=None, rateFactors=None, decayFactors=None) -> AdamWTensors:
         """The list of a step, in place or into ``outputs`` (parameters and an AdamWState); rateFactors and decayFactors: a
-        factor of each tensor's rate and weight decay.  Allocates and waits."""
+        factor of each tensor's rate and weight decay.  Allocates and waits; refused while the context's stream is captured."""
         return AdamWTensors(self.context, parameters, gradients, state, outputs, rateFactors, decayFactors)
 
     def encode(self, tensors: AdamWTensors, step, learningRate, beta1: float = 0.9, beta2: float = 0.999, epsilon: float = 1e-8,
