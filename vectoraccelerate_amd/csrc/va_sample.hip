@@ -1066,6 +1066,7 @@ __device__ void pass_two_falling(const Logits<T>& x, const Settings& s, const Pa
     const Bins bins(m, s);
     const float past = nextafterf(m.ref, __builtin_inff());
     const float up = m.first < 0 ? __builtin_inff() : m.first == 0 ? past : edge_of(bins, m.first - 1), down = m.end < 0 ? past : edge_of(bins, m.end);
+    const bool apart = !again && least > up;  // min-p leaves out some of what lies above
     through(x, part, [&](uint32_t i, const float(&v)[8]) {
         bool high = false, in = false;
 #pragma unroll
@@ -1078,7 +1079,7 @@ __device__ void pass_two_falling(const Logits<T>& x, const Settings& s, const Pa
             for (int e = 0; e < 8; ++e) {
                 const double w = exp2_of((double(v[e]) - double(m.ref)) * s.c);
                 above += v[e] >= up ? w : 0.0;
-                kept += v[e] >= up && v[e] >= least ? w : 0.0;
+                if (apart) kept += v[e] >= least ? w : 0.0;
             }
         }
         if (__any(in)) {
@@ -1091,7 +1092,7 @@ __device__ void pass_two_falling(const Logits<T>& x, const Settings& s, const Pa
         }
     }, [](uint32_t) {});
     m.above = quick_sum(above, q);
-    if (!again && m.target < 0.0) m.kept = quick_sum(kept, q);
+    if (!again && m.target < 0.0) m.kept = apart ? quick_sum(kept, q) : m.above;
 }
 
 // From the list, and from what lies above it, the cut and the item.
