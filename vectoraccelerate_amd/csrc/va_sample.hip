@@ -43,7 +43,6 @@ struct Row {
     int64_t* items;
     float* log_probability;
     uint32_t rows, V;
-    bool falling;  // drawn along falling logits
 };
 
 // What a row is drawn by.  Values on the device that make no sense are taken as the nearest that does.
@@ -246,7 +245,7 @@ __device__ uint32_t last_tie(const Logits<T>& x, const Cut& cut, bool of, Shared
 
 // Any row, whatever it holds, one pass after another: what the quick way below does not take.  (By value: by reference the caller keeps
 // its arguments in private memory.)
-template <class T>
+template <bool FALLING, class T>
 __device__ __noinline__ void sample_slowly(Row a, uint32_t row, Logits<T> x, Shared& sh) {
     const Settings s = settings_of(a, row);
     uint32_t top_key = 0, n = 0;
@@ -294,7 +293,7 @@ __device__ __noinline__ void sample_slowly(Row a, uint32_t row, Logits<T> x, Sha
         const uint32_t k = key_of(v);
         return k > cut.key || (k == cut.key && i <= last);
     };
-    if (a.falling) {
+    if constexpr (FALLING) {
         double sum = 0.0;
         for (uint32_t i = threadIdx.x; i < x.n; i += kThreads) {
             const float v = x(i);
@@ -826,7 +825,7 @@ __device__ Counts counts_of(Quick& q) {
 #pragma unroll
     for (int e = 1; e < 4; ++e) c.mine[e] += c.mine[e - 1];
     static_assert(kBins == 4 * kThreads, "four bins a thread");
-    __syncthreads();
+    // (every thread has read its own, and the last one, behind a barrier of quick_before)
 #pragma unroll
     for (int e = 0; e < 4; ++e) q.count[4 * threadIdx.x + e] = c.mine[e];
     __syncthreads();
@@ -1322,7 +1321,7 @@ __global__ __launch_bounds__(kThreads, 4) void sample_kernel(Row a) {
         const Logits<T> x{static_cast<const T*>(a.logits) + row * a.stride, a.V};
         if (!sample_quickly<FALLING>(a, row, x, sh.quick)) {
             __syncthreads();
-            sample_slowly(a, row, x, sh.slow);
+            sample_slowly<FALLING>(a, row, x, sh.slow);
         }
         __syncthreads();
     }
@@ -1495,7 +1494,7 @@ __global__ __launch_bounds__(kThreads, 4) void sample_three_kernel(Row a, Joined
     }
     if (!done) {
         __syncthreads();
-        sample_slowly(a, row, x, sh.slow);
+        sample_slowly<false>(a, row, x, sh.slow);
     }
 }
 
@@ -1595,7 +1594,7 @@ __global__ __launch_bounds__(kThreads, 4) void sample_three_falling_kernel(Row a
     }
     if (found == Found::nothing) {
         __syncthreads();
-        sample_slowly(a, row, x, sh.slow);
+        sample_slowly<true>(a, row, x, sh.slow);
     }
 }
 
@@ -1622,7 +1621,7 @@ __global__ __launch_bounds__(kThreads, 4) void sample_whole_kernel(Row a, Joined
     for (uint32_t i = 0; i < uint32_t(kWaves); ++i)
         if (left[i]) {
             const uint32_t r = blockIdx.x * kWaves + i;
-            sample_slowly(a, r, Logits<T>{static_cast<const T*>(a.logits) + r * a.stride, a.V}, slow);
+            sample_slowly<false>(a, r, Logits<T>{static_cast<const T*>(a.logits) + r * a.stride, a.V}, slow);
             __syncthreads();
         }
 }
@@ -1712,10 +1711,10 @@ va_status va_sample(va_context* ctx, const va_sample_desc* d, int64_t* out_items
     a.temperatures = d->temperatures, a.top_ps = d->top_ps, a.min_ps = d->min_ps, a.top_ks = d->top_ks;
     a.temperature = d->temperature, a.top_p = d->top_p, a.min_p = d->min_p, a.top_k = uint32_t(d->top_k);
     a.items = out_items, a.log_probability = out_log_probability, a.rows = d->rows, a.V = d->num_items;
-    a.falling = d->order == VA_SAMPLE_BY_LOGIT;
+    const bool falling = d->order == VA_SAMPLE_BY_LOGIT;
     // no row is cut, as the host can tell
     const bool whole = !a.temperatures && !a.top_ps && !a.min_ps && !a.top_ks && a.temperature > 0.0f && a.top_p >= 1.0f && a.min_p == 0.0f && (a.top_k == 0 || a.top_k >= a.V);
-    uint32_t slices = slices_of(ctx, d->rows, d->num_items, whole && !a.falling);
+    uint32_t slices = slices_of(ctx, d->rows, d->num_items, whole && !falling);
     Joined* joined = nullptr;
     if (slices) {
         const uint64_t need = uint64_t(std::min(d->rows, kBatch)) * sizeof(Joined);
@@ -1738,7 +1737,7 @@ va_status va_sample(va_context* ctx, const va_sample_desc* d, int64_t* out_items
     }
     const auto go = [&](auto t) {
         using T = decltype(t);
-        return a.falling ? run<T, true>(ctx, a, whole, joined, slices) : run<T, false>(ctx, a, whole, joined, slices);
+        return falling ? run<T, true>(ctx, a, whole, joined, slices) : run<T, false>(ctx, a, whole, joined, slices);
     };
     if (d->dtype == VA_DTYPE_F32) return go(0.0f);
     if (d->dtype == VA_DTYPE_F16) return go(_Float16(0));
