@@ -81,3 +81,17 @@ def test_nothing_random_draws_the_first_kept_item(ctx, V, s):
         want, share = _first_kept(x[t].double().numpy(), **settings)
         assert items[t] == want, f"row {t}: item {items[t]} where {want} is right"
         assert abs(logs[t] - np.log(share)) <= 2.0**-22 * abs(np.log(share)) + 1e-10, f"row {t}"
+
+
+@pytest.mark.parametrize("V", [900, 10_000, 50_000])
+def test_fewer_items_than_top_k_keeps(ctx, V):
+    """Masked rows: one item left, some, as many as top-k keeps, one more; in either order of the draw."""
+    from tests.test_gpu_sampling_order import _check as check_falling
+
+    x, u = _logits(24, V, torch.float32, V)
+    g = torch.Generator().manual_seed(V)
+    for t, left in enumerate([1, 2, 3, 40, 49, 50, 51, 64, 65, 300, 500, 850] * 2):
+        x[t, torch.randperm(V, generator=g)[left:]] = -torch.inf if t < 12 else torch.nan
+    for s in (dict(topK=50), dict(topK=300, topP=0.9), dict(topK=600, minP=0.01), dict(topK=899), dict(topK=50, topP=0.5, minP=0.1)):
+        _check(ctx, x, u, **s)
+        check_falling(ctx, x, u, **s)

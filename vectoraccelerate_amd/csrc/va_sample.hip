@@ -834,9 +834,10 @@ __device__ Counts counts_of(Quick& q) {
 // items of the bins up to b, whose counts are added up
 __device__ __forceinline__ uint32_t upto(const Quick& q, int b) { return b < 0 ? 0u : q.count[min(b, int(kBins) - 1)]; }
 
-// The bin with the k-th item.
+// The bin with the k-th item, or, of a row that has fewer (a mask leaves them), with the last.
 __device__ void range_by_count(uint32_t k, const Counts& counts, Quick& q, Mid& m) {
     uint32_t c = 0;
+    k = min(k, m.tops + counts.items);
 #pragma unroll
     for (int e = 0; e < 4; ++e) c += m.tops + counts.mine[e] < k;
     m.end = int(quick_count(c, q));
@@ -893,7 +894,6 @@ __device__ bool between(uint32_t n, const Settings& s, Quick& q, Mid& m) {
     }
     const Counts counts = counts_of(q);
     if (kind.by_count) {
-        if (s.k > m.tops + counts.items) return false;
         range_by_count(s.k, counts, q, m);
         if (m.tops + upto(q, m.end) > kListed) return false;
     } else if (!narrow(range_by_weight(s, (1.0 - s.p) * m.all, counts, q, m), q, m)) {
@@ -915,7 +915,6 @@ __device__ bool between_falling(uint32_t n, const Settings& s, double u, Quick& 
     m.least = s.m > 0.0 ? least_key(s.m, m.top, s.c) : kLowest;
     const Counts counts = counts_of(q);
     if (kind.by_count) {
-        if (s.k > m.tops + counts.items) return false;
         range_by_count(s.k, counts, q, m);
         return m.tops + upto(q, m.end) <= kListed;
     }
