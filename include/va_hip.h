@@ -636,12 +636,10 @@ va_status va_mx_product_rows(va_context* ctx, const void* queries, uint64_t quer
 
 /* An item for each row of logits.  With M a row's largest logit, item j weighs w_j = exp((x_j - M) / temperature).  Ordered by (x
  * descending, index ascending), top_k keeps the first k items (0: all); top_p the fewest whose weights add up to
- * p of those that top_k keeps; min_p those with w_j >= min_p.  The drawn item is the first, in the order of the items or
- * (VA_SAMPLE_BY_LOGIT) in that of the truncations, at which the kept weights added up exceed u times their sum: along falling
- * logits a smaller u draws a more likely item, wherever it lies.  A temperature of 0 draws the most likely item, the first of
+ * p of those that top_k keeps; min_p those with w_j >= min_p.  The drawn item is the first, in the order of the items, at which
+ * the kept weights added up exceed u times their sum.  A temperature of 0 draws the most likely item, the first of
  * those that are as likely.  NaN and -inf are never drawn (+inf: those items alone, as likely as each other); a
  * row without an item gives -1 and a log probability of -inf.  Weights and sums are fp64. */
-typedef enum { VA_SAMPLE_BY_ITEM = 0, VA_SAMPLE_BY_LOGIT = 1 } va_sample_order;
 typedef struct {
     const void* logits;          /* [rows x num_items] */
     const float* uniforms;       /* u in [0, 1), [rows] */
@@ -656,7 +654,6 @@ typedef struct {
     int32_t top_k;               /* 0: all */
     float top_p;                 /* (0, 1] */
     float min_p;                 /* [0, 1] */
-    int32_t order;               /* va_sample_order */
     void* workspace;             /* device memory at a multiple of 16 bytes, or NULL: the context's scratch arena; a captured call */
     uint64_t workspace_bytes;    /* without one does all in one launch, which takes longer for much to do */
 } va_sample_desc;
@@ -664,6 +661,11 @@ typedef struct {
 uint64_t va_sample_workspace(va_context* ctx, uint32_t rows, uint32_t num_items);
 /* out_log_probability (may be NULL): of the drawn item among those that were kept. */
 va_status va_sample(va_context* ctx, const va_sample_desc* desc, int64_t* out_items, float* out_log_probability);
+/* The same, drawn in the given order: VA_SAMPLE_BY_ITEM as va_sample does, VA_SAMPLE_BY_LOGIT in the order of the
+ * truncations, so that a smaller u draws a more likely item, wherever it lies. */
+typedef enum { VA_SAMPLE_BY_ITEM = 0, VA_SAMPLE_BY_LOGIT = 1 } va_sample_order;
+va_status va_sample_in_order(va_context* ctx, const va_sample_desc* desc, va_sample_order order, int64_t* out_items,
+                             float* out_log_probability);
 
 #ifdef __cplusplus
 }

@@ -683,9 +683,9 @@ class SoftmaxSamplingKernel {
         d.temperature = 1.0f, d.top_p = 1.0f;
         return d;
     }
-    Result sample(const va_sample_desc& d) const {
+    Result sample(const va_sample_desc& d, va_sample_order order = VA_SAMPLE_BY_ITEM) const {
         Result r{DeviceBuffer<int64_t>(ctx_, d.rows), DeviceBuffer<float>(ctx_, d.rows)};
-        ctx_.check(va_sample(ctx_.handle(), &d, r.items.data(), r.logProbability.data()), "va_sample");
+        ctx_.check(va_sample_in_order(ctx_.handle(), &d, order, r.items.data(), r.logProbability.data()), "va_sample_in_order");
         return r;
     }
 

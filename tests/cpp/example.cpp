@@ -201,6 +201,9 @@ int main(int argc, char** argv) {
             auto drawn = sampling.sample(sd);
             save(dir + "/sample_items.bin", drawn.items.download());
             save(dir + "/sample_log.bin", drawn.logProbability.download());
+            auto falling = sampling.sample(sd, VA_SAMPLE_BY_LOGIT);
+            save(dir + "/falling_items.bin", falling.items.download());
+            save(dir + "/falling_log.bin", falling.logProbability.download());
         }
 
         std::string kind = "none";

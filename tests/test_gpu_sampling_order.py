@@ -3,6 +3,7 @@ from the middle, draws that need a list of their own, ties, masks, rows that the
 from __future__ import annotations
 
 import ctypes as C
+import subprocess
 
 import numpy as np
 import pytest
@@ -270,6 +271,27 @@ def test_refusals(ctx):
         with pytest.raises(VectorError):
             k.sample(x, u, order=order)
     for order in (-1, 2):
-        d = _lib.SampleDesc(logits=x.data_ptr(), uniforms=u.data_ptr(), stride=50, rows=4, num_items=50, dtype=0, temperature=1.0, top_p=1.0, order=order)
-        assert ctx.lib.va_sample(ctx.handle, C.byref(d), items.data_ptr(), None) == 1
+        d = _lib.SampleDesc(logits=x.data_ptr(), uniforms=u.data_ptr(), stride=50, rows=4, num_items=50, dtype=0, temperature=1.0, top_p=1.0)
+        assert ctx.lib.va_sample_in_order(ctx.handle, C.byref(d), order, items.data_ptr(), None) == 1
     assert items.tolist() == [9] * 4
+
+
+def test_cpp_class(tmp_path):
+    """SoftmaxSamplingKernel::sample with an order, run by tests/cpp/va_example."""
+    from tests.test_gpu_learning_run import EXE
+
+    if not EXE.exists():
+        from vectoraccelerate_amd.build import build_cpp_example
+
+        build_cpp_example()
+    Q, N, D, classes = 40, 1500, 32, 8
+    g = np.random.default_rng(4)
+    for name, n in (("q", Q), ("x", N), ("c", classes)):
+        g.standard_normal((n, D), np.float32).tofile(tmp_path / f"{name}.bin")
+    proc = subprocess.run([str(EXE), str(tmp_path), str(Q), str(N), str(D), str(classes), "5", "4"], capture_output=True, text=True, timeout=120)
+    assert proc.returncode == 0, proc.stderr
+    rd = lambda n, kind: np.fromfile(tmp_path / f"{n}.bin", kind)  # noqa: E731
+    scores, items, logs = rd("mx_scores", np.float32).reshape(Q, N), rd("falling_items", np.int64), rd("falling_log", np.float32)
+    for t in range(Q):
+        item, probability, near = drawn(scores[t], 0.375, 1.0, 10, 1.0, 0.0)
+        assert near > 2.0**-40 and int(items[t]) == item and abs(float(logs[t]) - np.log(probability)) < 2.0**-22 * abs(np.log(probability)) + 1e-9

@@ -104,3 +104,12 @@ def test_a_list_is_not_made_while_its_stream_is_captured(lib, tmp_path):
     assert proc.returncode == 0, proc.stderr
     run = subprocess.run([str(exe)], capture_output=True, text=True, timeout=60)
     assert run.returncode == 0 and "ok" in run.stdout, run.stdout + run.stderr
+
+
+def test_an_order_needs_a_context(lib):
+    for order in (0, 1, 2):
+        assert lib.va_sample_in_order(None, C.byref(_lib.SampleDesc()), order, None, None) == 1
+    sampling = SoftmaxSamplingKernel(NoDevice())
+    for order in ("", "falling", None):
+        with pytest.raises(VectorError):
+            sampling.encode(torch.zeros(4, 4), torch.zeros(4), torch.zeros(4, dtype=torch.int64), order=order)

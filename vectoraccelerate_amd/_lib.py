@@ -137,6 +137,7 @@ SIGNATURES: dict[str, tuple] = {
     "va_mx_product": (_st, [_p, _p, _p, C.c_float, _p, _i32, _p, _u64]),
     "va_mx_product_rows": (_st, [_p, _p, _u64, _i32, _u32, _p, C.c_float, _p, _i32, _p, _u64]),
     "va_sample": (_st, [_p, _p, _p, _p]),
+    "va_sample_in_order": (_st, [_p, _p, _i32, _p, _p]),
     "va_sample_workspace": (_u64, [_p, _u32, _u32]),
     "va_probe_mfma": (_st, [_p, _i32, _i32, _u32, _p]),
 }
@@ -321,7 +322,6 @@ class SampleDesc(C.Structure):
         ("top_k", C.c_int32),
         ("top_p", C.c_float),
         ("min_p", C.c_float),
-        ("order", C.c_int32),
         ("workspace", C.c_void_p),
         ("workspace_bytes", C.c_uint64),
     ]

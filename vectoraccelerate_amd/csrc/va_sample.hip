@@ -1689,6 +1689,10 @@ using namespace va;
 extern "C" {
 
 va_status va_sample(va_context* ctx, const va_sample_desc* d, int64_t* out_items, float* out_log_probability) {
+    return va_sample_in_order(ctx, d, VA_SAMPLE_BY_ITEM, out_items, out_log_probability);
+}
+
+va_status va_sample_in_order(va_context* ctx, const va_sample_desc* d, va_sample_order order, int64_t* out_items, float* out_log_probability) {
     if (!ctx) return VA_ERR_INVALID_ARG;
     VA_REQUIRE(ctx, d, "va_sample: NULL description");
     VA_REQUIRE(ctx, d->dtype == VA_DTYPE_F32 || d->dtype == VA_DTYPE_F16 || d->dtype == VA_DTYPE_BF16, "va_sample: unknown type %d", int(d->dtype));
@@ -1696,7 +1700,7 @@ va_status va_sample(va_context* ctx, const va_sample_desc* d, int64_t* out_items
     VA_REQUIRE(ctx, d->temperatures || (std::isfinite(d->temperature) && d->temperature >= 0.0f), "va_sample: the temperature must be finite and not negative");
     VA_REQUIRE(ctx, d->top_ks || d->top_k >= 0, "va_sample: top_k must not be negative");
     VA_REQUIRE(ctx, d->top_ps || (d->top_p > 0.0f && d->top_p <= 1.0f), "va_sample: top_p must lie in (0, 1]");
-    VA_REQUIRE(ctx, d->order == VA_SAMPLE_BY_ITEM || d->order == VA_SAMPLE_BY_LOGIT, "va_sample: unknown order %d", int(d->order));
+    VA_REQUIRE(ctx, order == VA_SAMPLE_BY_ITEM || order == VA_SAMPLE_BY_LOGIT, "va_sample_in_order: unknown order %d", int(order));
     VA_REQUIRE(ctx, d->min_ps || (d->min_p >= 0.0f && d->min_p <= 1.0f), "va_sample: min_p must lie in [0, 1]");
     if (!d->rows) return VA_OK;
     VA_REQUIRE(ctx, d->logits && d->uniforms && out_items, "va_sample: NULL pointer");
@@ -1710,7 +1714,7 @@ va_status va_sample(va_context* ctx, const va_sample_desc* d, int64_t* out_items
     a.temperatures = d->temperatures, a.top_ps = d->top_ps, a.min_ps = d->min_ps, a.top_ks = d->top_ks;
     a.temperature = d->temperature, a.top_p = d->top_p, a.min_p = d->min_p, a.top_k = uint32_t(d->top_k);
     a.items = out_items, a.log_probability = out_log_probability, a.rows = d->rows, a.V = d->num_items;
-    const bool falling = d->order == VA_SAMPLE_BY_LOGIT;
+    const bool falling = order == VA_SAMPLE_BY_LOGIT;
     // no row is cut, as the host can tell
     const bool whole = !a.temperatures && !a.top_ps && !a.min_ps && !a.top_ks && a.temperature > 0.0f && a.top_p >= 1.0f && a.min_p == 0.0f && (a.top_k == 0 || a.top_k >= a.V);
     uint32_t slices = slices_of(ctx, d->rows, d->num_items, whole && !falling);

@@ -48,7 +48,7 @@ class SoftmaxSamplingKernel:
         p, stride = _rows(logits, "logits", c.device)
         T, V = logits.shape
         d = _lib.SampleDesc(logits=p, uniforms=_vector(uniforms, "uniforms", torch.float32, T, c.device), stride=stride, rows=T, num_items=V, dtype=dtype,
-                            temperature=1.0, top_p=1.0, order=self.orders[order])
+                            temperature=1.0, top_p=1.0)
         for name, value, one, many, of in (("temperature", temperature, "temperature", "temperatures", torch.float32), ("topK", topK, "top_k", "top_ks", torch.int32),
                                            ("topP", topP, "top_p", "top_ps", torch.float32), ("minP", minP, "min_p", "min_ps", torch.float32)):
             if isinstance(value, torch.Tensor):
@@ -61,9 +61,9 @@ class SoftmaxSamplingKernel:
                 setattr(d, one, float(value))
         if workspace is not None:
             d.workspace, d.workspace_bytes = _vector(workspace, "workspace", torch.uint8, workspace.numel(), c.device), workspace.numel()
-        c.check(c.lib.va_sample(c.handle, C.byref(d), _vector(outItems, "outItems", torch.int64, T, c.device),
-                                _vector(outLogProbability, "outLogProbability", torch.float32, T, c.device) if outLogProbability is not None else None),
-                "va_sample")
+        c.check(c.lib.va_sample_in_order(c.handle, C.byref(d), self.orders[order], _vector(outItems, "outItems", torch.int64, T, c.device),
+                                         _vector(outLogProbability, "outLogProbability", torch.float32, T, c.device) if outLogProbability is not None else None),
+                "va_sample_in_order")
 
     def sample(self, logits, uniforms, temperature=1.0, topK=0, topP=1.0, minP=0.0, order: str = "items"):
         """(items, log probabilities)."""
