@@ -574,7 +574,7 @@ va_status va_grad_clip(va_context* ctx, const va_tensor_list* list, float max_no
  * one that holds NaN or inf has a scale that is not finite.
  * Each array is read from one pointer and written to another, which may be the same. */
 typedef struct {
-    const void* param;          /* not read where there is a master */
+    const void* param;          /* where there is a master, read only to be copied by a step that is not taken */
     const void* grad;           /* of the parameters' type, or fp32 */
     const void* first;          /* m: fp32, or e4m3 codes */
     const void* second;         /* v: fp32, or e4m3 codes of its root */
@@ -639,7 +639,8 @@ va_status va_mx_product_rows(va_context* ctx, const void* queries, uint64_t quer
  * p of those that top_k keeps; min_p those with w_j >= min_p.  The drawn item is the first, in the order of the items, at which
  * the kept weights added up exceed u times their sum.  A temperature of 0 draws the most likely item, the first of
  * those that are as likely.  NaN and -inf are never drawn (+inf: those items alone, as likely as each other); a
- * row without an item gives -1 and a log probability of -inf.  Weights and sums are fp64. */
+ * row without an item gives -1 and a log probability of -inf.  Weights and sums are fp64, a weight good to 4e-14 of itself;
+ * one below 2^-1000 of the largest may count as zero, and an item without weight is not drawn.  u = 0 draws the first item kept. */
 typedef struct {
     const void* logits;          /* [rows x num_items] */
     const float* uniforms;       /* u in [0, 1), [rows] */

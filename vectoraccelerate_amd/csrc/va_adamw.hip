@@ -8,9 +8,10 @@
 // with fp32 moments 22, with 8-bit ones 10.1).  The list lies in device memory, laid out once when it is made, so a step is
 // one launch whatever the number of tensors.  A tensor is cut into chunks of kChunk values; a workgroup takes a run of
 // chunks and goes from tensor to tensor as they end, and a launch is as many workgroups as the CUs hold at once.
-// Measured: 290 bf16 tensors, 38.6M values with fp32 moments and copies, 217 us, 5.0 TB/s, what a large copy reaches; 50 bf16
-// tensors of 228M values with 8-bit moments 541 us, 4.2 TB/s: beside memory by the vector instructions, of which the
-// random words' 64-bit products and the exact root are most; 6 tensors of a head 5 us, a launch.
+// Measured: 290 bf16 tensors, 38.6M values with fp32 moments and copies, 219 us, 4.9 TB/s, what a large copy reaches; 50 bf16
+// tensors of 228M values with 8-bit moments 522-555 us, 4.1-4.4 TB/s (to 680 in the first milliseconds of work, while the clock is
+// down): beside memory by the vector instructions, of which the random words' 64-bit products and the exact root are most; 6 tensors
+// of a head 5 us, a launch.
 //
 // 8-bit moments: e4m3 codes with an fp32 scale for each group of 256 values (a tensor's first value starts one), of m
 // and of r = sqrt(v), whose range is half of v's in binary orders.  Each group's largest value is code 448.  What

@@ -157,9 +157,11 @@ __device__ __forceinline__ void planes(const float (&v)[8], bf16x8 (&o)[P]) {
 // to bf16: 410 us of stores and 500 us of products took 1000).
 // The 16-byte chunks of an LDS row are swizzled by the row, so fragment reads meet in no bank.  An item goes to the LDS row that puts
 // two neighbours into one lane: a half-wave writes 64 neighbouring scores of a query, whole lines, from its registers.
-// Measured: 4096 x 262,144 x 768 to bf16 750 us, 2.2 PFLOP/s and 2.9 TB/s of scores: bound by LDS, whose reads for 64 x 64 products a
-// wave take as long as the products (470 us without the stores; the matrix instructions alone 300), and by the stores between them
-// (410 alone).  512 x 100,003 x 384 to fp32: 44 us, its scores at 4.7 TB/s.
+// Measured: 4096 x 262,144 x 768 to bf16 745-785 us, 2.2 PFLOP/s and 2.8 TB/s of scores (660 where the clock is up).  No unit is full: the
+// matrix cores are busy for 27 % of the time, LDS for 17 %; a wave spends 30 % at waits and barriers.  What bounds it is how little the products
+// (470 us without the stores; their instructions alone 300) and the stores (410 alone) overlap: a CU has one workgroup, whose eight
+// waves meet at a barrier a stage.  512 x 100,003 x 384 to fp32: 43-45 us, its scores at 4.7 TB/s with the outputs in cache, 63 from memory:
+// rows that begin inside lines are written in pieces of lines.
 template <int WQ_, int WI_, int GS_>
 struct Shape {
     static constexpr int WQ = WQ_, WI = WI_, GS = GS_, WAVES = WQ * WI, THREADS = 64 * WAVES;

@@ -7,7 +7,10 @@
 // times their sum.  NaN and -inf are no items.
 //
 // Weights and their sums are fp64 throughout: an item next to a border has to fall on its side of it, and fp32's weights of
-// 100,000 items would move one draw in a hundred.  A sum's order is fixed, so results repeat bit for bit.
+// 100,000 items would move one draw in a hundred.  A weight is off by 4e-14 of itself (exp2_of), and listed ones go to chunks in steps of
+// 2^-50 of the largest: both are far below the distance of a border from a u of 24 digits.  A weight below 2^-1000 of the largest may be
+// zero.  A sum's order is fixed, so results repeat bit for bit (a row's passes divided among workgroups and in one add up in other
+// orders, and may part at a border by such a difference).
 //
 // Two passes over a row.  What weights refer to is the largest of a sample, so the first pass needs no other before it: it counts
 // the items in 2048 bins of equal width, adds up all weights where top-p asks for the sum, and lists the few items
@@ -17,12 +20,16 @@
 // Along falling logits (FALLING) the drawn item is the end of a prefix too, that whose weights exceed u times what is kept.  A list
 // from the top holds it beside the cut.  Of long prefixes the list near the cut, or a pass without a list, gives what is kept, and a further
 // pass, its bins chosen as before, lists the items around u times that; where nothing is cut the second pass does.
-// A long row's passes are divided among workgroups, with a launch for each pass; a row that the quick way cannot take (+inf, more
-// items of one value than a list holds) goes through as many passes as it needs.
+// A long row's passes are divided among workgroups, with a launch for each pass.  A row that the quick way cannot take goes through as many
+// passes as it needs, by one workgroup: one with +inf, with no item in the sample, with more than 4096 items in the bins that hold the cut
+// (equal logits, top-k beyond that), with more than 1024 items above the sample's largest, or, divided, with one that weighs 2^900
+// times that (6.2 logits above it at a temperature of 0.01).  One row of 262,144: 51 us by the quick way at p 0.9, 2.3 ms so with a lone
+// peak at a temperature of 0.01, 3.3 ms with all logits alike; along falling logits 75 us, 3.8 and 6.1 ms.
 //
-// Bound by the weights' fp64 instructions where there are many (2048 x 100,003 fp16, uncut: 192 us, 1.07 G weights a ms, 2.1 TB/s), by
-// the chain of short steps where there are few (64 x 262,144 bf16, p 0.9: 77 us, of which clearing 5, the passes 27 and 38, the end
-// 15; 1 x 10,000, top 50: 23 us in one launch).
+// Bound by the weights' fp64 instructions where there are many (2048 x 100,003 fp16, uncut: 190 us, 1.07 G weights a ms, 2.1 TB/s), by
+// the chain of short steps where there are few (64 x 262,144 bf16, p 0.9: 78 us, of which clearing 5, the passes 25 and 35, the end
+// 16; 1 x 10,000, top 50: 23 us in one launch).  Along falling logits 521 us, of each 1024 rows' 260 the passes 107 and 124 and the end
+// 25; 60 us, as what min-p keeps is listed from the top and nothing above it weighed; 27 us.
 #include <algorithm>
 #include <cmath>
 #include <cstddef>

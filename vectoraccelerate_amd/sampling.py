@@ -21,7 +21,8 @@ class SoftmaxSamplingKernel:
     exceed u times their sum; u in [0, 1) is given.  With order "logits" it is the first in the order of the truncations: a smaller u draws
     a more likely item, wherever it lies.  A temperature of 0 draws the most likely item, the first of those as
     likely.  NaN and -inf (a masked item) are never drawn; a row without an item gives -1 and a log probability of -inf.
-    Weights and sums are fp64; the same inputs give the same items.
+    Weights and sums are fp64 (a weight is good to 4e-14 of itself; one below 2^-1000 of the largest may count as zero, and an item without
+    weight is not drawn); the same inputs give the same items.
 
     Each setting is one number, or a device tensor with a value for each row (float32, topK int32), where what lies outside a setting's
     range is taken as its nearest value, and NaN as "not truncated" (a temperature: as 0).
