@@ -295,3 +295,26 @@ def test_cpp_class(tmp_path):
     for t in range(Q):
         item, probability, near = drawn(scores[t], 0.375, 1.0, 10, 1.0, 0.0)
         assert near > 2.0**-40 and int(items[t]) == item and abs(float(logs[t]) - np.log(probability)) < 2.0**-22 * abs(np.log(probability)) + 1e-9
+
+
+def test_without_probabilities_and_far_rows(ctx):
+    """No log probabilities asked for; rows more than 2^32 bytes apart."""
+    k = _kernel(ctx)
+    stride = (1 << 31) + 64
+    room = torch.empty(2 * stride + 30_000, dtype=torch.float16, device="cuda")
+    for V in (1000, 30_000):
+        far = torch.as_strided(room, (3, V), (stride, 1))
+        x, u = _logits(3, V, torch.float16, V)
+        far.copy_(x)
+        dx, du = x.cuda(), u.cuda()
+        for s in (dict(), dict(topK=9), dict(topP=0.8, temperature=3.0)):
+            a = k.sample(dx, du, **s, order="logits")
+            b = k.sample(far, du, **s, order="logits")
+            assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+            items = torch.full((5,), 7, device="cuda")
+            torch.cuda.synchronize()
+            k.encode(far, du, items[1:4], None, **s, order="logits")
+            ctx.synchronize()
+            assert items.tolist() == [7, *a[0].tolist(), 7]
+    del room, far
+    torch.cuda.empty_cache()
