@@ -95,3 +95,16 @@ def test_fewer_items_than_top_k_keeps(ctx, V):
     for s in (dict(topK=50), dict(topK=300, topP=0.9), dict(topK=600, minP=0.01), dict(topK=899), dict(topK=50, topP=0.5, minP=0.1)):
         _check(ctx, x, u, **s)
         check_falling(ctx, x, u, **s)
+
+
+@pytest.mark.parametrize("V", [2000, 300_000])
+def test_a_share_below_the_least_number(ctx, V):
+    """An item far below the row's largest, which no sample meets: if u = 0 draws it, its log probability is finite and its own."""
+    x = torch.zeros(3, V)
+    x[:, 0] = torch.tensor([-430.0, -600.0, -690.0])
+    x[:, 1711] = torch.tensor([600.0, 400.0, 620.0])
+    items, logs = (t.cpu().tolist() for t in _kernel(ctx).sample(x.cuda(), torch.zeros(3, device="cuda")))
+    for t in range(3):
+        a = x[t].double()
+        want = float(a[items[t]] - torch.logsumexp(a, 0))
+        assert items[t] in (0, 1) and abs(logs[t] - want) <= 2.0**-22 * abs(want), f"row {t}: {items[t]}, {logs[t]} where {want} is right"

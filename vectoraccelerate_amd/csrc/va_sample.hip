@@ -101,6 +101,12 @@ __device__ __forceinline__ double exp2_of(double t) {
 }
 __device__ __forceinline__ double weight(float x, double top, double c) { return double(x) == top ? 1.0 : exp2_of((double(x) - top) * c); }  // (x or top may be infinite)
 
+// The logarithm of a weight's share, also of one whose quotient fp64 does not hold (u = 0 may draw it).
+__device__ __forceinline__ float log_share(double w, double total) {
+    const double r = w / total;
+    return float(r >= 0x1p-1000 || !(w > 0.0) ? log(r) : log(w) - log(total));
+}
+
 constexpr int kThreads = 512, kWaves = kThreads / 64;
 constexpr int kDigits = 4;       // of a level of the search by weight
 constexpr uint32_t kMostChunks = 1024;
@@ -311,7 +317,7 @@ __device__ __noinline__ void sample_slowly(Row a, uint32_t row, Logits<T> x, Sha
         const uint32_t item = last_tie(x, by, true, sh);
         if (threadIdx.x == 0) {
             a.items[row] = item;
-            if (a.log_probability) a.log_probability[row] = float(log(weight(value_of(by.key), top, s.c) / sum));
+            if (a.log_probability) a.log_probability[row] = log_share(weight(value_of(by.key), top, s.c), sum);
         }
         return;
     }
@@ -366,7 +372,7 @@ __device__ __noinline__ void sample_slowly(Row a, uint32_t row, Logits<T> x, Sha
         }
         if (lane == 0) {
             a.items[row] = item;
-            if (a.log_probability) a.log_probability[row] = float(log(w / total));
+            if (a.log_probability) a.log_probability[row] = log_share(w, total);
         }
     }
 }
@@ -680,7 +686,7 @@ __device__ void draw(const Row& a, uint32_t row, const Logits<T>& x, const Part&
     }
     if (lane == 0) {
         a.items[row] = item;
-        if (a.log_probability) a.log_probability[row] = float(log(w / total));
+        if (a.log_probability) a.log_probability[row] = log_share(w, total);
     }
 }
 
@@ -692,8 +698,9 @@ struct Mid {
     int first, end;        // the bins whose items are listed (first -1: and what lies above them)
     uint32_t least;        // the least key that min-p keeps
     // along falling logits
-    double kept, target;   // what is kept weighs (the second pass: that of it which lies above the listed items); the drawn item is the first past
-    bool whole;            // target, which is negative as long as it is not known; whether all that min-p keeps is listed
+    double kept;           // the sum of the kept weights; out of the second pass, of those above the listed items
+    double target;         // the drawn item is the first at which the sum exceeds it; negative: not known yet
+    bool whole;            // all that min-p keeps is listed
 };
 struct Kind {
     bool by_count, by_weight;
@@ -832,7 +839,7 @@ __device__ Counts counts_of(Quick& q) {
 #pragma unroll
     for (int e = 1; e < 4; ++e) c.mine[e] += c.mine[e - 1];
     static_assert(kBins == 4 * kThreads, "four bins a thread");
-    // (every thread has read its own, and the last one, behind a barrier of quick_before)
+    // (every thread has read its own, and the last one, before the barriers of quick_before)
 #pragma unroll
     for (int e = 0; e < 4; ++e) q.count[4 * threadIdx.x + e] = c.mine[e];
     __syncthreads();
@@ -1172,7 +1179,7 @@ __device__ Found finish_falling(const Row& a, uint32_t row, const Logits<T>& x, 
     for (int e = 0; e < 8; ++e)
         if (from + e == at) {
             a.items[row] = int64_t(uint32_t(q.list[at]));
-            if (a.log_probability) a.log_probability[row] = float(log(w[e] / m.kept));
+            if (a.log_probability) a.log_probability[row] = log_share(w[e], m.kept);
         }
     return Found::item;
 }
@@ -1258,7 +1265,7 @@ __device__ bool finish(const Row& a, uint32_t row, const Logits<T>& x, const Set
         const uint32_t item = best ? 0x80000000u - best : far - 1;
         if (mine && index == item) {
             a.items[row] = int64_t(item);
-            if (a.log_probability) a.log_probability[row] = float(log(ws[threadIdx.x] / kept));
+            if (a.log_probability) a.log_probability[row] = log_share(ws[threadIdx.x], kept);
         }
         return true;
     }
